@@ -43,7 +43,8 @@ typedef enum {
     MPS_ERR_STATE = -9        /* e.g. mps_spmm before mps_plan_partition                        */
 } mps_status;
 
-typedef enum { MPS_F32 = 0, MPS_F16 = 1 } mps_dtype;
+/* MPS_BF16 is taken by the routed operators (mps_route ... mps_adapters_backward) only. */
+typedef enum { MPS_F32 = 0, MPS_F16 = 1, MPS_BF16 = 2 } mps_dtype;
 
 MPS_API const char *mps_last_error(void);
 MPS_API const char *mps_version(void);
@@ -374,6 +375,103 @@ MPS_API int mps_multi_slab(const mps_multi *m, int32_t g, int32_t *device, int32
 MPS_API int mps_multi_set_b(mps_multi *m, const void *host_B);
 MPS_API int mps_multi_spmm(mps_multi *m, int32_t repeat, int32_t gather_c, float *ms_spmm, float *ms_gather);
 MPS_API int mps_multi_get_c(mps_multi *m, void *host_C, int32_t from_gpu);
+
+/* ------------------------------------------------------------------ routed rows ---------- */
+
+/* Products in which every row is multiplied by the matrix it is routed to: mixtures of experts, weights per relation or
+ * node type, low-rank adapters.  The routing is a sparse matrix like A above, kept as the rows listed by group:
+ *   group_ptr[g] .. group_ptr[g + 1]   the slots of group g (a row_ptr: n_groups + 1 entries, from 0, never falling),
+ *   slot_row[slot]                     the input row in that slot (a col_idx), -1 behind the last slot in use,
+ *   slot_of[row, j]                    the slot of the row's j-th choice, -1 for none.
+ * mps_group_rows builds the three from ids, mps_route from router logits.  No reference counterpart.
+ *
+ * All of these launch asynchronously on `stream`, allocate nothing, keep nothing between calls, may be captured into a graph,
+ * and run side by side on different streams.  Types are MPS_F32, MPS_F16 and MPS_BF16 (weights, biases and scales always
+ * fp32); every sum is kept in fp32 and rounded once.  Arrays are contiguous; results do not depend on the run.  The device
+ * checks what it indexes by: a bad id, slot or group offset is skipped (no access outside the arrays, what it named is
+ * undefined) and reported by mps_routed_check. */
+
+/* Waits for the stream and returns MPS_ERR_ARG if a routed operator on the current device met an index out of range since
+ * the last check, MPS_ERR_DEVICE if one gave up a wait (its result is undefined); clears both. */
+MPS_API int mps_routed_check(void *stream);
+
+typedef enum { MPS_SCORE_SOFTMAX = 0, MPS_SCORE_SIGMOID = 1 } mps_score;
+
+typedef struct {
+    int32_t n_experts;   /* 1 .. 1024                                                                          */
+    int32_t top_k;       /* experts per row, 1 .. 32                                                           */
+    int32_t score;       /* mps_score                                                                          */
+    int32_t n_groups;    /* experts fall into this many equal contiguous groups, 1 .. 32 (1: no groups)        */
+    int32_t top_groups;  /* groups kept per row; top_k <= top_groups * n_experts / n_groups                    */
+    int32_t group_top;   /* a group ranks by its largest key (1) or the sum of its two largest scores + b (2)  */
+    int32_t renormalise; /* weights divided by their sum over the chosen                                       */
+    float scale;         /* and multiplied by this                                                             */
+} mps_route_spec;
+
+/* Experts of every row of d_logits (n_rows x n_experts, dtype): s = softmax or sigmoid of the logits, choice by s + d_bias
+ * (fp32, n_experts; NULL: none, then by the logits themselves), ties to the lowest index, weights from s alone:
+ *   d_weights[row, j] = scale * s_j  or  scale * s_j / sum of the chosen s  (n_rows x top_k fp32), largest key first.
+ * The choice is that of exact arithmetic up to fp64 rounding: where fp32 scores lie too close to tell, the row is decided
+ * in fp64.  An expert with a logit (or s + bias) of -inf or NaN is never chosen; where none is left the id is -1 and the
+ * weight 0.  A NaN logit (softmax: also +inf) makes all weights of its row NaN.  Where the chosen scores underflow together
+ * their ratios are still right.  The group arrays (all three or none NULL) receive the rows listed by expert as from
+ * mps_group_rows: n_experts + 1, n_rows * top_k and n_rows x top_k entries. */
+MPS_API int mps_route(int32_t n_rows, const mps_route_spec *spec, int dtype, const void *d_logits, const float *d_bias, int32_t *d_ids,
+              float *d_weights, int32_t *d_group_ptr, int32_t *d_slot_row, int32_t *d_slot_of, void *stream);
+
+/* Gradient of mps_route's weights by the logits, d_dlogits (n_rows x n_experts, dtype) written whole; the choice d_ids and
+ * the bias are constants.  spec as for mps_route (its group fields only have to be valid).  Ids below 0 are skipped. */
+MPS_API int mps_route_backward(int32_t n_rows, const mps_route_spec *spec, int dtype, const void *d_logits, const int32_t *d_ids,
+                       const float *d_dweights, void *d_dlogits, void *stream);
+
+/* Rows listed by group from d_ids (n_rows x per_row; a negative id is no group): d_group_ptr n_groups + 1 entries, d_slot_row
+ * n_rows * per_row (-1 behind the last slot in use), d_slot_of n_rows x per_row.  Within a group slots keep the order of the
+ * ids.  n_groups <= 1024. */
+MPS_API int mps_group_rows(int32_t n_rows, int32_t per_row, int32_t n_groups, const int32_t *d_ids, int32_t *d_group_ptr, int32_t *d_slot_row,
+                   int32_t *d_slot_of, void *stream);
+
+/* y[s, :] = x[slot_row[s], :] * W[g]^T for the slots s of every group g: d_x n_rows x k, d_w n_groups x n x k, d_y n_slots x n.
+ * transpose != 0: y[s, :] = x[slot_row[s], :] * W[g] with d_x n_rows x n and d_y n_slots x k - the gradient by the rows.
+ * d_slot_row == NULL: x has a row per slot (n_rows >= n_slots).  Rows of d_y outside the groups are left as they were.
+ * n_groups <= 1024; k and n up to 2^21. */
+MPS_API int mps_routed_product(int32_t n_slots, int32_t n_rows, int32_t n_groups, int32_t k, int32_t n, int dtype, int transpose,
+                       const int32_t *d_group_ptr, const int32_t *d_slot_row, const void *d_x, const void *d_w, void *d_y, void *stream);
+
+/* The gradient by the matrices: dW[g] = sum over the slots s of g of dy[s, :]^T x[slot_row[s], :], n_groups x n x k, zero for
+ * a group without slots.  d_dy n_slots x n, d_x n_rows x k; d_slot_row as above. */
+MPS_API int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_groups, int32_t k, int32_t n, int dtype, const int32_t *d_group_ptr,
+                     const int32_t *d_slot_row, const void *d_x, const void *d_dy, void *d_dw, void *stream);
+
+/* y[t, :] = sum over j of weights[t, j] * rows[slot_of[t, j], :] (d_weights NULL: 1 each; no term for a slot below 0):
+ * mps_spmm with the routing as A, for a fixed number of terms per row, without a plan.  d_rows n_slots x dim, d_y n_rows x dim.
+ * Summed in the order of j. */
+MPS_API int mps_routed_combine(int32_t n_rows, int32_t per_row, int32_t n_slots, int32_t dim, int dtype, const int32_t *d_slot_of,
+                       const float *d_weights, const void *d_rows, void *d_y, void *stream);
+
+/* Its gradients: d_drows[slot_of[t, j], :] = weights[t, j] * dy[t, :] (slots that no (t, j) names are left as they were; a
+ * slot may be named once) and d_dweights[t, j] = <dy[t, :], rows[slot_of[t, j], :]> in fp32, 0 for a slot below 0
+ * (d_dweights NULL: not wanted, d_rows may be NULL then). */
+MPS_API int mps_routed_combine_backward(int32_t n_rows, int32_t per_row, int32_t n_slots, int32_t dim, int dtype, const int32_t *d_slot_of,
+                                const float *d_weights, const void *d_dy, const void *d_rows, void *d_drows, float *d_dweights,
+                                void *stream);
+
+/* A shared projection with the low-rank pair of the adapter each row asks for:
+ *   y[t, :] = x[t, :] W^T + scale[a] (x[t, :] A[a]^T) B[a]^T,  a = ids[t]; a row with a negative id gets the projection alone.
+ * d_x n_rows x k, d_w n x k, d_a n_adapters x rank x k, d_b n_adapters x n x rank, d_scale n_adapters fp32 (NULL: 1), d_y
+ * n_rows x n.  d_group_ptr and d_slot_row list the rows by adapter (mps_group_rows of d_ids, per_row 1).  n_adapters <= 1024,
+ * rank <= 4096.  d_workspace: mps_adapters_workspace bytes (a negative return is an error), 256-byte aligned, for this call
+ * alone while it runs. */
+MPS_API int64_t mps_adapters_workspace(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, int backward);
+MPS_API int mps_adapters(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, const int32_t *d_ids,
+                 const int32_t *d_group_ptr, const int32_t *d_slot_row, const float *d_scale, const void *d_x, const void *d_w,
+                 const void *d_a, const void *d_b, void *d_y, void *d_workspace, int64_t workspace_bytes, void *stream);
+
+/* Its gradients by x, A and B (the shared projection and the scales are constants), each written whole:
+ *   dx = dy W + scale (dy B) A,   dA[a] = scale sum (dy B)^T x,   dB[a] = scale sum dy^T (x A^T)   over the rows of a. */
+MPS_API int mps_adapters_backward(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, const int32_t *d_ids,
+                          const int32_t *d_group_ptr, const int32_t *d_slot_row, const float *d_scale, const void *d_dy,
+                          const void *d_x, const void *d_w, const void *d_a, const void *d_b, void *d_dx, void *d_da, void *d_db,
+                          void *d_workspace, int64_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

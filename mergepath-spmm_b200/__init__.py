@@ -12,6 +12,7 @@ the stream), each a thin wrapper of one C-ABI entry point of libmps_b200.so (inc
     Plan / spmm                    the kernels and their launch loops    (ref :223-264, :388-574)
     spmm_host                      the whole program body on host arrays (ref :187-267)
     slab_bounds                    nnz-balanced row slabs for several GPUs (new)
+    route / routed_* / adapters    rows multiplied by the matrix each is routed to (new, routed.py)
 
 Nothing here computes on the CPU; without the CUDA library these calls raise.
 """
@@ -22,7 +23,9 @@ import ctypes as C
 import numpy as np
 
 from . import capi
-from .capi import F16, F32, MpsError  # noqa: F401
+from .capi import BF16, F16, F32, MpsError  # noqa: F401
+from .routed import *  # noqa: F401,F403
+from .routed import __all__ as _routed_all
 
 try:
     import torch
@@ -30,7 +33,7 @@ except Exception:  # pragma: no cover
     torch = None
 
 __all__ = ["Plan", "MultiGpu", "layout_query", "coo_to_csr", "coo_to_csr_device", "npz_to_csr", "spmm", "spmm_host", "spmm_host_resident_b", "spmm_host_scaled", "gather_probe", "gather_probe_stream", "partition_host", "schedule_host", "load_csr_rect", "spmm_noalloc", "partition_device", "schedule_device", "chunk_count", "load_csr", "save_csr",
-           "save_csr_bin", "load_csr_bin", "slab_bounds", "slab_rebase", "algorithmic_bytes", "F32", "F16", "MpsError"]
+           "save_csr_bin", "load_csr_bin", "slab_bounds", "slab_rebase", "algorithmic_bytes", "F32", "F16", "BF16", "MpsError"] + _routed_all
 
 
 def _stream_ptr(stream=None):

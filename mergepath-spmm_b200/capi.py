@@ -12,7 +12,8 @@ from . import build as _build
 
 OK = 0
 ERR_ARG, ERR_IO, ERR_FORMAT, ERR_CUDA, ERR_UNSUPPORTED, ERR_NOMEM, ERR_DEVICE, ERR_ALIGN, ERR_STATE = range(-1, -10, -1)
-F32, F16 = 0, 1
+F32, F16, BF16 = 0, 1, 2
+SCORES = {"softmax": 0, "sigmoid": 1}
 
 SYMBOLS = [
     "mps_last_error", "mps_version", "mps_csr_load", "mps_csr_load_rect", "mps_csr_free", "mps_csr_save", "mps_csr_save_bin",
@@ -20,6 +21,8 @@ SYMBOLS = [
     "mps_plan_destroy", "mps_plan_tune", "mps_plan_partition", "mps_spmm", "mps_spmm_scaled", "mps_plan_sync_check", "mps_plan_info", "mps_plan_set_walk", "mps_plan_layout", "mps_layout_query", "mps_plan_profile", "mps_plan_profile_read",
     "mps_algorithmic_bytes", "mps_gather_probe", "mps_gather_probe_stream", "mps_spmm_host", "mps_spmm_host_resident_b", "mps_spmm_host_scaled", "mps_partition_host", "mps_schedule_host", "mps_host_workspace_release", "mps_spmm_noalloc", "mps_slab_bounds", "mps_slab_bounds_items", "mps_slab_rebase", "mps_multi_create", "mps_multi_destroy", "mps_multi_slab",
     "mps_multi_set_b", "mps_multi_spmm", "mps_multi_get_c",
+    "mps_routed_check", "mps_route", "mps_route_backward", "mps_group_rows", "mps_routed_product", "mps_routed_wgrad", "mps_routed_combine",
+    "mps_routed_combine_backward", "mps_adapters_workspace", "mps_adapters", "mps_adapters_backward",
 ]
 
 
@@ -32,6 +35,11 @@ class MpsError(RuntimeError):
 class Csr(C.Structure):
     _fields_ = [("n_rows", C.c_int32), ("nnz", C.c_int32),
                 ("row_ptr", C.POINTER(C.c_int32)), ("col_idx", C.POINTER(C.c_int32))]
+
+
+class RouteSpec(C.Structure):
+    _fields_ = [("n_experts", C.c_int32), ("top_k", C.c_int32), ("score", C.c_int32), ("n_groups", C.c_int32), ("top_groups", C.c_int32),
+                ("group_top", C.c_int32), ("renormalise", C.c_int32), ("scale", C.c_float)]
 
 
 _lib = None
@@ -98,6 +106,18 @@ def lib():
     L.mps_multi_set_b.argtypes = [vp, vp]
     L.mps_multi_spmm.argtypes = [vp, i32, i32, C.POINTER(C.c_float), C.POINTER(C.c_float)]
     L.mps_multi_get_c.argtypes = [vp, vp, i32]
+    L.mps_routed_check.argtypes = [vp]
+    L.mps_route.argtypes = [i32, C.POINTER(RouteSpec), C.c_int] + [vp] * 8
+    L.mps_route_backward.argtypes = [i32, C.POINTER(RouteSpec), C.c_int] + [vp] * 5
+    L.mps_group_rows.argtypes = [i32] * 3 + [vp] * 5
+    L.mps_routed_product.argtypes = [i32] * 5 + [C.c_int] * 2 + [vp] * 6
+    L.mps_routed_wgrad.argtypes = [i32] * 5 + [C.c_int] + [vp] * 6
+    L.mps_routed_combine.argtypes = [i32] * 4 + [C.c_int] + [vp] * 5
+    L.mps_routed_combine_backward.argtypes = [i32] * 4 + [C.c_int] + [vp] * 7
+    L.mps_adapters_workspace.argtypes = [i32] * 5 + [C.c_int] * 2
+    L.mps_adapters_workspace.restype = i64
+    L.mps_adapters.argtypes = [i32] * 5 + [C.c_int] + [vp] * 10 + [i64, vp]
+    L.mps_adapters_backward.argtypes = [i32] * 5 + [C.c_int] + [vp] * 13 + [i64, vp]
     _lib = L
     return L
 

@@ -16,4 +16,6 @@ int32_t max_column(const int32_t *col_idx, long long nnz, int threads);
 // row_ptr[0] == 0, row_ptr non-decreasing, every column index inside [0, n_cols) (col_idx may be NULL): MPS_OK or
 // MPS_ERR_ARG with the offending position in the message.
 int check_csr_host(const char *who, int32_t n_rows, int32_t n_cols, const int32_t *row_ptr, const int32_t *col_idx, int threads);
+// Status word of the routing kernels on the current device (mps_route.cu): waits for the stream, returns it and clears it.
+int take_route_status(void *stream, int *status);
 }  // namespace mps

@@ -1,0 +1,589 @@
+// Routing rows to experts: scores, the choice, its weights and their gradient, and the rows listed by expert.
+//
+// With logits l[row, e] and an optional bias b[e]
+//     s = softmax(l) or sigmoid(l),   key = s + b   (without a bias key = l, which orders like s),
+// the experts of the best `top_groups` of `n_groups` equal groups stay (a group ranks by its largest key, or by the sum of
+// its two largest values s + b), the top_k largest keys of those are chosen, the lowest index first among equals, and
+//     w_j = scale * s_j      or, renormalised,   w_j = scale * s_j / sum over the chosen i of s_i.
+// An expert whose logit or key is -inf or NaN is never chosen; where fewer than top_k are left the id is -1, the weight 0.
+#include "mps.h"
+
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include <cmath>
+
+#include "mps_internal.h"
+#include "mps_types.cuh"
+
+namespace cg = cooperative_groups;
+using mps::fail;
+using mps::to_f32;
+
+namespace {
+
+#define RT_CUDA(call)                                                                               \
+    do {                                                                                            \
+        cudaError_t e_ = (call);                                                                    \
+        if (e_ != cudaSuccess) return fail(MPS_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_));  \
+    } while (0)
+
+__device__ int g_status;
+
+constexpr int kMaxExperts = 1024;   // 32 keys per lane
+constexpr int kMaxTop = 32;         // one chosen expert per lane
+constexpr int kMaxGroups = 32;      // one bit per expert group
+constexpr int kRouteWarps = 4;
+constexpr unsigned kAll = 0xffffffffu;
+
+struct RouteArgs {
+    int n_rows, n_experts, top_k, n_groups, per_group, top_groups, group_top;
+    bool renormalise;
+    float scale;
+};
+
+template <typename F>
+__device__ __forceinline__ F neg_inf();
+template <>
+__device__ __forceinline__ float neg_inf<float>() { return -INFINITY; }
+template <>
+__device__ __forceinline__ double neg_inf<double>() { return -(double)INFINITY; }
+
+__device__ __forceinline__ float exp_of(float x) { return expf(x); }
+__device__ __forceinline__ double exp_of(double x) { return exp(x); }
+
+template <typename F>
+__device__ __forceinline__ F sigmoid(F x) {  // exp of a number <= 0 only: no overflow, and small scores keep their digits
+    const F e = exp_of(x < (F)0 ? x : -x);
+    return (x < (F)0 ? e : (F)1) / ((F)1 + e);
+}
+
+template <typename F>
+__device__ __forceinline__ F warp_sum(F v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) v += __shfl_xor_sync(kAll, v, d);
+    return v;
+}
+
+template <typename F>
+__device__ __forceinline__ F warp_max(F v) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        const F o = __shfl_xor_sync(kAll, v, d);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+// fp32 -> unsigned with the same order (no NaN comes in; -0 counts as 0)
+__device__ __forceinline__ unsigned ordered(float v) {
+    const unsigned b = __float_as_uint(v + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// the largest (value, lowest index) of the warp's candidates
+__device__ __forceinline__ void warp_best(float &v, int &at) {
+    const unsigned mine = ordered(v), top = __reduce_max_sync(kAll, mine);
+    at = (int)__reduce_min_sync(kAll, mine == top ? (unsigned)at : 0x7fffffffu);
+    v = __uint_as_float(top & 0x80000000u ? top ^ 0x80000000u : ~top);
+}
+__device__ __forceinline__ void warp_best(double &v, int &at) {
+#pragma unroll
+    for (int d = 16; d; d >>= 1) {
+        const double ov = __shfl_xor_sync(kAll, v, d);
+        const int oa = __shfl_xor_sync(kAll, at, d);
+        if (ov > v || (ov == v && oa < at)) { v = ov; at = oa; }
+    }
+}
+
+// How far apart two fp32 keys must be for their order to be that of the exact ones: a score in [0, 1] is off by less than
+// 1e-6 (exponential, sum and quotient, a few units in the last place each), a key s + b by another half unit of itself.
+__device__ __forceinline__ float clearance(float key) { return 4e-6f + 2.5e-7f * fabsf(key); }
+
+// Keeps the experts of the best groups: key of the others becomes -inf.  `cells` is this warp's shared row of n_experts
+// (+ padding) values.  Returns false where fp32 cannot tell the last group kept from the first one dropped.
+template <typename F, int VPL>
+__device__ __forceinline__ bool keep_groups(F (&key)[VPL], const F (&value)[VPL], const RouteArgs &a, F *cells, int lane) {
+    // groups are contiguous runs of experts; `parts` lanes share a group, each scanning every parts-th member
+    int parts = 32;
+    while (parts * a.n_groups > 32) parts >>= 1;
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        const int e = lane + 32 * i;
+        if (e < a.n_experts) cells[e + (e >> 5)] = value[i];
+    }
+    __syncwarp();
+    const int g = lane / parts;
+    F one = neg_inf<F>(), two = neg_inf<F>();
+    if (g < a.n_groups)
+        for (int m = lane % parts; m < a.per_group; m += parts) {
+            const int e = g * a.per_group + m;
+            const F v = cells[e + (e >> 5)];
+            if (v > one) { two = one; one = v; }
+            else if (v > two) two = v;
+        }
+    for (int d = 1; d < parts; d <<= 1) {
+        const F o1 = __shfl_xor_sync(kAll, one, d), o2 = __shfl_xor_sync(kAll, two, d);
+        const F low = one < o1 ? one : o1;
+        one = one > o1 ? one : o1;
+        two = two > o2 ? two : o2;
+        two = two > low ? two : low;
+    }
+    F rank = one;
+    if (a.group_top == 2 && two > neg_inf<F>()) rank = one + two;
+    if (g >= a.n_groups || lane % parts) rank = neg_inf<F>();
+    unsigned kept = 0;
+    F last = neg_inf<F>();
+    for (int j = 0; j < a.top_groups; ++j) {
+        F best = rank;
+        int at = lane;
+        warp_best(best, at);
+        if (!(best > neg_inf<F>())) break;
+        kept |= 1u << (at / parts);
+        last = best;
+        if (lane == at) rank = neg_inf<F>();
+    }
+    bool clear = true;
+    if (sizeof(F) == 4) {
+        const float next = (float)warp_max(rank);
+        clear = !((float)last - next <= 2 * clearance((float)last)) || !(next > -INFINITY);
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        const int e = lane + 32 * i;
+        if (e < a.n_experts && !((kept >> (e / a.per_group)) & 1)) key[i] = neg_inf<F>();
+    }
+    return clear;
+}
+
+// The top_k largest keys: lane j returns the j-th expert (or -1) in `mine`.  EXACT keys are compared as they are; others
+// must be `clearance` apart unless they belong to equal logits and equal biases.  Returns false where they are not.
+template <bool EXACT, typename F, int VPL, typename T>
+__device__ __forceinline__ bool choose(F (&key)[VPL], const RouteArgs &a, const T *logits, const float *bias, int lane, int &mine) {
+    mine = -1;
+    bool clear = true;
+    float prev = INFINITY;
+    int prev_at = -1;
+    for (int j = 0; j < a.top_k + (EXACT ? 0 : 1); ++j) {
+        F best = key[0];
+        int at = lane;
+#pragma unroll
+        for (int i = 1; i < VPL; ++i)
+            if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+        warp_best(best, at);
+        if (!(best > neg_inf<F>())) break;
+        if (!EXACT) {
+            const float v = (float)best;
+            if (prev_at >= 0 && prev - v <= clearance(v))
+                clear = clear && to_f32(logits[prev_at]) == to_f32(logits[at]) && bias[prev_at] == bias[at];
+            prev = v;
+            prev_at = at;
+        }
+        if (lane == j && j < a.top_k) mine = at;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (at == lane + 32 * i) key[i] = neg_inf<F>();
+    }
+    return clear;
+}
+
+// keys and group values of one row in F; -inf where the expert may not be chosen
+template <typename F, int VPL, bool SIGMOID>
+__device__ __forceinline__ void row_keys(const float (&l)[VPL], const float (&b)[VPL], bool has_bias, bool need_score, F (&key)[VPL], F (&value)[VPL]) {
+    F peak = neg_inf<F>(), total = 0;
+    if (need_score && !SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if ((F)l[i] > peak) peak = (F)l[i];
+        peak = warp_max(peak);
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (l[i] > -INFINITY) total += exp_of((F)l[i] - peak);
+        total = warp_sum(total);
+    }
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        const bool open = l[i] > -INFINITY;
+        F s = 0;
+        if (need_score && open) s = SIGMOID ? sigmoid((F)l[i]) : exp_of((F)l[i] - peak) / total;
+        F k = has_bias ? s + (F)b[i] : (F)l[i];
+        if (!open || !(k > neg_inf<F>())) k = neg_inf<F>();
+        key[i] = k;
+        value[i] = has_bias || !need_score ? k : (open ? s : neg_inf<F>());
+    }
+}
+
+// One warp per row.  The row's logits stay in registers (lane + 32 i); the choice runs on fp32 keys, and a row in which two
+// keys that decide it lie closer together than fp32 can tell is decided again on fp64 keys.  That keeps the choice the
+// definition's at a fraction of the cost of fp64 throughout.
+template <typename T, int VPL, bool SIGMOID>
+__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
+                                                                int *__restrict__ ids, float *__restrict__ weights) {
+    extern __shared__ double s_cells[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int pitch = a.n_experts + (a.n_experts >> 5) + 1;
+    double *cells = s_cells + (size_t)warp * pitch;
+    const bool has_bias = bias != nullptr, grouped = a.n_groups > 1;
+    const bool need_score = has_bias || (grouped && a.group_top == 2);
+    float b[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        const int e = lane + 32 * i;
+        b[i] = has_bias && e < a.n_experts ? bias[e] : 0.0f;
+    }
+    for (long long row = (long long)blockIdx.x * kRouteWarps + warp; row < a.n_rows; row += (long long)gridDim.x * kRouteWarps) {
+        const T *line = logits + row * a.n_experts;
+        float l[VPL];
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const int e = lane + 32 * i;
+            l[i] = e < a.n_experts ? to_f32(line[e]) : -INFINITY;
+            if (l[i] != l[i] || (!SIGMOID && l[i] == INFINITY)) nan = true;  // the row's scores are not numbers: neither are its weights
+            if (l[i] != l[i]) l[i] = -INFINITY;
+        }
+        nan = __any_sync(kAll, nan);
+        float key[VPL], value[VPL];
+        row_keys<float, VPL, SIGMOID>(l, b, has_bias, need_score, key, value);
+        bool clear = true;
+        int mine;
+        if (grouped) {
+            clear = keep_groups(key, value, a, (float *)cells, lane);
+            if (!need_score) clear = true;  // logits compare exactly
+        }
+        if (has_bias) clear = choose<false>(key, a, line, bias, lane, mine) && clear;
+        else choose<true>(key, a, line, bias, lane, mine);
+        if (!clear) {
+            double key64[VPL], value64[VPL];
+            row_keys<double, VPL, SIGMOID>(l, b, has_bias, need_score, key64, value64);
+            if (grouped) keep_groups(key64, value64, a, cells, lane);
+            choose<true>(key64, a, line, bias, lane, mine);
+        }
+        // weights of the chosen, lane j the j-th
+        const bool live = mine >= 0;
+        const float lm = live ? to_f32(line[mine]) : -INFINITY;
+        float w;
+        const float top = warp_max(lm);
+        // the chosen scores' ratios: by exponentials of differences where the scores are exponentials (softmax, or a sigmoid so
+        // far down that 1 + e^l is 1), so that they do not underflow together
+        if (a.renormalise && (!SIGMOID || top < -30.0f)) {
+            const float e = live ? expf(lm - top) : 0.0f;
+            w = e / warp_sum(e);
+        } else if (SIGMOID) {
+            w = live ? sigmoid(lm) : 0.0f;
+            if (a.renormalise) w = w / warp_sum(w);
+        } else {
+            float peak = l[0], total = 0.0f;
+#pragma unroll
+            for (int i = 1; i < VPL; ++i) peak = fmaxf(peak, l[i]);
+            peak = warp_max(peak);
+#pragma unroll
+            for (int i = 0; i < VPL; ++i)
+                if (l[i] > -INFINITY) total += expf(l[i] - peak);
+            w = expf(lm - peak) / warp_sum(total);
+        }
+        if (lane < a.top_k) {
+            ids[row * a.top_k + lane] = mine;
+            weights[row * a.top_k + lane] = nan ? NAN : live ? w * a.scale : 0.0f;
+        }
+    }
+}
+
+// Gradient by the logits, all of the row written.  With r = the chosen scores' shares and g = the weights' gradient:
+//   renormalised: dl_j = scale r_j (g_j - sum_i g_i r_i) (times 1 - s_j for a sigmoid), nothing for the others;
+//   softmax:      dl_e = scale p_e (g_e - sum_i g_i p_i);      sigmoid: dl_j = scale g_j s_j (1 - s_j).
+// An expert named twice gets both contributions, in the order of the choices.
+template <typename T, bool SIGMOID>
+__global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(RouteArgs a, const T *__restrict__ logits, const int *__restrict__ ids,
+                                                                         const float *__restrict__ d_weights, T *__restrict__ d_logits) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const bool dense = !SIGMOID && !a.renormalise;
+    for (long long row = (long long)blockIdx.x * kRouteWarps + warp; row < a.n_rows; row += (long long)gridDim.x * kRouteWarps) {
+        const T *line = logits + row * a.n_experts;
+        int id = -1;
+        float g = 0.0f;
+        if (lane < a.top_k) {
+            id = ids[row * a.top_k + lane];
+            if (id >= a.n_experts) {
+                atomicOr(&g_status, mps::kStatusBadIndex);
+                id = -1;
+            }
+            if (id >= 0) g = d_weights[row * a.top_k + lane];
+        }
+        const float l = id >= 0 ? to_f32(line[id]) : -INFINITY;
+        float peak = 0.0f, total = 1.0f, own, common = 0.0f;
+        if (dense) {
+            float p = -INFINITY, t = 0.0f;
+            for (int e = lane; e < a.n_experts; e += 32) p = fmaxf(p, to_f32(line[e]));
+            peak = warp_max(p);
+            for (int e = lane; e < a.n_experts; e += 32) {
+                const float v = to_f32(line[e]);
+                if (v != -INFINITY) t += expf(v - peak);
+            }
+            total = warp_sum(t);
+            const float share = l != -INFINITY ? expf(l - peak) / total : 0.0f;
+            own = a.scale * g * share;
+            common = warp_sum(own);
+        } else {
+            const float s = SIGMOID ? (id >= 0 ? sigmoid(l) : 0.0f) : 0.0f, slope = SIGMOID ? sigmoid(-l) : 1.0f;
+            if (a.renormalise) {
+                const float top = warp_max(l);
+                float share;
+                if (!SIGMOID || top < -30.0f) {
+                    const float e = l != -INFINITY ? expf(l - top) : 0.0f, sum = warp_sum(e);
+                    share = sum != 0.0f ? e / sum : 0.0f;
+                } else share = s / warp_sum(s);
+                own = a.scale * share * (g - warp_sum(g * share)) * (id >= 0 ? slope : 0.0f);
+            } else own = id >= 0 ? a.scale * g * s * slope : 0.0f;
+        }
+        for (int e0 = 0; e0 < a.n_experts; e0 += 32) {
+            const int e = e0 + lane;
+            float d = 0.0f;
+            if (dense && e < a.n_experts) {
+                const float v = to_f32(line[e]);
+                d = v != -INFINITY ? -(expf(v - peak) / total) * common : 0.0f;
+            }
+            for (int j = 0; j < a.top_k; ++j) {
+                const int at = __shfl_sync(kAll, id, j);
+                const float c = __shfl_sync(kAll, own, j);
+                if (at == e) d += c;
+            }
+            if (e < a.n_experts) d_logits[row * a.n_experts + e] = mps::from_f32<T>(d);
+        }
+    }
+}
+
+// Rows listed by group: a stable counting sort of the pairs (row, choice) by id in one launch.  The pairs are cut into one
+// contiguous run per warp of the cluster; a warp counts its run's ids in shared memory (lanes of equal id are found with
+// match.any, so no atomics and one order), the counts are scanned over warps, blocks (distributed shared memory) and groups,
+// and the warp walks its run again and places every pair.
+constexpr int kGroupThreads = 1024, kGroupWarps = kGroupThreads / 32, kGroupMax = 1024;
+constexpr int kGroupCluster = 8;
+
+__global__ void __launch_bounds__(kGroupThreads) group_kernel(long long n_pairs, int per_row, int n_groups, const int *__restrict__ ids,
+                                                             int *__restrict__ group_ptr, int *__restrict__ slot_row, int *__restrict__ slot_of) {
+    extern __shared__ int s_int[];
+    int *count = s_int;                             // [warps][n_groups], later the next free slot
+    int *total = s_int + kGroupWarps * n_groups;    // this block's pairs per group
+    __shared__ int s_scan[kGroupWarps];
+    cg::cluster_group cluster = cg::this_cluster();
+    const int rank = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const long long steps = (n_pairs + 31) / 32, runs = (long long)blocks * kGroupWarps;
+    const long long run = rank * kGroupWarps + warp;
+    const long long lo = steps * run / runs, hi = steps * (run + 1) / runs;
+    int *own = count + warp * n_groups;
+    for (int g = lane; g < n_groups; g += 32) own[g] = 0;
+    __syncwarp();
+    for (long long s = lo; s < hi; ++s) {
+        const long long i = s * 32 + lane;
+        int id = i < n_pairs ? ids[i] : -1;
+        if (id >= n_groups) {
+            atomicOr(&g_status, mps::kStatusBadIndex);
+            id = -1;
+        }
+        const unsigned same = __match_any_sync(kAll, id);
+        if (id >= 0 && lane == __ffs(same) - 1) own[id] += __popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    if (tid < n_groups) {
+        int sum = 0;
+        for (int w = 0; w < kGroupWarps; ++w) {
+            const int c = count[w * n_groups + tid];
+            count[w * n_groups + tid] = sum;
+            sum += c;
+        }
+        total[tid] = sum;
+    }
+    cluster.sync();
+    int before = 0, all = 0;
+    if (tid < n_groups)
+        for (int r = 0; r < blocks; ++r) {
+            const int c = cluster.map_shared_rank(total, r)[tid];
+            if (r < rank) before += c;
+            all += c;
+        }
+    int scan = all;  // inclusive scan over groups
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(kAll, scan, d);
+        if (lane >= d) scan += o;
+    }
+    if (lane == 31) s_scan[warp] = scan;
+    __syncthreads();
+    if (warp == 0) {
+        int v = s_scan[lane];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(kAll, v, d);
+            if (lane >= d) v += o;
+        }
+        s_scan[lane] = v;
+    }
+    __syncthreads();
+    const int start = scan - all + (warp ? s_scan[warp - 1] : 0);
+    const int used = s_scan[kGroupWarps - 1];
+    if (tid < n_groups) {
+        if (rank == 0) {
+            group_ptr[tid] = start;
+            if (tid == n_groups - 1) group_ptr[n_groups] = used;
+        }
+        for (int w = 0; w < kGroupWarps; ++w) count[w * n_groups + tid] += start + before;
+    }
+    cluster.sync();  // also: no block leaves while another still reads its totals
+    for (long long s = lo; s < hi; ++s) {
+        const long long i = s * 32 + lane;
+        int id = i < n_pairs ? ids[i] : -1;
+        if (id >= n_groups) id = -1;
+        const unsigned same = __match_any_sync(kAll, id);
+        int at = -1;
+        if (id >= 0) at = own[id] + __popc(same & ((1u << lane) - 1));
+        __syncwarp();
+        if (id >= 0 && lane == __ffs(same) - 1) own[id] += __popc(same);
+        __syncwarp();
+        if (i < n_pairs) {
+            slot_of[i] = at;
+            if (at >= 0) slot_row[at] = (int)(i / per_row);
+            if (i >= used) slot_row[i] = -1;
+        }
+    }
+}
+
+int launch_group(long long n_pairs, int per_row, int n_groups, const int *ids, int *ptr, int *row, int *slot, cudaStream_t st) {
+    const size_t smem = (size_t)(kGroupWarps + 1) * n_groups * sizeof(int);
+    if (smem > 40 * 1024)
+        RT_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kGroupWarps + 1) * kGroupMax * (int)sizeof(int)));
+    const int blocks = n_pairs > 2048 ? kGroupCluster : 1;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = blocks;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks);
+    cfg.blockDim = dim3(kGroupThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    RT_CUDA(cudaLaunchKernelEx(&cfg, group_kernel, n_pairs, per_row, n_groups, ids, ptr, row, slot));
+    return MPS_OK;
+}
+
+template <typename T, bool SIGMOID>
+int launch_route(const RouteArgs &a, const void *logits, const float *bias, int *ids, float *weights, cudaStream_t st) {
+    const size_t smem = (size_t)kRouteWarps * (a.n_experts + (a.n_experts >> 5) + 1) * sizeof(double);
+    const long long want = ((long long)a.n_rows + kRouteWarps - 1) / kRouteWarps;
+    const unsigned blocks = (unsigned)(want < 148 * 16 ? want : 148 * 16);
+    const int per_lane = (a.n_experts + 31) / 32;
+#define RT_LAUNCH(V) route_kernel<T, V, SIGMOID><<<blocks, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, bias, ids, weights)
+    if (per_lane <= 1) RT_LAUNCH(1);
+    else if (per_lane <= 2) RT_LAUNCH(2);
+    else if (per_lane <= 4) RT_LAUNCH(4);
+    else if (per_lane <= 8) RT_LAUNCH(8);
+    else if (per_lane <= 16) RT_LAUNCH(16);
+    else RT_LAUNCH(32);
+#undef RT_LAUNCH
+    RT_CUDA(cudaGetLastError());
+    return MPS_OK;
+}
+
+int check_spec(const char *who, int n_rows, const mps_route_spec *spec, int dtype, RouteArgs *a) {
+    if (!spec) return fail(MPS_ERR_ARG, "%s: spec is NULL", who);
+    if (n_rows < 0) return fail(MPS_ERR_ARG, "%s: n_rows = %d", who, n_rows);
+    if (dtype != MPS_F32 && dtype != MPS_F16 && dtype != MPS_BF16) return fail(MPS_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    if (spec->score != MPS_SCORE_SOFTMAX && spec->score != MPS_SCORE_SIGMOID) return fail(MPS_ERR_ARG, "%s: unknown score %d", who, spec->score);
+    if (spec->n_experts < 1 || spec->top_k < 1 || spec->n_groups < 1 || spec->n_experts % spec->n_groups)
+        return fail(MPS_ERR_ARG, "%s: %d experts, top %d, %d groups (experts must divide into the groups)", who, spec->n_experts, spec->top_k,
+                    spec->n_groups);
+    if (spec->top_groups < 1 || spec->top_groups > spec->n_groups || (spec->group_top != 1 && spec->group_top != 2))
+        return fail(MPS_ERR_ARG, "%s: top_groups %d of %d, group_top %d (1 or 2)", who, spec->top_groups, spec->n_groups, spec->group_top);
+    if (spec->top_k > spec->n_experts / spec->n_groups * spec->top_groups)
+        return fail(MPS_ERR_ARG, "%s: top %d of %d experts in the groups kept", who, spec->top_k, spec->n_experts / spec->n_groups * spec->top_groups);
+    if (!std::isfinite(spec->scale)) return fail(MPS_ERR_ARG, "%s: scale is not finite", who);
+    if (spec->n_experts > kMaxExperts || spec->top_k > kMaxTop || spec->n_groups > kMaxGroups)
+        return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d experts, top %d, %d groups", who, kMaxExperts, kMaxTop, kMaxGroups);
+    if ((long long)n_rows * spec->top_k >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "%s: rows * top_k does not fit 31 bits", who);
+    *a = RouteArgs{n_rows, spec->n_experts, spec->top_k, spec->n_groups, spec->n_experts / spec->n_groups, spec->top_groups, spec->group_top,
+                   spec->renormalise != 0, spec->scale};
+    return MPS_OK;
+}
+
+bool misaligned(const void *p, size_t size) { return ((uintptr_t)p & (size - 1)) != 0; }
+
+}  // namespace
+
+namespace mps {
+int take_route_status(void *stream, int *status) {
+    cudaStream_t st = (cudaStream_t)stream;
+    static const int zero = 0;
+    RT_CUDA(cudaMemcpyFromSymbolAsync(status, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+    RT_CUDA(cudaStreamSynchronize(st));
+    if (*status) RT_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+    return MPS_OK;
+}
+}  // namespace mps
+
+extern "C" int mps_group_rows(int32_t n_rows, int32_t per_row, int32_t n_groups, const int32_t *d_ids, int32_t *d_group_ptr, int32_t *d_slot_row,
+                              int32_t *d_slot_of, void *stream) {
+    if (n_rows < 0 || per_row < 1 || n_groups < 1) return fail(MPS_ERR_ARG, "mps_group_rows: %d rows, %d per row, %d groups", n_rows, per_row, n_groups);
+    const long long pairs = (long long)n_rows * per_row;
+    if (!d_group_ptr || (pairs > 0 && (!d_ids || !d_slot_row || !d_slot_of))) return fail(MPS_ERR_ARG, "mps_group_rows: NULL pointer");
+    if (n_groups > kGroupMax) return fail(MPS_ERR_UNSUPPORTED, "mps_group_rows: at most %d groups", kGroupMax);
+    if (pairs >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "mps_group_rows: rows * per_row does not fit 31 bits");
+    if (misaligned(d_ids, 4) || misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_slot_of, 4))
+        return fail(MPS_ERR_ALIGN, "mps_group_rows: pointers must be 4-byte aligned");
+    return launch_group(pairs, per_row, n_groups, d_ids, d_group_ptr, d_slot_row, d_slot_of, (cudaStream_t)stream);
+}
+
+extern "C" int mps_route(int32_t n_rows, const mps_route_spec *spec, int dtype, const void *d_logits, const float *d_bias, int32_t *d_ids,
+                         float *d_weights, int32_t *d_group_ptr, int32_t *d_slot_row, int32_t *d_slot_of, void *stream) {
+    RouteArgs a;
+    if (int rc = check_spec("mps_route", n_rows, spec, dtype, &a)) return rc;
+    const bool list = d_group_ptr || d_slot_row || d_slot_of;
+    if (n_rows > 0 && (!d_logits || !d_ids || !d_weights)) return fail(MPS_ERR_ARG, "mps_route: NULL pointer");
+    if (list && (!d_group_ptr || (n_rows > 0 && (!d_slot_row || !d_slot_of))))
+        return fail(MPS_ERR_ARG, "mps_route: the three group arrays go together (all or none NULL)");
+    if (misaligned(d_logits, dtype == MPS_F32 ? 4 : 2) || misaligned(d_bias, 4) || misaligned(d_ids, 4) || misaligned(d_weights, 4) ||
+        misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_slot_of, 4))
+        return fail(MPS_ERR_ALIGN, "mps_route: a pointer is not aligned to its element size");
+    cudaStream_t st = (cudaStream_t)stream;
+    if (n_rows > 0) {
+        const bool sig = spec->score == MPS_SCORE_SIGMOID;
+        int rc;
+        if (dtype == MPS_F32) rc = sig ? launch_route<float, true>(a, d_logits, d_bias, d_ids, d_weights, st) : launch_route<float, false>(a, d_logits, d_bias, d_ids, d_weights, st);
+        else if (dtype == MPS_F16) rc = sig ? launch_route<__half, true>(a, d_logits, d_bias, d_ids, d_weights, st) : launch_route<__half, false>(a, d_logits, d_bias, d_ids, d_weights, st);
+        else rc = sig ? launch_route<__nv_bfloat16, true>(a, d_logits, d_bias, d_ids, d_weights, st) : launch_route<__nv_bfloat16, false>(a, d_logits, d_bias, d_ids, d_weights, st);
+        if (rc) return rc;
+    }
+    if (list) return launch_group((long long)n_rows * a.top_k, a.top_k, a.n_experts, d_ids, d_group_ptr, d_slot_row, d_slot_of, st);
+    return MPS_OK;
+}
+
+template <typename T>
+static int launch_route_backward(const RouteArgs &a, bool sigmoid_score, const void *logits, const int *ids, const float *d_weights, void *d_logits,
+                                 cudaStream_t st) {
+    const long long want = ((long long)a.n_rows + kRouteWarps - 1) / kRouteWarps;
+    const unsigned blocks = (unsigned)(want < 148 * 16 ? want : 148 * 16);
+    if (sigmoid_score) route_backward_kernel<T, true><<<blocks, 32 * kRouteWarps, 0, st>>>(a, (const T *)logits, ids, d_weights, (T *)d_logits);
+    else route_backward_kernel<T, false><<<blocks, 32 * kRouteWarps, 0, st>>>(a, (const T *)logits, ids, d_weights, (T *)d_logits);
+    RT_CUDA(cudaGetLastError());
+    return MPS_OK;
+}
+
+extern "C" int mps_route_backward(int32_t n_rows, const mps_route_spec *spec, int dtype, const void *d_logits, const int32_t *d_ids,
+                                  const float *d_dweights, void *d_dlogits, void *stream) {
+    RouteArgs a;
+    if (int rc = check_spec("mps_route_backward", n_rows, spec, dtype, &a)) return rc;
+    if (n_rows == 0) return MPS_OK;
+    if (!d_logits || !d_ids || !d_dweights || !d_dlogits) return fail(MPS_ERR_ARG, "mps_route_backward: NULL pointer");
+    const size_t size = dtype == MPS_F32 ? 4 : 2;
+    if (misaligned(d_logits, size) || misaligned(d_dlogits, size) || misaligned(d_ids, 4) || misaligned(d_dweights, 4))
+        return fail(MPS_ERR_ALIGN, "mps_route_backward: a pointer is not aligned to its element size");
+    const bool sig = spec->score == MPS_SCORE_SIGMOID;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (dtype == MPS_F32) return launch_route_backward<float>(a, sig, d_logits, d_ids, d_dweights, d_dlogits, st);
+    if (dtype == MPS_F16) return launch_route_backward<__half>(a, sig, d_logits, d_ids, d_dweights, d_dlogits, st);
+    return launch_route_backward<__nv_bfloat16>(a, sig, d_logits, d_ids, d_dweights, d_dlogits, st);
+}

@@ -1,0 +1,419 @@
+// Entry points of the products of routed rows: experts' products, their combination, low-rank adapters, and the gradients.
+#include "mps.h"
+
+#include <cuda_runtime.h>
+
+#include "mps_internal.h"
+#include "mps_routed_plain.cuh"
+#include "mps_types.cuh"
+
+using mps::fail;
+using mps::OuterArgs;
+using mps::RowsArgs;
+
+namespace {
+
+#define RD_CUDA(call)                                                                               \
+    do {                                                                                            \
+        cudaError_t e_ = (call);                                                                    \
+        if (e_ != cudaSuccess) return fail(MPS_ERR_CUDA, "%s: %s", #call, cudaGetErrorString(e_));  \
+    } while (0)
+
+__device__ int g_status;
+
+int status_pointer(int **p) {
+    RD_CUDA(cudaGetSymbolAddress((void **)p, g_status));
+    return MPS_OK;
+}
+
+bool misaligned(const void *p, size_t size) { return ((uintptr_t)p & (size - 1)) != 0; }
+size_t size_of(int dtype) { return dtype == MPS_F32 ? 4 : 2; }
+bool known(int dtype) { return dtype == MPS_F32 || dtype == MPS_F16 || dtype == MPS_BF16; }
+
+// ---------------------------------------------------------------------------------------------- combine
+
+// y[t] = sum over j of weight[t, j] * rows[slot[t, j]].  Moves bytes only: a thread owns 16 bytes of a row of y (one element
+// where the row's pitch or a pointer is not a multiple of 16 bytes) and keeps the loads of all of the row's terms in flight.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) combine_kernel(int n_rows, int per_row, int n_slots, int dim, const int *__restrict__ slot_of,
+                                                      const float *__restrict__ weights, const T *__restrict__ rows, T *__restrict__ y, int *status) {
+    const int per = dim / VEC;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)n_rows * per; i += (long long)gridDim.x * 256) {
+        const long long t = i / per;
+        const int c = (int)(i - t * per) * VEC;
+        float acc[VEC] = {};
+#pragma unroll 4
+        for (int j = 0; j < per_row; ++j) {
+            const int s = slot_of[t * per_row + j];
+            if (s < 0) continue;
+            if (s >= n_slots) {
+                atomicOr(status, mps::kStatusBadIndex);
+                continue;
+            }
+            const float w = weights ? weights[t * per_row + j] : 1.0f;
+            const T *src = rows + (long long)s * dim + c;
+            if constexpr (VEC > 1) {
+                const mps::Pack<T> p = *reinterpret_cast<const mps::Pack<T> *>(src);
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) acc[v] = fmaf(w, mps::to_f32(p.v[v]), acc[v]);
+            } else acc[0] = fmaf(w, mps::to_f32(*src), acc[0]);
+        }
+        if constexpr (VEC > 1) {
+            mps::Pack<T> p;
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) p.v[v] = mps::from_f32<T>(acc[v]);
+            *reinterpret_cast<mps::Pack<T> *>(y + t * dim + c) = p;
+        } else y[t * dim + c] = mps::from_f32<T>(acc[0]);
+    }
+}
+
+// d_rows[slot[t, j]] = weight[t, j] * dy[t] and d_weights[t, j] = <dy[t], rows[slot[t, j]]>, one warp per (t, j): rows is read
+// and d_rows written once, the repeated reads of dy[t] meet the cache.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(256) combine_backward_kernel(int n_rows, int per_row, int n_slots, int dim, const int *__restrict__ slot_of,
+                                                               const float *__restrict__ weights, const T *__restrict__ dy, const T *__restrict__ rows,
+                                                               T *__restrict__ d_rows, float *__restrict__ d_weights, int *status) {
+    const int lane = threadIdx.x & 31;
+    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < (long long)n_rows * per_row; i += (long long)gridDim.x * 8) {
+        const long long t = i / per_row;
+        int s = slot_of[i];
+        if (s >= n_slots) {
+            if (lane == 0) atomicOr(status, mps::kStatusBadIndex);
+            s = -1;
+        }
+        float dot = 0.0f;
+        if (s >= 0) {
+            const float w = weights ? weights[i] : 1.0f;
+            const T *g = dy + t * dim, *src = rows + (long long)s * dim;
+            T *dst = d_rows + (long long)s * dim;
+#pragma unroll 4
+            for (int c = lane * VEC; c < dim; c += 32 * VEC) {
+                if constexpr (VEC > 1) {
+                    const mps::Pack<T> p = *reinterpret_cast<const mps::Pack<T> *>(g + c);
+                    mps::Pack<T> q = {}, o;
+                    if (d_weights) q = *reinterpret_cast<const mps::Pack<T> *>(src + c);
+#pragma unroll
+                    for (int v = 0; v < VEC; ++v) {
+                        const float d = mps::to_f32(p.v[v]);
+                        dot = fmaf(d, mps::to_f32(q.v[v]), dot);
+                        o.v[v] = mps::from_f32<T>(w * d);
+                    }
+                    *reinterpret_cast<mps::Pack<T> *>(dst + c) = o;
+                } else {
+                    const float d = mps::to_f32(g[c]);
+                    if (d_weights) dot = fmaf(d, mps::to_f32(src[c]), dot);
+                    dst[c] = mps::from_f32<T>(w * d);
+                }
+            }
+        }
+        if (d_weights) {
+#pragma unroll
+            for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+            if (lane == 0) d_weights[i] = dot;
+        }
+    }
+}
+
+template <typename T>
+int launch_combine(int n_rows, int per_row, int n_slots, int dim, const int *slot_of, const float *weights, const void *rows, void *y, cudaStream_t st) {
+    int *status;
+    if (int rc = status_pointer(&status)) return rc;
+    constexpr int VEC = mps::Pack<T>::N;
+    const bool wide = dim % VEC == 0 && !misaligned(rows, 16) && !misaligned(y, 16);
+    const long long blocks = ((long long)n_rows * (wide ? dim / VEC : dim) + 255) / 256;
+    const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20);
+    if (wide) combine_kernel<T, VEC><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)rows, (T *)y, status);
+    else combine_kernel<T, 1><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)rows, (T *)y, status);
+    RD_CUDA(cudaGetLastError());
+    return MPS_OK;
+}
+
+template <typename T>
+int launch_combine_backward(int n_rows, int per_row, int n_slots, int dim, const int *slot_of, const float *weights, const void *dy, const void *rows,
+                            void *d_rows, float *d_weights, cudaStream_t st) {
+    int *status;
+    if (int rc = status_pointer(&status)) return rc;
+    constexpr int VEC = mps::Pack<T>::N;
+    const bool wide = dim % VEC == 0 && !misaligned(rows, 16) && !misaligned(dy, 16) && !misaligned(d_rows, 16);
+    const long long blocks = ((long long)n_rows * per_row + 7) / 8;
+    const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20);
+    if (wide)
+        combine_backward_kernel<T, VEC><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)dy, (const T *)rows, (T *)d_rows,
+                                                              d_weights, status);
+    else
+        combine_backward_kernel<T, 1><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)dy, (const T *)rows, (T *)d_rows,
+                                                            d_weights, status);
+    RD_CUDA(cudaGetLastError());
+    return MPS_OK;
+}
+
+// ---------------------------------------------------------------------------------------------- products
+
+template <typename T, typename TO, bool LOWRANK>
+int launch_plain_rows(RowsArgs a, const void *x, const void *w, const void *b, void *out, cudaStream_t st) {
+    if (int rc = status_pointer(&a.status)) return rc;
+    const long long tiles = (a.n_slots + mps::kPlainTile - 1) / mps::kPlainTile + (a.group_ptr ? a.n_groups : 0);  // every group ends in a part of a tile
+    const dim3 grid((unsigned)tiles, (unsigned)((a.n + mps::kPlainTile - 1) / mps::kPlainTile));
+    mps::plain_rows_kernel<T, TO, LOWRANK><<<grid, mps::kPlainThreads, 0, st>>>(a, (const T *)x, (const T *)w, (const T *)b, (TO *)out);
+    RD_CUDA(cudaGetLastError());
+    return MPS_OK;
+}
+
+template <typename TP, typename TQ, typename TO>
+int launch_plain_outer(OuterArgs a, const void *p, const void *q, void *out, cudaStream_t st) {
+    if (int rc = status_pointer(&a.status)) return rc;
+    const dim3 grid((unsigned)((a.i + mps::kPlainTile - 1) / mps::kPlainTile), (unsigned)((a.j + mps::kPlainTile - 1) / mps::kPlainTile),
+                    (unsigned)a.n_groups);
+    mps::plain_outer_kernel<TP, TQ, TO><<<grid, mps::kPlainThreads, 0, st>>>(a, (const TP *)p, (const TQ *)q, (TO *)out);
+    RD_CUDA(cudaGetLastError());
+    return MPS_OK;
+}
+
+int check_product(const char *who, int n_slots, int n_rows, int n_groups, int k, int n, int dtype) {
+    if (n_slots < 0 || n_rows < 0 || n_groups < 1 || k < 1 || n < 1)
+        return fail(MPS_ERR_ARG, "%s: %d slots, %d rows, %d groups, k = %d, n = %d", who, n_slots, n_rows, n_groups, k, n);
+    if (!known(dtype)) return fail(MPS_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    if (n_groups > mps::kMaxRowGroups) return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d groups", who, mps::kMaxRowGroups);
+    if (k > 1 << 21 || n > 1 << 21) return fail(MPS_ERR_UNSUPPORTED, "%s: k and n may be up to %d", who, 1 << 21);
+    return MPS_OK;
+}
+
+template <typename T>
+int product(const RowsArgs &a, const void *x, const void *w, void *y, cudaStream_t st) {
+    return launch_plain_rows<T, T, false>(a, x, w, nullptr, y, st);
+}
+
+template <typename T>
+int wgrad(const OuterArgs &a, const void *dy, const void *x, void *dw, cudaStream_t st) {
+    return launch_plain_outer<T, T, T>(a, dy, x, dw, st);
+}
+
+// ---------------------------------------------------------------------------------------------- adapters
+
+struct AdapterShape {
+    int n_rows, k, n, n_adapters, rank;
+    const int *ids, *group_ptr, *slot_row;
+    const float *scale;
+};
+
+// u[row] = scale * (x[row] times the row's adapter matrix), fp32, rows without an adapter left as they were
+template <typename T>
+int adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m, long long m_k, long long m_r, float *u, cudaStream_t st) {
+    RowsArgs a = {};
+    a.group_ptr = s.group_ptr;
+    a.slot_row = s.slot_row;
+    a.n_groups = s.n_adapters;
+    a.n_slots = a.n_x_rows = s.n_rows;
+    a.k = k;
+    a.n = s.rank;
+    a.w_group = (long long)k * s.rank;
+    a.w_k = m_k;
+    a.w_n = m_r;
+    a.group_scale = s.scale;
+    a.out_by_row = true;
+    return launch_plain_rows<T, float, false>(a, x, m, nullptr, u, st);
+}
+
+// out = x times the shared matrix + u times the row's adapter matrix
+template <typename T>
+int adapter_wide(const AdapterShape &s, int k, int n, const void *x, const void *w, long long w_k, long long w_n, const float *u, const void *m,
+                 long long m_r, long long m_n, void *out, cudaStream_t st) {
+    RowsArgs a = {};
+    a.n_slots = a.n_x_rows = s.n_rows;
+    a.k = k;
+    a.n = n;
+    a.w_k = w_k;
+    a.w_n = w_n;
+    a.ids = s.ids;
+    a.u = u;
+    a.n_adapters = s.n_adapters;
+    a.rank = s.rank;
+    a.b_group = (long long)n * s.rank;
+    a.b_r = m_r;
+    a.b_n = m_n;
+    return launch_plain_rows<T, T, true>(a, x, w, m, out, st);
+}
+
+template <typename T>
+int adapters(const AdapterShape &s, const void *x, const void *w, const void *a, const void *b, void *y, void *workspace, cudaStream_t st) {
+    float *u = (float *)workspace;
+    if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
+    return adapter_wide<T>(s, s.k, s.n, x, w, 1, s.k, u, b, 1, s.rank, y, st);
+}
+
+template <typename T>
+int adapters_backward(const AdapterShape &s, const void *dy, const void *x, const void *w, const void *a, const void *b, void *dx, void *da, void *db,
+                      void *workspace, cudaStream_t st) {
+    float *u = (float *)workspace, *v = u + (size_t)s.n_rows * s.rank;
+    if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;    // scale * x A^T
+    if (int rc = adapter_narrow<T>(s, s.n, dy, b, s.rank, 1, v, st)) return rc;  // scale * dy B
+    if (int rc = adapter_wide<T>(s, s.n, s.k, dy, w, s.k, 1, v, a, s.k, 1, dx, st)) return rc;
+    OuterArgs o = {};
+    o.group_ptr = s.group_ptr;
+    o.slot_row = s.slot_row;
+    o.n_groups = s.n_adapters;
+    o.n_slots = o.n_rows = s.n_rows;
+    o.p_by_row = o.q_by_row = true;
+    o.i = s.rank;
+    o.j = s.k;
+    if (int rc = launch_plain_outer<float, T, T>(o, v, x, da, st)) return rc;
+    o.i = s.n;
+    o.j = s.rank;
+    return launch_plain_outer<T, float, T>(o, dy, u, db, st);
+}
+
+int64_t adapters_bytes(int n_rows, int rank, bool backward) { return (int64_t)n_rows * rank * 4 * (backward ? 2 : 1) + 256; }
+
+int check_adapters(const char *who, const AdapterShape &s, int dtype, const void *workspace, int64_t bytes, bool backward) {
+    if (s.n_rows < 0 || s.k < 1 || s.n < 1 || s.n_adapters < 1 || s.rank < 1)
+        return fail(MPS_ERR_ARG, "%s: %d rows, k = %d, n = %d, %d adapters of rank %d", who, s.n_rows, s.k, s.n, s.n_adapters, s.rank);
+    if (!known(dtype)) return fail(MPS_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    if (s.n_adapters > mps::kMaxRowGroups) return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d adapters", who, mps::kMaxRowGroups);
+    if (s.k > 1 << 21 || s.n > 1 << 21 || s.rank > 1 << 12) return fail(MPS_ERR_UNSUPPORTED, "%s: k and n may be up to %d, the rank up to %d", who, 1 << 21, 1 << 12);
+    if (!s.group_ptr || (s.n_rows > 0 && (!s.ids || !s.slot_row))) return fail(MPS_ERR_ARG, "%s: NULL pointer", who);
+    if (misaligned(s.ids, 4) || misaligned(s.group_ptr, 4) || misaligned(s.slot_row, 4) || misaligned(s.scale, 4))
+        return fail(MPS_ERR_ALIGN, "%s: a pointer is not aligned to its element size", who);
+    if (s.n_rows > 0) {
+        const int64_t need = mps_adapters_workspace(s.n_rows, s.k, s.n, s.n_adapters, s.rank, dtype, backward);
+        if (need < 0) return (int)need;
+        if (!workspace || bytes < need) return fail(MPS_ERR_ARG, "%s: the workspace needs %lld bytes, %lld given", who, (long long)need, (long long)bytes);
+        if (misaligned(workspace, 256)) return fail(MPS_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", who);
+    }
+    return MPS_OK;
+}
+
+}  // namespace
+
+#define RD_BY_TYPE(dtype, call)                     \
+    do {                                            \
+        if ((dtype) == MPS_F32) { using T = float; return call; }      \
+        if ((dtype) == MPS_F16) { using T = __half; return call; }     \
+        using T = __nv_bfloat16;                    \
+        return call;                                \
+    } while (0)
+
+extern "C" int mps_routed_product(int32_t n_slots, int32_t n_rows, int32_t n_groups, int32_t k, int32_t n, int dtype, int transpose,
+                                  const int32_t *d_group_ptr, const int32_t *d_slot_row, const void *d_x, const void *d_w, void *d_y, void *stream) {
+    if (int rc = check_product("mps_routed_product", n_slots, n_rows, n_groups, k, n, dtype)) return rc;
+    if (n_slots == 0) return MPS_OK;
+    if (!d_group_ptr || !d_x || !d_w || !d_y) return fail(MPS_ERR_ARG, "mps_routed_product: NULL pointer");
+    if (!d_slot_row && n_rows < n_slots) return fail(MPS_ERR_ARG, "mps_routed_product: %d rows for %d slots read in order", n_rows, n_slots);
+    const size_t size = size_of(dtype);
+    if (misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_x, size) || misaligned(d_w, size) || misaligned(d_y, size))
+        return fail(MPS_ERR_ALIGN, "mps_routed_product: a pointer is not aligned to its element size");
+    RowsArgs a = {};
+    a.group_ptr = d_group_ptr;
+    a.slot_row = d_slot_row;
+    a.n_groups = n_groups;
+    a.n_slots = n_slots;
+    a.n_x_rows = n_rows;
+    a.k = transpose ? n : k;
+    a.n = transpose ? k : n;
+    a.w_group = (long long)k * n;
+    a.w_k = transpose ? k : 1;
+    a.w_n = transpose ? 1 : k;
+    RD_BY_TYPE(dtype, product<T>(a, d_x, d_w, d_y, (cudaStream_t)stream));
+}
+
+extern "C" int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_groups, int32_t k, int32_t n, int dtype, const int32_t *d_group_ptr,
+                                const int32_t *d_slot_row, const void *d_x, const void *d_dy, void *d_dw, void *stream) {
+    if (int rc = check_product("mps_routed_wgrad", n_slots, n_rows, n_groups, k, n, dtype)) return rc;
+    if (!d_group_ptr || !d_dw || (n_slots > 0 && (!d_x || !d_dy))) return fail(MPS_ERR_ARG, "mps_routed_wgrad: NULL pointer");
+    if (!d_slot_row && n_rows < n_slots) return fail(MPS_ERR_ARG, "mps_routed_wgrad: %d rows for %d slots read in order", n_rows, n_slots);
+    const size_t size = size_of(dtype);
+    if (misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_x, size) || misaligned(d_dy, size) || misaligned(d_dw, size))
+        return fail(MPS_ERR_ALIGN, "mps_routed_wgrad: a pointer is not aligned to its element size");
+    OuterArgs a = {};
+    a.group_ptr = d_group_ptr;
+    a.slot_row = d_slot_row;
+    a.n_groups = n_groups;
+    a.n_slots = n_slots;
+    a.n_rows = n_rows;
+    a.i = n;
+    a.j = k;
+    a.q_by_row = true;
+    RD_BY_TYPE(dtype, wgrad<T>(a, d_dy, d_x, d_dw, (cudaStream_t)stream));
+}
+
+static int check_combine(const char *who, int n_rows, int per_row, int n_slots, int dim, int dtype) {
+    if (n_rows < 0 || per_row < 1 || n_slots < 0 || dim < 1) return fail(MPS_ERR_ARG, "%s: %d rows of %d terms, %d slots, dim %d", who, n_rows, per_row, n_slots, dim);
+    if (!known(dtype)) return fail(MPS_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    if ((long long)n_rows * per_row >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "%s: rows * per_row does not fit 31 bits", who);
+    return MPS_OK;
+}
+
+extern "C" int mps_routed_combine(int32_t n_rows, int32_t per_row, int32_t n_slots, int32_t dim, int dtype, const int32_t *d_slot_of,
+                                  const float *d_weights, const void *d_rows, void *d_y, void *stream) {
+    if (int rc = check_combine("mps_routed_combine", n_rows, per_row, n_slots, dim, dtype)) return rc;
+    if (n_rows == 0) return MPS_OK;
+    if (!d_slot_of || !d_y || (n_slots > 0 && !d_rows)) return fail(MPS_ERR_ARG, "mps_routed_combine: NULL pointer");
+    const size_t size = size_of(dtype);
+    if (misaligned(d_slot_of, 4) || misaligned(d_weights, 4) || misaligned(d_rows, size) || misaligned(d_y, size))
+        return fail(MPS_ERR_ALIGN, "mps_routed_combine: a pointer is not aligned to its element size");
+    RD_BY_TYPE(dtype, launch_combine<T>(n_rows, per_row, n_slots, dim, d_slot_of, d_weights, d_rows, d_y, (cudaStream_t)stream));
+}
+
+extern "C" int mps_routed_combine_backward(int32_t n_rows, int32_t per_row, int32_t n_slots, int32_t dim, int dtype, const int32_t *d_slot_of,
+                                           const float *d_weights, const void *d_dy, const void *d_rows, void *d_drows, float *d_dweights, void *stream) {
+    if (int rc = check_combine("mps_routed_combine_backward", n_rows, per_row, n_slots, dim, dtype)) return rc;
+    if (n_rows == 0) return MPS_OK;
+    if (!d_slot_of || !d_dy || (n_slots > 0 && (!d_drows || (d_dweights && !d_rows)))) return fail(MPS_ERR_ARG, "mps_routed_combine_backward: NULL pointer");
+    const size_t size = size_of(dtype);
+    if (misaligned(d_slot_of, 4) || misaligned(d_weights, 4) || misaligned(d_dweights, 4) || misaligned(d_dy, size) || misaligned(d_rows, size) ||
+        misaligned(d_drows, size))
+        return fail(MPS_ERR_ALIGN, "mps_routed_combine_backward: a pointer is not aligned to its element size");
+    RD_BY_TYPE(dtype, launch_combine_backward<T>(n_rows, per_row, n_slots, dim, d_slot_of, d_weights, d_dy, d_rows, d_drows, d_dweights, (cudaStream_t)stream));
+}
+
+extern "C" int64_t mps_adapters_workspace(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, int backward) {
+    if (n_rows < 0 || k < 1 || n < 1 || n_adapters < 1 || rank < 1 || !known(dtype))
+        return fail(MPS_ERR_ARG, "mps_adapters_workspace: %d rows, k = %d, n = %d, %d adapters of rank %d, dtype %d", n_rows, k, n, n_adapters, rank, dtype);
+    return adapters_bytes(n_rows, rank, backward != 0);
+}
+
+extern "C" int mps_adapters(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, const int32_t *d_ids,
+                            const int32_t *d_group_ptr, const int32_t *d_slot_row, const float *d_scale, const void *d_x, const void *d_w,
+                            const void *d_a, const void *d_b, void *d_y, void *d_workspace, int64_t workspace_bytes, void *stream) {
+    const AdapterShape s = {n_rows, k, n, n_adapters, rank, d_ids, d_group_ptr, d_slot_row, d_scale};
+    if (int rc = check_adapters("mps_adapters", s, dtype, d_workspace, workspace_bytes, false)) return rc;
+    if (n_rows == 0) return MPS_OK;
+    if (!d_x || !d_w || !d_a || !d_b || !d_y) return fail(MPS_ERR_ARG, "mps_adapters: NULL pointer");
+    const size_t size = size_of(dtype);
+    if (misaligned(d_x, size) || misaligned(d_w, size) || misaligned(d_a, size) || misaligned(d_b, size) || misaligned(d_y, size))
+        return fail(MPS_ERR_ALIGN, "mps_adapters: a pointer is not aligned to its element size");
+    RD_BY_TYPE(dtype, adapters<T>(s, d_x, d_w, d_a, d_b, d_y, d_workspace, (cudaStream_t)stream));
+}
+
+extern "C" int mps_adapters_backward(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, const int32_t *d_ids,
+                                     const int32_t *d_group_ptr, const int32_t *d_slot_row, const float *d_scale, const void *d_dy, const void *d_x,
+                                     const void *d_w, const void *d_a, const void *d_b, void *d_dx, void *d_da, void *d_db, void *d_workspace,
+                                     int64_t workspace_bytes, void *stream) {
+    const AdapterShape s = {n_rows, k, n, n_adapters, rank, d_ids, d_group_ptr, d_slot_row, d_scale};
+    if (int rc = check_adapters("mps_adapters_backward", s, dtype, d_workspace, workspace_bytes, true)) return rc;
+    if (!d_w || !d_a || !d_b || !d_da || !d_db || (n_rows > 0 && (!d_dy || !d_x || !d_dx))) return fail(MPS_ERR_ARG, "mps_adapters_backward: NULL pointer");
+    const size_t size = size_of(dtype);
+    if (misaligned(d_dy, size) || misaligned(d_x, size) || misaligned(d_w, size) || misaligned(d_a, size) || misaligned(d_b, size) ||
+        misaligned(d_dx, size) || misaligned(d_da, size) || misaligned(d_db, size))
+        return fail(MPS_ERR_ALIGN, "mps_adapters_backward: a pointer is not aligned to its element size");
+    if (n_rows == 0) {  // no rows: the adapters' gradients are zero
+        const size_t bytes = (size_t)n_adapters * rank * size;
+        RD_CUDA(cudaMemsetAsync(d_da, 0, bytes * k, (cudaStream_t)stream));
+        RD_CUDA(cudaMemsetAsync(d_db, 0, bytes * n, (cudaStream_t)stream));
+        return MPS_OK;
+    }
+    RD_BY_TYPE(dtype, adapters_backward<T>(s, d_dy, d_x, d_w, d_a, d_b, d_dx, d_da, d_db, d_workspace, (cudaStream_t)stream));
+}
+
+extern "C" int mps_routed_check(void *stream) {
+    cudaStream_t st = (cudaStream_t)stream;
+    int routed = 0, route = 0;
+    static const int zero = 0;
+    RD_CUDA(cudaMemcpyFromSymbolAsync(&routed, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
+    RD_CUDA(cudaStreamSynchronize(st));
+    if (routed) RD_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+    if (int rc = mps::take_route_status(st, &route)) return rc;
+    const int status = routed | route;
+    if (status & mps::kStatusTimeout) return fail(MPS_ERR_DEVICE, "mps_routed_check: a kernel gave up a wait");
+    if (status & mps::kStatusBadIndex) return fail(MPS_ERR_ARG, "mps_routed_check: an id, a slot or a group offset was out of range");
+    return MPS_OK;
+}

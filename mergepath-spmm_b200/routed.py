@@ -1,0 +1,233 @@
+"""Rows that are each multiplied by the matrix they are routed to: experts, weights per node type, low-rank adapters.
+
+The routing is kept as the rows listed by group (`Groups`): `ptr` is the row_ptr over groups, `row` the col_idx (the input row
+in every slot), `slot` the slot of every (row, choice).  Thin wrappers of the mps_route* / mps_routed_* / mps_adapters* entry
+points of include/mps.h over torch CUDA tensors (float32, float16 or bfloat16); no reference counterpart.  Gradients are
+functions of their own.  Nothing synchronises; `routed_check()` waits and reports what the device met out of range.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+from . import capi
+
+try:
+    import torch
+except Exception:  # pragma: no cover
+    torch = None
+
+__all__ = ["Groups", "route", "route_backward", "group_rows", "routed_product", "routed_wgrad", "routed_combine", "routed_combine_backward",
+           "adapters", "adapters_backward", "routed_check"]
+
+_DTYPES = {} if torch is None else {torch.float32: capi.F32, torch.float16: capi.F16, torch.bfloat16: capi.BF16}
+
+
+class Groups(NamedTuple):
+    """Rows listed by group: int32 CUDA tensors ptr (groups + 1), row (slots, -1 behind the last one in use) and slot (the
+    shape of the ids, -1 for none)."""
+    ptr: "torch.Tensor"
+    row: "torch.Tensor"
+    slot: "torch.Tensor"
+
+
+def _dtype(t) -> int:
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise ValueError(f"expected float32, float16 or bfloat16, got {t.dtype}")
+    return d
+
+
+def _check(device, *named):
+    """Every (name, tensor, dtype, shape): a contiguous CUDA tensor on `device` of that dtype and shape (None: not given)."""
+    for name, t, dtype, shape in named:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name}: expected a CUDA tensor (there is no CPU path)")
+        if t.device != device:
+            raise ValueError(f"{name}: on {t.device}, expected {device}")
+        if not t.is_contiguous():
+            raise ValueError(f"{name}: expected a contiguous tensor")
+        if t.dtype != dtype:
+            raise ValueError(f"{name}: expected {dtype}, got {t.dtype}")
+        if tuple(t.shape) != tuple(shape):
+            raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _call(device, stream, name, *args):
+    """The entry point on `device` and `stream` (default: torch's current stream of that device)."""
+    fn = getattr(capi.lib(), name)
+    if device.index == torch.cuda.current_device():
+        capi.check(fn(*args, (torch.cuda.current_stream() if stream is None else stream).cuda_stream))
+        return
+    with torch.cuda.device(device):
+        capi.check(fn(*args, (torch.cuda.current_stream() if stream is None else stream).cuda_stream))
+
+
+def _matrix(name, t, dims=2):
+    if t.dim() != dims:
+        raise ValueError(f"{name}: expected {dims} dimensions, got {t.dim()}")
+    if not t.is_cuda:
+        raise ValueError(f"{name}: expected a CUDA tensor (there is no CPU path)")
+    return t
+
+
+def _spec(n_experts, top_k, score, n_groups, top_groups, group_top, renormalise, scale):
+    if score not in capi.SCORES:
+        raise ValueError(f"score: expected one of {sorted(capi.SCORES)}, got {score!r}")
+    return capi.RouteSpec(n_experts, top_k, capi.SCORES[score], n_groups, top_groups, group_top, int(renormalise), scale)
+
+
+def route(logits, top_k: int, *, score: str = "softmax", bias=None, n_groups: int = 1, top_groups: int = 1, group_top: int = 1,
+          renormalise: bool = True, scale: float = 1.0, group: bool = True, stream=None):
+    """(ids, weights, groups): the top_k experts of every row of `logits` (rows, experts) by score + bias among the best
+    `top_groups` of `n_groups` expert groups, their weights (fp32), and the rows listed by expert (None with group=False)."""
+    rows, experts = _matrix("logits", logits).shape
+    dev = logits.device
+    _check(dev, ("logits", logits, logits.dtype, (rows, experts)), ("bias", bias, torch.float32, (experts,)))
+    spec = _spec(experts, top_k, score, n_groups, top_groups, group_top, renormalise, scale)
+    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
+    weights = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
+    groups = None
+    if group:
+        groups = Groups(torch.empty(experts + 1, dtype=torch.int32, device=dev), torch.empty(rows * top_k, dtype=torch.int32, device=dev),
+                        torch.empty((rows, top_k), dtype=torch.int32, device=dev))
+    ptr, row, slot = groups or (None, None, None)
+    _call(dev, stream, "mps_route", rows, C.byref(spec), _dtype(logits), _ptr(logits), _ptr(bias), _ptr(ids), _ptr(weights), _ptr(ptr), _ptr(row), _ptr(slot))
+    return ids, weights, groups
+
+
+def route_backward(logits, ids, d_weights, *, score: str = "softmax", renormalise: bool = True, scale: float = 1.0, stream=None):
+    """Gradient by the logits of route's weights for the choice `ids` and the weights' gradient (fp32)."""
+    rows, experts = _matrix("logits", logits).shape
+    dev = logits.device
+    top_k = _matrix("ids", ids).shape[1]
+    _check(dev, ("logits", logits, logits.dtype, (rows, experts)), ("ids", ids, torch.int32, (rows, top_k)),
+           ("d_weights", d_weights, torch.float32, (rows, top_k)))
+    spec = _spec(experts, top_k, score, 1, 1, 1, renormalise, scale)
+    out = torch.empty_like(logits)
+    _call(dev, stream, "mps_route_backward", rows, C.byref(spec), _dtype(logits), _ptr(logits), _ptr(ids), _ptr(d_weights), _ptr(out))
+    return out
+
+
+def group_rows(ids, n_groups: int, *, stream=None) -> Groups:
+    """Rows listed by group from int32 `ids` of shape (rows,) or (rows, choices); a negative id is no group."""
+    dev = ids.device
+    if ids.dim() not in (1, 2):
+        raise ValueError(f"ids: expected 1 or 2 dimensions, got {ids.dim()}")
+    _check(dev, ("ids", ids, torch.int32, ids.shape))
+    rows, per_row = ids.shape[0], 1 if ids.dim() == 1 else ids.shape[1]
+    groups = Groups(torch.empty(max(n_groups, 0) + 1, dtype=torch.int32, device=dev), torch.empty(ids.numel(), dtype=torch.int32, device=dev),
+                    torch.empty_like(ids))
+    _call(dev, stream, "mps_group_rows", rows, per_row, n_groups, _ptr(ids), _ptr(groups.ptr), _ptr(groups.row), _ptr(groups.slot))
+    return groups
+
+
+def routed_product(x, w, groups: Groups, *, gather: bool = True, transpose: bool = False, out=None, stream=None):
+    """y[s] = x[groups.row[s]] @ w[g].T for the slots s of every group g (x[s] itself with gather=False); transpose=True
+    multiplies by w[g] instead.  w (groups, n, k).  Rows of `out` behind the last slot in use are left as they were."""
+    n_groups, n, k = _matrix("w", w, 3).shape
+    inner, outer = (n, k) if transpose else (k, n)
+    dev, rows, slots = x.device, _matrix("x", x).shape[0], groups.row.numel()
+    if out is None:
+        out = torch.empty((slots, outer), dtype=x.dtype, device=dev)
+    _check(dev, ("x", x, x.dtype, (rows, inner)), ("w", w, x.dtype, (n_groups, n, k)), ("groups.ptr", groups.ptr, torch.int32, (n_groups + 1,)),
+           ("groups.row", groups.row, torch.int32, (slots,)), ("out", out, x.dtype, (slots, outer)))
+    _call(dev, stream, "mps_routed_product", slots, rows, n_groups, k, n, _dtype(x), int(transpose), _ptr(groups.ptr),
+          _ptr(groups.row) if gather else None, _ptr(x), _ptr(w), _ptr(out))
+    return out
+
+
+def routed_wgrad(x, dy, groups: Groups, *, gather: bool = True, out=None, stream=None):
+    """dw[g] = sum over the slots s of g of outer(dy[s], x[groups.row[s]]) (x[s] with gather=False): (groups, n, k), zero for
+    a group without slots."""
+    dev, slots, n_groups = x.device, groups.row.numel(), groups.ptr.numel() - 1
+    (rows, k), n = _matrix("x", x).shape, _matrix("dy", dy).shape[1]
+    if out is None:
+        out = torch.empty((n_groups, n, k), dtype=x.dtype, device=dev)
+    _check(dev, ("x", x, x.dtype, (rows, k)), ("dy", dy, x.dtype, (slots, n)), ("groups.ptr", groups.ptr, torch.int32, (n_groups + 1,)),
+           ("groups.row", groups.row, torch.int32, (slots,)), ("out", out, x.dtype, (n_groups, n, k)))
+    _call(dev, stream, "mps_routed_wgrad", slots, rows, n_groups, k, n, _dtype(x), _ptr(groups.ptr), _ptr(groups.row) if gather else None,
+          _ptr(x), _ptr(dy), _ptr(out))
+    return out
+
+
+def routed_combine(rows, slot, weights=None, *, out=None, stream=None):
+    """y[t] = sum over j of weights[t, j] * rows[slot[t, j]]; no term for a negative slot, weights None: 1 each."""
+    dev, (n_slots, dim), (n, per_row) = rows.device, _matrix("rows", rows).shape, _matrix("slot", slot).shape
+    if out is None:
+        out = torch.empty((n, dim), dtype=rows.dtype, device=dev)
+    _check(dev, ("rows", rows, rows.dtype, (n_slots, dim)), ("slot", slot, torch.int32, (n, per_row)), ("weights", weights, torch.float32, (n, per_row)),
+           ("out", out, rows.dtype, (n, dim)))
+    _call(dev, stream, "mps_routed_combine", n, per_row, n_slots, dim, _dtype(rows), _ptr(slot), _ptr(weights), _ptr(rows), _ptr(out))
+    return out
+
+
+def routed_combine_backward(dy, rows, slot, weights=None, *, out=None, stream=None):
+    """(d_rows, d_weights) of routed_combine; `out` receives d_rows, whose rows that no slot names are left as they were."""
+    dev, (n_slots, dim), (n, per_row) = rows.device, _matrix("rows", rows).shape, _matrix("slot", slot).shape
+    if out is None:
+        out = torch.empty_like(rows)
+    _check(dev, ("dy", dy, rows.dtype, (n, dim)), ("rows", rows, rows.dtype, (n_slots, dim)), ("slot", slot, torch.int32, (n, per_row)),
+           ("weights", weights, torch.float32, (n, per_row)), ("out", out, rows.dtype, (n_slots, dim)))
+    d_weights = torch.empty((n, per_row), dtype=torch.float32, device=dev)
+    _call(dev, stream, "mps_routed_combine_backward", n, per_row, n_slots, dim, _dtype(rows), _ptr(slot), _ptr(weights), _ptr(dy), _ptr(rows), _ptr(out),
+          _ptr(d_weights))
+    return out, d_weights
+
+
+def _adapter_sizes(x, w, a, b, ids, groups, scale):
+    rows, (n, k), (n_adapters, rank) = _matrix("x", x).shape[0], _matrix("w", w).shape, _matrix("a", a, 3).shape[:2]
+    _check(x.device, ("x", x, x.dtype, (rows, k)), ("w", w, x.dtype, (n, k)), ("a", a, x.dtype, (n_adapters, rank, k)),
+           ("b", b, x.dtype, (n_adapters, n, rank)), ("ids", ids, torch.int32, (rows,)), ("groups.ptr", groups.ptr, torch.int32, (n_adapters + 1,)),
+           ("groups.row", groups.row, torch.int32, (rows,)), ("scale", scale, torch.float32, (n_adapters,)))
+    return rows, k, n, n_adapters, rank
+
+
+def _adapter_workspace(device, sizes, dtype, backward):
+    need = capi.lib().mps_adapters_workspace(*sizes, dtype, int(backward))
+    if need < 0:
+        capi.check(int(need))
+    return torch.empty(need, dtype=torch.uint8, device=device)
+
+
+def adapters(x, w, a, b, ids, groups: Groups, scale=None, *, out=None, stream=None):
+    """y[t] = x[t] @ w.T + scale[i] * (x[t] @ a[i].T) @ b[i].T with i = ids[t] (a negative id: the projection alone).
+    w (n, k), a (adapters, rank, k), b (adapters, n, rank), groups = group_rows(ids, adapters), scale fp32 or None (1)."""
+    sizes = rows, k, n, _, _ = _adapter_sizes(x, w, a, b, ids, groups, scale)
+    if out is None:
+        out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
+    _check(x.device, ("out", out, x.dtype, (rows, n)))
+    dtype = _dtype(x)
+    ws = _adapter_workspace(x.device, sizes, dtype, False)
+    if stream is not None:
+        ws.record_stream(stream)
+    _call(x.device, stream, "mps_adapters", *sizes, dtype, _ptr(ids), _ptr(groups.ptr), _ptr(groups.row), _ptr(scale), _ptr(x), _ptr(w), _ptr(a), _ptr(b),
+          _ptr(out), _ptr(ws), ws.numel())
+    return out
+
+
+def adapters_backward(dy, x, w, a, b, ids, groups: Groups, scale=None, *, stream=None):
+    """(dx, da, db) of adapters; the shared projection and the scales are constants."""
+    sizes = rows, k, n, _, _ = _adapter_sizes(x, w, a, b, ids, groups, scale)
+    _check(x.device, ("dy", dy, x.dtype, (rows, n)))
+    dx, da, db = torch.empty_like(x), torch.empty_like(a), torch.empty_like(b)
+    dtype = _dtype(x)
+    ws = _adapter_workspace(x.device, sizes, dtype, True)
+    if stream is not None:
+        ws.record_stream(stream)
+    _call(x.device, stream, "mps_adapters_backward", *sizes, dtype, _ptr(ids), _ptr(groups.ptr), _ptr(groups.row), _ptr(scale), _ptr(dy), _ptr(x), _ptr(w),
+          _ptr(a), _ptr(b), _ptr(dx), _ptr(da), _ptr(db), _ptr(ws), ws.numel())
+    return dx, da, db
+
+
+def routed_check(device=None, stream=None) -> None:
+    """Waits for the stream and raises if a routed operator on the device met an index out of range or gave up a wait since
+    the last check."""
+    with torch.cuda.device(torch.cuda.current_device() if device is None else device):
+        capi.check(capi.lib().mps_routed_check((torch.cuda.current_stream() if stream is None else stream).cuda_stream))
