@@ -38,7 +38,7 @@ def build_library(force: bool = False, verbose: bool = False) -> str:
     """Compiles every source to an object (in parallel) and links libmps_b200.so."""
     from concurrent.futures import ThreadPoolExecutor
     srcs = _sources(["mps_api.cu", "mps_spmm_f32.cu", "mps_spmm_f32_scaled.cu", "mps_spmm_f16.cu", "mps_noalloc.cu", "mps_multi.cu", "mps_probe.cu", "mps_route.cu", "mps_routed.cu", "convert_device.cu", "csr_io.cpp", "convert.cpp", "host_check.cpp", "partition_host.cpp"])
-    deps = srcs + _sources(["mps_kernels.cuh", "mps_dispatch.cuh", "mps_internal.h", "mps_plan.h", "mps_types.cuh", "mps_routed_plain.cuh"]) + [os.path.join(ROOT, "include", "mps.h")]
+    deps = srcs + _sources(["mps_kernels.cuh", "mps_dispatch.cuh", "mps_internal.h", "mps_plan.h", "mps_types.cuh", "mps_routed_plain.cuh", "mps_tc.cuh", "mps_routed_tc.cuh"]) + [os.path.join(ROOT, "include", "mps.h")]
     if not force and _newer(LIB, deps):
         return LIB
     os.makedirs(LIBDIR, exist_ok=True)

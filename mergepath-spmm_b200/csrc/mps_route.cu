@@ -357,15 +357,16 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(RouteA
 // Rows listed by group: a stable counting sort of the pairs (row, choice) by id in one launch.  The pairs are cut into one
 // contiguous run per warp of the cluster; a warp counts its run's ids in shared memory (lanes of equal id are found with
 // match.any, so no atomics and one order), the counts are scanned over warps, blocks (distributed shared memory) and groups,
-// and the warp walks its run again and places every pair.
+// and the warp walks its run again and places every pair.  With `rest` the pairs without a group form one group more, the last.
 constexpr int kGroupThreads = 1024, kGroupWarps = kGroupThreads / 32, kGroupMax = 1024;
 constexpr int kGroupCluster = 8;
 
-__global__ void __launch_bounds__(kGroupThreads) group_kernel(long long n_pairs, int per_row, int n_groups, const int *__restrict__ ids,
+__global__ void __launch_bounds__(kGroupThreads) group_kernel(long long n_pairs, int per_row, int n_groups, bool rest, const int *__restrict__ ids,
                                                              int *__restrict__ group_ptr, int *__restrict__ slot_row, int *__restrict__ slot_of) {
     extern __shared__ int s_int[];
-    int *count = s_int;                             // [warps][n_groups], later the next free slot
-    int *total = s_int + kGroupWarps * n_groups;    // this block's pairs per group
+    const int columns = n_groups + (rest ? 1 : 0), none = rest ? n_groups : -1;
+    int *count = s_int;                            // [warps][columns], later the next free slot
+    int *total = s_int + kGroupWarps * columns;    // this block's pairs per column
     __shared__ int s_scan[kGroupWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks();
@@ -373,29 +374,27 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(long long n_pairs,
     const long long steps = (n_pairs + 31) / 32, runs = (long long)blocks * kGroupWarps;
     const long long run = rank * kGroupWarps + warp;
     const long long lo = steps * run / runs, hi = steps * (run + 1) / runs;
-    int *own = count + warp * n_groups;
-    for (int g = lane; g < n_groups; g += 32) own[g] = 0;
+    int *own = count + warp * columns;
+    for (int g = lane; g < columns; g += 32) own[g] = 0;
     __syncwarp();
     for (long long s = lo; s < hi; ++s) {
         const long long i = s * 32 + lane;
         int id = i < n_pairs ? ids[i] : -1;
-        if (id >= n_groups) {
-            atomicOr(&g_status, mps::kStatusBadIndex);
-            id = -1;
-        }
+        if (id >= n_groups) atomicOr(&g_status, mps::kStatusBadIndex);
+        if ((unsigned)id >= (unsigned)n_groups) id = i < n_pairs ? none : -1;
         const unsigned same = __match_any_sync(kAll, id);
         if (id >= 0 && lane == __ffs(same) - 1) own[id] += __popc(same);
         __syncwarp();
     }
     __syncthreads();
-    if (tid < n_groups) {
+    for (int g = tid; g < columns; g += kGroupThreads) {
         int sum = 0;
         for (int w = 0; w < kGroupWarps; ++w) {
-            const int c = count[w * n_groups + tid];
-            count[w * n_groups + tid] = sum;
+            const int c = count[w * columns + g];
+            count[w * columns + g] = sum;
             sum += c;
         }
-        total[tid] = sum;
+        total[g] = sum;
     }
     cluster.sync();
     int before = 0, all = 0;
@@ -430,13 +429,19 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(long long n_pairs,
             group_ptr[tid] = start;
             if (tid == n_groups - 1) group_ptr[n_groups] = used;
         }
-        for (int w = 0; w < kGroupWarps; ++w) count[w * n_groups + tid] += start + before;
+        for (int w = 0; w < kGroupWarps; ++w) count[w * columns + tid] += start + before;
+    }
+    if (rest && tid < 32) {  // behind the groups
+        int ahead = used;
+        for (int r = 0; r < rank; ++r) ahead += cluster.map_shared_rank(total, r)[n_groups];
+        count[tid * columns + n_groups] += ahead;
+        if (tid == 0 && rank == 0) group_ptr[columns] = (int)n_pairs;
     }
     cluster.sync();  // also: no block leaves while another still reads its totals
     for (long long s = lo; s < hi; ++s) {
         const long long i = s * 32 + lane;
         int id = i < n_pairs ? ids[i] : -1;
-        if (id >= n_groups) id = -1;
+        if ((unsigned)id >= (unsigned)n_groups) id = i < n_pairs ? none : -1;
         const unsigned same = __match_any_sync(kAll, id);
         int at = -1;
         if (id >= 0) at = own[id] + __popc(same & ((1u << lane) - 1));
@@ -444,17 +449,17 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(long long n_pairs,
         if (id >= 0 && lane == __ffs(same) - 1) own[id] += __popc(same);
         __syncwarp();
         if (i < n_pairs) {
-            slot_of[i] = at;
+            if (slot_of) slot_of[i] = at;
             if (at >= 0) slot_row[at] = (int)(i / per_row);
-            if (i >= used) slot_row[i] = -1;
+            if (!rest && i >= used) slot_row[i] = -1;
         }
     }
 }
 
-int launch_group(long long n_pairs, int per_row, int n_groups, const int *ids, int *ptr, int *row, int *slot, cudaStream_t st) {
-    const size_t smem = (size_t)(kGroupWarps + 1) * n_groups * sizeof(int);
+int launch_group(long long n_pairs, int per_row, int n_groups, bool rest, const int *ids, int *ptr, int *row, int *slot, cudaStream_t st) {
+    const size_t smem = (size_t)(kGroupWarps + 1) * (n_groups + (rest ? 1 : 0)) * sizeof(int);
     if (smem > 40 * 1024)
-        RT_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kGroupWarps + 1) * kGroupMax * (int)sizeof(int)));
+        RT_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kGroupWarps + 1) * (kGroupMax + 1) * (int)sizeof(int)));
     const int blocks = n_pairs > 2048 ? kGroupCluster : 1;
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
@@ -467,7 +472,7 @@ int launch_group(long long n_pairs, int per_row, int n_groups, const int *ids, i
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, group_kernel, n_pairs, per_row, n_groups, ids, ptr, row, slot));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, group_kernel, n_pairs, per_row, n_groups, rest, ids, ptr, row, slot));
     return MPS_OK;
 }
 
@@ -523,6 +528,9 @@ int take_route_status(void *stream, int *status) {
     if (*status) RT_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
     return MPS_OK;
 }
+int list_rows_and_rest(int n_rows, int n_groups, const int32_t *ids, int32_t *group_ptr, int32_t *slot_row, void *stream) {
+    return launch_group(n_rows, 1, n_groups, true, ids, group_ptr, slot_row, nullptr, (cudaStream_t)stream);
+}
 }  // namespace mps
 
 extern "C" int mps_group_rows(int32_t n_rows, int32_t per_row, int32_t n_groups, const int32_t *d_ids, int32_t *d_group_ptr, int32_t *d_slot_row,
@@ -534,7 +542,7 @@ extern "C" int mps_group_rows(int32_t n_rows, int32_t per_row, int32_t n_groups,
     if (pairs >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "mps_group_rows: rows * per_row does not fit 31 bits");
     if (misaligned(d_ids, 4) || misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_slot_of, 4))
         return fail(MPS_ERR_ALIGN, "mps_group_rows: pointers must be 4-byte aligned");
-    return launch_group(pairs, per_row, n_groups, d_ids, d_group_ptr, d_slot_row, d_slot_of, (cudaStream_t)stream);
+    return launch_group(pairs, per_row, n_groups, false, d_ids, d_group_ptr, d_slot_row, d_slot_of, (cudaStream_t)stream);
 }
 
 extern "C" int mps_route(int32_t n_rows, const mps_route_spec *spec, int dtype, const void *d_logits, const float *d_bias, int32_t *d_ids,
@@ -557,7 +565,7 @@ extern "C" int mps_route(int32_t n_rows, const mps_route_spec *spec, int dtype, 
         else rc = sig ? launch_route<__nv_bfloat16, true>(a, d_logits, d_bias, d_ids, d_weights, st) : launch_route<__nv_bfloat16, false>(a, d_logits, d_bias, d_ids, d_weights, st);
         if (rc) return rc;
     }
-    if (list) return launch_group((long long)n_rows * a.top_k, a.top_k, a.n_experts, d_ids, d_group_ptr, d_slot_row, d_slot_of, st);
+    if (list) return launch_group((long long)n_rows * a.top_k, a.top_k, a.n_experts, false, d_ids, d_group_ptr, d_slot_row, d_slot_of, st);
     return MPS_OK;
 }
 

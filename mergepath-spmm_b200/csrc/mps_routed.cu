@@ -3,13 +3,18 @@
 
 #include <cuda_runtime.h>
 
+#include <initializer_list>
+
 #include "mps_internal.h"
 #include "mps_routed_plain.cuh"
+#include "mps_routed_tc.cuh"
 #include "mps_types.cuh"
 
 using mps::fail;
 using mps::OuterArgs;
 using mps::RowsArgs;
+using mps::TcOuter;
+using mps::TcRows;
 
 namespace {
 
@@ -169,6 +174,132 @@ int launch_plain_outer(OuterArgs a, const void *p, const void *q, void *out, cud
     return MPS_OK;
 }
 
+// ---- tensor cores
+
+int sm_count(int *n) {
+    int dev = 0;
+    RD_CUDA(cudaGetDevice(&dev));
+    RD_CUDA(cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev));
+    return MPS_OK;
+}
+
+// Tensor map of `dims` sizes (innermost first, rows packed) of a 16-bit type, read in boxes of 64 elements by box_rows.
+int tensor_map(CUtensorMap *map, bool bf16, const void *base, int dims, unsigned long long d0, unsigned long long d1, unsigned long long d2, int box_rows) {
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &fn, 12000, cudaEnableDefault, &found) != cudaSuccess) fn = nullptr;
+        return (Encode)fn;
+    }();
+    if (!encode) return fail(MPS_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+    const cuuint64_t size[3] = {d0, d1, d2}, pitch[2] = {d0 * 2, d0 * d1 * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    const CUresult rc = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims, const_cast<void *>(base), size, pitch,
+                               box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fail(MPS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu x %llu", (int)rc, d0, d1, d2);
+    return MPS_OK;
+}
+
+// A launch of `blocks` blocks in clusters of `split`.
+template <typename Kernel, typename Args>
+int launch_tc(Kernel kernel, const Args &args, long long blocks, int split, size_t smem, cudaStream_t st) {
+    RD_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = split;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)blocks);
+    cfg.blockDim = dim3(mps::kTcThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    RD_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
+    return MPS_OK;
+}
+
+// Blocks that share a tile's sum: as many as leave no SM without work, but two slices each at least.
+int split_of(long long tiles, int steps, int sms) {
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= sms && split * 4 <= steps) split *= 2;
+    return split;
+}
+
+template <int NT>
+int launch_tc_rows(TcRows a, int sms, cudaStream_t st) {
+    // a group ends in a part of a tile, so there are at most this many
+    const long long most = a.n_slots / NT + (a.n_groups < a.n_slots ? a.n_groups : a.n_slots);
+    const long long tiles = most * ((a.n + mps::kTcFeatures - 1) / mps::kTcFeatures);
+    a.split = NT <= 64 ? split_of(tiles, (a.k + mps::kTcDepth - 1) / mps::kTcDepth, sms) : 1;
+    const long long workers = sms / a.split;
+    return launch_tc(mps::tc_rows_kernel<NT>, a, (tiles < workers ? tiles : workers) * a.split, a.split, mps::TcShape<NT>::bytes(a.n_groups), st);
+}
+
+// The rest of a filled in: what every use has in common, and the tile for the mean number of rows per group.
+int tc_rows(TcRows a, const void *x, long long x_rows, cudaStream_t st) {
+    if (int rc = status_pointer(&a.status)) return rc;
+    int sms;
+    if (int rc = sm_count(&sms)) return rc;
+    const int groups = a.n_groups < a.n_slots ? a.n_groups : a.n_slots;
+    const long long mean = a.n_slots / groups;
+    const int nt = mean <= 8 ? 16 : mean <= 20 ? 32 : mean <= 48 ? 64 : mean <= 128 ? 128 : 256;
+    if (int rc = tensor_map(&a.x, a.bf16, x, 2, a.k, x_rows, 1, a.gather ? 1 : nt)) return rc;
+    if (a.rank) {
+        if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, nt)) return rc;
+    }
+    if (nt == 16) return launch_tc_rows<16>(a, sms, st);
+    if (nt == 32) return launch_tc_rows<32>(a, sms, st);
+    if (nt == 64) return launch_tc_rows<64>(a, sms, st);
+    if (nt == 128) return launch_tc_rows<128>(a, sms, st);
+    return launch_tc_rows<256>(a, sms, st);
+}
+
+// The matrices of a: stored features x summed (MN-major: summed x features), `groups` of them.
+int tc_matrix(CUtensorMap *map, TcRows *a, const void *w, int summed, int features, long long groups) {
+    a->w_rows = features < mps::kTcFeatures ? (features + 7) / 8 * 8 : mps::kTcFeatures;
+    return a->mn_major ? tensor_map(map, a->bf16, w, 3, features, summed, groups, mps::kTcDepth)
+                       : tensor_map(map, a->bf16, w, 3, summed, features, groups, a->w_rows);
+}
+
+template <int NT>
+int launch_tc_outer(TcOuter a, int sms, cudaStream_t st) {
+    const int cols = a.pair ? NT / 2 : NT;
+    const long long tiles = (long long)a.n_groups * ((a.i + mps::kTcFeatures - 1) / mps::kTcFeatures) * ((a.j + cols - 1) / cols);
+    const int steps = (a.n_slots / a.n_groups + mps::kTcDepth - 1) / mps::kTcDepth;  // of the mean group
+    a.split = NT <= 128 ? split_of(tiles, steps, sms) : 1;
+    const long long workers = sms / a.split;
+    return launch_tc(mps::tc_outer_kernel<NT>, a, (tiles < workers ? tiles : workers) * a.split, a.split, mps::TcOuterShape<NT>::kBytes, st);
+}
+
+// P: n_p_rows rows of a.i, by a.slot_row or in slot order; Q: rows of a.j in slot order (pair: two planes of them).
+int tc_outer(TcOuter a, const void *p, const void *q, cudaStream_t st) {
+    if (int rc = status_pointer(&a.status)) return rc;
+    int sms;
+    if (int rc = sm_count(&sms)) return rc;
+    a.q_plane = a.n_slots;
+    a.q_rows_all = a.pair ? 2 * a.n_slots : a.n_slots;
+    if (int rc = tensor_map(&a.p_rows, a.bf16, p, 2, a.i, a.n_p_rows, 1, 1)) return rc;
+    if (int rc = tensor_map(&a.p_tile, a.bf16, p, 2, a.i, a.n_p_rows, 1, mps::kTcDepth)) return rc;
+    if (int rc = tensor_map(&a.q_rows, a.bf16, q, 2, a.j, a.q_rows_all, 1, 1)) return rc;
+    if (int rc = tensor_map(&a.q_tile, a.bf16, q, 2, a.j, a.q_rows_all, 1, mps::kTcDepth)) return rc;
+    if (a.pair || a.j <= 128) return launch_tc_outer<128>(a, sms, st);
+    return launch_tc_outer<256>(a, sms, st);
+}
+
+// Whether tensor maps can describe the operands: a 16-bit type, row pitches and addresses in multiples of 16 bytes.
+bool tc_widths(int dtype, std::initializer_list<int> pitches, std::initializer_list<const void *> pointers) {
+    if (dtype == MPS_F32) return false;
+    for (int p : pitches)
+        if (p % 8) return false;
+    for (const void *p : pointers)
+        if (misaligned(p, 16)) return false;
+    return true;
+}
+
 int check_product(const char *who, int n_slots, int n_rows, int n_groups, int k, int n, int dtype) {
     if (n_slots < 0 || n_rows < 0 || n_groups < 1 || k < 1 || n < 1)
         return fail(MPS_ERR_ARG, "%s: %d slots, %d rows, %d groups, k = %d, n = %d", who, n_slots, n_rows, n_groups, k, n);
@@ -178,20 +309,10 @@ int check_product(const char *who, int n_slots, int n_rows, int n_groups, int k,
     return MPS_OK;
 }
 
-template <typename T>
-int product(const RowsArgs &a, const void *x, const void *w, void *y, cudaStream_t st) {
-    return launch_plain_rows<T, T, false>(a, x, w, nullptr, y, st);
-}
-
-template <typename T>
-int wgrad(const OuterArgs &a, const void *dy, const void *x, void *dw, cudaStream_t st) {
-    return launch_plain_outer<T, T, T>(a, dy, x, dw, st);
-}
-
 // ---------------------------------------------------------------------------------------------- adapters
 
 struct AdapterShape {
-    int n_rows, k, n, n_adapters, rank;
+    int n_rows, k, n, n_adapters, rank, dtype;
     const int *ids, *group_ptr, *slot_row;
     const float *scale;
 };
@@ -234,9 +355,95 @@ int adapter_wide(const AdapterShape &s, int k, int n, const void *x, const void 
     return launch_plain_rows<T, T, true>(a, x, w, m, out, st);
 }
 
+// Workspace: the two intermediates (fp32 by row, or hi and lo planes by slot: 4 bytes a value either way), then the rows listed
+// with those that ask for no adapter behind the others.
+struct AdapterSpace {
+    char *u, *v;
+    int *ptr, *row;
+    int64_t bytes;
+    AdapterSpace(void *base, int n_rows, int n_adapters, int rank, bool backward) {
+        char *at = (char *)base;
+        auto take = [&](int64_t size) {
+            char *p = at;
+            at += (size + 255) / 256 * 256;
+            return p;
+        };
+        u = take((int64_t)n_rows * rank * 4);
+        v = backward ? take((int64_t)n_rows * rank * 4) : nullptr;
+        ptr = (int *)take(4ll * (n_adapters + 2));
+        row = (int *)take(4ll * n_rows);
+        bytes = at - (char *)base;
+    }
+};
+
+// u (two planes, slot order) = scale * rows of x times the adapters' matrices (mn_major: stored summed x rank)
+int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m, bool mn_major, void *u, cudaStream_t st) {
+    TcRows a = {};
+    a.bf16 = s.dtype == MPS_BF16;
+    a.mn_major = mn_major;
+    a.group_ptr = s.group_ptr;
+    a.slot_row = s.slot_row;
+    a.n_groups = s.n_adapters;
+    a.n_slots = a.n_x_rows = s.n_rows;
+    a.k = k;
+    a.n = s.rank;
+    a.gather = a.pair = true;
+    a.group_scale = s.scale;
+    a.out = u;
+    a.out_plane = (long long)s.n_rows * s.rank;
+    if (int rc = tc_matrix(&a.w, &a, m, k, s.rank, s.n_adapters)) return rc;
+    return tc_rows(a, x, s.n_rows, st);
+}
+
+// out = x times the shared matrix, the sum going on with u times the adapter's matrix; rows by adapter, those without one last
+int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, int k, int n, const void *x, const void *w, const void *u, const void *m, bool mn_major,
+                    void *out, cudaStream_t st) {
+    TcRows a = {};
+    a.bf16 = s.dtype == MPS_BF16;
+    a.mn_major = mn_major;
+    a.group_ptr = ws.ptr;
+    a.slot_row = ws.row;
+    a.n_groups = s.n_adapters + 1;
+    a.n_slots = a.n_x_rows = s.n_rows;
+    a.k = k;
+    a.n = n;
+    a.rank = s.rank;
+    a.rank_groups = s.n_adapters;
+    a.u_base = u;
+    a.u_plane = s.n_rows;
+    a.w_shared = a.gather = a.scatter = true;
+    a.out = out;
+    if (int rc = tc_matrix(&a.w, &a, w, k, n, 1)) return rc;
+    if (int rc = tc_matrix(&a.w2, &a, m, s.rank, n, s.n_adapters)) return rc;
+    return tc_rows(a, x, s.n_rows, st);
+}
+
+int tc_adapter_outer(const AdapterShape &s, int features, const void *p, const void *q, void *out, long long out_f, long long out_c, cudaStream_t st) {
+    TcOuter a = {};
+    a.bf16 = s.dtype == MPS_BF16;
+    a.group_ptr = s.group_ptr;
+    a.slot_row = s.slot_row;
+    a.n_groups = s.n_adapters;
+    a.n_slots = a.n_p_rows = s.n_rows;
+    a.i = features;
+    a.j = s.rank;
+    a.pair = true;
+    a.out = out;
+    a.out_group = (long long)features * s.rank;
+    a.out_f = out_f;
+    a.out_c = out_c;
+    return tc_outer(a, p, q, st);
+}
+
 template <typename T>
 int adapters(const AdapterShape &s, const void *x, const void *w, const void *a, const void *b, void *y, void *workspace, cudaStream_t st) {
-    float *u = (float *)workspace;
+    const AdapterSpace ws(workspace, s.n_rows, s.n_adapters, s.rank, false);
+    if (tc_widths(s.dtype, {s.k, s.rank}, {x, w, a, b})) {
+        if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
+        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, st)) return rc;
+        return tc_adapter_wide(s, ws, s.k, s.n, x, w, ws.u, b, false, y, st);
+    }
+    float *u = (float *)ws.u;
     if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
     return adapter_wide<T>(s, s.k, s.n, x, w, 1, s.k, u, b, 1, s.rank, y, st);
 }
@@ -244,9 +451,18 @@ int adapters(const AdapterShape &s, const void *x, const void *w, const void *a,
 template <typename T>
 int adapters_backward(const AdapterShape &s, const void *dy, const void *x, const void *w, const void *a, const void *b, void *dx, void *da, void *db,
                       void *workspace, cudaStream_t st) {
-    float *u = (float *)workspace, *v = u + (size_t)s.n_rows * s.rank;
-    if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;    // scale * x A^T
-    if (int rc = adapter_narrow<T>(s, s.n, dy, b, s.rank, 1, v, st)) return rc;  // scale * dy B
+    const AdapterSpace ws(workspace, s.n_rows, s.n_adapters, s.rank, true);
+    if (tc_widths(s.dtype, {s.k, s.n, s.rank}, {dy, x, w, a, b})) {
+        if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
+        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, st)) return rc;    // scale * x A^T
+        if (int rc = tc_adapter_narrow(s, s.n, dy, b, true, ws.v, st)) return rc;    // scale * dy B
+        if (int rc = tc_adapter_wide(s, ws, s.n, s.k, dy, w, ws.v, a, true, dx, st)) return rc;
+        if (int rc = tc_adapter_outer(s, s.k, x, ws.v, da, 1, s.k, st)) return rc;
+        return tc_adapter_outer(s, s.n, dy, ws.u, db, s.rank, 1, st);
+    }
+    float *u = (float *)ws.u, *v = (float *)ws.v;
+    if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
+    if (int rc = adapter_narrow<T>(s, s.n, dy, b, s.rank, 1, v, st)) return rc;
     if (int rc = adapter_wide<T>(s, s.n, s.k, dy, w, s.k, 1, v, a, s.k, 1, dx, st)) return rc;
     OuterArgs o = {};
     o.group_ptr = s.group_ptr;
@@ -262,20 +478,18 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
     return launch_plain_outer<T, float, T>(o, dy, u, db, st);
 }
 
-int64_t adapters_bytes(int n_rows, int rank, bool backward) { return (int64_t)n_rows * rank * 4 * (backward ? 2 : 1) + 256; }
-
-int check_adapters(const char *who, const AdapterShape &s, int dtype, const void *workspace, int64_t bytes, bool backward) {
+int check_adapters(const char *who, const AdapterShape &s, const void *workspace, int64_t bytes, bool backward) {
     if (s.n_rows < 0 || s.k < 1 || s.n < 1 || s.n_adapters < 1 || s.rank < 1)
         return fail(MPS_ERR_ARG, "%s: %d rows, k = %d, n = %d, %d adapters of rank %d", who, s.n_rows, s.k, s.n, s.n_adapters, s.rank);
-    if (!known(dtype)) return fail(MPS_ERR_ARG, "%s: unknown dtype %d", who, dtype);
+    if (!known(s.dtype)) return fail(MPS_ERR_ARG, "%s: unknown dtype %d", who, s.dtype);
     if (s.n_adapters > mps::kMaxRowGroups) return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d adapters", who, mps::kMaxRowGroups);
     if (s.k > 1 << 21 || s.n > 1 << 21 || s.rank > 1 << 12) return fail(MPS_ERR_UNSUPPORTED, "%s: k and n may be up to %d, the rank up to %d", who, 1 << 21, 1 << 12);
+    if (s.n_rows >= 1 << 30) return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d rows", who, (1 << 30) - 1);
     if (!s.group_ptr || (s.n_rows > 0 && (!s.ids || !s.slot_row))) return fail(MPS_ERR_ARG, "%s: NULL pointer", who);
     if (misaligned(s.ids, 4) || misaligned(s.group_ptr, 4) || misaligned(s.slot_row, 4) || misaligned(s.scale, 4))
         return fail(MPS_ERR_ALIGN, "%s: a pointer is not aligned to its element size", who);
     if (s.n_rows > 0) {
-        const int64_t need = mps_adapters_workspace(s.n_rows, s.k, s.n, s.n_adapters, s.rank, dtype, backward);
-        if (need < 0) return (int)need;
+        const int64_t need = AdapterSpace(nullptr, s.n_rows, s.n_adapters, s.rank, backward).bytes;
         if (!workspace || bytes < need) return fail(MPS_ERR_ARG, "%s: the workspace needs %lld bytes, %lld given", who, (long long)need, (long long)bytes);
         if (misaligned(workspace, 256)) return fail(MPS_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", who);
     }
@@ -301,18 +515,35 @@ extern "C" int mps_routed_product(int32_t n_slots, int32_t n_rows, int32_t n_gro
     const size_t size = size_of(dtype);
     if (misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_x, size) || misaligned(d_w, size) || misaligned(d_y, size))
         return fail(MPS_ERR_ALIGN, "mps_routed_product: a pointer is not aligned to its element size");
+    const int summed = transpose ? n : k, features = transpose ? k : n;
+    if (n_rows > 0 && tc_widths(dtype, {k, summed}, {d_x, d_w})) {
+        TcRows a = {};
+        a.bf16 = dtype == MPS_BF16;
+        a.mn_major = transpose != 0;
+        a.group_ptr = d_group_ptr;
+        a.slot_row = d_slot_row;
+        a.n_groups = n_groups;
+        a.n_slots = n_slots;
+        a.n_x_rows = n_rows;
+        a.k = summed;
+        a.n = features;
+        a.gather = d_slot_row != nullptr;
+        a.out = d_y;
+        if (int rc = tc_matrix(&a.w, &a, d_w, summed, features, n_groups)) return rc;
+        return tc_rows(a, d_x, n_rows, (cudaStream_t)stream);
+    }
     RowsArgs a = {};
     a.group_ptr = d_group_ptr;
     a.slot_row = d_slot_row;
     a.n_groups = n_groups;
     a.n_slots = n_slots;
     a.n_x_rows = n_rows;
-    a.k = transpose ? n : k;
-    a.n = transpose ? k : n;
+    a.k = summed;
+    a.n = features;
     a.w_group = (long long)k * n;
     a.w_k = transpose ? k : 1;
     a.w_n = transpose ? 1 : k;
-    RD_BY_TYPE(dtype, product<T>(a, d_x, d_w, d_y, (cudaStream_t)stream));
+    RD_BY_TYPE(dtype, (launch_plain_rows<T, T, false>(a, d_x, d_w, nullptr, d_y, (cudaStream_t)stream)));
 }
 
 extern "C" int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_groups, int32_t k, int32_t n, int dtype, const int32_t *d_group_ptr,
@@ -323,6 +554,22 @@ extern "C" int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_group
     const size_t size = size_of(dtype);
     if (misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_x, size) || misaligned(d_dy, size) || misaligned(d_dw, size))
         return fail(MPS_ERR_ALIGN, "mps_routed_wgrad: a pointer is not aligned to its element size");
+    if (n_slots > 0 && n_rows > 0 && tc_widths(dtype, {k, n}, {d_x, d_dy})) {
+        TcOuter a = {};
+        a.bf16 = dtype == MPS_BF16;
+        a.group_ptr = d_group_ptr;
+        a.slot_row = d_slot_row;
+        a.n_groups = n_groups;
+        a.n_slots = n_slots;
+        a.n_p_rows = n_rows;
+        a.i = k;
+        a.j = n;
+        a.out = d_dw;
+        a.out_group = (long long)k * n;
+        a.out_f = 1;
+        a.out_c = k;
+        return tc_outer(a, d_x, d_dy, (cudaStream_t)stream);
+    }
     OuterArgs a = {};
     a.group_ptr = d_group_ptr;
     a.slot_row = d_slot_row;
@@ -332,7 +579,7 @@ extern "C" int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_group
     a.i = n;
     a.j = k;
     a.q_by_row = true;
-    RD_BY_TYPE(dtype, wgrad<T>(a, d_dy, d_x, d_dw, (cudaStream_t)stream));
+    RD_BY_TYPE(dtype, (launch_plain_outer<T, T, T>(a, d_dy, d_x, d_dw, (cudaStream_t)stream)));
 }
 
 static int check_combine(const char *who, int n_rows, int per_row, int n_slots, int dim, int dtype) {
@@ -368,14 +615,14 @@ extern "C" int mps_routed_combine_backward(int32_t n_rows, int32_t per_row, int3
 extern "C" int64_t mps_adapters_workspace(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, int backward) {
     if (n_rows < 0 || k < 1 || n < 1 || n_adapters < 1 || rank < 1 || !known(dtype))
         return fail(MPS_ERR_ARG, "mps_adapters_workspace: %d rows, k = %d, n = %d, %d adapters of rank %d, dtype %d", n_rows, k, n, n_adapters, rank, dtype);
-    return adapters_bytes(n_rows, rank, backward != 0);
+    return AdapterSpace(nullptr, n_rows, n_adapters, rank, backward != 0).bytes;
 }
 
 extern "C" int mps_adapters(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, const int32_t *d_ids,
                             const int32_t *d_group_ptr, const int32_t *d_slot_row, const float *d_scale, const void *d_x, const void *d_w,
                             const void *d_a, const void *d_b, void *d_y, void *d_workspace, int64_t workspace_bytes, void *stream) {
-    const AdapterShape s = {n_rows, k, n, n_adapters, rank, d_ids, d_group_ptr, d_slot_row, d_scale};
-    if (int rc = check_adapters("mps_adapters", s, dtype, d_workspace, workspace_bytes, false)) return rc;
+    const AdapterShape s = {n_rows, k, n, n_adapters, rank, dtype, d_ids, d_group_ptr, d_slot_row, d_scale};
+    if (int rc = check_adapters("mps_adapters", s, d_workspace, workspace_bytes, false)) return rc;
     if (n_rows == 0) return MPS_OK;
     if (!d_x || !d_w || !d_a || !d_b || !d_y) return fail(MPS_ERR_ARG, "mps_adapters: NULL pointer");
     const size_t size = size_of(dtype);
@@ -388,8 +635,8 @@ extern "C" int mps_adapters_backward(int32_t n_rows, int32_t k, int32_t n, int32
                                      const int32_t *d_group_ptr, const int32_t *d_slot_row, const float *d_scale, const void *d_dy, const void *d_x,
                                      const void *d_w, const void *d_a, const void *d_b, void *d_dx, void *d_da, void *d_db, void *d_workspace,
                                      int64_t workspace_bytes, void *stream) {
-    const AdapterShape s = {n_rows, k, n, n_adapters, rank, d_ids, d_group_ptr, d_slot_row, d_scale};
-    if (int rc = check_adapters("mps_adapters_backward", s, dtype, d_workspace, workspace_bytes, true)) return rc;
+    const AdapterShape s = {n_rows, k, n, n_adapters, rank, dtype, d_ids, d_group_ptr, d_slot_row, d_scale};
+    if (int rc = check_adapters("mps_adapters_backward", s, d_workspace, workspace_bytes, true)) return rc;
     if (!d_w || !d_a || !d_b || !d_da || !d_db || (n_rows > 0 && (!d_dy || !d_x || !d_dx))) return fail(MPS_ERR_ARG, "mps_adapters_backward: NULL pointer");
     const size_t size = size_of(dtype);
     if (misaligned(d_dy, size) || misaligned(d_x, size) || misaligned(d_w, size) || misaligned(d_a, size) || misaligned(d_b, size) ||
