@@ -1,11 +1,12 @@
 // Products of routed rows on the tensor cores (tcgen05), 16-bit types.
 //
 // tc_rows_kernel: out[slot, f] = sum_i W[g(slot)][f, i] x[row(slot), i].  The matrix is the first operand, so its result rows
-// fill the 128 lanes of TMEM whatever the number of routed rows is; the slots are the columns, NT of them per tile (16 where a
-// few rows meet each matrix and its bytes are what counts, 256 where the arithmetic does).  Both operands come by TMA in
-// 64-deep slices through a ring of stages, the gathered rows by row number (four per instruction), straight into the swizzled
-// layout the tensor cores read; rows behind a group's end are named out of range and arrive as zeros.  Two accumulators in
-// TMEM alternate, so a tile is stored while the next one is summed.
+// fill the 128 lanes of TMEM whatever the number of routed rows is; the slots are the columns, NT of them per tile (32 where a
+// few rows meet each matrix and its bytes are what counts, 256 where the arithmetic does).  The matrices come by TMA in 64-deep
+// slices through a ring of stages, rows in slot order too; gathered rows are fetched by four warps with 16-byte asynchronous
+// copies into the same swizzled layout (TMA loads by row number took 67 cycles for four rows, four times what the tensor cores
+// leave).  Two accumulators in TMEM alternate, so a tile is stored while the next one is summed; results go through shared
+// memory, where 32 slots by 128 features become whole 256-byte rows.
 //
 // A tile's sum may go on with a second product (`rank` > 0): the group's low-rank matrix times rows u that were computed before,
 // kept as hi + lo pairs of the 16-bit type (two planes), so that the intermediate's rounding (2^-16 in bf16, 2^-22 in fp16)
@@ -19,10 +20,13 @@
 
 namespace mps {
 
-constexpr int kTcThreads = 256;  // warps: 0 matrix loads, 1 products, 2 row loads, 3 idle, 4-7 results
+constexpr int kTcThreads = 384;  // warps: 0 TMA, 1 products, 2-3 idle, 4-7 results (TMEM lanes go by warp number mod 4), 8-11 row copies
 constexpr int kTcFeatures = 128;
 constexpr int kTcDepth = 64;
-constexpr int kTcRing = 192 * 1024;  // shared memory of the stages
+constexpr int kTcRing = 192 * 1024;            // shared memory of the stages
+constexpr int kOutPitch = kTcFeatures * 2 + 16;  // a result row in shared memory; the pad spreads 16-byte reads over the banks
+constexpr int kOutBytes = 2 * 32 * kOutPitch;    // two chunks of 32 rows
+constexpr int kOutTotal = (kOutBytes + 1023) / 1024 * 1024;
 
 struct TcRows {
     CUtensorMap w, x, w2, u;  // matrices {i, f, group} or {f, i, group}; rows {i, row}; the low-rank pair's matrix and rows
@@ -30,6 +34,7 @@ struct TcRows {
     const int *slot_row;      // row behind a slot; NULL: the slot itself
     int n_groups, n_slots, n_x_rows;
     int k, n;                 // summed index, result features
+    const uint16_t *rows;     // gathered rows: x itself
     int rank, rank_groups;    // depth of the second product; groups that have one (the first rank_groups)
     const void *u_base;       // rows of the second product (host side)
     int u_plane;              // rows between the hi and the lo plane of u
@@ -43,27 +48,45 @@ struct TcRows {
 };
 
 struct TcPipe {
-    uint64_t full[16], empty[16], tmem_full[2], tmem_empty[2];
+    uint64_t full[12], empty[12], tmem_full[2], tmem_empty[2];
     uint32_t tmem;
     int gave_up;
 };
 
+__device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, int full_count) {
+    for (int i = 0; i < stages; ++i) {
+        mbar_init(smem_addr(&pipe.full[i]), full_count);
+        mbar_init(smem_addr(&pipe.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_addr(&pipe.tmem_full[i]), 1);
+        mbar_init(smem_addr(&pipe.tmem_empty[i]), 128);
+    }
+    pipe.gave_up = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+
+constexpr int stages_for(int bytes, int stage) { return bytes / stage < 12 ? bytes / stage : 12; }
+
 template <int NT>
 struct TcShape {
-    static constexpr uint32_t kStage = kTcFeatures * 128 + NT * 128;
-    static constexpr int kStages = kTcRing / kStage < 12 ? kTcRing / kStage : 12;
-    static constexpr uint32_t kColumns = 2 * NT < 32 ? 32 : 2 * NT;
-    static constexpr uint32_t kReduce = NT <= 64 ? NT * kTcFeatures * 4 : 0;  // only small tiles are split
-    static constexpr int kSplitStages = (kTcRing - (int)kReduce) / kStage < 12 ? (kTcRing - (int)kReduce) / kStage : 12;
-    static size_t bytes(int n_groups) { return 1024 + kTcRing + (size_t)(3 * n_groups + 1) * sizeof(int); }
+    static constexpr int kStage = kTcFeatures * 128 + NT * 128;
+    static constexpr int kStages = stages_for(kTcRing, kStage);
+    static constexpr int kColumns = 2 * NT;
+    static constexpr int kReduce = NT <= 64 ? NT * kTcFeatures * 4 : 0;  // only small tiles are split
+    static constexpr int kSplitStages = stages_for(kTcRing - kReduce, kStage);
+    static constexpr int kLag = NT > 128 ? 2 : 3;  // slices of row copies in flight
+    static size_t bytes(int n_groups) { return 1024 + kTcRing + kOutTotal + (size_t)(3 * n_groups + 1) * sizeof(int); }
 };
 
 // A cursor over the tiles of all groups: tile numbers only rise, so the group is found by walking on.
 struct TcCursor {
     const int *first, *lo, *hi;  // first tile of every group (n_groups + 1), its slots
-    int group = 0;
-    __device__ __forceinline__ void seek(int tile) {
+    int group, slot0, slot1;
+    __device__ __forceinline__ void seek(int tile, int nt) {
         while (tile >= first[group + 1]) ++group;
+        slot0 = lo[group] + (tile - first[group]) * nt;
+        slot1 = min(slot0 + nt, hi[group]);
     }
 };
 
@@ -74,8 +97,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     __shared__ TcPipe pipe;
     __shared__ int s_sum[kTcThreads / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t ring = (smem_addr(s_raw) + 1023) & ~1023u;
-    int *first = reinterpret_cast<int *>(s_raw + (ring - smem_addr(s_raw)) + kTcRing);
+    const uint32_t ring = (smem_addr(s_raw) + 1023) & ~1023u, staging = ring + kTcRing;
+    int *first = reinterpret_cast<int *>(s_raw + (ring - smem_addr(s_raw)) + kTcRing + kOutTotal);
     int *lo = first + a.n_groups + 1, *hi = lo + a.n_groups;
     const int split = a.split, part = split > 1 ? (int)cluster_rank() : 0;
     const int stages = split > 1 ? S::kSplitStages : S::kStages;
@@ -105,18 +128,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (lane >= d) scan += o;
         }
         if (lane == 31) s_sum[warp] = scan;
-        if (tid == 0) {
-            for (int i = 0; i < stages; ++i) {
-                mbar_init(smem_addr(&pipe.full[i]), 1);
-                mbar_init(smem_addr(&pipe.empty[i]), 1);
-            }
-            for (int i = 0; i < 2; ++i) {
-                mbar_init(smem_addr(&pipe.tmem_full[i]), 1);
-                mbar_init(smem_addr(&pipe.tmem_empty[i]), 128);
-            }
-            pipe.gave_up = 0;
-            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        }
+        if (tid == 0) pipe_init(pipe, stages, a.gather ? 1 + 128 : 1);
         if (warp == 1) tmem_alloc(smem_addr(&pipe.tmem), S::kColumns);
         __syncthreads();
         for (int w = 0; w < warp; ++w) scan += s_sum[w];
@@ -138,7 +150,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     const int rank_steps = 2 * ((a.rank + kTcDepth - 1) / kTcDepth);
     const long long n_tiles = (long long)first[a.n_groups] * feature_tiles;
     const long long worker = blockIdx.x / split, workers = gridDim.x / split;
-    TcCursor cur = {first, lo, hi};
+    TcCursor cur = {first, lo, hi, 0, 0, 0};
 
     // steps of this block for a tile of group g
     auto range = [&](int g, int &s0, int &s1) {
@@ -147,12 +159,41 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
         s1 = (int)((long long)total * (part + 1) / split);
     };
 
-    int it = 0;        // stages used so far, this warp's count
-    int turn = 0;      // tiles done so far
+    // row copies: a thread owns 16 bytes of every 16th row of a slice
+    constexpr int RPT = NT / 16;
+    const int chunk = tid & 7, row0 = (tid - 256) >> 3;
+    int row[RPT], next_row[RPT];
+    TcCursor ahead = cur;
+    auto fetch_rows = [&](long long tile) {
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) next_row[i] = -1;
+        if (tile >= n_tiles) return;
+        ahead.seek((int)(tile / feature_tiles), NT);
+#pragma unroll
+        for (int i = 0; i < RPT; ++i) {
+            const int slot = ahead.slot0 + row0 + 16 * i;
+            if (slot < ahead.slot1) {
+                next_row[i] = a.slot_row[slot];
+                if ((unsigned)next_row[i] >= (unsigned)a.n_x_rows) {
+                    atomicOr(a.status, kStatusBadIndex);
+                    next_row[i] = -1;
+                }
+            }
+        }
+    };
+    const bool copies = warp >= 8 && a.gather;
+    if (copies) fetch_rows(worker);
+    int it = 0, told = 0;  // stages used by this warp; of those, copies reported as landed
+    auto report = [&](int until) {
+        fence_async();
+        for (; told < until; ++told) mbar_arrive(smem_addr(&pipe.full[told % stages]));
+    };
+
+    int turn = 0;  // tiles done so far
     for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
         const int tt = (int)(tile / feature_tiles), f0 = (int)(tile - (long long)tt * feature_tiles) * kTcFeatures;
-        cur.seek(tt);
-        const int g = cur.group, slot0 = lo[g] + (tt - first[g]) * NT, slot1 = min(slot0 + NT, hi[g]);
+        cur.seek(tt, NT);
+        const int g = cur.group, slot0 = cur.slot0, slot1 = cur.slot1;
         int s0, s1;
         range(g, s0, s1);
         const int buf = turn & 1;
@@ -160,27 +201,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (lane == 0) {
                 const int z = a.w_shared ? 0 : g;
                 const int halves = a.n - f0 > 64 ? 2 : 1;  // MN-major: boxes of 64 features
-                const uint32_t bytes = (a.mn_major ? halves * kBlock64 : a.w_rows * 128u) + NT * 128u;
+                const uint32_t w_bytes = a.mn_major ? halves * kBlock64 : a.w_rows * 128u;
                 for (int s = s0; s < s1; ++s, ++it) {
                     const int st = it % stages;
                     mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
                     const uint32_t bar = smem_addr(&pipe.full[st]), dst = ring + st * S::kStage;
-                    const bool second = s >= main_steps;
+                    const bool second = s >= main_steps, rows = second || !a.gather;
                     const int e = s - main_steps, i0 = (second ? e >> 1 : s) * kTcDepth;
-                    mbar_expect(bar, bytes);
+                    mbar_expect(bar, w_bytes + (rows ? NT * 128u : 0u));
                     const CUtensorMap *m = second ? &a.w2 : &a.w;
                     if (a.mn_major)
                         for (int h = 0; h < halves; ++h) tma_3d(dst + h * kBlock64, m, f0 + h * 64, i0, second ? g : z, bar);
                     else tma_3d(dst, m, i0, f0, second ? g : z, bar);
                     if (second) tma_2d(dst + kTcFeatures * 128, &a.u, i0, (e & 1) * a.u_plane + slot0, bar);
-                    else if (!a.gather) tma_2d(dst + kTcFeatures * 128, &a.x, i0, slot0, bar);
+                    else if (rows) tma_2d(dst + kTcFeatures * 128, &a.x, i0, slot0, bar);
                 }
             }
         } else if (warp == 1) {
             if (lane == 0) {
                 mbar_wait(smem_addr(&pipe.tmem_empty[buf]), ((turn >> 1) & 1) ^ 1, gave_up, a.status);
                 tc_fence_after();
-                const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, a.mn_major, false, NT);
+                // only as many columns as there are slots: the last tile of a group costs what it holds
+                const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, a.mn_major, false, (slot1 - slot0 + 15) & ~15);
                 const uint64_t a_step = operand_step(a.mn_major), b_step = operand_step(false);
                 for (int s = s0; s < s1; ++s, ++it) {
                     const int st = it % stages;
@@ -195,69 +237,75 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 }
                 tc_commit(smem_addr(&pipe.tmem_full[buf]));
             }
-        } else if (warp == 2) {
-            if (a.gather) {
-                constexpr int SETS = (NT / 4 + 31) / 32;
-                int r[SETS][4];
+        } else if (copies) {
 #pragma unroll
-                for (int q = 0; q < SETS; ++q)
+            for (int i = 0; i < RPT; ++i) row[i] = next_row[i];
+            fetch_rows(tile + workers);  // under way while this tile is copied
+            for (int s = s0; s < s1; ++s, ++it) {
+                const int st = it % stages;
+                mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
+                const int col = s * kTcDepth + chunk * 8;
+                if (s < main_steps) {
+                    const uint32_t dst = ring + st * S::kStage + kTcFeatures * 128 + swizzled(row0, chunk);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int slot = slot0 + (lane + 32 * q) * 4 + i;
-                        r[q][i] = a.n_x_rows;  // out of range: zeros
-                        if (slot < slot1) {
-                            const int row = a.slot_row[slot];
-                            if ((unsigned)row < (unsigned)a.n_x_rows) r[q][i] = row;
-                            else atomicOr(a.status, kStatusBadIndex);
-                        }
+                    for (int i = 0; i < RPT; ++i) {
+                        const bool valid = row[i] >= 0 && col < a.k;
+                        copy_16(dst + i * 2048, valid ? a.rows + (long long)row[i] * a.k + col : a.rows, valid);
                     }
-                for (int s = s0; s < s1; ++s, ++it) {
-                    const int st = it % stages;
-                    // every use of a stage is waited for, also where nothing is loaded: a parity tells neighbouring uses apart only
-                    mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
-                    __syncwarp();  // nor may a lane without rows fall behind the others
-                    if (s >= main_steps) continue;
-                    const uint32_t dst = ring + st * S::kStage + kTcFeatures * 128;
-#pragma unroll
-                    for (int q = 0; q < SETS; ++q)
-                        if (lane + 32 * q < NT / 4) tma_rows(dst + (lane + 32 * q) * 512, &a.x, s * kTcDepth, r[q], smem_addr(&pipe.full[st]));
                 }
-                __syncwarp();
+                copy_commit();
+                copy_wait<S::kLag>();
+                report(it + 1 - S::kLag);
             }
-        } else if (warp >= 4) {
+            if (split > 1) {  // the cluster meets at the end of the tile: nothing may be left unreported
+                copy_wait<0>();
+                report(it);
+            }
+        } else if (warp >= 4 && warp < 8) {
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
             tc_fence_after();
-            const int quad = warp & 3, f = f0 + quad * 32 + lane;
+            const int quad = warp & 3, f = f0 + quad * 32 + lane, mine = tid - 128;
             const float scale = a.group_scale ? a.group_scale[g] : 1.0f;
             uint16_t *out = (uint16_t *)a.out;
-            auto store = [&](int slot, int row, float v) {
-                if (f >= a.n) return;
-                v *= scale;
-                const long long at = (long long)(a.scatter ? row : slot) * a.n + f;
+            auto out_row = [&](int slot) {  // where a slot's result goes, or -1
+                if (!a.scatter) return slot;
+                const int r = a.slot_row[slot];
+                return (unsigned)r < (unsigned)a.n_x_rows ? r : -1;
+            };
+            auto store = [&](int r, float v) {
+                if (f >= a.n || r < 0) return;
+                const long long at = (long long)r * a.n + f;
                 const uint16_t h = to_16(v, a.bf16);
                 out[at] = h;
                 if (a.pair) out[at + a.out_plane] = to_16(v - from_16(h, a.bf16), a.bf16);
             };
+            const bool wide = !a.pair && a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
 #pragma unroll 1
-            for (int c0 = 0; c0 < NT; c0 += 16) {
-                if (slot0 + c0 >= slot1) break;
-                float v[16];
+            for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 32) {
+                float v[32];
                 tmem_load(tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + c0, v);
                 if (split > 1) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
+                    for (int j = 0; j < 32; ++j)
                         asm volatile("st.shared.f32 [%0], %1;" ::"r"(partial + ((c0 + j) * kTcFeatures + quad * 32 + lane) * 4), "f"(v[j]) : "memory");
-                    continue;
-                }
-                int rows = 0;
-                if (a.scatter && slot0 + c0 + (lane & 15) < slot1) {
-                    rows = a.slot_row[slot0 + c0 + (lane & 15)];
-                    if ((unsigned)rows >= (unsigned)a.n_x_rows) rows = -1;
-                }
+                } else if (wide) {
+                    const uint32_t at = staging + (c0 >> 5 & 1) * (32 * kOutPitch);
 #pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    const int row = __shfl_sync(0xffffffffu, rows, j);
-                    if (slot0 + c0 + j < slot1 && row >= 0) store(slot0 + c0 + j, row, v[j]);
+                    for (int j = 0; j < 32; ++j) store_shared_16(at + j * kOutPitch + (quad * 32 + lane) * 2, to_16(v[j] * scale, a.bf16));
+                    results_sync();  // one per chunk is enough: the other buffer's readers have passed it too
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int c = (mine >> 4) + 8 * j, fc = (mine & 15) * 8;
+                        const uint4 q = load_shared_128(at + c * kOutPitch + fc * 2);
+                        if (slot0 + c0 + c < slot1 && f0 + fc < a.n) {
+                            const int r = out_row(slot0 + c0 + c);
+                            if (r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = q;
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j)
+                        if (slot0 + c0 + j < slot1) store(out_row(slot0 + c0 + j), v[j] * scale);
                 }
             }
             tc_fence_before();
@@ -268,21 +316,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 for (int c = part; slot0 + c < slot1; c += split) {
                     float v = 0.0f;
                     for (int p = 0; p < split; ++p) v += load_peer(partial + (c * kTcFeatures + quad * 32 + lane) * 4, p);
-                    int row = 0;
-                    if (a.scatter) {
-                        row = a.slot_row[slot0 + c];
-                        if ((unsigned)row >= (unsigned)a.n_x_rows) row = -1;
-                    }
-                    if (row >= 0) store(slot0 + c, row, v);
+                    store(out_row(slot0 + c), v * scale);
                 }
                 cluster_sync();  // the partial results may be overwritten, and no block leaves while one still reads its own
-            }
+            } else if (wide) results_sync();  // the next tile starts with the first buffer again
         }
-        if (split > 1 && warp < 4) {
+        if (split > 1 && (warp < 4 || warp >= 8)) {
             __syncwarp();
             cluster_sync();
             cluster_sync();
         }
+    }
+    if (copies) {
+        copy_wait<0>();
+        report(it);
     }
     if (*gave_up) __nanosleep(1000000);  // copies in flight land before the block's memory is given back
     tc_fence_before();
@@ -295,16 +342,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
 
 // tc_outer_kernel: out[g][f, c] = sum over the slots s of group g of P[.., f] Q[s, c] - the gradient by a group's matrix.  The
 // summed index is the slot, so both operands lie across it (MN-major): a stage holds 64 slots of 128 features of P and of up
-// to NT columns of Q in blocks of 64.  Whole slices of rows in slot order come as one box per block, gathered rows and the
-// last slice of a group by row number, with the rows behind the group's end named out of range: zeros, whatever lies there.
+// to NT columns of Q in blocks of 64.  Whole slices of rows in slot order come by TMA, a box per block; gathered rows and the
+// last slice of a group by the copying warps, which put zeros behind the group's end, whatever lies there.
 // With `pair` a block of columns of Q is a hi and a lo plane, added up when the result is stored.
 struct TcOuter {
-    CUtensorMap p_rows, p_tile, q_rows, q_tile;  // boxes of one row / of 64
-    const int *group_ptr, *slot_row;             // slot_row: rows of P (NULL: in slot order)
+    CUtensorMap p, q;
+    const uint16_t *p_base, *q_base;
+    const int *group_ptr, *slot_row;  // slot_row: rows of P (NULL: in slot order)
     int n_groups, n_slots, n_p_rows;
-    int i, j;                                    // features of P, columns of Q
-    int q_plane, q_rows_all;                     // rows between the planes of Q; rows of the tensor
-    bool bf16, pair;
+    int i, j;                         // features of P, columns of Q
+    bool bf16, pair;                  // pair: Q is two planes of n_slots rows
     void *out;
     long long out_group, out_f, out_c;
     int split;
@@ -313,11 +360,12 @@ struct TcOuter {
 
 template <int NT>
 struct TcOuterShape {
-    static constexpr uint32_t kStage = 2 * kBlock64 + NT / 64 * kBlock64;
-    static constexpr int kStages = kTcRing / kStage;
-    static constexpr uint32_t kReduce = NT <= 128 ? NT * kTcFeatures * 4 : 0;
-    static constexpr int kSplitStages = (kTcRing - (int)kReduce) / kStage;
-    static constexpr size_t kBytes = 1024 + kTcRing;
+    static constexpr int kStage = 2 * kBlock64 + NT / 64 * kBlock64;
+    static constexpr int kStages = stages_for(kTcRing, kStage);
+    static constexpr int kReduce = NT <= 128 ? NT * kTcFeatures * 4 : 0;
+    static constexpr int kSplitStages = stages_for(kTcRing - kReduce, kStage);
+    static constexpr int kLag = 2;
+    static constexpr size_t kBytes = 1024 + kTcRing + kOutTotal;
 };
 
 template <int NT>
@@ -326,34 +374,27 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     extern __shared__ uint8_t s_raw[];
     __shared__ TcPipe pipe;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t ring = (smem_addr(s_raw) + 1023) & ~1023u;
+    const uint32_t ring = (smem_addr(s_raw) + 1023) & ~1023u, staging = ring + kTcRing;
     const int split = a.split, part = split > 1 ? (int)cluster_rank() : 0;
     const int stages = split > 1 ? S::kSplitStages : S::kStages;
     const uint32_t partial = ring + (uint32_t)S::kSplitStages * S::kStage;
-    if (tid == 0) {
-        for (int i = 0; i < stages; ++i) {
-            mbar_init(smem_addr(&pipe.full[i]), 1);
-            mbar_init(smem_addr(&pipe.empty[i]), 1);
-        }
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_addr(&pipe.tmem_full[i]), 1);
-            mbar_init(smem_addr(&pipe.tmem_empty[i]), 128);
-        }
-        pipe.gave_up = 0;
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
+    if (tid == 0) pipe_init(pipe, stages, 1 + 128);
     if (warp == 1) tmem_alloc(smem_addr(&pipe.tmem), 2 * NT);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = pipe.tmem;
     volatile int *gave_up = &pipe.gave_up;
-    constexpr int COLS = NT;
-    const int cols = a.pair ? COLS / 2 : COLS;  // result columns per tile
+    const int cols = a.pair ? NT / 2 : NT;  // result columns per tile
     const int i_tiles = (a.i + kTcFeatures - 1) / kTcFeatures, j_tiles = (a.j + cols - 1) / cols;
     const long long n_tiles = (long long)a.n_groups * i_tiles * j_tiles;
     const long long worker = blockIdx.x / split, workers = gridDim.x / split;
-    int it = 0, turn = 0;
+    const bool gather = a.slot_row != nullptr;
+    int it = 0, told = 0, turn = 0;
+    auto report = [&](int until) {
+        fence_async();
+        for (; told < until; ++told) mbar_arrive(smem_addr(&pipe.full[told % stages]));
+    };
     for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
         const int g = (int)(tile / ((long long)i_tiles * j_tiles)), rest = (int)(tile - (long long)g * i_tiles * j_tiles);
         const int f0 = rest / j_tiles * kTcFeatures, c0 = rest % j_tiles * cols;
@@ -368,12 +409,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     const int st = it % stages, slot = slots.x + s * kTcDepth;
                     mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
                     const uint32_t bar = smem_addr(&pipe.full[st]), dst = ring + st * S::kStage;
-                    mbar_expect(bar, (p_blocks + q_blocks) * kBlock64);
-                    if (slot + kTcDepth > slots.y) continue;  // a part of a slice: by row number
-                    if (!a.slot_row)
-                        for (int b = 0; b < p_blocks; ++b) tma_2d(dst + b * kBlock64, &a.p_tile, f0 + b * 64, slot, bar);
+                    if (slot + kTcDepth > slots.y) {
+                        mbar_arrive(bar);
+                        continue;
+                    }
+                    mbar_expect(bar, ((gather ? 0 : p_blocks) + q_blocks) * kBlock64);
+                    if (!gather)
+                        for (int b = 0; b < p_blocks; ++b) tma_2d(dst + b * kBlock64, &a.p, f0 + b * 64, slot, bar);
                     for (int b = 0; b < q_blocks; ++b)
-                        tma_2d(dst + (2 + b) * kBlock64, &a.q_tile, a.pair ? c0 : c0 + b * 64, a.pair ? b * a.q_plane + slot : slot, bar);
+                        tma_2d(dst + (2 + b) * kBlock64, &a.q, a.pair ? c0 : c0 + b * 64, a.pair ? b * a.n_slots + slot : slot, bar);
                 }
             }
         } else if (warp == 1) {
@@ -394,78 +438,106 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
                 tc_commit(smem_addr(&pipe.tmem_full[buf]));
             }
-        } else if (warp == 2) {
-            const int q = lane & 15, half = lane >> 4;  // four slots of a slice; every other block
+        } else if (warp >= 8) {
+            // a thread owns 16 bytes of every 16th slot of a block
+            const int chunk = tid & 7, row0 = (tid - 256) >> 3;
             int next[4];
             auto fetch = [&](int s) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int slot = slots.x + s * kTcDepth + q * 4 + i;
-                    next[i] = a.n_p_rows;
+                    const int slot = slots.x + s * kTcDepth + row0 + 16 * i;
+                    next[i] = -1;
                     if (s < s1 && slot < slots.y) {
-                        const int row = a.slot_row ? a.slot_row[slot] : slot;
-                        if ((unsigned)row < (unsigned)a.n_p_rows) next[i] = row;
-                        else atomicOr(a.status, kStatusBadIndex);
+                        next[i] = gather ? a.slot_row[slot] : slot;
+                        if ((unsigned)next[i] >= (unsigned)a.n_p_rows) {
+                            atomicOr(a.status, kStatusBadIndex);
+                            next[i] = -1;
+                        }
                     }
                 }
             };
             fetch(s0);
             for (int s = s0; s < s1; ++s, ++it) {
-                int r[4];
+                int row[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) r[i] = next[i];
+                for (int i = 0; i < 4; ++i) row[i] = next[i];
+                fetch(s + 1);  // under way while this slice is copied
                 const int st = it % stages, slot = slots.x + s * kTcDepth;
-                const bool part_slice = slot + kTcDepth > slots.y;
-                if (a.slot_row) fetch(s + 1);
-                else {  // the last slice of rows in slot order
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) r[i] = slot + q * 4 + i < slots.y ? slot + q * 4 + i : a.n_p_rows;
-                }
-                // every use of a stage is waited for, also where nothing is loaded: a parity tells neighbouring uses apart only
+                const bool last = slot + kTcDepth > slots.y;
                 mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
-                __syncwarp();  // nor may a lane without rows fall behind the others
-                if (!a.slot_row && !part_slice) continue;
-                const uint32_t bar = smem_addr(&pipe.full[st]), dst = ring + st * S::kStage + q * 512;
-                if (half < p_blocks) tma_rows(dst + half * kBlock64, &a.p_rows, f0 + half * 64, r, bar);
-                if (part_slice) {
-                    for (int b = half; b < q_blocks; b += 2) {
-                        int rq[4];
+                const uint32_t dst = ring + st * S::kStage + swizzled(row0, chunk);
+                if (gather || last)
+                    for (int b = 0; b < p_blocks; ++b) {
+                        const int f = f0 + b * 64 + chunk * 8;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const int at = slot + q * 4 + i;
-                            rq[i] = at < slots.y ? (a.pair ? b * a.q_plane : 0) + at : a.q_rows_all;
+                            const bool valid = row[i] >= 0 && f < a.i;
+                            copy_16(dst + b * kBlock64 + i * 2048, valid ? a.p_base + (long long)row[i] * a.i + f : a.p_base, valid);
                         }
-                        tma_rows(dst + (2 + b) * kBlock64, &a.q_rows, a.pair ? c0 : c0 + b * 64, rq, bar);
                     }
+                if (last)
+                    for (int b = 0; b < q_blocks; ++b) {
+                        const int c = (a.pair ? c0 : c0 + b * 64) + chunk * 8;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = slot + row0 + 16 * i;
+                            const bool valid = at < slots.y && c < a.j;
+                            const long long line = (a.pair ? (long long)b * a.n_slots : 0) + at;
+                            copy_16(dst + (2 + b) * kBlock64 + i * 2048, valid ? a.q_base + line * a.j + c : a.q_base, valid);
+                        }
+                    }
+                copy_commit();
+                if (gather) {
+                    copy_wait<S::kLag>();
+                    report(it + 1 - S::kLag);
+                } else {
+                    copy_wait<0>();
+                    report(it + 1);
                 }
             }
-            __syncwarp();
+            if (split > 1) {
+                copy_wait<0>();
+                report(it);
+            }
         } else if (warp >= 4) {
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
             tc_fence_after();
-            const int quad = warp & 3, f = f0 + quad * 32 + lane;
-            uint16_t *out = (uint16_t *)a.out + g * a.out_group + f * a.out_f;
+            const int quad = warp & 3, f = f0 + quad * 32 + lane, mine = tid - 128;
+            uint16_t *out = (uint16_t *)a.out + g * a.out_group;
             const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT;
             const bool none = s0 == s1;
+            const bool wide = a.out_f == 1 && a.i % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
 #pragma unroll 1
-            for (int c = 0; c < cols && c0 + c < a.j; c += 16) {
-                float v[16] = {}, w[16];
+            for (int c = 0; c < cols && c0 + c < a.j; c += 32) {
+                float v[32] = {};
                 if (!none) {
                     tmem_load(lanes + c, v);
                     if (a.pair) {
+                        float w[32];
                         tmem_load(lanes + cols + c, w);
 #pragma unroll
-                        for (int x = 0; x < 16; ++x) v[x] += w[x];
+                        for (int x = 0; x < 32; ++x) v[x] += w[x];
                     }
                 }
                 if (split > 1) {
 #pragma unroll
-                    for (int x = 0; x < 16; ++x)
+                    for (int x = 0; x < 32; ++x)
                         asm volatile("st.shared.f32 [%0], %1;" ::"r"(partial + ((c + x) * kTcFeatures + quad * 32 + lane) * 4), "f"(v[x]) : "memory");
+                } else if (wide) {
+                    const uint32_t at = staging + (c >> 5 & 1) * (32 * kOutPitch);
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) store_shared_16(at + x * kOutPitch + (quad * 32 + lane) * 2, to_16(v[x], a.bf16));
+                    results_sync();
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const int cc = (mine >> 4) + 8 * x, fc = (mine & 15) * 8;
+                        const uint4 q = load_shared_128(at + cc * kOutPitch + fc * 2);
+                        if (c0 + c + cc < a.j && f0 + fc < a.i) *reinterpret_cast<uint4 *>(out + (c0 + c + cc) * a.out_c + f0 + fc) = q;
+                    }
                 } else {
 #pragma unroll
-                    for (int x = 0; x < 16; ++x)
-                        if (f < a.i && c0 + c + x < a.j) out[(c0 + c + x) * a.out_c] = to_16(v[x], a.bf16);
+                    for (int x = 0; x < 32; ++x)
+                        if (f < a.i && c0 + c + x < a.j) out[f * a.out_f + (c0 + c + x) * a.out_c] = to_16(v[x], a.bf16);
                 }
             }
             tc_fence_before();
@@ -475,16 +547,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 for (int c = part; c < cols && c0 + c < a.j; c += split) {
                     float v = 0.0f;
                     for (int p = 0; p < split; ++p) v += load_peer(partial + (c * kTcFeatures + quad * 32 + lane) * 4, p);
-                    if (f < a.i) out[(c0 + c) * a.out_c] = to_16(v, a.bf16);
+                    if (f < a.i) out[f * a.out_f + (c0 + c) * a.out_c] = to_16(v, a.bf16);
                 }
                 cluster_sync();
-            }
+            } else if (wide) results_sync();
         }
-        if (split > 1 && warp < 4) {
+        if (split > 1 && (warp < 4 || warp >= 8)) {
             __syncwarp();
             cluster_sync();
             cluster_sync();
         }
+    }
+    if (warp >= 8) {
+        copy_wait<0>();
+        report(it);
     }
     if (*gave_up) __nanosleep(1000000);
     tc_fence_before();
