@@ -233,10 +233,12 @@ template <int NT>
 int launch_tc_rows(TcRows a, int sms, cudaStream_t st) {
     // a group ends in a part of a tile, so there are at most this many
     const long long most = a.n_slots / NT + (a.n_groups < a.n_slots ? a.n_groups : a.n_slots);
-    const long long tiles = most * ((a.n + mps::kTcFeatures - 1) / mps::kTcFeatures);
+    const int tile_f = mps::kTcFeatures * (mps::TcShape<NT>::kPaired ? 2 : 1);
+    const long long tiles = most * ((a.n + tile_f - 1) / tile_f);
     a.split = NT <= 64 ? split_of(tiles, (a.k + mps::kTcDepth - 1) / mps::kTcDepth, sms) : 1;
-    const long long workers = sms / a.split;
-    return launch_tc(mps::tc_rows_kernel<NT>, a, (tiles < workers ? tiles : workers) * a.split, a.split, mps::TcShape<NT>::bytes(a.n_groups), st);
+    const int cluster = mps::TcShape<NT>::kPaired ? 2 : a.split;
+    const long long workers = sms / cluster;
+    return launch_tc(mps::tc_rows_kernel<NT>, a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcShape<NT>::bytes(a.n_groups), st);
 }
 
 // The rest of a filled in: what every use has in common, and the tile for the mean number of rows per group.
@@ -247,11 +249,12 @@ int tc_rows(TcRows a, const void *x, long long x_rows, cudaStream_t st) {
     const int groups = a.n_groups < a.n_slots ? a.n_groups : a.n_slots;
     const long long mean = a.n_slots / groups;
     const int nt = mean <= 20 ? 32 : mean <= 48 ? 64 : mean <= 128 ? 128 : 256;
+    const int loaded = nt == 256 ? mps::TcShape<256>::kRows : nt;  // slots a block loads
     a.rows = (const uint16_t *)x;
     if (!a.gather)
-        if (int rc = tensor_map(&a.x, a.bf16, x, 2, a.k, x_rows, 1, nt)) return rc;
+        if (int rc = tensor_map(&a.x, a.bf16, x, 2, a.k, x_rows, 1, loaded)) return rc;
     if (a.rank) {
-        if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, nt)) return rc;
+        if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded)) return rc;
     }
     if (nt == 32) return launch_tc_rows<32>(a, sms, st);
     if (nt == 64) return launch_tc_rows<64>(a, sms, st);
@@ -269,11 +272,13 @@ int tc_matrix(CUtensorMap *map, TcRows *a, const void *w, int summed, int featur
 template <int NT>
 int launch_tc_outer(TcOuter a, int sms, cudaStream_t st) {
     const int cols = a.pair ? NT / 2 : NT;
-    const long long tiles = (long long)a.n_groups * ((a.i + mps::kTcFeatures - 1) / mps::kTcFeatures) * ((a.j + cols - 1) / cols);
+    const int tile_f = mps::kTcFeatures * (mps::TcOuterShape<NT>::kPaired ? 2 : 1);
+    const long long tiles = (long long)a.n_groups * ((a.i + tile_f - 1) / tile_f) * ((a.j + cols - 1) / cols);
     const int steps = (a.n_slots / a.n_groups + mps::kTcDepth - 1) / mps::kTcDepth;  // of the mean group
     a.split = NT <= 128 ? split_of(tiles, steps, sms) : 1;
-    const long long workers = sms / a.split;
-    return launch_tc(mps::tc_outer_kernel<NT>, a, (tiles < workers ? tiles : workers) * a.split, a.split, mps::TcOuterShape<NT>::kBytes, st);
+    const int cluster = mps::TcOuterShape<NT>::kPaired ? 2 : a.split;
+    const long long workers = sms / cluster;
+    return launch_tc(mps::tc_outer_kernel<NT>, a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcOuterShape<NT>::kBytes, st);
 }
 
 // P: n_p_rows rows of a.i, by a.slot_row or in slot order; Q: rows of a.j in slot order (pair: two planes of them).

@@ -12,6 +12,10 @@
 // kept as hi + lo pairs of the 16-bit type (two planes), so that the intermediate's rounding (2^-16 in bf16, 2^-22 in fp16)
 // stays below the result's.
 //
+// The widest tiles (NT = 256) belong to a pair of neighbouring blocks (cta_group::2): 256 features by 256 slots, each block
+// loading its 128 features and half of the slots, so that a block's slice is 32 KB instead of 48 and six of them are in flight.
+// Both blocks' loads arrive at the first one's barriers; it issues the products for both, and each stores the features it holds.
+//
 // Few tiles with long sums are cut along the sum over the blocks of a cluster; the partial results meet in distributed shared
 // memory, added in the order of the blocks.
 #pragma once
@@ -48,19 +52,19 @@ struct TcRows {
 };
 
 struct TcPipe {
-    uint64_t full[12], empty[12], tmem_full[2], tmem_empty[2];
+    uint64_t full[12], empty[12], tmem_full[2], tmem_empty[2];  // of a pair's full and tmem_empty the first block's count
     uint32_t tmem;
     int gave_up;
 };
 
-__device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, int full_count) {
+__device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, int full_count, bool paired) {
     for (int i = 0; i < stages; ++i) {
         mbar_init(smem_addr(&pipe.full[i]), full_count);
         mbar_init(smem_addr(&pipe.empty[i]), 1);
     }
     for (int i = 0; i < 2; ++i) {
         mbar_init(smem_addr(&pipe.tmem_full[i]), 1);
-        mbar_init(smem_addr(&pipe.tmem_empty[i]), 128);
+        mbar_init(smem_addr(&pipe.tmem_empty[i]), paired ? 256 : 128);
     }
     pipe.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -70,12 +74,14 @@ constexpr int stages_for(int bytes, int stage) { return bytes / stage < 12 ? byt
 
 template <int NT>
 struct TcShape {
-    static constexpr int kStage = kTcFeatures * 128 + NT * 128;
+    static constexpr bool kPaired = NT == 256;
+    static constexpr int kRows = kPaired ? NT / 2 : NT;  // slots a block loads
+    static constexpr int kStage = kTcFeatures * 128 + kRows * 128;
     static constexpr int kStages = stages_for(kTcRing, kStage);
     static constexpr int kColumns = 2 * NT;
     static constexpr int kReduce = NT <= 64 ? NT * kTcFeatures * 4 : 0;  // only small tiles are split
     static constexpr int kSplitStages = stages_for(kTcRing - kReduce, kStage);
-    static constexpr int kLag = NT > 128 ? 2 : 3;  // slices of row copies in flight
+    static constexpr int kLag = kPaired ? 4 : 3;  // slices of row copies in flight
     static size_t bytes(int n_groups) { return 1024 + kTcRing + kOutTotal + (size_t)(3 * n_groups + 1) * sizeof(int); }
 };
 
@@ -103,6 +109,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     const int split = a.split, part = split > 1 ? (int)cluster_rank() : 0;
     const int stages = split > 1 ? S::kSplitStages : S::kStages;
     const uint32_t partial = ring + (uint32_t)S::kSplitStages * S::kStage;  // split only
+    constexpr bool PAIRED = S::kPaired;
+    const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
 
     // ---- tiles of the groups
     {
@@ -128,8 +136,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (lane >= d) scan += o;
         }
         if (lane == 31) s_sum[warp] = scan;
-        if (tid == 0) pipe_init(pipe, stages, a.gather ? 1 + 128 : 1);
-        if (warp == 1) tmem_alloc(smem_addr(&pipe.tmem), S::kColumns);
+        if (tid == 0) pipe_init(pipe, stages, a.gather ? 1 + 4 * (PAIRED ? 2 : 1) : 1, PAIRED);
+        if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), S::kColumns);
         __syncthreads();
         for (int w = 0; w < warp; ++w) scan += s_sum[w];
         int at = scan - sum;
@@ -142,14 +150,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
         }
         tc_fence_before();
         __syncthreads();
+        if (PAIRED) cluster_sync();  // the pair's barriers exist before either arrives at them
         tc_fence_after();
     }
     const uint32_t tmem = pipe.tmem;
     volatile int *gave_up = &pipe.gave_up;
-    const int feature_tiles = (a.n + kTcFeatures - 1) / kTcFeatures, main_steps = (a.k + kTcDepth - 1) / kTcDepth;
+    constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
+    const int feature_tiles = (a.n + TILE_F - 1) / TILE_F, main_steps = (a.k + kTcDepth - 1) / kTcDepth;
     const int rank_steps = 2 * ((a.rank + kTcDepth - 1) / kTcDepth);
     const long long n_tiles = (long long)first[a.n_groups] * feature_tiles;
-    const long long worker = blockIdx.x / split, workers = gridDim.x / split;
+    const long long worker = blockIdx.x / group_blocks, workers = gridDim.x / group_blocks;
     TcCursor cur = {first, lo, hi, 0, 0, 0};
 
     // steps of this block for a tile of group g
@@ -159,8 +169,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
         s1 = (int)((long long)total * (part + 1) / split);
     };
 
+    // columns of a tile's products: only as many as there are slots, so that the last tile of a group costs what it holds
+    auto columns_of = [](const TcCursor &c) { return PAIRED ? (c.slot1 - c.slot0 + 31) & ~31 : (c.slot1 - c.slot0 + 15) & ~15; };
+
     // row copies: a thread owns 16 bytes of every 16th row of a slice
-    constexpr int RPT = NT / 16;
+    constexpr int RPT = S::kRows / 16;
     const int chunk = tid & 7, row0 = (tid - 256) >> 3;
     int row[RPT], next_row[RPT];
     TcCursor ahead = cur;
@@ -171,8 +184,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
         ahead.seek((int)(tile / feature_tiles), NT);
 #pragma unroll
         for (int i = 0; i < RPT; ++i) {
-            const int slot = ahead.slot0 + row0 + 16 * i;
-            if (slot < ahead.slot1) {
+            const int at = row0 + 16 * i, slot = ahead.slot0 + half * columns_of(ahead) / 2 + at;
+            if (slot < ahead.slot1 && (!PAIRED || at < columns_of(ahead) / 2)) {
                 next_row[i] = a.slot_row[slot];
                 if ((unsigned)next_row[i] >= (unsigned)a.n_x_rows) {
                     atomicOr(a.status, kStatusBadIndex);
@@ -184,45 +197,48 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     const bool copies = warp >= 8 && a.gather;
     if (copies) fetch_rows(worker);
     int it = 0, told = 0;  // stages used by this warp; of those, copies reported as landed
+    const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);  // where loads are reported
     auto report = [&](int until) {
         fence_async();
-        for (; told < until; ++told) mbar_arrive(smem_addr(&pipe.full[told % stages]));
+        __syncwarp();
+        for (; told < until; ++told)
+            if (lane == 0) mbar_arrive_cluster(full0 + told % stages * 8);
     };
 
     int turn = 0;  // tiles done so far
     for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
-        const int tt = (int)(tile / feature_tiles), f0 = (int)(tile - (long long)tt * feature_tiles) * kTcFeatures;
+        const int tt = (int)(tile / feature_tiles), f0 = (int)(tile - (long long)tt * feature_tiles) * TILE_F + half * kTcFeatures;
         cur.seek(tt, NT);
-        const int g = cur.group, slot0 = cur.slot0, slot1 = cur.slot1;
+        const int g = cur.group, slot0 = cur.slot0, slot1 = cur.slot1, columns = columns_of(cur);
         int s0, s1;
         range(g, s0, s1);
         const int buf = turn & 1;
         if (warp == 0) {
             if (lane == 0) {
                 const int z = a.w_shared ? 0 : g;
-                const int halves = a.n - f0 > 64 ? 2 : 1;  // MN-major: boxes of 64 features
+                const int halves = PAIRED || a.n - f0 > 64 ? 2 : 1;  // MN-major: boxes of 64 features (as many in both blocks)
                 const uint32_t w_bytes = a.mn_major ? halves * kBlock64 : a.w_rows * 128u;
                 for (int s = s0; s < s1; ++s, ++it) {
                     const int st = it % stages;
                     mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
-                    const uint32_t bar = smem_addr(&pipe.full[st]), dst = ring + st * S::kStage;
+                    const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
                     const bool second = s >= main_steps, rows = second || !a.gather;
                     const int e = s - main_steps, i0 = (second ? e >> 1 : s) * kTcDepth;
-                    mbar_expect(bar, w_bytes + (rows ? NT * 128u : 0u));
+                    if (half == 0) mbar_expect(bar, (PAIRED ? 2 : 1) * (w_bytes + (rows ? S::kRows * 128u : 0u)));
                     const CUtensorMap *m = second ? &a.w2 : &a.w;
                     if (a.mn_major)
-                        for (int h = 0; h < halves; ++h) tma_3d(dst + h * kBlock64, m, f0 + h * 64, i0, second ? g : z, bar);
-                    else tma_3d(dst, m, i0, f0, second ? g : z, bar);
-                    if (second) tma_2d(dst + kTcFeatures * 128, &a.u, i0, (e & 1) * a.u_plane + slot0, bar);
-                    else if (rows) tma_2d(dst + kTcFeatures * 128, &a.x, i0, slot0, bar);
+                        for (int h = 0; h < halves; ++h) tma_3d<PAIRED>(dst + h * kBlock64, m, f0 + h * 64, i0, second ? g : z, bar);
+                    else tma_3d<PAIRED>(dst, m, i0, f0, second ? g : z, bar);
+                    const int own = slot0 + half * columns / 2;
+                    if (second) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.u, i0, (e & 1) * a.u_plane + own, bar);
+                    else if (rows) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);
                 }
             }
         } else if (warp == 1) {
-            if (lane == 0) {
+            if (lane == 0 && half == 0) {
                 mbar_wait(smem_addr(&pipe.tmem_empty[buf]), ((turn >> 1) & 1) ^ 1, gave_up, a.status);
                 tc_fence_after();
-                // only as many columns as there are slots: the last tile of a group costs what it holds
-                const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, a.mn_major, false, (slot1 - slot0 + 15) & ~15);
+                const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, a.mn_major, false, TILE_F, columns);
                 const uint64_t a_step = operand_step(a.mn_major), b_step = operand_step(false);
                 for (int s = s0; s < s1; ++s, ++it) {
                     const int st = it % stages;
@@ -232,10 +248,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     const uint64_t da = operand(src, a.mn_major), db = operand(src + kTcFeatures * 128, false);
                     const int left = s >= main_steps ? a.rank - ((s - main_steps) >> 1) * kTcDepth : a.k - s * kTcDepth;
                     const int steps = min(4, (left + 15) >> 4);
-                    for (int i = 0; i < steps; ++i) tc_mma(d, da + i * a_step, db + i * b_step, idesc, s > s0 || i > 0);
-                    tc_commit(smem_addr(&pipe.empty[st]));
+                    for (int i = 0; i < steps; ++i) tc_mma<PAIRED>(d, da + i * a_step, db + i * b_step, idesc, s > s0 || i > 0);
+                    tc_commit<PAIRED>(smem_addr(&pipe.empty[st]));
                 }
-                tc_commit(smem_addr(&pipe.tmem_full[buf]));
+                tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
         } else if (copies) {
 #pragma unroll
@@ -309,7 +325,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 }
             }
             tc_fence_before();
-            mbar_arrive(smem_addr(&pipe.tmem_empty[buf]));
+            if (PAIRED) mbar_arrive_cluster(in_first(smem_addr(&pipe.tmem_empty[buf])));
+            else mbar_arrive(smem_addr(&pipe.tmem_empty[buf]));
             if (split > 1) {
                 // every block of the cluster adds up and stores its share of the columns
                 cluster_sync();
@@ -334,9 +351,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     if (*gave_up) __nanosleep(1000000);  // copies in flight land before the block's memory is given back
     tc_fence_before();
     __syncthreads();
+    if (PAIRED) cluster_sync();  // neither block leaves while the other's products or arrivals still reach it
     if (warp == 1) {
         tc_fence_after();
-        tmem_free(tmem, S::kColumns);
+        tmem_free<PAIRED>(tmem, S::kColumns);
     }
 }
 
@@ -360,11 +378,12 @@ struct TcOuter {
 
 template <int NT>
 struct TcOuterShape {
-    static constexpr int kStage = 2 * kBlock64 + NT / 64 * kBlock64;
+    static constexpr bool kPaired = NT == 256;
+    static constexpr int kStage = 2 * kBlock64 + 2 * kBlock64;  // a block of a pair loads half of the columns
     static constexpr int kStages = stages_for(kTcRing, kStage);
     static constexpr int kReduce = NT <= 128 ? NT * kTcFeatures * 4 : 0;
     static constexpr int kSplitStages = stages_for(kTcRing - kReduce, kStage);
-    static constexpr int kLag = 2;
+    static constexpr int kLag = kPaired ? 4 : 3;
     static constexpr size_t kBytes = 1024 + kTcRing + kOutTotal;
 };
 
@@ -378,53 +397,61 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     const int split = a.split, part = split > 1 ? (int)cluster_rank() : 0;
     const int stages = split > 1 ? S::kSplitStages : S::kStages;
     const uint32_t partial = ring + (uint32_t)S::kSplitStages * S::kStage;
-    if (tid == 0) pipe_init(pipe, stages, 1 + 128);
-    if (warp == 1) tmem_alloc(smem_addr(&pipe.tmem), 2 * NT);
+    constexpr bool PAIRED = S::kPaired;
+    constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
+    const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
+    if (tid == 0) pipe_init(pipe, stages, 1 + 4 * (PAIRED ? 2 : 1), PAIRED);
+    if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), 2 * NT);
     tc_fence_before();
     __syncthreads();
+    if (PAIRED) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = pipe.tmem;
     volatile int *gave_up = &pipe.gave_up;
     const int cols = a.pair ? NT / 2 : NT;  // result columns per tile
-    const int i_tiles = (a.i + kTcFeatures - 1) / kTcFeatures, j_tiles = (a.j + cols - 1) / cols;
+    const int i_tiles = (a.i + TILE_F - 1) / TILE_F, j_tiles = (a.j + cols - 1) / cols;
     const long long n_tiles = (long long)a.n_groups * i_tiles * j_tiles;
-    const long long worker = blockIdx.x / split, workers = gridDim.x / split;
+    const long long worker = blockIdx.x / group_blocks, workers = gridDim.x / group_blocks;
     const bool gather = a.slot_row != nullptr;
     int it = 0, told = 0, turn = 0;
+    const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);  // where loads are reported
     auto report = [&](int until) {
         fence_async();
-        for (; told < until; ++told) mbar_arrive(smem_addr(&pipe.full[told % stages]));
+        __syncwarp();
+        for (; told < until; ++told)
+            if (lane == 0) mbar_arrive_cluster(full0 + told % stages * 8);
     };
     for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
         const int g = (int)(tile / ((long long)i_tiles * j_tiles)), rest = (int)(tile - (long long)g * i_tiles * j_tiles);
-        const int f0 = rest / j_tiles * kTcFeatures, c0 = rest % j_tiles * cols;
+        const int f0 = rest / j_tiles * TILE_F + half * kTcFeatures, c0 = rest % j_tiles * cols;
         const int2 slots = group_range(a.group_ptr, g, a.n_slots, a.status);
         const int total = (slots.y - slots.x + kTcDepth - 1) / kTcDepth;
         const int s0 = (int)((long long)total * part / split), s1 = (int)((long long)total * (part + 1) / split);
         const int buf = turn & 1;
-        const int p_blocks = a.i - f0 > 64 ? 2 : 1, q_blocks = a.pair ? 2 : min(NT / 64, (a.j - c0 + 63) / 64);
+        const int p_blocks = PAIRED || a.i - f0 > 64 ? 2 : 1, q_blocks = a.pair || a.j - c0 > NT / 2 ? 2 : 1;
+        const int q0 = c0 + half * q_blocks * 64;  // the columns this block loads
         if (warp == 0) {
             if (lane == 0) {
                 for (int s = s0; s < s1; ++s, ++it) {
                     const int st = it % stages, slot = slots.x + s * kTcDepth;
                     mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
-                    const uint32_t bar = smem_addr(&pipe.full[st]), dst = ring + st * S::kStage;
+                    const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
                     if (slot + kTcDepth > slots.y) {
-                        mbar_arrive(bar);
+                        if (half == 0) mbar_arrive(bar);
                         continue;
                     }
-                    mbar_expect(bar, ((gather ? 0 : p_blocks) + q_blocks) * kBlock64);
+                    if (half == 0) mbar_expect(bar, (PAIRED ? 2 : 1) * ((gather ? 0 : p_blocks) + q_blocks) * kBlock64);
                     if (!gather)
-                        for (int b = 0; b < p_blocks; ++b) tma_2d(dst + b * kBlock64, &a.p, f0 + b * 64, slot, bar);
+                        for (int b = 0; b < p_blocks; ++b) tma_2d<PAIRED>(dst + b * kBlock64, &a.p, f0 + b * 64, slot, bar);
                     for (int b = 0; b < q_blocks; ++b)
-                        tma_2d(dst + (2 + b) * kBlock64, &a.q, a.pair ? c0 : c0 + b * 64, a.pair ? b * a.n_slots + slot : slot, bar);
+                        tma_2d<PAIRED>(dst + (2 + b) * kBlock64, &a.q, a.pair ? c0 : q0 + b * 64, a.pair ? b * a.n_slots + slot : slot, bar);
                 }
             }
         } else if (warp == 1) {
-            if (lane == 0) {
+            if (lane == 0 && half == 0) {
                 mbar_wait(smem_addr(&pipe.tmem_empty[buf]), ((turn >> 1) & 1) ^ 1, gave_up, a.status);
                 tc_fence_after();
-                const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, true, true, q_blocks * 64);
+                const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, true, true, TILE_F, q_blocks * (PAIRED ? 128 : 64));
                 const uint64_t step = operand_step(true);
                 for (int s = s0; s < s1; ++s, ++it) {
                     const int st = it % stages;
@@ -433,35 +460,38 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     const uint32_t src = ring + st * S::kStage;
                     const uint64_t da = operand(src, true), db = operand(src + 2 * kBlock64, true);
                     const int steps = min(4, (slots.y - slots.x - s * kTcDepth + 15) >> 4);
-                    for (int i = 0; i < steps; ++i) tc_mma(d, da + i * step, db + i * step, idesc, s > s0 || i > 0);
-                    tc_commit(smem_addr(&pipe.empty[st]));
+                    for (int i = 0; i < steps; ++i) tc_mma<PAIRED>(d, da + i * step, db + i * step, idesc, s > s0 || i > 0);
+                    tc_commit<PAIRED>(smem_addr(&pipe.empty[st]));
                 }
-                tc_commit(smem_addr(&pipe.tmem_full[buf]));
+                tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
         } else if (warp >= 8) {
             // a thread owns 16 bytes of every 16th slot of a block
             const int chunk = tid & 7, row0 = (tid - 256) >> 3;
-            int next[4];
+            // row numbers are read four slices ahead: a lane holds one of the warp's 16 rows of two neighbouring slices
             auto fetch = [&](int s) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int slot = slots.x + s * kTcDepth + row0 + 16 * i;
-                    next[i] = -1;
-                    if (s < s1 && slot < slots.y) {
-                        next[i] = gather ? a.slot_row[slot] : slot;
-                        if ((unsigned)next[i] >= (unsigned)a.n_p_rows) {
-                            atomicOr(a.status, kStatusBadIndex);
-                            next[i] = -1;
-                        }
+                const int at = (s + (lane >> 4)) * kTcDepth + (lane >> 2 & 3) * 16 + (warp - 8) * 4 + (lane & 3), slot = slots.x + at;
+                int r = -1;
+                if (s + (lane >> 4) < s1 && slot < slots.y) {
+                    r = gather ? a.slot_row[slot] : slot;
+                    if ((unsigned)r >= (unsigned)a.n_p_rows) {
+                        atomicOr(a.status, kStatusBadIndex);
+                        r = -1;
                     }
                 }
+                return r;
             };
-            fetch(s0);
+            int now = fetch(s0), next = fetch(s0 + 2), later = -1;
             for (int s = s0; s < s1; ++s, ++it) {
+                const int odd = (s - s0) & 1;
+                if (!odd) later = fetch(s + 4);
                 int row[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) row[i] = next[i];
-                fetch(s + 1);  // under way while this slice is copied
+                for (int i = 0; i < 4; ++i) row[i] = __shfl_sync(0xffffffffu, now, odd * 16 + i * 4 + (lane >> 3));
+                if (odd) {
+                    now = next;
+                    next = later;
+                }
                 const int st = it % stages, slot = slots.x + s * kTcDepth;
                 const bool last = slot + kTcDepth > slots.y;
                 mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
@@ -477,7 +507,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     }
                 if (last)
                     for (int b = 0; b < q_blocks; ++b) {
-                        const int c = (a.pair ? c0 : c0 + b * 64) + chunk * 8;
+                        const int c = (a.pair ? c0 : q0 + b * 64) + chunk * 8;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const int at = slot + row0 + 16 * i;
@@ -541,7 +571,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
             }
             tc_fence_before();
-            mbar_arrive(smem_addr(&pipe.tmem_empty[buf]));
+            if (PAIRED) mbar_arrive_cluster(in_first(smem_addr(&pipe.tmem_empty[buf])));
+            else mbar_arrive(smem_addr(&pipe.tmem_empty[buf]));
             if (split > 1) {
                 cluster_sync();
                 for (int c = part; c < cols && c0 + c < a.j; c += split) {
@@ -565,9 +596,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     if (*gave_up) __nanosleep(1000000);
     tc_fence_before();
     __syncthreads();
+    if (PAIRED) cluster_sync();
     if (warp == 1) {
         tc_fence_after();
-        tmem_free(tmem, 2 * NT);
+        tmem_free<PAIRED>(tmem, 2 * NT);
     }
 }
 

@@ -51,13 +51,24 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatil
 
 // ---- TMA: boxes of 64 elements (128 bytes, 128-byte swizzle) by some rows.  The x coordinate is a multiple of 64 elements
 // throughout, so every copy starts on a 128-byte multiple of its row.
+// PAIRED: the barrier may be the other block's.
+template <bool PAIRED>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x),
+    if constexpr (PAIRED)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                     "l"(map), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
+    else asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map), "r"(x),
                  "r"(y), "r"(bar)
                  : "memory");
 }
+template <bool PAIRED>
 __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
+    if constexpr (PAIRED)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                     "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                     : "memory");
+    else asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map),
                  "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
@@ -77,24 +88,44 @@ __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.
 // byte offset of 16-byte chunk c (0..7) of a 128-byte row in the 128-byte swizzle
 __device__ __forceinline__ uint32_t swizzled(int row, int c) { return (uint32_t)row * 128 + (uint32_t)((c ^ (row & 7)) << 4); }
 
-// ---- tcgen05
+// ---- tcgen05; PAIRED: by two neighbouring blocks of a cluster as one, the products issued by the first for both
+template <bool PAIRED>
 __device__ __forceinline__ void tmem_alloc(uint32_t where, uint32_t columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if constexpr (PAIRED) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(where), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
 }
+template <bool PAIRED>
 __device__ __forceinline__ void tmem_free(uint32_t base, uint32_t columns) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
+    if constexpr (PAIRED) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "r"(columns));
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// arrives at the barrier (PAIRED: at both blocks' barriers of that address) once the products issued so far are done
+template <bool PAIRED>
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if constexpr (PAIRED)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                     : "memory");
+    else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+template <bool PAIRED>
 __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
-        "r"((uint32_t)add)
-        : "memory");
+    if constexpr (PAIRED)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+            "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+            "r"(idesc), "r"((uint32_t)add)
+            : "memory");
 }
 
 // Shared-memory operand in 128-byte swizzled atoms of eight 128-byte rows.  Summed index contiguous: the rows are the tile's
@@ -108,9 +139,9 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, bool mn_major) {
 // 16 summed elements further, in units of the descriptor's address field
 __device__ __forceinline__ uint64_t operand_step(bool mn_major) { return mn_major ? (16 * 128) >> 4 : 32 >> 4; }
 
-// fp32 result, both operands of one 16-bit type, 128 result rows by n columns
-__device__ __forceinline__ uint32_t mma_desc(bool bf16, bool a_mn, bool b_mn, int n) {
-    return 1u << 4 | (uint32_t)bf16 << 7 | (uint32_t)bf16 << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+// fp32 result, both operands of one 16-bit type, m result rows (128; 256 by a pair of blocks) by n columns
+__device__ __forceinline__ uint32_t mma_desc(bool bf16, bool a_mn, bool b_mn, int m, int n) {
+    return 1u << 4 | (uint32_t)bf16 << 7 | (uint32_t)bf16 << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
 // 32 consecutive columns of the calling warp's 32 TMEM lanes, one lane per thread
@@ -150,6 +181,15 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// the address of block 0's variable of that address in this block
+__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(addr));
+    return remote;
+}
+// Arrives at a barrier of either block.  (With .release.cluster the arrival waits for the thread's writes to reach the cluster,
+// about a microsecond; what it orders here are writes of the asynchronous proxy that had landed before, see fence_async.)
+__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
     uint32_t remote;
     float v;
