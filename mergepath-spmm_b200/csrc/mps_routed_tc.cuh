@@ -24,7 +24,7 @@
 
 namespace mps {
 
-constexpr int kTcThreads = 384;  // warps: 0 TMA, 1 products, 2-3 idle, 4-7 results (TMEM lanes go by warp number mod 4), 8-11 row copies
+constexpr int kTcThreads = 384;  // warps: 0 TMA, 1 products, 2 reports of row copies, 4-7 results (TMEM lanes go by warp number mod 4), 8-11 row copies
 constexpr int kTcFeatures = 128;
 constexpr int kTcDepth = 64;
 constexpr int kTcRing = 192 * 1024;            // shared memory of the stages
@@ -52,7 +52,7 @@ struct TcRows {
 };
 
 struct TcPipe {
-    uint64_t full[12], empty[12], tmem_full[2], tmem_empty[2];  // of a pair's full and tmem_empty the first block's count
+    uint64_t full[12], empty[12], landed[12], tmem_full[2], tmem_empty[2];  // of a pair's full and tmem_empty the first block's count
     uint32_t tmem;
     int gave_up;
 };
@@ -61,6 +61,7 @@ __device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, int full_cou
     for (int i = 0; i < stages; ++i) {
         mbar_init(smem_addr(&pipe.full[i]), full_count);
         mbar_init(smem_addr(&pipe.empty[i]), 1);
+        mbar_init(smem_addr(&pipe.landed[i]), 128);  // every copying thread, as its copies land
     }
     for (int i = 0; i < 2; ++i) {
         mbar_init(smem_addr(&pipe.tmem_full[i]), 1);
@@ -81,7 +82,6 @@ struct TcShape {
     static constexpr int kColumns = 2 * NT;
     static constexpr int kReduce = NT <= 64 ? NT * kTcFeatures * 4 : 0;  // only small tiles are split
     static constexpr int kSplitStages = stages_for(kTcRing - kReduce, kStage);
-    static constexpr int kLag = kPaired ? 4 : 3;  // slices of row copies in flight
     static size_t bytes(int n_groups) { return 1024 + kTcRing + kOutTotal + (size_t)(3 * n_groups + 1) * sizeof(int); }
 };
 
@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (lane >= d) scan += o;
         }
         if (lane == 31) s_sum[warp] = scan;
-        if (tid == 0) pipe_init(pipe, stages, a.gather ? 1 + 4 * (PAIRED ? 2 : 1) : 1, PAIRED);
+        if (tid == 0) pipe_init(pipe, stages, 1 + (a.gather ? PAIRED ? 2 : 1 : 0), PAIRED);
         if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), S::kColumns);
         __syncthreads();
         for (int w = 0; w < warp; ++w) scan += s_sum[w];
@@ -196,14 +196,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     };
     const bool copies = warp >= 8 && a.gather;
     if (copies) fetch_rows(worker);
-    int it = 0, told = 0;  // stages used by this warp; of those, copies reported as landed
     const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);  // where loads are reported
-    auto report = [&](int until) {
-        fence_async();
-        __syncwarp();
-        for (; told < until; ++told)
-            if (lane == 0) mbar_arrive_cluster(full0 + told % stages * 8);
-    };
+    int it = 0;  // stages used by this warp
 
     int turn = 0;  // tiles done so far
     for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
@@ -253,6 +247,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 }
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
+        } else if (warp == 2) {
+            if (lane == 0 && a.gather)  // row copies that have landed: made visible to the tensor cores and reported
+                for (int s = s0; s < s1; ++s, ++it) {
+                    const int st = it % stages;
+                    mbar_wait(smem_addr(&pipe.landed[st]), (it / stages) & 1, gave_up, a.status);
+                    fence_async();
+                    mbar_arrive_cluster(full0 + st * 8);
+                }
         } else if (copies) {
 #pragma unroll
             for (int i = 0; i < RPT; ++i) row[i] = next_row[i];
@@ -269,13 +271,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                         copy_16(dst + i * 2048, valid ? a.rows + (long long)row[i] * a.k + col : a.rows, valid);
                     }
                 }
-                copy_commit();
-                copy_wait<S::kLag>();
-                report(it + 1 - S::kLag);
-            }
-            if (split > 1) {  // the cluster meets at the end of the tile: nothing may be left unreported
-                copy_wait<0>();
-                report(it);
+                copy_arrive(smem_addr(&pipe.landed[st]));
             }
         } else if (warp >= 4 && warp < 8) {
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
@@ -344,10 +340,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             cluster_sync();
         }
     }
-    if (copies) {
-        copy_wait<0>();
-        report(it);
-    }
+    if (copies) copy_drain();
     if (*gave_up) __nanosleep(1000000);  // copies in flight land before the block's memory is given back
     tc_fence_before();
     __syncthreads();
@@ -383,7 +376,6 @@ struct TcOuterShape {
     static constexpr int kStages = stages_for(kTcRing, kStage);
     static constexpr int kReduce = NT <= 128 ? NT * kTcFeatures * 4 : 0;
     static constexpr int kSplitStages = stages_for(kTcRing - kReduce, kStage);
-    static constexpr int kLag = kPaired ? 4 : 3;
     static constexpr size_t kBytes = 1024 + kTcRing + kOutTotal;
 };
 
@@ -400,7 +392,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     constexpr bool PAIRED = S::kPaired;
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
-    if (tid == 0) pipe_init(pipe, stages, 1 + 4 * (PAIRED ? 2 : 1), PAIRED);
+    if (tid == 0) pipe_init(pipe, stages, 1 + (PAIRED ? 2 : 1), PAIRED);
     if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), 2 * NT);
     tc_fence_before();
     __syncthreads();
@@ -413,14 +405,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     const long long n_tiles = (long long)a.n_groups * i_tiles * j_tiles;
     const long long worker = blockIdx.x / group_blocks, workers = gridDim.x / group_blocks;
     const bool gather = a.slot_row != nullptr;
-    int it = 0, told = 0, turn = 0;
-    const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);  // where loads are reported
-    auto report = [&](int until) {
-        fence_async();
-        __syncwarp();
-        for (; told < until; ++told)
-            if (lane == 0) mbar_arrive_cluster(full0 + told % stages * 8);
-    };
+    const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);
+    int it = 0, turn = 0;
     for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
         const int g = (int)(tile / ((long long)i_tiles * j_tiles)), rest = (int)(tile - (long long)g * i_tiles * j_tiles);
         const int f0 = rest / j_tiles * TILE_F + half * kTcFeatures, c0 = rest % j_tiles * cols;
@@ -465,6 +451,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
+        } else if (warp == 2) {
+            if (lane == 0)  // row copies that have landed: made visible to the tensor cores and reported
+                for (int s = s0; s < s1; ++s, ++it) {
+                    const int st = it % stages;
+                    mbar_wait(smem_addr(&pipe.landed[st]), (it / stages) & 1, gave_up, a.status);
+                    fence_async();
+                    mbar_arrive_cluster(full0 + st * 8);
+                }
         } else if (warp >= 8) {
             // a thread owns 16 bytes of every 16th slot of a block
             const int chunk = tid & 7, row0 = (tid - 256) >> 3;
@@ -516,18 +510,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                             copy_16(dst + (2 + b) * kBlock64 + i * 2048, valid ? a.q_base + line * a.j + c : a.q_base, valid);
                         }
                     }
-                copy_commit();
-                if (gather) {
-                    copy_wait<S::kLag>();
-                    report(it + 1 - S::kLag);
-                } else {
-                    copy_wait<0>();
-                    report(it + 1);
-                }
-            }
-            if (split > 1) {
-                copy_wait<0>();
-                report(it);
+                copy_arrive(smem_addr(&pipe.landed[st]));
             }
         } else if (warp >= 4) {
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
@@ -589,10 +572,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             cluster_sync();
         }
     }
-    if (warp >= 8) {
-        copy_wait<0>();
-        report(it);
-    }
+    if (warp >= 8) copy_drain();
     if (*gave_up) __nanosleep(1000000);
     tc_fence_before();
     __syncthreads();

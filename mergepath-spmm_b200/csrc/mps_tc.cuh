@@ -78,12 +78,10 @@ __device__ __forceinline__ void tma_prefetch(const CUtensorMap *map) { asm volat
 __device__ __forceinline__ void copy_16(uint32_t dst, const void *src, bool valid) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-// what this thread wrote to shared memory becomes visible to the tensor cores' reads that are ordered behind it
+// an arrival at the barrier once all of this thread's copies so far have landed
+__device__ __forceinline__ void copy_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void copy_drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// ordinary writes to shared memory that this thread knows of become visible to the tensor cores' reads ordered behind it
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // byte offset of 16-byte chunk c (0..7) of a 128-byte row in the 128-byte swizzle
 __device__ __forceinline__ uint32_t swizzled(int row, int c) { return (uint32_t)row * 128 + (uint32_t)((c ^ (row & 7)) << 4); }
