@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     const bool copies = warp >= 8 && a.gather;
     if (copies) fetch_rows(worker);
     const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);  // where loads are reported
-    int it = 0;  // stages used by this warp
+    RingAt pos;  // this warp's place in the ring
 
     int turn = 0;  // tiles done so far
     for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
@@ -208,13 +208,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
         range(g, s0, s1);
         const int buf = turn & 1;
         if (warp == 0) {
-            if (lane == 0) {
+            if (elect_one()) {
                 const int z = a.w_shared ? 0 : g;
                 const int halves = PAIRED || a.n - f0 > 64 ? 2 : 1;  // MN-major: boxes of 64 features (as many in both blocks)
                 const uint32_t w_bytes = a.mn_major ? halves * kBlock64 : a.w_rows * 128u;
-                for (int s = s0; s < s1; ++s, ++it) {
-                    const int st = it % stages;
-                    mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
+                for (int s = s0; s < s1; ++s, pos.next(stages)) {
+                    const int st = pos.stage;
+                    mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                     const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
                     const bool second = s >= main_steps, rows = second || !a.gather;
                     const int e = s - main_steps, i0 = (second ? e >> 1 : s) * kTcDepth;
@@ -229,29 +229,28 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 }
             }
         } else if (warp == 1) {
-            if (lane == 0 && half == 0) {
+            if (half == 0 && elect_one()) {
                 mbar_wait(smem_addr(&pipe.tmem_empty[buf]), ((turn >> 1) & 1) ^ 1, gave_up, a.status);
                 tc_fence_after();
                 const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, a.mn_major, false, TILE_F, columns);
                 const uint64_t a_step = operand_step(a.mn_major), b_step = operand_step(false);
-                for (int s = s0; s < s1; ++s, ++it) {
-                    const int st = it % stages;
-                    mbar_wait(smem_addr(&pipe.full[st]), (it / stages) & 1, gave_up, a.status);
+                const uint64_t a0 = operand(ring, a.mn_major), b0 = operand(ring + kTcFeatures * 128, false);
+                for (int s = s0; s < s1; ++s, pos.next(stages)) {
+                    const int st = pos.stage;
+                    mbar_wait(smem_addr(&pipe.full[st]), pos.parity, gave_up, a.status);
                     tc_fence_after();
-                    const uint32_t src = ring + st * S::kStage;
-                    const uint64_t da = operand(src, a.mn_major), db = operand(src + kTcFeatures * 128, false);
+                    const uint64_t da = operand_at(a0, st * S::kStage), db = operand_at(b0, st * S::kStage);
                     const int left = s >= main_steps ? a.rank - ((s - main_steps) >> 1) * kTcDepth : a.k - s * kTcDepth;
-                    const int steps = min(4, (left + 15) >> 4);
-                    for (int i = 0; i < steps; ++i) tc_mma<PAIRED>(d, da + i * a_step, db + i * b_step, idesc, s > s0 || i > 0);
+                    tc_slice<PAIRED>(d, da, db, a_step, b_step, idesc, min(4, (left + 15) >> 4), s > s0);
                     tc_commit<PAIRED>(smem_addr(&pipe.empty[st]));
                 }
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
         } else if (warp == 2) {
-            if (lane == 0 && a.gather)  // row copies that have landed: made visible to the tensor cores and reported
-                for (int s = s0; s < s1; ++s, ++it) {
-                    const int st = it % stages;
-                    mbar_wait(smem_addr(&pipe.landed[st]), (it / stages) & 1, gave_up, a.status);
+            if (a.gather && elect_one())  // row copies that have landed: made visible to the tensor cores and reported
+                for (int s = s0; s < s1; ++s, pos.next(stages)) {
+                    const int st = pos.stage;
+                    mbar_wait(smem_addr(&pipe.landed[st]), pos.parity, gave_up, a.status);
                     fence_async();
                     mbar_arrive_cluster(full0 + st * 8);
                 }
@@ -259,9 +258,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
 #pragma unroll
             for (int i = 0; i < RPT; ++i) row[i] = next_row[i];
             fetch_rows(tile + workers);  // under way while this tile is copied
-            for (int s = s0; s < s1; ++s, ++it) {
-                const int st = it % stages;
-                mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
+            for (int s = s0; s < s1; ++s, pos.next(stages)) {
+                const int st = pos.stage;
+                mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                 const int col = s * kTcDepth + chunk * 8;
                 if (s < main_steps) {
                     const uint32_t dst = ring + st * S::kStage + kTcFeatures * 128 + swizzled(row0, chunk);
@@ -406,7 +405,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     const long long worker = blockIdx.x / group_blocks, workers = gridDim.x / group_blocks;
     const bool gather = a.slot_row != nullptr;
     const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);
-    int it = 0, turn = 0;
+    RingAt pos;
+    int turn = 0;
     for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
         const int g = (int)(tile / ((long long)i_tiles * j_tiles)), rest = (int)(tile - (long long)g * i_tiles * j_tiles);
         const int f0 = rest / j_tiles * TILE_F + half * kTcFeatures, c0 = rest % j_tiles * cols;
@@ -417,10 +417,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
         const int p_blocks = PAIRED || a.i - f0 > 64 ? 2 : 1, q_blocks = a.pair || a.j - c0 > NT / 2 ? 2 : 1;
         const int q0 = c0 + half * q_blocks * 64;  // the columns this block loads
         if (warp == 0) {
-            if (lane == 0) {
-                for (int s = s0; s < s1; ++s, ++it) {
-                    const int st = it % stages, slot = slots.x + s * kTcDepth;
-                    mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
+            if (elect_one()) {
+                for (int s = s0; s < s1; ++s, pos.next(stages)) {
+                    const int st = pos.stage, slot = slots.x + s * kTcDepth;
+                    mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                     const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
                     if (slot + kTcDepth > slots.y) {
                         if (half == 0) mbar_arrive(bar);
@@ -434,28 +434,26 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
             }
         } else if (warp == 1) {
-            if (lane == 0 && half == 0) {
+            if (half == 0 && elect_one()) {
                 mbar_wait(smem_addr(&pipe.tmem_empty[buf]), ((turn >> 1) & 1) ^ 1, gave_up, a.status);
                 tc_fence_after();
                 const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, true, true, TILE_F, q_blocks * (PAIRED ? 128 : 64));
-                const uint64_t step = operand_step(true);
-                for (int s = s0; s < s1; ++s, ++it) {
-                    const int st = it % stages;
-                    mbar_wait(smem_addr(&pipe.full[st]), (it / stages) & 1, gave_up, a.status);
+                const uint64_t step = operand_step(true), a0 = operand(ring, true), b0 = operand(ring + 2 * kBlock64, true);
+                for (int s = s0; s < s1; ++s, pos.next(stages)) {
+                    const int st = pos.stage;
+                    mbar_wait(smem_addr(&pipe.full[st]), pos.parity, gave_up, a.status);
                     tc_fence_after();
-                    const uint32_t src = ring + st * S::kStage;
-                    const uint64_t da = operand(src, true), db = operand(src + 2 * kBlock64, true);
-                    const int steps = min(4, (slots.y - slots.x - s * kTcDepth + 15) >> 4);
-                    for (int i = 0; i < steps; ++i) tc_mma<PAIRED>(d, da + i * step, db + i * step, idesc, s > s0 || i > 0);
+                    tc_slice<PAIRED>(d, operand_at(a0, st * S::kStage), operand_at(b0, st * S::kStage), step, step, idesc,
+                                     min(4, (slots.y - slots.x - s * kTcDepth + 15) >> 4), s > s0);
                     tc_commit<PAIRED>(smem_addr(&pipe.empty[st]));
                 }
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
         } else if (warp == 2) {
-            if (lane == 0)  // row copies that have landed: made visible to the tensor cores and reported
-                for (int s = s0; s < s1; ++s, ++it) {
-                    const int st = it % stages;
-                    mbar_wait(smem_addr(&pipe.landed[st]), (it / stages) & 1, gave_up, a.status);
+            if (elect_one())  // row copies that have landed: made visible to the tensor cores and reported
+                for (int s = s0; s < s1; ++s, pos.next(stages)) {
+                    const int st = pos.stage;
+                    mbar_wait(smem_addr(&pipe.landed[st]), pos.parity, gave_up, a.status);
                     fence_async();
                     mbar_arrive_cluster(full0 + st * 8);
                 }
@@ -476,7 +474,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 return r;
             };
             int now = fetch(s0), next = fetch(s0 + 2), later = -1;
-            for (int s = s0; s < s1; ++s, ++it) {
+            for (int s = s0; s < s1; ++s, pos.next(stages)) {
                 const int odd = (s - s0) & 1;
                 if (!odd) later = fetch(s + 4);
                 int row[4];
@@ -486,9 +484,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     now = next;
                     next = later;
                 }
-                const int st = it % stages, slot = slots.x + s * kTcDepth;
+                const int st = pos.stage, slot = slots.x + s * kTcDepth;
                 const bool last = slot + kTcDepth > slots.y;
-                mbar_wait(smem_addr(&pipe.empty[st]), ((it / stages) & 1) ^ 1, gave_up, a.status);
+                mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                 const uint32_t dst = ring + st * S::kStage + swizzled(row0, chunk);
                 if (gather || last)
                     for (int b = 0; b < p_blocks; ++b) {

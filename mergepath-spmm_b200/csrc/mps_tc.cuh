@@ -30,6 +30,27 @@ __device__ __forceinline__ unsigned long long now_ns() {
     return t;
 }
 
+// one lane of a converged warp, in the form the compiler knows to be a single thread (products and their descriptors then stay
+// in uniform registers)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.b32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+    return ok != 0;
+}
+
+// The stage a warp is at in the ring, and the parity of its use.  Counted up: a division per slice costs the thread that issues
+// the products more than the products take.
+struct RingAt {
+    int stage = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ void next(int stages) {
+        if (++stage == stages) {
+            stage = 0;
+            parity ^= 1;
+        }
+    }
+};
+
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // no wait of a working kernel comes near two seconds
 
 // Waits for the phase; after kWaitLimitNs (or once another thread of the block gave up) it records that and returns.  The
@@ -136,6 +157,8 @@ __device__ __forceinline__ uint64_t operand(uint32_t addr, bool mn_major) {
 }
 // 16 summed elements further, in units of the descriptor's address field
 __device__ __forceinline__ uint64_t operand_step(bool mn_major) { return mn_major ? (16 * 128) >> 4 : 32 >> 4; }
+// the same operand `bytes` further on (addresses stay below 2^18, so the field does not overflow)
+__device__ __forceinline__ uint64_t operand_at(uint64_t first, uint32_t bytes) { return first + (bytes >> 4); }
 
 // fp32 result, both operands of one 16-bit type, m result rows (128; 256 by a pair of blocks) by n columns
 __device__ __forceinline__ uint32_t mma_desc(bool bf16, bool a_mn, bool b_mn, int m, int n) {
@@ -194,6 +217,17 @@ __device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
     asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
     return v;
+}
+
+// the products of one slice: `steps` (1..4) times 16 summed elements, the first overwriting the accumulator unless `add`
+template <bool PAIRED>
+__device__ __forceinline__ void tc_slice(uint32_t d, uint64_t a, uint64_t b, uint64_t a_step, uint64_t b_step, uint32_t idesc, int steps, bool add) {
+    if (steps == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tc_mma<PAIRED>(d, a + i * a_step, b + i * b_step, idesc, add || i > 0);
+    } else {
+        for (int i = 0; i < steps; ++i) tc_mma<PAIRED>(d, a + i * a_step, b + i * b_step, idesc, add || i > 0);
+    }
 }
 
 }  // namespace mps
