@@ -251,8 +251,7 @@ int tc_rows(TcRows a, const void *x, long long x_rows, cudaStream_t st) {
     const int nt = mean <= 20 ? 32 : mean <= 48 ? 64 : mean <= 128 ? 128 : 256;
     const int loaded = nt == 256 ? mps::TcShape<256>::kRows : nt;  // slots a block loads
     a.rows = (const uint16_t *)x;
-    if (!a.gather)
-        if (int rc = tensor_map(&a.x, a.bf16, x, 2, a.k, x_rows, 1, loaded)) return rc;
+    if (int rc = tensor_map(&a.x, a.bf16, x, 2, a.k, x_rows, 1, a.gather ? 1 : loaded)) return rc;
     if (a.rank) {
         if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded)) return rc;
     }

@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (lane >= d) scan += o;
         }
         if (lane == 31) s_sum[warp] = scan;
-        if (tid == 0) pipe_init(pipe, stages, 1 + (a.gather ? PAIRED ? 2 : 1 : 0), PAIRED);
+        if (tid == 0) pipe_init(pipe, stages, 1, PAIRED);
         if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), S::kColumns);
         __syncthreads();
         for (int w = 0; w < warp; ++w) scan += s_sum[w];
@@ -172,26 +172,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     // columns of a tile's products: only as many as there are slots, so that the last tile of a group costs what it holds
     auto columns_of = [](const TcCursor &c) { return PAIRED ? (c.slot1 - c.slot0 + 31) & ~31 : (c.slot1 - c.slot0 + 15) & ~15; };
 
-    // row copies: a thread owns 16 bytes of every 16th row of a slice
-    constexpr int RPT = S::kRows / 16;
-    const int chunk = tid & 7, row0 = (tid - 256) >> 3;
-    int row[RPT], next_row[RPT];
+    // gathered rows: a warp loads a quarter of a slice's, a lane holding one row's number
+    constexpr int RPW = S::kRows / 4;
+    int row = 0, next_row = 0;
     TcCursor ahead = cur;
     auto fetch_rows = [&](long long tile) {
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) next_row[i] = -1;
+        next_row = a.n_x_rows;  // out of range: zeros
         if (tile >= n_tiles) return;
         ahead.seek((int)(tile / feature_tiles), NT);
-#pragma unroll
-        for (int i = 0; i < RPT; ++i) {
-            const int at = row0 + 16 * i, slot = ahead.slot0 + half * columns_of(ahead) / 2 + at;
-            if (slot < ahead.slot1 && (!PAIRED || at < columns_of(ahead) / 2)) {
-                next_row[i] = a.slot_row[slot];
-                if ((unsigned)next_row[i] >= (unsigned)a.n_x_rows) {
-                    atomicOr(a.status, kStatusBadIndex);
-                    next_row[i] = -1;
-                }
-            }
+        const int at = (warp - 8) * RPW + lane, slot = ahead.slot0 + half * columns_of(ahead) / 2 + at;
+        if (lane < RPW && slot < ahead.slot1 && (!PAIRED || at < columns_of(ahead) / 2)) {
+            const int r = a.slot_row[slot];
+            if ((unsigned)r < (unsigned)a.n_x_rows) next_row = r;
+            else atomicOr(a.status, kStatusBadIndex);
         }
     };
     const bool copies = warp >= 8 && a.gather;
@@ -216,16 +209,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     const int st = pos.stage;
                     mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                     const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
-                    const bool second = s >= main_steps, rows = second || !a.gather;
+                    const bool second = s >= main_steps;
                     const int e = s - main_steps, i0 = (second ? e >> 1 : s) * kTcDepth;
-                    if (half == 0) mbar_expect(bar, (PAIRED ? 2 : 1) * (w_bytes + (rows ? S::kRows * 128u : 0u)));
+                    if (half == 0) mbar_expect(bar, (PAIRED ? 2 : 1) * (w_bytes + S::kRows * 128u));
                     const CUtensorMap *m = second ? &a.w2 : &a.w;
                     if (a.mn_major)
                         for (int h = 0; h < halves; ++h) tma_3d<PAIRED>(dst + h * kBlock64, m, f0 + h * 64, i0, second ? g : z, bar);
                     else tma_3d<PAIRED>(dst, m, i0, f0, second ? g : z, bar);
                     const int own = slot0 + half * columns / 2;
                     if (second) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.u, i0, (e & 1) * a.u_plane + own, bar);
-                    else if (rows) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);
+                    else if (!a.gather) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);
                 }
             }
         } else if (warp == 1) {
@@ -246,31 +239,21 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 }
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
-        } else if (warp == 2) {
-            if (a.gather && elect_one())  // row copies that have landed: made visible to the tensor cores and reported
-                for (int s = s0; s < s1; ++s, pos.next(stages)) {
-                    const int st = pos.stage;
-                    mbar_wait(smem_addr(&pipe.landed[st]), pos.parity, gave_up, a.status);
-                    fence_async();
-                    mbar_arrive_cluster(full0 + st * 8);
-                }
         } else if (copies) {
-#pragma unroll
-            for (int i = 0; i < RPT; ++i) row[i] = next_row[i];
-            fetch_rows(tile + workers);  // under way while this tile is copied
+            row = next_row;
+            fetch_rows(tile + workers);  // under way while this tile is loaded
             for (int s = s0; s < s1; ++s, pos.next(stages)) {
                 const int st = pos.stage;
                 mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
-                const int col = s * kTcDepth + chunk * 8;
-                if (s < main_steps) {
-                    const uint32_t dst = ring + st * S::kStage + kTcFeatures * 128 + swizzled(row0, chunk);
+                __syncwarp();
+                if (s >= main_steps) continue;
+                const uint32_t dst = ring + st * S::kStage + kTcFeatures * 128 + (warp - 8) * RPW * 128;
 #pragma unroll
-                    for (int i = 0; i < RPT; ++i) {
-                        const bool valid = row[i] >= 0 && col < a.k;
-                        copy_16(dst + i * 2048, valid ? a.rows + (long long)row[i] * a.k + col : a.rows, valid);
-                    }
+                for (int q = 0; q < RPW / 4; ++q) {
+                    const int r0 = __shfl_sync(0xffffffffu, row, 4 * q), r1 = __shfl_sync(0xffffffffu, row, 4 * q + 1);
+                    const int r2 = __shfl_sync(0xffffffffu, row, 4 * q + 2), r3 = __shfl_sync(0xffffffffu, row, 4 * q + 3);
+                    if (elect_one()) tma_rows<PAIRED>(dst + q * 512, &a.x, s * kTcDepth, r0, r1, r2, r3, full0 + st * 8);
                 }
-                copy_arrive(smem_addr(&pipe.landed[st]));
             }
         } else if (warp >= 4 && warp < 8) {
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
@@ -339,7 +322,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             cluster_sync();
         }
     }
-    if (copies) copy_drain();
     if (*gave_up) __nanosleep(1000000);  // copies in flight land before the block's memory is given back
     tc_fence_before();
     __syncthreads();

@@ -93,6 +93,21 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, int
                  "r"(x), "r"(y), "r"(z), "r"(bar)
                  : "memory");
 }
+// four rows by number, one under the other; a row number outside the tensor gives zeros
+template <bool PAIRED>
+__device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, int x, int r0, int r1, int r2, int r3, uint32_t bar) {
+    if constexpr (PAIRED)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
+                dst),
+            "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
+            : "memory");
+}
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // ---- 16 bytes from global to shared memory without a register between; zeros where !valid (nothing is read then)
