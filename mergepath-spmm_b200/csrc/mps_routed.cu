@@ -250,7 +250,6 @@ int tc_rows(TcRows a, const void *x, long long x_rows, cudaStream_t st) {
     const long long mean = a.n_slots / groups;
     const int nt = mean <= 20 ? 32 : mean <= 48 ? 64 : mean <= 128 ? 128 : 256;
     const int loaded = nt == 256 ? mps::TcShape<256>::kRows : nt;  // slots a block loads
-    a.rows = (const uint16_t *)x;
     if (int rc = tensor_map(&a.x, a.bf16, x, 2, a.k, x_rows, 1, a.gather ? 1 : loaded)) return rc;
     if (a.rank) {
         if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded)) return rc;
@@ -285,11 +284,11 @@ int tc_outer(TcOuter a, const void *p, const void *q, cudaStream_t st) {
     if (int rc = status_pointer(&a.status)) return rc;
     int sms;
     if (int rc = sm_count(&sms)) return rc;
-    a.p_base = (const uint16_t *)p;
-    a.q_base = (const uint16_t *)q;
-    if (!a.slot_row)
-        if (int rc = tensor_map(&a.p, a.bf16, p, 2, a.i, a.n_p_rows, 1, mps::kTcDepth)) return rc;
-    if (int rc = tensor_map(&a.q, a.bf16, q, 2, a.j, (a.pair ? 2ull : 1ull) * a.n_slots, 1, mps::kTcDepth)) return rc;
+    const unsigned long long q_rows = (a.pair ? 2ull : 1ull) * a.n_slots;
+    if (int rc = tensor_map(&a.p_rows, a.bf16, p, 2, a.i, a.n_p_rows, 1, 1)) return rc;
+    if (int rc = tensor_map(&a.p_tile, a.bf16, p, 2, a.i, a.n_p_rows, 1, mps::kTcDepth)) return rc;
+    if (int rc = tensor_map(&a.q_rows, a.bf16, q, 2, a.j, q_rows, 1, 1)) return rc;
+    if (int rc = tensor_map(&a.q_tile, a.bf16, q, 2, a.j, q_rows, 1, mps::kTcDepth)) return rc;
     if (a.pair || a.j <= 128) return launch_tc_outer<128>(a, sms, st);
     return launch_tc_outer<256>(a, sms, st);
 }

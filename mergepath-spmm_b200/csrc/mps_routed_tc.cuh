@@ -3,9 +3,9 @@
 // tc_rows_kernel: out[slot, f] = sum_i W[g(slot)][f, i] x[row(slot), i].  The matrix is the first operand, so its result rows
 // fill the 128 lanes of TMEM whatever the number of routed rows is; the slots are the columns, NT of them per tile (32 where a
 // few rows meet each matrix and its bytes are what counts, 256 where the arithmetic does).  The matrices come by TMA in 64-deep
-// slices through a ring of stages, rows in slot order too; gathered rows are fetched by four warps with 16-byte asynchronous
-// copies into the same swizzled layout (TMA loads by row number took 67 cycles for four rows, four times what the tensor cores
-// leave).  Two accumulators in TMEM alternate, so a tile is stored while the next one is summed; results go through shared
+// slices through a ring of stages, rows in slot order too; gathered rows by number, four per TMA instruction, issued by one
+// elected lane of each of four warps (2.3 us a slice of 256 rows from 32 diverged lanes of one warp; 16-byte asynchronous copies
+// by 128 threads took 0.45 us for 128 rows, these 0.3).  Two accumulators in TMEM alternate, so a tile is stored while the next one is summed; results go through shared
 // memory, where 32 slots by 128 features become whole 256-byte rows.
 //
 // A tile's sum may go on with a second product (`rank` > 0): the group's low-rank matrix times rows u that were computed before,
@@ -24,7 +24,7 @@
 
 namespace mps {
 
-constexpr int kTcThreads = 384;  // warps: 0 TMA, 1 products, 2 reports of row copies, 4-7 results (TMEM lanes go by warp number mod 4), 8-11 row copies
+constexpr int kTcThreads = 384;  // warps: 0 TMA, 1 products, 2-3 none, 4-7 results (TMEM lanes go by warp number mod 4), 8-11 row loads
 constexpr int kTcFeatures = 128;
 constexpr int kTcDepth = 64;
 constexpr int kTcRing = 192 * 1024;            // shared memory of the stages
@@ -38,7 +38,6 @@ struct TcRows {
     const int *slot_row;      // row behind a slot; NULL: the slot itself
     int n_groups, n_slots, n_x_rows;
     int k, n;                 // summed index, result features
-    const uint16_t *rows;     // gathered rows: x itself
     int rank, rank_groups;    // depth of the second product; groups that have one (the first rank_groups)
     const void *u_base;       // rows of the second product (host side)
     int u_plane;              // rows between the hi and the lo plane of u
@@ -52,16 +51,15 @@ struct TcRows {
 };
 
 struct TcPipe {
-    uint64_t full[12], empty[12], landed[12], tmem_full[2], tmem_empty[2];  // of a pair's full and tmem_empty the first block's count
+    uint64_t full[12], empty[12], tmem_full[2], tmem_empty[2];  // of a pair's full and tmem_empty the first block's count
     uint32_t tmem;
     int gave_up;
 };
 
-__device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, int full_count, bool paired) {
+__device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, bool paired) {
     for (int i = 0; i < stages; ++i) {
-        mbar_init(smem_addr(&pipe.full[i]), full_count);
+        mbar_init(smem_addr(&pipe.full[i]), 1);
         mbar_init(smem_addr(&pipe.empty[i]), 1);
-        mbar_init(smem_addr(&pipe.landed[i]), 128);  // every copying thread, as its copies land
     }
     for (int i = 0; i < 2; ++i) {
         mbar_init(smem_addr(&pipe.tmem_full[i]), 1);
@@ -136,7 +134,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (lane >= d) scan += o;
         }
         if (lane == 31) s_sum[warp] = scan;
-        if (tid == 0) pipe_init(pipe, stages, 1, PAIRED);
+        if (tid == 0) pipe_init(pipe, stages, PAIRED);
         if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), S::kColumns);
         __syncthreads();
         for (int w = 0; w < warp; ++w) scan += s_sum[w];
@@ -187,8 +185,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             else atomicOr(a.status, kStatusBadIndex);
         }
     };
-    const bool copies = warp >= 8 && a.gather;
-    if (copies) fetch_rows(worker);
+    const bool loads_rows = warp >= 8 && a.gather;
+    if (loads_rows) fetch_rows(worker);
     const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);  // where loads are reported
     RingAt pos;  // this warp's place in the ring
 
@@ -239,11 +237,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 }
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
-        } else if (copies) {
+        } else if (loads_rows) {
             row = next_row;
             fetch_rows(tile + workers);  // under way while this tile is loaded
             for (int s = s0; s < s1; ++s, pos.next(stages)) {
                 const int st = pos.stage;
+                // every use of a stage is waited for, also where nothing is loaded: a parity tells neighbouring uses apart only
                 mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                 __syncwarp();
                 if (s >= main_steps) continue;
@@ -334,12 +333,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
 
 // tc_outer_kernel: out[g][f, c] = sum over the slots s of group g of P[.., f] Q[s, c] - the gradient by a group's matrix.  The
 // summed index is the slot, so both operands lie across it (MN-major): a stage holds 64 slots of 128 features of P and of up
-// to NT columns of Q in blocks of 64.  Whole slices of rows in slot order come by TMA, a box per block; gathered rows and the
-// last slice of a group by the copying warps, which put zeros behind the group's end, whatever lies there.
+// to NT columns of Q in blocks of 64.  Whole slices of rows in slot order come as a box per block; gathered rows and the last
+// slice of a group by row number, those behind the group's end named out of range: zeros, whatever lies there.
 // With `pair` a block of columns of Q is a hi and a lo plane, added up when the result is stored.
 struct TcOuter {
-    CUtensorMap p, q;
-    const uint16_t *p_base, *q_base;
+    CUtensorMap p_rows, p_tile, q_rows, q_tile;  // boxes of one row / of 64
     const int *group_ptr, *slot_row;  // slot_row: rows of P (NULL: in slot order)
     int n_groups, n_slots, n_p_rows;
     int i, j;                         // features of P, columns of Q
@@ -373,7 +371,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     constexpr bool PAIRED = S::kPaired;
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
-    if (tid == 0) pipe_init(pipe, stages, 1 + (PAIRED ? 2 : 1), PAIRED);
+    if (tid == 0) pipe_init(pipe, stages, PAIRED);
     if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), 2 * NT);
     tc_fence_before();
     __syncthreads();
@@ -404,15 +402,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     const int st = pos.stage, slot = slots.x + s * kTcDepth;
                     mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                     const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
-                    if (slot + kTcDepth > slots.y) {
-                        if (half == 0) mbar_arrive(bar);
-                        continue;
-                    }
-                    if (half == 0) mbar_expect(bar, (PAIRED ? 2 : 1) * ((gather ? 0 : p_blocks) + q_blocks) * kBlock64);
+                    if (half == 0) mbar_expect(bar, (PAIRED ? 2 : 1) * (p_blocks + q_blocks) * kBlock64);
+                    if (slot + kTcDepth > slots.y) continue;  // part of a slice: by row number
                     if (!gather)
-                        for (int b = 0; b < p_blocks; ++b) tma_2d<PAIRED>(dst + b * kBlock64, &a.p, f0 + b * 64, slot, bar);
+                        for (int b = 0; b < p_blocks; ++b) tma_2d<PAIRED>(dst + b * kBlock64, &a.p_tile, f0 + b * 64, slot, bar);
                     for (int b = 0; b < q_blocks; ++b)
-                        tma_2d<PAIRED>(dst + (2 + b) * kBlock64, &a.q, a.pair ? c0 : q0 + b * 64, a.pair ? b * a.n_slots + slot : slot, bar);
+                        tma_2d<PAIRED>(dst + (2 + b) * kBlock64, &a.q_tile, a.pair ? c0 : q0 + b * 64, a.pair ? b * a.n_slots + slot : slot, bar);
                 }
             }
         } else if (warp == 1) {
@@ -431,66 +426,59 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
-        } else if (warp == 2) {
-            if (elect_one())  // row copies that have landed: made visible to the tensor cores and reported
-                for (int s = s0; s < s1; ++s, pos.next(stages)) {
-                    const int st = pos.stage;
-                    mbar_wait(smem_addr(&pipe.landed[st]), pos.parity, gave_up, a.status);
-                    fence_async();
-                    mbar_arrive_cluster(full0 + st * 8);
-                }
         } else if (warp >= 8) {
-            // a thread owns 16 bytes of every 16th slot of a block
-            const int chunk = tid & 7, row0 = (tid - 256) >> 3;
-            // row numbers are read four slices ahead: a lane holds one of the warp's 16 rows of two neighbouring slices
+            // rows by number, a quarter of a slice's per warp.  The numbers are read four slices ahead: a lane holds one of the
+            // warp's 16 of two neighbouring slices.
             auto fetch = [&](int s) {
-                const int at = (s + (lane >> 4)) * kTcDepth + (lane >> 2 & 3) * 16 + (warp - 8) * 4 + (lane & 3), slot = slots.x + at;
-                int r = -1;
+                const int slot = slots.x + (s + (lane >> 4)) * kTcDepth + (warp - 8) * 16 + (lane & 15);
+                int r = a.n_p_rows;  // out of range: zeros
                 if (s + (lane >> 4) < s1 && slot < slots.y) {
                     r = gather ? a.slot_row[slot] : slot;
                     if ((unsigned)r >= (unsigned)a.n_p_rows) {
                         atomicOr(a.status, kStatusBadIndex);
-                        r = -1;
+                        r = a.n_p_rows;
                     }
                 }
                 return r;
             };
-            int now = fetch(s0), next = fetch(s0 + 2), later = -1;
+            const int q_end = (a.pair ? 2 : 1) * a.n_slots;  // out of range of Q
+            int now = fetch(s0), next = fetch(s0 + 2), later = a.n_p_rows;
             for (int s = s0; s < s1; ++s, pos.next(stages)) {
-                const int odd = (s - s0) & 1;
+                const int odd = (s - s0) & 1, mine = now;
                 if (!odd) later = fetch(s + 4);
-                int row[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) row[i] = __shfl_sync(0xffffffffu, now, odd * 16 + i * 4 + (lane >> 3));
-                if (odd) {
+                else {
                     now = next;
                     next = later;
                 }
                 const int st = pos.stage, slot = slots.x + s * kTcDepth;
                 const bool last = slot + kTcDepth > slots.y;
+                // every use of a stage is waited for, also where nothing is loaded: a parity tells neighbouring uses apart only
                 mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
-                const uint32_t dst = ring + st * S::kStage + swizzled(row0, chunk);
-                if (gather || last)
-                    for (int b = 0; b < p_blocks; ++b) {
-                        const int f = f0 + b * 64 + chunk * 8;
+                __syncwarp();
+                const uint32_t dst = ring + st * S::kStage + (warp - 8) * 16 * 128, bar = full0 + st * 8;
+                if (gather || last) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const bool valid = row[i] >= 0 && f < a.i;
-                            copy_16(dst + b * kBlock64 + i * 2048, valid ? a.p_base + (long long)row[i] * a.i + f : a.p_base, valid);
+                    for (int q = 0; q < 4; ++q) {
+                        const int from = odd * 16 + 4 * q;
+                        const int r0 = __shfl_sync(0xffffffffu, mine, from), r1 = __shfl_sync(0xffffffffu, mine, from + 1);
+                        const int r2 = __shfl_sync(0xffffffffu, mine, from + 2), r3 = __shfl_sync(0xffffffffu, mine, from + 3);
+                        if (elect_one()) {
+                            tma_rows<PAIRED>(dst + q * 512, &a.p_rows, f0, r0, r1, r2, r3, bar);
+                            if (p_blocks > 1) tma_rows<PAIRED>(dst + kBlock64 + q * 512, &a.p_rows, f0 + 64, r0, r1, r2, r3, bar);
                         }
                     }
-                if (last)
-                    for (int b = 0; b < q_blocks; ++b) {
-                        const int c = (a.pair ? c0 : q0 + b * 64) + chunk * 8;
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const int at = slot + row0 + 16 * i;
-                            const bool valid = at < slots.y && c < a.j;
-                            const long long line = (a.pair ? (long long)b * a.n_slots : 0) + at;
-                            copy_16(dst + (2 + b) * kBlock64 + i * 2048, valid ? a.q_base + line * a.j + c : a.q_base, valid);
+                }
+                if (last) {
+                    for (int q = 0; q < 4; ++q) {
+                        const int first = slot + (warp - 8) * 16 + 4 * q;
+                        for (int b = 0; b < q_blocks; ++b) {
+                            const int plane = a.pair ? b * a.n_slots : 0;
+                            auto line = [&](int i) { return first + i < slots.y ? plane + first + i : q_end; };
+                            if (elect_one())
+                                tma_rows<PAIRED>(dst + (2 + b) * kBlock64 + q * 512, &a.q_rows, a.pair ? c0 : q0 + b * 64, line(0), line(1), line(2), line(3), bar);
                         }
                     }
-                copy_arrive(smem_addr(&pipe.landed[st]));
+                }
             }
         } else if (warp >= 4) {
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
@@ -552,7 +540,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             cluster_sync();
         }
     }
-    if (warp >= 8) copy_drain();
     if (*gave_up) __nanosleep(1000000);
     tc_fence_before();
     __syncthreads();

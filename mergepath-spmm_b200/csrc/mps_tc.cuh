@@ -110,18 +110,6 @@ __device__ __forceinline__ void tma_rows(uint32_t dst, const CUtensorMap *map, i
 }
 __device__ __forceinline__ void tma_prefetch(const CUtensorMap *map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
-// ---- 16 bytes from global to shared memory without a register between; zeros where !valid (nothing is read then)
-__device__ __forceinline__ void copy_16(uint32_t dst, const void *src, bool valid) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
-}
-// an arrival at the barrier once all of this thread's copies so far have landed
-__device__ __forceinline__ void copy_arrive(uint32_t bar) { asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory"); }
-__device__ __forceinline__ void copy_drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
-// ordinary writes to shared memory that this thread knows of become visible to the tensor cores' reads ordered behind it
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-// byte offset of 16-byte chunk c (0..7) of a 128-byte row in the 128-byte swizzle
-__device__ __forceinline__ uint32_t swizzled(int row, int c) { return (uint32_t)row * 128 + (uint32_t)((c ^ (row & 7)) << 4); }
-
 // ---- tcgen05; PAIRED: by two neighbouring blocks of a cluster as one, the products issued by the first for both
 template <bool PAIRED>
 __device__ __forceinline__ void tmem_alloc(uint32_t where, uint32_t columns) {
@@ -224,7 +212,7 @@ __device__ __forceinline__ uint32_t in_first(uint32_t addr) {
     return remote;
 }
 // Arrives at a barrier of either block.  (With .release.cluster the arrival waits for the thread's writes to reach the cluster,
-// about a microsecond; what it orders here are writes of the asynchronous proxy that had landed before, see fence_async.)
+// about a microsecond; it follows no writes here that the other block reads.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
     uint32_t remote;
