@@ -3,6 +3,7 @@
 
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <initializer_list>
 
 #include "mps_internal.h"
@@ -203,21 +204,23 @@ int tensor_map(CUtensorMap *map, bool bf16, const void *base, int dims, unsigned
     return MPS_OK;
 }
 
-// A launch of `blocks` blocks in clusters of `split`.
+// A launch of `blocks` blocks in clusters; `ahead`: it may start before the launch in front of it has ended.
 template <typename Kernel, typename Args>
-int launch_tc(Kernel kernel, const Args &args, long long blocks, int split, size_t smem, cudaStream_t st) {
+int launch_tc(Kernel kernel, const Args &args, long long blocks, int cluster, size_t smem, bool ahead, cudaStream_t st) {
     RD_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = split;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = cluster;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)blocks);
     cfg.blockDim = dim3(mps::kTcThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = ahead ? 2 : 1;
     RD_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
     return MPS_OK;
 }
@@ -229,36 +232,61 @@ int split_of(long long tiles, int steps, int sms) {
     return split;
 }
 
+// How the rows of a product are cut: slots per tile and blocks per tile's sum, by an estimate of the time in SM cycles.  A step of
+// 64 summed elements takes the longest of its products (2 cycles a slot and 128 features), its bytes (64 a cycle and SM out of
+// L2) and its gathered rows (4.3 cycles each); a tile costs 1,500 cycles more where nothing overlaps its first loads and last
+// stores, 2,500 where a cluster adds its parts.  Measured: 32,768 slots of 32 groups, 2048 x 2048: 250 us with 256 slots per
+// tile; 32 slots of 64 groups, 1024 x 2048: 28 us with 32.
+struct Cut {
+    int nt, split;
+    double cycles;
+};
+Cut best_cut(int slots, int groups, int features, int steps, bool gather, int sms, int most_nt) {
+    const double active = groups == 1 ? 1.0 : groups * (1.0 - std::pow(1.0 - 1.0 / groups, (double)slots));  // groups that slots chosen evenly meet
+    Cut best = {32, 1, 1e30};
+    for (int nt = 32; nt <= most_nt; nt *= 2) {
+        const bool paired = nt == 256;
+        const int loaded = paired ? mps::TcShape<256>::kRows : nt, tile_f = paired ? 256 : 128;
+        const double per = slots / active, tiles_of_group = groups == 1 ? std::ceil(per / nt) : std::fmax(1.0, per / nt + 0.5);
+        const double tiles = active * tiles_of_group * ((features + tile_f - 1) / tile_f);
+        const double bytes = 128.0 * ((features < 128 ? features : 128) + loaded);
+        const double step = std::fmax(std::fmax(2.0 * nt + 20, bytes / 64), gather ? 4.3 * loaded : 0.0);
+        for (int split = 1; split <= (nt <= 64 ? 8 : 1); split *= 2) {
+            if (split > 1 && steps < 2 * split) break;  // two slices each at least
+            const double waves = std::ceil(tiles / (sms / (paired ? 2 : split)) - 0.05);
+            const double cycles = waves * (std::ceil((double)steps / split) * step + (split > 1 ? 2500 : 1500));
+            if (cycles < best.cycles) best = {nt, split, cycles};
+        }
+    }
+    return best;
+}
+
 template <int NT>
-int launch_tc_rows(TcRows a, int sms, cudaStream_t st) {
+int launch_tc_rows(const TcRows &a, int sms, cudaStream_t st) {
     // a group ends in a part of a tile, so there are at most this many
     const long long most = a.n_slots / NT + (a.n_groups < a.n_slots ? a.n_groups : a.n_slots);
     const int tile_f = mps::kTcFeatures * (mps::TcShape<NT>::kPaired ? 2 : 1);
     const long long tiles = most * ((a.n + tile_f - 1) / tile_f);
-    a.split = NT <= 64 ? split_of(tiles, (a.k + mps::kTcDepth - 1) / mps::kTcDepth, sms) : 1;
     const int cluster = mps::TcShape<NT>::kPaired ? 2 : a.split;
     const long long workers = sms / cluster;
-    return launch_tc(mps::tc_rows_kernel<NT>, a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcShape<NT>::bytes(a.n_groups), st);
+    return launch_tc(mps::tc_rows_kernel<NT>, a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcShape<NT>::bytes(a.n_groups), a.ahead, st);
 }
 
-// The rest of a filled in: what every use has in common, and the tile for the mean number of rows per group.
-int tc_rows(TcRows a, const void *x, long long x_rows, cudaStream_t st) {
+// The rest of a filled in: what every use has in common.
+int tc_rows(TcRows a, const Cut &cut, const void *x, long long x_rows, int sms, cudaStream_t st) {
     if (int rc = status_pointer(&a.status)) return rc;
-    int sms;
-    if (int rc = sm_count(&sms)) return rc;
-    const int groups = a.n_groups < a.n_slots ? a.n_groups : a.n_slots;
-    const long long mean = a.n_slots / groups;
-    const int nt = mean <= 20 ? 32 : mean <= 48 ? 64 : mean <= 128 ? 128 : 256;
-    const int loaded = nt == 256 ? mps::TcShape<256>::kRows : nt;  // slots a block loads
+    a.split = cut.split;
+    const int loaded = cut.nt == 256 ? mps::TcShape<256>::kRows : cut.nt;  // slots a block loads
     if (int rc = tensor_map(&a.x, a.bf16, x, 2, a.k, x_rows, 1, a.gather ? 1 : loaded)) return rc;
-    if (a.rank) {
+    if (a.rank)
         if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded)) return rc;
-    }
-    if (nt == 32) return launch_tc_rows<32>(a, sms, st);
-    if (nt == 64) return launch_tc_rows<64>(a, sms, st);
-    if (nt == 128) return launch_tc_rows<128>(a, sms, st);
+    if (cut.nt == 32) return launch_tc_rows<32>(a, sms, st);
+    if (cut.nt == 64) return launch_tc_rows<64>(a, sms, st);
+    if (cut.nt == 128) return launch_tc_rows<128>(a, sms, st);
     return launch_tc_rows<256>(a, sms, st);
 }
+
+int steps_of(int summed) { return (summed + mps::kTcDepth - 1) / mps::kTcDepth; }
 
 // The matrices of a: stored features x summed (MN-major: summed x features), `groups` of them.
 int tc_matrix(CUtensorMap *map, TcRows *a, const void *w, int summed, int features, long long groups) {
@@ -276,7 +304,7 @@ int launch_tc_outer(TcOuter a, int sms, cudaStream_t st) {
     a.split = NT <= 128 ? split_of(tiles, steps, sms) : 1;
     const int cluster = mps::TcOuterShape<NT>::kPaired ? 2 : a.split;
     const long long workers = sms / cluster;
-    return launch_tc(mps::tc_outer_kernel<NT>, a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcOuterShape<NT>::kBytes, st);
+    return launch_tc(mps::tc_outer_kernel<NT>, a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcOuterShape<NT>::kBytes, false, st);
 }
 
 // P: n_p_rows rows of a.i, by a.slot_row or in slot order; Q: rows of a.j in slot order (pair: two planes of them).
@@ -358,10 +386,10 @@ int adapter_wide(const AdapterShape &s, int k, int n, const void *x, const void 
     return launch_plain_rows<T, T, true>(a, x, w, m, out, st);
 }
 
-// Workspace: the two intermediates (fp32 by row, or hi and lo planes by slot: 4 bytes a value either way), then the rows listed
-// with those that ask for no adapter behind the others.
+// Workspace: the two intermediates (fp32 by row, or hi and lo planes by slot: 4 bytes a value either way), the gradient's second
+// one in fp32 as well, then the rows listed with those that ask for no adapter behind the others.
 struct AdapterSpace {
-    char *u, *v;
+    char *u, *v, *v_f32;
     int *ptr, *row;
     int64_t bytes;
     AdapterSpace(void *base, int n_rows, int n_adapters, int rank, bool backward) {
@@ -373,14 +401,16 @@ struct AdapterSpace {
         };
         u = take((int64_t)n_rows * rank * 4);
         v = backward ? take((int64_t)n_rows * rank * 4) : nullptr;
+        v_f32 = backward ? take((int64_t)n_rows * rank * 4) : nullptr;
         ptr = (int *)take(4ll * (n_adapters + 2));
         row = (int *)take(4ll * n_rows);
         bytes = at - (char *)base;
     }
 };
 
-// u (two planes, slot order) = scale * rows of x times the adapters' matrices (mn_major: stored summed x rank)
-int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m, bool mn_major, void *u, cudaStream_t st) {
+// u (two planes, slot order) = scale * rows of x times the adapters' matrices (mn_major: stored summed x rank); u_f32 (or NULL)
+// the same by row
+int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m, bool mn_major, void *u, float *u_f32, int sms, cudaStream_t st) {
     TcRows a = {};
     a.bf16 = s.dtype == MPS_BF16;
     a.mn_major = mn_major;
@@ -394,31 +424,59 @@ int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m
     a.group_scale = s.scale;
     a.out = u;
     a.out_plane = (long long)s.n_rows * s.rank;
+    a.out_f32 = u_f32;
     if (int rc = tc_matrix(&a.w, &a, m, k, s.rank, s.n_adapters)) return rc;
-    return tc_rows(a, x, s.n_rows, st);
+    return tc_rows(a, best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(k), true, sms, 256), x, s.n_rows, sms, st);
 }
 
-// out = x times the shared matrix, the sum going on with u times the adapter's matrix; rows by adapter, those without one last
-int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, int k, int n, const void *x, const void *w, const void *u, const void *m, bool mn_major,
-                    void *out, cudaStream_t st) {
+// Whether the shared matrix is read once for rows of any adapter, the low-rank part added in fp32 by the warps that store the
+// results (about a quarter of an SM's 128 multiply-adds a cycle), or per adapter, the low-rank part summed on the tensor cores.
+// Measured at 4096 x 4096 in bf16: 64 rows of 24 adapters of rank 16 take ADAPT_A us by rows and ADAPT_B by adapter, 4096 rows
+// of 8 adapters of rank 64 ADAPT_C by adapter and ADAPT_D by rows.
+bool by_rows(const AdapterShape &s, int k, int n, int sms, Cut *cut) {
+    const Cut grouped = best_cut(s.n_rows, s.n_adapters + 1, n, steps_of(k) + 2 * steps_of(s.rank), true, sms, 256);
+    const Cut rows = best_cut(s.n_rows, 1, n, steps_of(k), false, sms, 64);
+    const double low_rank = (double)s.n_rows * n * s.rank / (32.0 * sms);
+    *cut = rows.cycles + low_rank < grouped.cycles ? rows : grouped;
+    return rows.cycles + low_rank < grouped.cycles;
+}
+
+// out = x times the shared matrix plus u times the row's adapter matrix m; u_f32 by row (by_rows) or u in planes by slot.
+int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cut, bool rows, int k, int n, const void *x, const void *w, const void *u,
+                    const float *u_f32, const void *m, bool mn_major, void *out, bool ahead, int sms, cudaStream_t st) {
     TcRows a = {};
     a.bf16 = s.dtype == MPS_BF16;
     a.mn_major = mn_major;
-    a.group_ptr = ws.ptr;
-    a.slot_row = ws.row;
-    a.n_groups = s.n_adapters + 1;
     a.n_slots = a.n_x_rows = s.n_rows;
     a.k = k;
     a.n = n;
+    a.w_shared = true;
+    a.out = out;
+    if (int rc = tc_matrix(&a.w, &a, w, k, n, 1)) return rc;
+    if (rows) {
+        a.n_groups = 1;
+        a.ids = s.ids;
+        a.delta_u = u_f32;
+        a.delta_m = (const uint16_t *)m;
+        a.delta_adapters = s.n_adapters;
+        a.delta_rank = s.rank;
+        a.delta_group = (long long)n * s.rank;
+        a.delta_f = mn_major ? 1 : s.rank;
+        a.delta_r = mn_major ? n : 1;
+        a.ahead = ahead;
+        return tc_rows(a, cut, x, s.n_rows, sms, st);
+    }
+    if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
+    a.group_ptr = ws.ptr;
+    a.slot_row = ws.row;
+    a.n_groups = s.n_adapters + 1;
     a.rank = s.rank;
     a.rank_groups = s.n_adapters;
     a.u_base = u;
     a.u_plane = s.n_rows;
-    a.w_shared = a.gather = a.scatter = true;
-    a.out = out;
-    if (int rc = tc_matrix(&a.w, &a, w, k, n, 1)) return rc;
+    a.gather = a.scatter = true;
     if (int rc = tc_matrix(&a.w2, &a, m, s.rank, n, s.n_adapters)) return rc;
-    return tc_rows(a, x, s.n_rows, st);
+    return tc_rows(a, cut, x, s.n_rows, sms, st);
 }
 
 int tc_adapter_outer(const AdapterShape &s, int features, const void *p, const void *q, void *out, long long out_f, long long out_c, cudaStream_t st) {
@@ -442,9 +500,18 @@ template <typename T>
 int adapters(const AdapterShape &s, const void *x, const void *w, const void *a, const void *b, void *y, void *workspace, cudaStream_t st) {
     const AdapterSpace ws(workspace, s.n_rows, s.n_adapters, s.rank, false);
     if (tc_widths(s.dtype, {s.k, s.rank}, {x, w, a, b})) {
-        if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
-        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, st)) return rc;
-        return tc_adapter_wide(s, ws, s.k, s.n, x, w, ws.u, b, false, y, st);
+        int sms, *status;
+        Cut cut;
+        if (int rc = sm_count(&sms)) return rc;
+        if (int rc = status_pointer(&status)) return rc;
+        const bool rows = by_rows(s, s.k, s.n, sms, &cut);
+        if (rows) {
+            const dim3 grid((unsigned)s.n_rows, (unsigned)((s.rank + 7) / 8));
+            mps::adapter_dots_kernel<<<grid, 256, 0, st>>>(s.k, s.rank, s.n_adapters, s.dtype == MPS_BF16, s.ids, s.scale, (const uint16_t *)x,
+                                                           (const uint16_t *)a, (float *)ws.u, status);
+            RD_CUDA(cudaGetLastError());
+        } else if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, sms, st)) return rc;
+        return tc_adapter_wide(s, ws, cut, rows, s.k, s.n, x, w, ws.u, (const float *)ws.u, b, false, y, rows, sms, st);
     }
     float *u = (float *)ws.u;
     if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
@@ -456,10 +523,13 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
                       void *workspace, cudaStream_t st) {
     const AdapterSpace ws(workspace, s.n_rows, s.n_adapters, s.rank, true);
     if (tc_widths(s.dtype, {s.k, s.n, s.rank}, {dy, x, w, a, b})) {
-        if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
-        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, st)) return rc;    // scale * x A^T
-        if (int rc = tc_adapter_narrow(s, s.n, dy, b, true, ws.v, st)) return rc;    // scale * dy B
-        if (int rc = tc_adapter_wide(s, ws, s.n, s.k, dy, w, ws.v, a, true, dx, st)) return rc;
+        int sms;
+        Cut cut;
+        if (int rc = sm_count(&sms)) return rc;
+        const bool rows = by_rows(s, s.n, s.k, sms, &cut);
+        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, sms, st)) return rc;                               // scale * x A^T
+        if (int rc = tc_adapter_narrow(s, s.n, dy, b, true, ws.v, rows ? (float *)ws.v_f32 : nullptr, sms, st)) return rc;  // scale * dy B
+        if (int rc = tc_adapter_wide(s, ws, cut, rows, s.n, s.k, dy, w, ws.v, (const float *)ws.v_f32, a, true, dx, false, sms, st)) return rc;
         if (int rc = tc_adapter_outer(s, s.k, x, ws.v, da, 1, s.k, st)) return rc;
         return tc_adapter_outer(s, s.n, dy, ws.u, db, s.rank, 1, st);
     }
@@ -532,8 +602,10 @@ extern "C" int mps_routed_product(int32_t n_slots, int32_t n_rows, int32_t n_gro
         a.n = features;
         a.gather = d_slot_row != nullptr;
         a.out = d_y;
+        int sms;
+        if (int rc = sm_count(&sms)) return rc;
         if (int rc = tc_matrix(&a.w, &a, d_w, summed, features, n_groups)) return rc;
-        return tc_rows(a, d_x, n_rows, (cudaStream_t)stream);
+        return tc_rows(a, best_cut(n_slots, n_groups, features, steps_of(summed), a.gather, sms, 256), d_x, n_rows, sms, (cudaStream_t)stream);
     }
     RowsArgs a = {};
     a.group_ptr = d_group_ptr;

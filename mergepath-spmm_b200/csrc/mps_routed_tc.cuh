@@ -4,8 +4,8 @@
 // fill the 128 lanes of TMEM whatever the number of routed rows is; the slots are the columns, NT of them per tile (32 where a
 // few rows meet each matrix and its bytes are what counts, 256 where the arithmetic does).  The matrices come by TMA in 64-deep
 // slices through a ring of stages, rows in slot order too; gathered rows by number, four per TMA instruction, issued by one
-// elected lane of each of four warps (2.3 us a slice of 256 rows from 32 diverged lanes of one warp; 16-byte asynchronous copies
-// by 128 threads took 0.45 us for 128 rows, these 0.3).  Two accumulators in TMEM alternate, so a tile is stored while the next one is summed; results go through shared
+// elected lane of each of eight warps: 0.29 us for 128 rows of a slice, about what the TMA unit gives (0.35 us from four warps,
+// 0.45 us as 16-byte asynchronous copies by 128 threads, 1.2 us from 32 diverged lanes of one warp).  Two accumulators in TMEM alternate, so a tile is stored while the next one is summed; results go through shared
 // memory, where 32 slots by 128 features become whole 256-byte rows.
 //
 // A tile's sum may go on with a second product (`rank` > 0): the group's low-rank matrix times rows u that were computed before,
@@ -17,14 +17,18 @@
 // Both blocks' loads arrive at the first one's barriers; it issues the products for both, and each stores the features it holds.
 //
 // Few tiles with long sums are cut along the sum over the blocks of a cluster; the partial results meet in distributed shared
-// memory, added in the order of the blocks.
+// memory, added in the order of the blocks by the warps that store results, while the others are at the next tile.
+//
+// For a few rows of many adapters the shared matrix must not be read once per adapter.  Then the tiles hold rows of any adapter,
+// and the result warps add u times the row's own low-rank matrix themselves (`delta`), computed in fp32 while the slices of
+// the shared matrix are still coming.
 #pragma once
 #include "mps_routed_plain.cuh"
 #include "mps_tc.cuh"
 
 namespace mps {
 
-constexpr int kTcThreads = 384;  // warps: 0 TMA, 1 products, 2-3 none, 4-7 results (TMEM lanes go by warp number mod 4), 8-11 row loads
+constexpr int kTcThreads = 512;  // warps: 0 TMA, 1 products, 2-3 none, 4-7 results (TMEM lanes go by warp number mod 4), 8-15 row loads
 constexpr int kTcFeatures = 128;
 constexpr int kTcDepth = 64;
 constexpr int kTcRing = 192 * 1024;            // shared memory of the stages
@@ -46,17 +50,25 @@ struct TcRows {
     const float *group_scale;
     void *out;
     long long out_plane;
+    float *out_f32;           // pair: the result in fp32 too, by row (NULL: not wanted)
+    const int *ids;           // delta: adapter of a row,
+    const float *delta_u;     //   the rows' intermediates (by row, delta_rank each),
+    const uint16_t *delta_m;  //   the adapters' matrices with their strides by adapter, feature and rank index
+    int delta_adapters, delta_rank;
+    long long delta_group, delta_f, delta_r;
+    bool ahead;               // launched before the end of the launch that computes delta_u
     int split;                // blocks of a cluster, each with its part of the sum
     int *status;
 };
 
 struct TcPipe {
     uint64_t full[12], empty[12], tmem_full[2], tmem_empty[2];  // of a pair's full and tmem_empty the first block's count
+    uint64_t partials, freed;                                   // split: every block's part is in its shared memory / has been read
     uint32_t tmem;
     int gave_up;
 };
 
-__device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, bool paired) {
+__device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, bool paired, int split) {
     for (int i = 0; i < stages; ++i) {
         mbar_init(smem_addr(&pipe.full[i]), 1);
         mbar_init(smem_addr(&pipe.empty[i]), 1);
@@ -65,8 +77,17 @@ __device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, bool paired)
         mbar_init(smem_addr(&pipe.tmem_full[i]), 1);
         mbar_init(smem_addr(&pipe.tmem_empty[i]), paired ? 256 : 128);
     }
+    mbar_init(smem_addr(&pipe.partials), 4 * split);  // a lane of each of the four result warps of every block
+    mbar_init(smem_addr(&pipe.freed), 4 * split);
     pipe.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+
+// One of the result warps tells those of all blocks of the cluster.
+__device__ __forceinline__ void tell_cluster(uint32_t bar, int split, int lane) {
+    fence_cluster();
+    __syncwarp();
+    if (lane < split) mbar_arrive_at(bar, lane);
 }
 
 constexpr int stages_for(int bytes, int stage) { return bytes / stage < 12 ? bytes / stage : 12; }
@@ -105,14 +126,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     int *first = reinterpret_cast<int *>(s_raw + (ring - smem_addr(s_raw)) + kTcRing + kOutTotal);
     int *lo = first + a.n_groups + 1, *hi = lo + a.n_groups;
     const int split = a.split, part = split > 1 ? (int)cluster_rank() : 0;
-    const int stages = split > 1 ? S::kSplitStages : S::kStages;
-    const uint32_t partial = ring + (uint32_t)S::kSplitStages * S::kStage;  // split only
+    const bool reduce = split > 1 || a.ids;  // results meet in shared memory before they are stored
+    const int stages = reduce ? S::kSplitStages : S::kStages;
+    const uint32_t partial = ring + (uint32_t)S::kSplitStages * S::kStage;
     constexpr bool PAIRED = S::kPaired;
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
 
     // ---- tiles of the groups
     {
-        constexpr int PER = kMaxRowGroups / kTcThreads + 1;  // a list with the ungrouped rows has one group more
+        constexpr int PER = (kMaxRowGroups + 1 + kTcThreads - 1) / kTcThreads;  // a list with the ungrouped rows has one group more
         int tiles[PER], sum = 0;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
@@ -134,7 +156,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (lane >= d) scan += o;
         }
         if (lane == 31) s_sum[warp] = scan;
-        if (tid == 0) pipe_init(pipe, stages, PAIRED);
+        if (tid == 0) pipe_init(pipe, stages, PAIRED, split);
         if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), S::kColumns);
         __syncthreads();
         for (int w = 0; w < warp; ++w) scan += s_sum[w];
@@ -148,7 +170,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
         }
         tc_fence_before();
         __syncthreads();
-        if (PAIRED) cluster_sync();  // the pair's barriers exist before either arrives at them
+        if (PAIRED || split > 1) cluster_sync();  // the cluster's barriers exist before anyone arrives at them
         tc_fence_after();
     }
     const uint32_t tmem = pipe.tmem;
@@ -170,8 +192,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     // columns of a tile's products: only as many as there are slots, so that the last tile of a group costs what it holds
     auto columns_of = [](const TcCursor &c) { return PAIRED ? (c.slot1 - c.slot0 + 31) & ~31 : (c.slot1 - c.slot0 + 15) & ~15; };
 
-    // gathered rows: a warp loads a quarter of a slice's, a lane holding one row's number
-    constexpr int RPW = S::kRows / 4;
+    // gathered rows: a warp loads an eighth of a slice's, a lane holding one row's number
+    constexpr int RPW = S::kRows / 8;
     int row = 0, next_row = 0;
     TcCursor ahead = cur;
     auto fetch_rows = [&](long long tile) {
@@ -255,8 +277,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 }
             }
         } else if (warp >= 4 && warp < 8) {
-            mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
-            tc_fence_after();
             const int quad = warp & 3, f = f0 + quad * 32 + lane, mine = tid - 128;
             const float scale = a.group_scale ? a.group_scale[g] : 1.0f;
             uint16_t *out = (uint16_t *)a.out;
@@ -265,22 +285,84 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 const int r = a.slot_row[slot];
                 return (unsigned)r < (unsigned)a.n_x_rows ? r : -1;
             };
-            auto store = [&](int r, float v) {
+            auto store = [&](int slot, float v) {
+                const int r = out_row(slot);
                 if (f >= a.n || r < 0) return;
                 const long long at = (long long)r * a.n + f;
                 const uint16_t h = to_16(v, a.bf16);
                 out[at] = h;
-                if (a.pair) out[at + a.out_plane] = to_16(v - from_16(h, a.bf16), a.bf16);
+                if (a.pair) {
+                    out[at + a.out_plane] = to_16(v - from_16(h, a.bf16), a.bf16);
+                    if (a.out_f32) {
+                        const int line = a.slot_row[slot];
+                        if ((unsigned)line < (unsigned)a.n_x_rows) a.out_f32[(long long)line * a.n + f] = v;
+                    }
+                }
             };
-            const bool wide = !a.pair && a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
+            const uint32_t own_partial = partial + (quad * 32 + lane) * 4;  // this thread's feature, columns kTcFeatures * 4 bytes apart
+            if (reduce) {
+                mbar_wait(smem_addr(&pipe.freed), (turn & 1) ^ 1, gave_up, a.status);
+                if (a.ids) {
+                    // the columns this block stores start from u times the adapter's matrix: four columns' loads in flight
+                    if (a.ahead && turn == 0) wait_for_launch_before();
+                    for (int c = part; slot0 + c < slot1; c += 4 * split) {
+                        const float *u[4];
+                        const uint16_t *m[4];
+                        float v[4] = {};
+                        bool live[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int slot = slot0 + c + j * split;
+                            int id = slot < slot1 ? a.ids[slot] : -1;
+                            if (id >= a.delta_adapters) {
+                                atomicOr(a.status, kStatusBadIndex);
+                                id = -1;
+                            }
+                            live[j] = id >= 0 && f < a.n;
+                            u[j] = a.delta_u + (long long)(live[j] ? slot : 0) * a.delta_rank;
+                            m[j] = a.delta_m + (live[j] ? id * a.delta_group + f * a.delta_f : 0);
+                        }
+                        for (int r = 0; r < a.delta_rank; r += 8) {  // the rank is a multiple of eight here
+                            uint16_t w[4][8];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if (!live[j]) continue;
+                                if (a.delta_r == 1) *reinterpret_cast<uint4 *>(w[j]) = *reinterpret_cast<const uint4 *>(m[j] + r);
+                                else
+#pragma unroll
+                                    for (int i = 0; i < 8; ++i) w[j][i] = m[j][(r + i) * a.delta_r];
+                            }
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                if (!live[j]) continue;
+                                const float4 p = *reinterpret_cast<const float4 *>(u[j] + r), q = *reinterpret_cast<const float4 *>(u[j] + r + 4);
+                                const float x[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+                                for (int i = 0; i < 8; ++i) v[j] = fmaf(x[i], from_16(w[j][i], a.bf16), v[j]);
+                            }
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            if (slot0 + c + j * split < slot1)
+                                asm volatile("st.shared.f32 [%0], %1;" ::"r"(own_partial + (c + j * split) * (kTcFeatures * 4)), "f"(v[j]) : "memory");
+                    }
+                }
+            }
+            mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
+            tc_fence_after();
+            const bool wide = !reduce && !a.pair && a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
 #pragma unroll 1
             for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 32) {
                 float v[32];
                 tmem_load(tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + c0, v);
-                if (split > 1) {
+                if (reduce) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j)
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(partial + ((c0 + j) * kTcFeatures + quad * 32 + lane) * 4), "f"(v[j]) : "memory");
+                    for (int j = 0; j < 32; ++j) {
+                        const uint32_t at = own_partial + (c0 + j) * (kTcFeatures * 4);
+                        float have = 0.0f;
+                        if (a.ids && (c0 + j) % split == part && slot0 + c0 + j < slot1) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(have) : "r"(at) : "memory");
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v[j] + have) : "memory");
+                    }
                 } else if (wide) {
                     const uint32_t at = staging + (c0 >> 5 & 1) * (32 * kOutPitch);
 #pragma unroll
@@ -298,37 +380,61 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        if (slot0 + c0 + j < slot1) store(out_row(slot0 + c0 + j), v[j] * scale);
+                        if (slot0 + c0 + j < slot1) store(slot0 + c0 + j, v[j] * scale);
                 }
             }
             tc_fence_before();
             if (PAIRED) mbar_arrive_cluster(in_first(smem_addr(&pipe.tmem_empty[buf])));
             else mbar_arrive(smem_addr(&pipe.tmem_empty[buf]));
-            if (split > 1) {
+            if (reduce) {
                 // every block of the cluster adds up and stores its share of the columns
-                cluster_sync();
+                tell_cluster(smem_addr(&pipe.partials), split, lane);
+                mbar_wait(smem_addr(&pipe.partials), turn & 1, gave_up, a.status);
+                fence_cluster();
                 for (int c = part; slot0 + c < slot1; c += split) {
                     float v = 0.0f;
-                    for (int p = 0; p < split; ++p) v += load_peer(partial + (c * kTcFeatures + quad * 32 + lane) * 4, p);
-                    store(out_row(slot0 + c), v * scale);
+                    for (int p = 0; p < split; ++p) v += load_peer(own_partial + c * (kTcFeatures * 4), p);
+                    store(slot0 + c, v * scale);
                 }
-                cluster_sync();  // the partial results may be overwritten, and no block leaves while one still reads its own
+                tell_cluster(smem_addr(&pipe.freed), split, lane);
             } else if (wide) results_sync();  // the next tile starts with the first buffer again
-        }
-        if (split > 1 && (warp < 4 || warp >= 8)) {
-            __syncwarp();
-            cluster_sync();
-            cluster_sync();
         }
     }
     if (*gave_up) __nanosleep(1000000);  // copies in flight land before the block's memory is given back
     tc_fence_before();
     __syncthreads();
-    if (PAIRED) cluster_sync();  // neither block leaves while the other's products or arrivals still reach it
+    if (PAIRED || split > 1) cluster_sync();  // no block leaves while another's products, reads or arrivals still reach it
     if (warp == 1) {
         tc_fence_after();
         tmem_free<PAIRED>(tmem, S::kColumns);
     }
+}
+
+// u[row, r] = scale * <x[row], the row's adapter matrix [r]> in fp32, for a few rows: a warp per value, eight ranks per block.  The
+// launch behind it may start at once; it waits for these values where it needs them.
+__global__ void __launch_bounds__(256) adapter_dots_kernel(int k, int rank, int n_adapters, bool bf16, const int *__restrict__ ids,
+                                                           const float *__restrict__ scale, const uint16_t *__restrict__ x,
+                                                           const uint16_t *__restrict__ m, float *__restrict__ u, int *status) {
+    let_next_launch_start();
+    const int row = blockIdx.x, r = blockIdx.y * 8 + (threadIdx.x >> 5), lane = threadIdx.x & 31, id = ids[row];
+    if (id < 0 || r >= rank) return;
+    if (id >= n_adapters) {
+        if (lane == 0) atomicOr(status, kStatusBadIndex);
+        return;
+    }
+    const uint16_t *p = x + (long long)row * k, *q = m + ((long long)id * rank + r) * k;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int i = lane * 8; i < k; i += 256) {
+        const uint4 a = *reinterpret_cast<const uint4 *>(p + i), b = *reinterpret_cast<const uint4 *>(q + i);
+        const uint32_t v[4] = {a.x, a.y, a.z, a.w}, w[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            sum = fmaf(from_16((uint16_t)(v[j >> 1] >> (j & 1) * 16), bf16), from_16((uint16_t)(w[j >> 1] >> (j & 1) * 16), bf16), sum);
+    }
+#pragma unroll
+    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (lane == 0) u[(long long)row * rank + r] = scale ? sum * scale[id] : sum;
 }
 
 // tc_outer_kernel: out[g][f, c] = sum over the slots s of group g of P[.., f] Q[s, c] - the gradient by a group's matrix.  The
@@ -371,11 +477,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     constexpr bool PAIRED = S::kPaired;
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
-    if (tid == 0) pipe_init(pipe, stages, PAIRED);
+    if (tid == 0) pipe_init(pipe, stages, PAIRED, split);
     if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), 2 * NT);
     tc_fence_before();
     __syncthreads();
-    if (PAIRED) cluster_sync();
+    if (PAIRED || split > 1) cluster_sync();
     tc_fence_after();
     const uint32_t tmem = pipe.tmem;
     volatile int *gave_up = &pipe.gave_up;
@@ -427,12 +533,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
         } else if (warp >= 8) {
-            // rows by number, a quarter of a slice's per warp.  The numbers are read four slices ahead: a lane holds one of the
-            // warp's 16 of two neighbouring slices.
+            // rows by number, an eighth of a slice's per warp.  The numbers are read eight slices ahead: a lane holds one of the
+            // warp's eight of four neighbouring slices.
             auto fetch = [&](int s) {
-                const int slot = slots.x + (s + (lane >> 4)) * kTcDepth + (warp - 8) * 16 + (lane & 15);
+                const int slot = slots.x + (s + (lane >> 3)) * kTcDepth + (warp - 8) * 8 + (lane & 7);
                 int r = a.n_p_rows;  // out of range: zeros
-                if (s + (lane >> 4) < s1 && slot < slots.y) {
+                if (s + (lane >> 3) < s1 && slot < slots.y) {
                     r = gather ? a.slot_row[slot] : slot;
                     if ((unsigned)r >= (unsigned)a.n_p_rows) {
                         atomicOr(a.status, kStatusBadIndex);
@@ -442,26 +548,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 return r;
             };
             const int q_end = (a.pair ? 2 : 1) * a.n_slots;  // out of range of Q
-            int now = fetch(s0), next = fetch(s0 + 2), later = a.n_p_rows;
+            int now = fetch(s0), next = fetch(s0 + 4);
             for (int s = s0; s < s1; ++s, pos.next(stages)) {
-                const int odd = (s - s0) & 1, mine = now;
-                if (!odd) later = fetch(s + 4);
-                else {
+                const int which = (s - s0) & 3;
+                if (which == 0 && s > s0) {
                     now = next;
-                    next = later;
+                    next = fetch(s + 4);
                 }
                 const int st = pos.stage, slot = slots.x + s * kTcDepth;
                 const bool last = slot + kTcDepth > slots.y;
                 // every use of a stage is waited for, also where nothing is loaded: a parity tells neighbouring uses apart only
                 mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                 __syncwarp();
-                const uint32_t dst = ring + st * S::kStage + (warp - 8) * 16 * 128, bar = full0 + st * 8;
+                const uint32_t dst = ring + st * S::kStage + (warp - 8) * 8 * 128, bar = full0 + st * 8;
                 if (gather || last) {
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int from = odd * 16 + 4 * q;
-                        const int r0 = __shfl_sync(0xffffffffu, mine, from), r1 = __shfl_sync(0xffffffffu, mine, from + 1);
-                        const int r2 = __shfl_sync(0xffffffffu, mine, from + 2), r3 = __shfl_sync(0xffffffffu, mine, from + 3);
+                    for (int q = 0; q < 2; ++q) {
+                        const int from = which * 8 + 4 * q;
+                        const int r0 = __shfl_sync(0xffffffffu, now, from), r1 = __shfl_sync(0xffffffffu, now, from + 1);
+                        const int r2 = __shfl_sync(0xffffffffu, now, from + 2), r3 = __shfl_sync(0xffffffffu, now, from + 3);
                         if (elect_one()) {
                             tma_rows<PAIRED>(dst + q * 512, &a.p_rows, f0, r0, r1, r2, r3, bar);
                             if (p_blocks > 1) tma_rows<PAIRED>(dst + kBlock64 + q * 512, &a.p_rows, f0 + 64, r0, r1, r2, r3, bar);
@@ -469,8 +574,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     }
                 }
                 if (last) {
-                    for (int q = 0; q < 4; ++q) {
-                        const int first = slot + (warp - 8) * 16 + 4 * q;
+                    for (int q = 0; q < 2; ++q) {
+                        const int first = slot + (warp - 8) * 8 + 4 * q;
                         for (int b = 0; b < q_blocks; ++b) {
                             const int plane = a.pair ? b * a.n_slots : 0;
                             auto line = [&](int i) { return first + i < slots.y ? plane + first + i : q_end; };
@@ -481,6 +586,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
             }
         } else if (warp >= 4) {
+            if (split > 1) mbar_wait(smem_addr(&pipe.freed), (turn & 1) ^ 1, gave_up, a.status);
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
             tc_fence_after();
             const int quad = warp & 3, f = f0 + quad * 32 + lane, mine = tid - 128;
@@ -525,25 +631,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             if (PAIRED) mbar_arrive_cluster(in_first(smem_addr(&pipe.tmem_empty[buf])));
             else mbar_arrive(smem_addr(&pipe.tmem_empty[buf]));
             if (split > 1) {
-                cluster_sync();
+                tell_cluster(smem_addr(&pipe.partials), split, lane);
+                mbar_wait(smem_addr(&pipe.partials), turn & 1, gave_up, a.status);
+                fence_cluster();
                 for (int c = part; c < cols && c0 + c < a.j; c += split) {
                     float v = 0.0f;
                     for (int p = 0; p < split; ++p) v += load_peer(partial + (c * kTcFeatures + quad * 32 + lane) * 4, p);
                     if (f < a.i) out[f * a.out_f + (c0 + c) * a.out_c] = to_16(v, a.bf16);
                 }
-                cluster_sync();
+                tell_cluster(smem_addr(&pipe.freed), split, lane);
             } else if (wide) results_sync();
-        }
-        if (split > 1 && (warp < 4 || warp >= 8)) {
-            __syncwarp();
-            cluster_sync();
-            cluster_sync();
         }
     }
     if (*gave_up) __nanosleep(1000000);
     tc_fence_before();
     __syncthreads();
-    if (PAIRED) cluster_sync();
+    if (PAIRED || split > 1) cluster_sync();
     if (warp == 1) {
         tc_fence_after();
         tmem_free<PAIRED>(tmem, 2 * NT);

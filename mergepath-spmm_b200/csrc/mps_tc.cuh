@@ -214,6 +214,16 @@ __device__ __forceinline__ uint32_t in_first(uint32_t addr) {
 // Arrives at a barrier of either block.  (With .release.cluster the arrival waits for the thread's writes to reach the cluster,
 // about a microsecond; it follows no writes here that the other block reads.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// the same at block `rank`'s barrier of that address
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(bar), "r"(rank));
+    mbar_arrive_cluster(remote);
+}
+__device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
+// Waits for the launch before this one on the stream, where this one was allowed to start ahead of its end.
+__device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
     uint32_t remote;
     float v;
