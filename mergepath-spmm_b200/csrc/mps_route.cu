@@ -38,6 +38,7 @@ constexpr unsigned kAll = 0xffffffffu;
 
 struct RouteArgs {
     int n_rows, n_experts, top_k, n_groups, per_group, top_groups, group_top;
+    unsigned group_inverse;  // 2^32 / per_group rounded up: experts stay below 2^16, so mulhi by it is the quotient (0: per_group 1)
     bool renormalise;
     float scale;
 };
@@ -49,13 +50,9 @@ __device__ __forceinline__ float neg_inf<float>() { return -INFINITY; }
 template <>
 __device__ __forceinline__ double neg_inf<double>() { return -(double)INFINITY; }
 
-__device__ __forceinline__ float exp_of(float x) { return expf(x); }
-__device__ __forceinline__ double exp_of(double x) { return exp(x); }
-
-template <typename F>
-__device__ __forceinline__ F sigmoid(F x) {  // exp of a number <= 0 only: no overflow, and small scores keep their digits
-    const F e = exp_of(x < (F)0 ? x : -x);
-    return (x < (F)0 ? e : (F)1) / ((F)1 + e);
+__device__ __forceinline__ float sigmoid(float x) {  // exp of a number <= 0 only: no overflow, and small scores keep their digits
+    const float e = expf(x < 0.0f ? x : -x);
+    return (x < 0.0f ? e : 1.0f) / (1.0f + e);
 }
 
 template <typename F>
@@ -96,13 +93,27 @@ __device__ __forceinline__ void warp_best(double &v, int &at) {
     }
 }
 
-// How far apart two fp32 keys must be for their order to be that of the exact ones: a score in [0, 1] is off by less than
-// 1e-6 (exponential, sum and quotient, a few units in the last place each), a key s + b by another half unit of itself.
-__device__ __forceinline__ float clearance(float key) { return 4e-6f + 2.5e-7f * fabsf(key); }
+// Sigmoid and exponential of the keys, which only have to order.  __expf is off by (2 + 1.173 |x|) 2^-23 of the result, which
+// keeps 1 / (1 + e^-x) within 5e-7 (|x| e^-|x| is bounded; below -80 the score counts as e^-80).
+__device__ __forceinline__ float key_sigmoid(float x) { return __fdividef(1.0f, 1.0f + __expf(fminf(-x, 80.0f))); }
+__device__ __forceinline__ double key_sigmoid(double x) {
+    const double e = exp(x < 0 ? x : -x);
+    return (x < 0 ? e : 1.0) / (1.0 + e);
+}
+__device__ __forceinline__ float key_exp(float x) { return __expf(x); }
+__device__ __forceinline__ double key_exp(double x) { return exp(x); }
+__device__ __forceinline__ float key_div(float x, float y) { return __fdividef(x, y); }
+__device__ __forceinline__ double key_div(double x, double y) { return x / y; }
+
+// How far apart two fp32 keys must be for their order to be that of the exact ones.  A sigmoid is off by at most 5e-7 (the
+// errors above), a softmax by 3e-6 (its denominator adds up to 37 roundings), a key s + b by another half unit of itself; twice
+// that for two keys.
+template <bool SIGMOID>
+__device__ __forceinline__ float clearance(float key) { return (SIGMOID ? 1e-6f : 6e-6f) + 2.5e-7f * fabsf(key); }
 
 // Keeps the experts of the best groups: key of the others becomes -inf.  `cells` is this warp's shared row of n_experts
 // (+ padding) values.  Returns false where fp32 cannot tell the last group kept from the first one dropped.
-template <typename F, int VPL>
+template <bool SIGMOID, typename F, int VPL>
 __device__ __forceinline__ bool keep_groups(F (&key)[VPL], const F (&value)[VPL], const RouteArgs &a, F *cells, int lane) {
     // groups are contiguous runs of experts; `parts` lanes share a group, each scanning every parts-th member
     int parts = 32;
@@ -147,43 +158,65 @@ __device__ __forceinline__ bool keep_groups(F (&key)[VPL], const F (&value)[VPL]
     bool clear = true;
     if (sizeof(F) == 4) {
         const float next = (float)warp_max(rank);
-        clear = !((float)last - next <= 2 * clearance((float)last)) || !(next > -INFINITY);
+        clear = !((float)last - next <= 2 * clearance<SIGMOID>((float)last)) || !(next > -INFINITY);
     }
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
         const int e = lane + 32 * i;
-        if (e < a.n_experts && !((kept >> (e / a.per_group)) & 1)) key[i] = neg_inf<F>();
+        const int at = a.group_inverse ? (int)__umulhi((unsigned)e, a.group_inverse) : e;
+        if (e < a.n_experts && !((kept >> at) & 1)) key[i] = neg_inf<F>();
     }
     return clear;
 }
 
-// The top_k largest keys: lane j returns the j-th expert (or -1) in `mine`.  EXACT keys are compared as they are; others
-// must be `clearance` apart unless they belong to equal logits and equal biases.  Returns false where they are not.
-template <bool EXACT, typename F, int VPL, typename T>
+// The top_k largest keys: lane j returns the j-th expert (or -1) in `mine`.  Every lane keeps the best two of its keys at hand, so
+// that most picks cost two warp reductions and no pass over the keys.  EXACT keys are compared as they are; others must be
+// `clearance` apart unless they belong to equal logits and equal biases.  Returns false where they are not.
+template <bool EXACT, bool SIGMOID, typename F, int VPL, typename T>
 __device__ __forceinline__ bool choose(F (&key)[VPL], const RouteArgs &a, const T *logits, const float *bias, int lane, int &mine) {
+    F one, two;
+    int one_at, two_at;
+    auto scan = [&]() {  // the lane's best two, the lower index first among equals
+        one = two = neg_inf<F>();
+        one_at = two_at = 0;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const bool first = key[i] > one, second = key[i] > two;
+            two = first ? one : second ? key[i] : two;
+            two_at = first ? one_at : second ? i : two_at;
+            one = first ? key[i] : one;
+            one_at = first ? i : one_at;
+        }
+    };
+    scan();
     mine = -1;
     bool clear = true;
     float prev = INFINITY;
     int prev_at = -1;
-    for (int j = 0; j < a.top_k + (EXACT ? 0 : 1); ++j) {
-        F best = key[0];
-        int at = lane;
-#pragma unroll
-        for (int i = 1; i < VPL; ++i)
-            if (key[i] > best) { best = key[i]; at = lane + 32 * i; }
+    const int picks = a.top_k + (EXACT ? 0 : 1);
+    for (int j = 0; j < picks; ++j) {
+        F best = one;
+        int at = lane + 32 * one_at;
         warp_best(best, at);
         if (!(best > neg_inf<F>())) break;
         if (!EXACT) {
             const float v = (float)best;
-            if (prev_at >= 0 && prev - v <= clearance(v))
+            if (prev_at >= 0 && prev - v <= clearance<SIGMOID>(v))
                 clear = clear && to_f32(logits[prev_at]) == to_f32(logits[at]) && bias[prev_at] == bias[at];
             prev = v;
             prev_at = at;
         }
         if (lane == j && j < a.top_k) mine = at;
+        if ((at & 31) == lane) {
 #pragma unroll
-        for (int i = 0; i < VPL; ++i)
-            if (at == lane + 32 * i) key[i] = neg_inf<F>();
+            for (int i = 0; i < VPL; ++i)
+                if (i == one_at) key[i] = neg_inf<F>();
+            if (two > neg_inf<F>()) {
+                one = two;
+                one_at = two_at;
+                two = neg_inf<F>();
+            } else scan();
+        }
     }
     return clear;
 }
@@ -199,14 +232,16 @@ __device__ __forceinline__ void row_keys(const float (&l)[VPL], const float (&b)
         peak = warp_max(peak);
 #pragma unroll
         for (int i = 0; i < VPL; ++i)
-            if (l[i] > -INFINITY) total += exp_of((F)l[i] - peak);
+            if (l[i] > -INFINITY) total += key_exp((F)l[i] - peak);
         total = warp_sum(total);
     }
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
         const bool open = l[i] > -INFINITY;
         F s = 0;
-        if (need_score && open) s = SIGMOID ? sigmoid((F)l[i]) : exp_of((F)l[i] - peak) / total;
+        if (need_score && open) {
+            s = SIGMOID ? key_sigmoid((F)l[i]) : key_div(key_exp((F)l[i] - peak), total);
+        }
         F k = has_bias ? s + (F)b[i] : (F)l[i];
         if (!open || !(k > neg_inf<F>())) k = neg_inf<F>();
         key[i] = k;
@@ -214,11 +249,31 @@ __device__ __forceinline__ void row_keys(const float (&l)[VPL], const float (&b)
     }
 }
 
+// A row decided on fp64 keys: lane j returns the j-th expert.  Out of line, so that the few rows that need it do not cost the
+// others their registers.
+template <typename T, int VPL, bool SIGMOID>
+__device__ __noinline__ int decide_exactly(const RouteArgs &a, const T *line, const float *bias, double *cells, int lane) {
+    float l[VPL], b[VPL];
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) {
+        const int e = lane + 32 * i;
+        l[i] = e < a.n_experts ? to_f32(line[e]) : -INFINITY;
+        b[i] = bias && e < a.n_experts ? bias[e] : 0.0f;
+        if (l[i] != l[i]) l[i] = -INFINITY;
+    }
+    double key[VPL], value[VPL];
+    row_keys<double, VPL, SIGMOID>(l, b, bias != nullptr, true, key, value);
+    if (a.n_groups > 1) keep_groups<SIGMOID>(key, value, a, cells, lane);
+    int mine;
+    choose<true, SIGMOID>(key, a, line, bias, lane, mine);
+    return mine;
+}
+
 // One warp per row.  The row's logits stay in registers (lane + 32 i); the choice runs on fp32 keys, and a row in which two
 // keys that decide it lie closer together than fp32 can tell is decided again on fp64 keys.  That keeps the choice the
 // definition's at a fraction of the cost of fp64 throughout.
 template <typename T, int VPL, bool SIGMOID>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
+__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
                                                                 int *__restrict__ ids, float *__restrict__ weights) {
     extern __shared__ double s_cells[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -234,55 +289,49 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(RouteArgs a, co
     }
     for (long long row = (long long)blockIdx.x * kRouteWarps + warp; row < a.n_rows; row += (long long)gridDim.x * kRouteWarps) {
         const T *line = logits + row * a.n_experts;
-        float l[VPL];
+        float l[VPL], peak = 0.0f, total = 1.0f;
         bool nan = false;
 #pragma unroll
         for (int i = 0; i < VPL; ++i) {
             const int e = lane + 32 * i;
             l[i] = e < a.n_experts ? to_f32(line[e]) : -INFINITY;
-            if (l[i] != l[i] || (!SIGMOID && l[i] == INFINITY)) nan = true;  // the row's scores are not numbers: neither are its weights
+            nan = nan || !(SIGMOID ? l[i] <= INFINITY : l[i] < INFINITY);  // the row's scores are not numbers: neither are its weights
             if (l[i] != l[i]) l[i] = -INFINITY;
         }
         nan = __any_sync(kAll, nan);
-        float key[VPL], value[VPL];
-        row_keys<float, VPL, SIGMOID>(l, b, has_bias, need_score, key, value);
-        bool clear = true;
-        int mine;
-        if (grouped) {
-            clear = keep_groups(key, value, a, (float *)cells, lane);
-            if (!need_score) clear = true;  // logits compare exactly
-        }
-        if (has_bias) clear = choose<false>(key, a, line, bias, lane, mine) && clear;
-        else choose<true>(key, a, line, bias, lane, mine);
-        if (!clear) {
-            double key64[VPL], value64[VPL];
-            row_keys<double, VPL, SIGMOID>(l, b, has_bias, need_score, key64, value64);
-            if (grouped) keep_groups(key64, value64, a, cells, lane);
-            choose<true>(key64, a, line, bias, lane, mine);
-        }
-        // weights of the chosen, lane j the j-th
-        const bool live = mine >= 0;
-        const float lm = live ? to_f32(line[mine]) : -INFINITY;
-        float w;
-        const float top = warp_max(lm);
-        // the chosen scores' ratios: by exponentials of differences where the scores are exponentials (softmax, or a sigmoid so
-        // far down that 1 + e^l is 1), so that they do not underflow together
-        if (a.renormalise && (!SIGMOID || top < -30.0f)) {
-            const float e = live ? expf(lm - top) : 0.0f;
-            w = e / warp_sum(e);
-        } else if (SIGMOID) {
-            w = live ? sigmoid(lm) : 0.0f;
-            if (a.renormalise) w = w / warp_sum(w);
-        } else {
-            float peak = l[0], total = 0.0f;
+        if (!SIGMOID && !a.renormalise) {  // the denominator of the weights
+            peak = l[0];
+            total = 0.0f;
 #pragma unroll
             for (int i = 1; i < VPL; ++i) peak = fmaxf(peak, l[i]);
             peak = warp_max(peak);
 #pragma unroll
             for (int i = 0; i < VPL; ++i)
                 if (l[i] > -INFINITY) total += expf(l[i] - peak);
-            w = expf(lm - peak) / warp_sum(total);
+            total = warp_sum(total);
         }
+        float key[VPL], value[VPL];
+        row_keys<float, VPL, SIGMOID>(l, b, has_bias, need_score, key, value);
+        bool clear = true;
+        int mine;
+        if (grouped) {
+            clear = keep_groups<SIGMOID>(key, value, a, (float *)cells, lane);
+            if (!need_score) clear = true;  // logits compare exactly
+        }
+        if (has_bias) clear = choose<false, SIGMOID>(key, a, line, bias, lane, mine) && clear;
+        else choose<true, SIGMOID>(key, a, line, bias, lane, mine);
+        if (!clear) mine = decide_exactly<T, VPL, SIGMOID>(a, line, bias, cells, lane);
+        // weights of the chosen, lane j the j-th
+        const bool live = mine >= 0;
+        const float lm = live ? to_f32(line[mine]) : -INFINITY;
+        float w;
+        // the chosen scores' ratios: by exponentials of differences where the scores are exponentials (softmax, or a sigmoid so
+        // far down that 1 + e^l is 1), so that they do not underflow together
+        if (a.renormalise) {
+            const float top = warp_max(lm);
+            w = !SIGMOID || top < -30.0f ? (live ? expf(lm - top) : 0.0f) : (live ? sigmoid(lm) : 0.0f);
+            w = w / warp_sum(w);
+        } else w = SIGMOID ? (live ? sigmoid(lm) : 0.0f) : expf(lm - peak) / total;
         if (lane < a.top_k) {
             ids[row * a.top_k + lane] = mine;
             weights[row * a.top_k + lane] = nan ? NAN : live ? w * a.scale : 0.0f;
@@ -354,41 +403,75 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(RouteA
     }
 }
 
-// Rows listed by group: a stable counting sort of the pairs (row, choice) by id in one launch.  The pairs are cut into one
-// contiguous run per warp of the cluster; a warp counts its run's ids in shared memory (lanes of equal id are found with
-// match.any, so no atomics and one order), the counts are scanned over warps, blocks (distributed shared memory) and groups,
-// and the warp walks its run again and places every pair.  With `rest` the pairs without a group form one group more, the last.
+// Rows listed by group: a stable counting sort of the pairs (row, choice) by id in one launch of one cluster.  The pairs are cut
+// into one contiguous run per warp of the cluster; a warp counts its run's ids in shared memory, the counts are scanned over
+// warps, blocks (distributed shared memory) and groups, and the warp walks its run again, 32 pairs at a time, and places every
+// pair: lanes of equal id find one another by a ballot per bit of the id, so there is one order and no atomics in it (match.any
+// for the same took 45 us for 131,072 pairs of 256 groups).  A block first sorts its own pairs in shared memory and then writes
+// whole runs per group: scattered 4-byte writes straight to memory took 30 of 37 us there.  With `rest` the pairs without a
+// group form one group more, the last.
 constexpr int kGroupThreads = 1024, kGroupWarps = kGroupThreads / 32, kGroupMax = 1024;
-constexpr int kGroupCluster = 8;
+constexpr int kGroupCluster = 16;
+constexpr int kSortedMax = 16384;  // pairs a block sorts in shared memory
 
-__global__ void __launch_bounds__(kGroupThreads) group_kernel(long long n_pairs, int per_row, int n_groups, bool rest, const int *__restrict__ ids,
-                                                             int *__restrict__ group_ptr, int *__restrict__ slot_row, int *__restrict__ slot_of) {
+struct GroupArgs {
+    long long n_pairs;
+    int per_row, n_groups, sorted;  // sorted: pairs a block has room for (0: written straight to memory)
+    bool rest;
+    const int *ids;
+    int *group_ptr, *slot_row, *slot_of;
+};
+
+__global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a) {
     extern __shared__ int s_int[];
-    const int columns = n_groups + (rest ? 1 : 0), none = rest ? n_groups : -1;
-    int *count = s_int;                            // [warps][columns], later the next free slot
-    int *total = s_int + kGroupWarps * columns;    // this block's pairs per column
-    __shared__ int s_scan[kGroupWarps];
+    const int columns = a.n_groups + (a.rest ? 1 : 0), none = a.rest ? a.n_groups : -1;
+    int *count = s_int;                           // [warps][columns], later the next free place of the block's sorted pairs
+    int *total = count + kGroupWarps * columns;   // this block's pairs per column
+    int *local = total + columns;                 // where a column starts among the block's sorted pairs (columns + 1)
+    int *global = local + columns + 1;            // and among all
+    int *sorted = global + columns;
+    __shared__ int s_scan[kGroupWarps], s_own[kGroupWarps];
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = (int)cluster.block_rank(), blocks = (int)cluster.num_blocks();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long steps = (n_pairs + 31) / 32, runs = (long long)blocks * kGroupWarps;
-    const long long run = rank * kGroupWarps + warp;
-    const long long lo = steps * run / runs, hi = steps * (run + 1) / runs;
+    const int steps = (int)((a.n_pairs + 31) / 32), runs = blocks * kGroupWarps, run = rank * kGroupWarps + warp;
+    const int lo = (int)((long long)steps * run / runs), hi = (int)((long long)steps * (run + 1) / runs);
     int *own = count + warp * columns;
     for (int g = lane; g < columns; g += 32) own[g] = 0;
     __syncwarp();
-    for (long long s = lo; s < hi; ++s) {
-        const long long i = s * 32 + lane;
-        int id = i < n_pairs ? ids[i] : -1;
-        if (id >= n_groups) atomicOr(&g_status, mps::kStatusBadIndex);
-        if ((unsigned)id >= (unsigned)n_groups) id = i < n_pairs ? none : -1;
-        const unsigned same = __match_any_sync(kAll, id);
-        if (id >= 0 && lane == __ffs(same) - 1) own[id] += __popc(same);
-        __syncwarp();
+    const int bits = columns > 1 ? 32 - __clz(columns - 1) : 0;  // of an id
+    auto lanes_of = [&](int id) {                               // lanes with this lane's id, for an id >= 0
+        unsigned same = __ballot_sync(kAll, id >= 0);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned set = __ballot_sync(kAll, id >> b & 1);
+            same &= id >> b & 1 ? set : ~set;
+        }
+        return same;
+    };
+    constexpr int kBatch = 8;  // loads in flight
+    int batch[kBatch];
+    auto load = [&](int s) {
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            const long long i = (long long)(s + j) * 32 + lane;
+            const bool in = s + j < hi && i < a.n_pairs;
+            batch[j] = in ? a.ids[i] : -1;
+            if ((unsigned)batch[j] >= (unsigned)a.n_groups) {
+                if (batch[j] >= 0) atomicOr(&g_status, mps::kStatusBadIndex);
+                batch[j] = in ? none : -1;
+            }
+        }
+    };
+    for (int s = lo; s < hi; s += kBatch) {
+        load(s);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j)
+            if (batch[j] >= 0) atomicAdd(&own[batch[j]], 1);  // counts only: their order does not show
     }
     __syncthreads();
     for (int g = tid; g < columns; g += kGroupThreads) {
         int sum = 0;
+#pragma unroll
         for (int w = 0; w < kGroupWarps; ++w) {
             const int c = count[w * columns + g];
             count[w * columns + g] = sum;
@@ -397,70 +480,106 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(long long n_pairs,
         total[g] = sum;
     }
     cluster.sync();
-    int before = 0, all = 0;
-    if (tid < n_groups)
+    // exclusive scans over the columns: of this block's totals and of all blocks'
+    int before = 0, all = 0, mine = 0;
+    if (tid < a.n_groups) {
+        mine = total[tid];
         for (int r = 0; r < blocks; ++r) {
             const int c = cluster.map_shared_rank(total, r)[tid];
             if (r < rank) before += c;
             all += c;
         }
-    int scan = all;  // inclusive scan over groups
+    }
+    int scan = all, scan_own = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int o = __shfl_up_sync(kAll, scan, d);
-        if (lane >= d) scan += o;
+        const int o = __shfl_up_sync(kAll, scan, d), q = __shfl_up_sync(kAll, scan_own, d);
+        if (lane >= d) {
+            scan += o;
+            scan_own += q;
+        }
     }
-    if (lane == 31) s_scan[warp] = scan;
+    if (lane == 31) {
+        s_scan[warp] = scan;
+        s_own[warp] = scan_own;
+    }
     __syncthreads();
     if (warp == 0) {
-        int v = s_scan[lane];
+        int v = s_scan[lane], q = s_own[lane];
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int o = __shfl_up_sync(kAll, v, d);
-            if (lane >= d) v += o;
+            const int o = __shfl_up_sync(kAll, v, d), u = __shfl_up_sync(kAll, q, d);
+            if (lane >= d) {
+                v += o;
+                q += u;
+            }
         }
         s_scan[lane] = v;
+        s_own[lane] = q;
     }
     __syncthreads();
-    const int start = scan - all + (warp ? s_scan[warp - 1] : 0);
-    const int used = s_scan[kGroupWarps - 1];
-    if (tid < n_groups) {
+    const int start = scan - all + (warp ? s_scan[warp - 1] : 0), start_own = scan_own - mine + (warp ? s_own[warp - 1] : 0);
+    const int used = s_scan[kGroupWarps - 1], used_own = s_own[kGroupWarps - 1];
+    if (tid < a.n_groups) {
+        local[tid] = start_own;
+        global[tid] = start + before;
         if (rank == 0) {
-            group_ptr[tid] = start;
-            if (tid == n_groups - 1) group_ptr[n_groups] = used;
+            a.group_ptr[tid] = start;
+            if (tid == a.n_groups - 1) a.group_ptr[a.n_groups] = used;
         }
-        for (int w = 0; w < kGroupWarps; ++w) count[w * columns + tid] += start + before;
     }
-    if (rest && tid < 32) {  // behind the groups
-        int ahead = used;
-        for (int r = 0; r < rank; ++r) ahead += cluster.map_shared_rank(total, r)[n_groups];
-        count[tid * columns + n_groups] += ahead;
-        if (tid == 0 && rank == 0) group_ptr[columns] = (int)n_pairs;
+    if (tid == 0) {
+        local[a.n_groups] = used_own;
+        if (a.rest) {  // behind the groups
+            int ahead = used;
+            for (int r = 0; r < rank; ++r) ahead += cluster.map_shared_rank(total, r)[a.n_groups];
+            global[a.n_groups] = ahead;
+            local[columns] = used_own + total[a.n_groups];
+            if (rank == 0) a.group_ptr[columns] = (int)a.n_pairs;
+        }
     }
     cluster.sync();  // also: no block leaves while another still reads its totals
-    for (long long s = lo; s < hi; ++s) {
-        const long long i = s * 32 + lane;
-        int id = i < n_pairs ? ids[i] : -1;
-        if ((unsigned)id >= (unsigned)n_groups) id = i < n_pairs ? none : -1;
-        const unsigned same = __match_any_sync(kAll, id);
-        int at = -1;
-        if (id >= 0) at = own[id] + __popc(same & ((1u << lane) - 1));
-        __syncwarp();
-        if (id >= 0 && lane == __ffs(same) - 1) own[id] += __popc(same);
-        __syncwarp();
-        if (i < n_pairs) {
-            if (slot_of) slot_of[i] = at;
-            if (at >= 0) slot_row[at] = (int)(i / per_row);
-            if (!rest && i >= used) slot_row[i] = -1;
+    for (int s = lo; s < hi; s += kBatch) {
+        load(s);
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (s + j >= hi) break;
+            const long long i = (long long)(s + j) * 32 + lane;
+            const int id = batch[j];
+            const unsigned same = lanes_of(id);
+            int at = -1;
+            if (id >= 0) at = own[id] + __popc(same & ((1u << lane) - 1));  // among the block's pairs of the column
+            __syncwarp();
+            if (id >= 0 && lane == __ffs(same) - 1) own[id] += __popc(same);
+            __syncwarp();
+            if (i < a.n_pairs) {
+                const int slot = id >= 0 ? global[id] + at : -1;
+                if (a.slot_of) a.slot_of[i] = slot;
+                if (id >= 0) {
+                    if (a.sorted) sorted[local[id] + at] = (int)i / a.per_row;
+                    else a.slot_row[slot] = (int)i / a.per_row;
+                }
+                if (!a.rest && i >= used) a.slot_row[i] = -1;
+            }
         }
+    }
+    if (a.sorted) {
+        __syncthreads();
+        for (int g = warp; g < columns; g += kGroupWarps)
+            for (int j = local[g] + lane; j < local[g + 1]; j += 32) a.slot_row[global[g] + j - local[g]] = sorted[j];
     }
 }
 
 int launch_group(long long n_pairs, int per_row, int n_groups, bool rest, const int *ids, int *ptr, int *row, int *slot, cudaStream_t st) {
-    const size_t smem = (size_t)(kGroupWarps + 1) * (n_groups + (rest ? 1 : 0)) * sizeof(int);
+    const int columns = n_groups + (rest ? 1 : 0);
+    const int blocks = n_pairs > 16384 ? kGroupCluster : n_pairs > 2048 ? 8 : 1;
+    const long long runs = blocks * kGroupWarps, most = ((n_pairs + 31) / 32 + runs - 1) / runs * 32 * kGroupWarps;  // pairs of a block
+    const GroupArgs a = {n_pairs, per_row, n_groups, most <= kSortedMax ? (int)most : 0, rest, ids, ptr, row, slot};
+    const size_t smem = ((size_t)(kGroupWarps + 3) * columns + 1 + a.sorted) * sizeof(int);
     if (smem > 40 * 1024)
-        RT_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kGroupWarps + 1) * (kGroupMax + 1) * (int)sizeof(int)));
-    const int blocks = n_pairs > 2048 ? kGroupCluster : 1;
+        RT_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)(((kGroupWarps + 3) * (kGroupMax + 1) + 1 + kSortedMax) * sizeof(int))));
+    if (blocks > 8) RT_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     cudaLaunchAttribute attr;
     attr.id = cudaLaunchAttributeClusterDimension;
     attr.val.clusterDim.x = blocks;
@@ -472,7 +591,7 @@ int launch_group(long long n_pairs, int per_row, int n_groups, bool rest, const 
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    RT_CUDA(cudaLaunchKernelEx(&cfg, group_kernel, n_pairs, per_row, n_groups, rest, ids, ptr, row, slot));
+    RT_CUDA(cudaLaunchKernelEx(&cfg, group_kernel, a));
     return MPS_OK;
 }
 
@@ -480,7 +599,7 @@ template <typename T, bool SIGMOID>
 int launch_route(const RouteArgs &a, const void *logits, const float *bias, int *ids, float *weights, cudaStream_t st) {
     const size_t smem = (size_t)kRouteWarps * (a.n_experts + (a.n_experts >> 5) + 1) * sizeof(double);
     const long long want = ((long long)a.n_rows + kRouteWarps - 1) / kRouteWarps;
-    const unsigned blocks = (unsigned)(want < 148 * 16 ? want : 148 * 16);
+    const unsigned blocks = (unsigned)(want < 148 * 8 ? want : 148 * 8);  // what is resident at once
     const int per_lane = (a.n_experts + 31) / 32;
 #define RT_LAUNCH(V) route_kernel<T, V, SIGMOID><<<blocks, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, bias, ids, weights)
     if (per_lane <= 1) RT_LAUNCH(1);
@@ -511,6 +630,7 @@ int check_spec(const char *who, int n_rows, const mps_route_spec *spec, int dtyp
         return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d experts, top %d, %d groups", who, kMaxExperts, kMaxTop, kMaxGroups);
     if ((long long)n_rows * spec->top_k >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "%s: rows * top_k does not fit 31 bits", who);
     *a = RouteArgs{n_rows, spec->n_experts, spec->top_k, spec->n_groups, spec->n_experts / spec->n_groups, spec->top_groups, spec->group_top,
+                   spec->n_experts == spec->n_groups ? 0u : (unsigned)(((1ull << 32) + spec->n_experts / spec->n_groups - 1) / (spec->n_experts / spec->n_groups)),
                    spec->renormalise != 0, spec->scale};
     return MPS_OK;
 }

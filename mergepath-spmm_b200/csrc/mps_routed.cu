@@ -43,10 +43,11 @@ bool known(int dtype) { return dtype == MPS_F32 || dtype == MPS_F16 || dtype == 
 template <typename T, int VEC>
 __global__ void __launch_bounds__(256) combine_kernel(int n_rows, int per_row, int n_slots, int dim, const int *__restrict__ slot_of,
                                                       const float *__restrict__ weights, const T *__restrict__ rows, T *__restrict__ y, int *status) {
-    const int per = dim / VEC;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < (long long)n_rows * per; i += (long long)gridDim.x * 256) {
-        const long long t = i / per;
-        const int c = (int)(i - t * per) * VEC;
+    // blockIdx.x: rows (as many as fill 256 threads), blockIdx.y: stretches of a long row
+    const int per = dim / VEC, rows_here = per < 256 ? 256 / per : 1, local = per < 256 ? (int)threadIdx.x / per : 0;
+    const int c = ((int)threadIdx.x - local * per + (int)blockIdx.y * 256) * VEC;
+    if (local >= rows_here || c >= dim) return;
+    for (long long t = (long long)blockIdx.x * rows_here + local; t < n_rows; t += (long long)gridDim.x * rows_here) {
         float acc[VEC] = {};
 #pragma unroll 4
         for (int j = 0; j < per_row; ++j) {
@@ -126,8 +127,9 @@ int launch_combine(int n_rows, int per_row, int n_slots, int dim, const int *slo
     if (int rc = status_pointer(&status)) return rc;
     constexpr int VEC = mps::Pack<T>::N;
     const bool wide = dim % VEC == 0 && !misaligned(rows, 16) && !misaligned(y, 16);
-    const long long blocks = ((long long)n_rows * (wide ? dim / VEC : dim) + 255) / 256;
-    const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20);
+    const int per = wide ? dim / VEC : dim, rows_here = per < 256 ? 256 / per : 1;
+    const long long blocks = ((long long)n_rows + rows_here - 1) / rows_here;
+    const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20), (unsigned)((per + 255) / 256));
     if (wide) combine_kernel<T, VEC><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)rows, (T *)y, status);
     else combine_kernel<T, 1><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)rows, (T *)y, status);
     RD_CUDA(cudaGetLastError());
