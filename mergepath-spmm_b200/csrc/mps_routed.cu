@@ -28,7 +28,12 @@ namespace {
 __device__ int g_status;
 
 int status_pointer(int **p) {
+    static mps::PerDevice<int *> known;
+    int dev = 0;
+    RD_CUDA(cudaGetDevice(&dev));
+    if ((*p = known.get(dev))) return MPS_OK;
     RD_CUDA(cudaGetSymbolAddress((void **)p, g_status));
+    known.put(dev, *p);
     return MPS_OK;
 }
 
@@ -180,9 +185,12 @@ int launch_plain_outer(OuterArgs a, const void *p, const void *q, void *out, cud
 // ---- tensor cores
 
 int sm_count(int *n) {
+    static mps::PerDevice<int> known;
     int dev = 0;
     RD_CUDA(cudaGetDevice(&dev));
+    if ((*n = known.get(dev))) return MPS_OK;
     RD_CUDA(cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev));
+    known.put(dev, *n);
     return MPS_OK;
 }
 
@@ -207,9 +215,19 @@ int tensor_map(CUtensorMap *map, bool bf16, const void *base, int dims, unsigned
 }
 
 // A launch of `blocks` blocks in clusters; `ahead`: it may start before the launch in front of it has ended.
-template <typename Kernel, typename Args>
-int launch_tc(Kernel kernel, const Args &args, long long blocks, int cluster, size_t smem, bool ahead, cudaStream_t st) {
-    RD_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+template <auto Kernel, typename Args>
+int launch_tc(const Args &args, long long blocks, int cluster, size_t smem, bool ahead, cudaStream_t st) {
+    static mps::PerDevice<int> allowed;  // shared memory the kernel may ask for
+    int dev = 0;
+    RD_CUDA(cudaGetDevice(&dev));
+    if (allowed.get(dev) == 0) {
+        int most = 0;
+        RD_CUDA(cudaDeviceGetAttribute(&most, cudaDevAttrMaxSharedMemoryPerBlockOptin, dev));
+        cudaFuncAttributes at;
+        RD_CUDA(cudaFuncGetAttributes(&at, Kernel));
+        RD_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)at.sharedSizeBytes));
+        allowed.put(dev, most);
+    }
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
@@ -223,7 +241,7 @@ int launch_tc(Kernel kernel, const Args &args, long long blocks, int cluster, si
     cfg.stream = st;
     cfg.attrs = attr;
     cfg.numAttrs = ahead ? 2 : 1;
-    RD_CUDA(cudaLaunchKernelEx(&cfg, kernel, args));
+    RD_CUDA(cudaLaunchKernelEx(&cfg, Kernel, args));
     return MPS_OK;
 }
 
@@ -271,7 +289,7 @@ int launch_tc_rows(const TcRows &a, int sms, cudaStream_t st) {
     const long long tiles = most * ((a.n + tile_f - 1) / tile_f);
     const int cluster = mps::TcShape<NT>::kPaired ? 2 : a.split;
     const long long workers = sms / cluster;
-    return launch_tc(mps::tc_rows_kernel<NT>, a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcShape<NT>::bytes(a.n_groups), a.ahead, st);
+    return launch_tc<mps::tc_rows_kernel<NT>>(a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcShape<NT>::bytes(a.n_groups), a.ahead, st);
 }
 
 // The rest of a filled in: what every use has in common.
@@ -306,7 +324,7 @@ int launch_tc_outer(TcOuter a, int sms, cudaStream_t st) {
     a.split = NT <= 128 ? split_of(tiles, steps, sms) : 1;
     const int cluster = mps::TcOuterShape<NT>::kPaired ? 2 : a.split;
     const long long workers = sms / cluster;
-    return launch_tc(mps::tc_outer_kernel<NT>, a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcOuterShape<NT>::kBytes, false, st);
+    return launch_tc<mps::tc_outer_kernel<NT>>(a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcOuterShape<NT>::kBytes, false, st);
 }
 
 // P: n_p_rows rows of a.i, by a.slot_row or in slot order; Q: rows of a.j in slot order (pair: two planes of them).
