@@ -14,6 +14,7 @@
 #include <cmath>
 
 #include "mps_internal.h"
+#include "mps_tc.cuh"
 #include "mps_types.cuh"
 
 namespace cg = cooperative_groups;
@@ -276,6 +277,7 @@ template <typename T, int VPL, bool SIGMOID>
 __global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
                                                                 int *__restrict__ ids, float *__restrict__ weights) {
     extern __shared__ double s_cells[];
+    mps::let_next_launch_start();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int pitch = a.n_experts + (a.n_experts >> 5) + 1;
     double *cells = s_cells + (size_t)warp * pitch;
@@ -437,6 +439,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a)
     const int steps = (int)((a.n_pairs + 31) / 32), runs = blocks * kGroupWarps, run = rank * kGroupWarps + warp;
     const int lo = (int)((long long)steps * run / runs), hi = (int)((long long)steps * (run + 1) / runs);
     int *own = count + warp * columns;
+    mps::let_next_launch_start();
     for (int g = lane; g < columns; g += 32) own[g] = 0;
     __syncwarp();
     const int bits = columns > 1 ? 32 - __clz(columns - 1) : 0;  // of an id
@@ -448,6 +451,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a)
         }
         return same;
     };
+    mps::wait_for_launch_before();
     constexpr int kBatch = 8;  // loads in flight
     int batch[kBatch];
     auto load = [&](int s) {
@@ -570,7 +574,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_kernel(const GroupArgs a)
     }
 }
 
-int launch_group(long long n_pairs, int per_row, int n_groups, bool rest, const int *ids, int *ptr, int *row, int *slot, cudaStream_t st) {
+int launch_group(long long n_pairs, int per_row, int n_groups, bool rest, const int *ids, int *ptr, int *row, int *slot, bool follows, cudaStream_t st) {
     const int columns = n_groups + (rest ? 1 : 0);
     const int blocks = n_pairs > 16384 ? kGroupCluster : n_pairs > 2048 ? 8 : 1;
     const long long runs = blocks * kGroupWarps, most = ((n_pairs + 31) / 32 + runs - 1) / runs * 32 * kGroupWarps;  // pairs of a block
@@ -580,17 +584,19 @@ int launch_group(long long n_pairs, int per_row, int n_groups, bool rest, const 
         RT_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)(((kGroupWarps + 3) * (kGroupMax + 1) + 1 + kSortedMax) * sizeof(int))));
     if (blocks > 8) RT_CUDA(cudaFuncSetAttribute(group_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = blocks;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = blocks;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // see mps_tc.cuh
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks);
     cfg.blockDim = dim3(kGroupThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = follows ? 2 : 1;
     RT_CUDA(cudaLaunchKernelEx(&cfg, group_kernel, a));
     return MPS_OK;
 }
@@ -648,8 +654,8 @@ int take_route_status(void *stream, int *status) {
     if (*status) RT_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
     return MPS_OK;
 }
-int list_rows_and_rest(int n_rows, int n_groups, const int32_t *ids, int32_t *group_ptr, int32_t *slot_row, void *stream) {
-    return launch_group(n_rows, 1, n_groups, true, ids, group_ptr, slot_row, nullptr, (cudaStream_t)stream);
+int list_rows_and_rest(int n_rows, int n_groups, const int32_t *ids, int32_t *group_ptr, int32_t *slot_row, bool follows, void *stream) {
+    return launch_group(n_rows, 1, n_groups, true, ids, group_ptr, slot_row, nullptr, follows, (cudaStream_t)stream);
 }
 }  // namespace mps
 
@@ -662,7 +668,7 @@ extern "C" int mps_group_rows(int32_t n_rows, int32_t per_row, int32_t n_groups,
     if (pairs >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "mps_group_rows: rows * per_row does not fit 31 bits");
     if (misaligned(d_ids, 4) || misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_slot_of, 4))
         return fail(MPS_ERR_ALIGN, "mps_group_rows: pointers must be 4-byte aligned");
-    return launch_group(pairs, per_row, n_groups, false, d_ids, d_group_ptr, d_slot_row, d_slot_of, (cudaStream_t)stream);
+    return launch_group(pairs, per_row, n_groups, false, d_ids, d_group_ptr, d_slot_row, d_slot_of, false, (cudaStream_t)stream);
 }
 
 extern "C" int mps_route(int32_t n_rows, const mps_route_spec *spec, int dtype, const void *d_logits, const float *d_bias, int32_t *d_ids,
@@ -685,7 +691,7 @@ extern "C" int mps_route(int32_t n_rows, const mps_route_spec *spec, int dtype, 
         else rc = sig ? launch_route<__nv_bfloat16, true>(a, d_logits, d_bias, d_ids, d_weights, st) : launch_route<__nv_bfloat16, false>(a, d_logits, d_bias, d_ids, d_weights, st);
         if (rc) return rc;
     }
-    if (list) return launch_group((long long)n_rows * a.top_k, a.top_k, a.n_experts, false, d_ids, d_group_ptr, d_slot_row, d_slot_of, st);
+    if (list) return launch_group((long long)n_rows * a.top_k, a.top_k, a.n_experts, false, d_ids, d_group_ptr, d_slot_row, d_slot_of, n_rows > 0, st);
     return MPS_OK;
 }
 

@@ -214,9 +214,10 @@ int tensor_map(CUtensorMap *map, bool bf16, const void *base, int dims, unsigned
     return MPS_OK;
 }
 
-// A launch of `blocks` blocks in clusters; `ahead`: it may start before the launch in front of it has ended.
+// A launch of `blocks` blocks in clusters; `follows`: the launch before it on the stream is one of the same call, and this one may
+// start before that has ended.
 template <auto Kernel, typename Args>
-int launch_tc(const Args &args, long long blocks, int cluster, size_t smem, bool ahead, cudaStream_t st) {
+int launch_tc(const Args &args, long long blocks, int cluster, size_t smem, bool follows, cudaStream_t st) {
     static mps::PerDevice<int> allowed;  // shared memory the kernel may ask for
     int dev = 0;
     RD_CUDA(cudaGetDevice(&dev));
@@ -240,7 +241,7 @@ int launch_tc(const Args &args, long long blocks, int cluster, size_t smem, bool
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     cfg.attrs = attr;
-    cfg.numAttrs = ahead ? 2 : 1;
+    cfg.numAttrs = follows ? 2 : 1;
     RD_CUDA(cudaLaunchKernelEx(&cfg, Kernel, args));
     return MPS_OK;
 }
@@ -289,7 +290,7 @@ int launch_tc_rows(const TcRows &a, int sms, cudaStream_t st) {
     const long long tiles = most * ((a.n + tile_f - 1) / tile_f);
     const int cluster = mps::TcShape<NT>::kPaired ? 2 : a.split;
     const long long workers = sms / cluster;
-    return launch_tc<mps::tc_rows_kernel<NT>>(a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcShape<NT>::bytes(a.n_groups), a.ahead, st);
+    return launch_tc<mps::tc_rows_kernel<NT>>(a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcShape<NT>::bytes(a.n_groups), a.follows, st);
 }
 
 // The rest of a filled in: what every use has in common.
@@ -298,6 +299,8 @@ int tc_rows(TcRows a, const Cut &cut, const void *x, long long x_rows, int sms, 
     a.split = cut.split;
     const int loaded = cut.nt == 256 ? mps::TcShape<256>::kRows : cut.nt;  // slots a block loads
     if (int rc = tensor_map(&a.x, a.bf16, x, 2, a.k, x_rows, 1, a.gather ? 1 : loaded)) return rc;
+    if (a.gather)
+        if (int rc = tensor_map(&a.x_run, a.bf16, x, 2, a.k, x_rows, 1, loaded / 8)) return rc;
     if (a.rank)
         if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded)) return rc;
     if (cut.nt == 32) return launch_tc_rows<32>(a, sms, st);
@@ -324,7 +327,7 @@ int launch_tc_outer(TcOuter a, int sms, cudaStream_t st) {
     a.split = NT <= 128 ? split_of(tiles, steps, sms) : 1;
     const int cluster = mps::TcOuterShape<NT>::kPaired ? 2 : a.split;
     const long long workers = sms / cluster;
-    return launch_tc<mps::tc_outer_kernel<NT>>(a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcOuterShape<NT>::kBytes, false, st);
+    return launch_tc<mps::tc_outer_kernel<NT>>(a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcOuterShape<NT>::kBytes, a.follows, st);
 }
 
 // P: n_p_rows rows of a.i, by a.slot_row or in slot order; Q: rows of a.j in slot order (pair: two planes of them).
@@ -430,7 +433,7 @@ struct AdapterSpace {
 
 // u (two planes, slot order) = scale * rows of x times the adapters' matrices (mn_major: stored summed x rank); u_f32 (or NULL)
 // the same by row
-int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m, bool mn_major, void *u, float *u_f32, int sms, cudaStream_t st) {
+int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m, bool mn_major, void *u, float *u_f32, bool follows, int sms, cudaStream_t st) {
     TcRows a = {};
     a.bf16 = s.dtype == MPS_BF16;
     a.mn_major = mn_major;
@@ -443,6 +446,7 @@ int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m
     a.gather = a.pair = true;
     a.group_scale = s.scale;
     a.out = u;
+    a.follows = follows;
     a.out_plane = (long long)s.n_rows * s.rank;
     a.out_f32 = u_f32;
     if (int rc = tc_matrix(&a.w, &a, m, k, s.rank, s.n_adapters)) return rc;
@@ -470,7 +474,7 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cu
     a.n_slots = a.n_x_rows = s.n_rows;
     a.k = k;
     a.n = n;
-    a.w_shared = true;
+    a.w_shared = a.follows = true;
     a.out = out;
     if (int rc = tc_matrix(&a.w, &a, w, k, n, 1)) return rc;
     if (rows) {
@@ -486,7 +490,7 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cu
         a.ahead = ahead;
         return tc_rows(a, cut, x, s.n_rows, sms, st);
     }
-    if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
+    if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, true, st)) return rc;
     a.group_ptr = ws.ptr;
     a.slot_row = ws.row;
     a.n_groups = s.n_adapters + 1;
@@ -508,7 +512,7 @@ int tc_adapter_outer(const AdapterShape &s, int features, const void *p, const v
     a.n_slots = a.n_p_rows = s.n_rows;
     a.i = features;
     a.j = s.rank;
-    a.pair = true;
+    a.pair = a.follows = true;
     a.out = out;
     a.out_group = (long long)features * s.rank;
     a.out_f = out_f;
@@ -530,7 +534,7 @@ int adapters(const AdapterShape &s, const void *x, const void *w, const void *a,
             mps::adapter_dots_kernel<<<grid, 256, 0, st>>>(s.k, s.rank, s.n_adapters, s.dtype == MPS_BF16, s.ids, s.scale, (const uint16_t *)x,
                                                            (const uint16_t *)a, (float *)ws.u, status);
             RD_CUDA(cudaGetLastError());
-        } else if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, sms, st)) return rc;
+        } else if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, false, sms, st)) return rc;
         return tc_adapter_wide(s, ws, cut, rows, s.k, s.n, x, w, ws.u, (const float *)ws.u, b, false, y, rows, sms, st);
     }
     float *u = (float *)ws.u;
@@ -547,8 +551,8 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
         Cut cut;
         if (int rc = sm_count(&sms)) return rc;
         const bool rows = by_rows(s, s.n, s.k, sms, &cut);
-        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, sms, st)) return rc;                               // scale * x A^T
-        if (int rc = tc_adapter_narrow(s, s.n, dy, b, true, ws.v, rows ? (float *)ws.v_f32 : nullptr, sms, st)) return rc;  // scale * dy B
+        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, false, sms, st)) return rc;                               // scale * x A^T
+        if (int rc = tc_adapter_narrow(s, s.n, dy, b, true, ws.v, rows ? (float *)ws.v_f32 : nullptr, true, sms, st)) return rc;  // scale * dy B
         if (int rc = tc_adapter_wide(s, ws, cut, rows, s.n, s.k, dy, w, ws.v, (const float *)ws.v_f32, a, true, dx, false, sms, st)) return rc;
         if (int rc = tc_adapter_outer(s, s.k, x, ws.v, da, 1, s.k, st)) return rc;
         return tc_adapter_outer(s, s.n, dy, ws.u, db, s.rank, 1, st);

@@ -38,6 +38,7 @@ constexpr int kOutTotal = (kOutBytes + 1023) / 1024 * 1024;
 
 struct TcRows {
     CUtensorMap w, x, w2, u;  // matrices {i, f, group} or {f, i, group}; rows {i, row}; the low-rank pair's matrix and rows
+    CUtensorMap x_run;        // gathered rows: as many neighbouring ones as a warp loads
     const int *group_ptr;     // NULL: one group of all slots
     const int *slot_row;      // row behind a slot; NULL: the slot itself
     int n_groups, n_slots, n_x_rows;
@@ -56,8 +57,9 @@ struct TcRows {
     const uint16_t *delta_m;  //   the adapters' matrices with their strides by adapter, feature and rank index
     int delta_adapters, delta_rank;
     long long delta_group, delta_f, delta_r;
-    bool ahead;               // launched before the end of the launch that computes delta_u
-    int split;                // blocks of a cluster, each with its part of the sum
+    bool ahead;               // only delta_u comes from the launch before this one
+    int split;                // blocks of a cluster, each with its part of the sum (a power of two)
+    bool follows;             // the launch before is one of the same call (host side)
     int *status;
 };
 
@@ -88,6 +90,24 @@ __device__ __forceinline__ void tell_cluster(uint32_t bar, int split, int lane) 
     fence_cluster();
     __syncwarp();
     if (lane < split) mbar_arrive_at(bar, lane);
+}
+
+// The parts of all blocks, in their order, for columns a `split` apart (kTogether of them, those below `columns`): the loads of
+// a block's part are in flight together, one by one they took 13 us for 32 columns.
+constexpr int kTogether = 8;
+__device__ __forceinline__ void add_partials(float (&v)[kTogether], uint32_t addr, int split, int columns) {
+    for (int p = 0; p < split; p += 2) {  // split is 1 or even
+        float w[2][kTogether];
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j)
+                w[q][j] = j * split < columns && p + q < split ? load_peer(addr + j * split * (kTcFeatures * 4), p + q) : 0.0f;
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int j = 0; j < kTogether; ++j) v[j] += w[q][j];
+    }
 }
 
 constexpr int stages_for(int bytes, int stage) { return bytes / stage < 12 ? bytes / stage : 12; }
@@ -132,6 +152,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     constexpr bool PAIRED = S::kPaired;
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
 
+    let_next_launch_start();
+    if (!a.ahead) wait_for_launch_before();
     // ---- tiles of the groups
     {
         constexpr int PER = (kMaxRowGroups + 1 + kTcThreads - 1) / kTcThreads;  // a list with the ungrouped rows has one group more
@@ -261,6 +283,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             }
         } else if (loads_rows) {
             row = next_row;
+            // neighbouring rows in order (a request's, listed by adapter) come as one box
+            const int row0 = __shfl_sync(0xffffffffu, row, 0);
+            const bool run = __all_sync(0xffffffffu, lane >= RPW || row == row0 + lane);
             fetch_rows(tile + workers);  // under way while this tile is loaded
             for (int s = s0; s < s1; ++s, pos.next(stages)) {
                 const int st = pos.stage;
@@ -269,6 +294,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 __syncwarp();
                 if (s >= main_steps) continue;
                 const uint32_t dst = ring + st * S::kStage + kTcFeatures * 128 + (warp - 8) * RPW * 128;
+                if (run) {
+                    if (elect_one()) tma_2d<PAIRED>(dst, &a.x_run, s * kTcDepth, row0, full0 + st * 8);
+                    continue;
+                }
 #pragma unroll
                 for (int q = 0; q < RPW / 4; ++q) {
                     const int r0 = __shfl_sync(0xffffffffu, row, 4 * q), r1 = __shfl_sync(0xffffffffu, row, 4 * q + 1);
@@ -303,8 +332,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (reduce) {
                 mbar_wait(smem_addr(&pipe.freed), (turn & 1) ^ 1, gave_up, a.status);
                 if (a.ids) {
-                    // the columns this block stores start from u times the adapter's matrix: four columns' loads in flight
-                    if (a.ahead && turn == 0) wait_for_launch_before();
+                    // the columns this block stores start from u times the adapter's matrix: four columns' loads in flight, the
+                    // matrices asked for before the wait for u
+                    if (turn == 0) {
+                        for (int c = part; slot0 + c < slot1; c += split) {
+                            const int id = a.ids[slot0 + c];
+                            if ((unsigned)id < (unsigned)a.delta_adapters && f < a.n)
+                                for (int r = 0; r < a.delta_rank; r += a.delta_r == 1 ? 64 : 1)
+                                    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.delta_m + id * a.delta_group + f * a.delta_f + r * a.delta_r));
+                        }
+                        if (a.ahead) wait_for_launch_before();
+                    }
                     for (int c = part; slot0 + c < slot1; c += 4 * split) {
                         const float *u[4];
                         const uint16_t *m[4];
@@ -360,7 +398,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     for (int j = 0; j < 32; ++j) {
                         const uint32_t at = own_partial + (c0 + j) * (kTcFeatures * 4);
                         float have = 0.0f;
-                        if (a.ids && (c0 + j) % split == part && slot0 + c0 + j < slot1) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(have) : "r"(at) : "memory");
+                        if (a.ids && ((c0 + j) & (split - 1)) == part && slot0 + c0 + j < slot1) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(have) : "r"(at) : "memory");
                         asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v[j] + have) : "memory");
                     }
                 } else if (wide) {
@@ -391,10 +429,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 tell_cluster(smem_addr(&pipe.partials), split, lane);
                 mbar_wait(smem_addr(&pipe.partials), turn & 1, gave_up, a.status);
                 fence_cluster();
-                for (int c = part; slot0 + c < slot1; c += split) {
-                    float v = 0.0f;
-                    for (int p = 0; p < split; ++p) v += load_peer(own_partial + c * (kTcFeatures * 4), p);
-                    store(slot0 + c, v * scale);
+                for (int c = part; slot0 + c < slot1; c += kTogether * split) {
+                    float v[kTogether] = {};
+                    add_partials(v, own_partial + c * (kTcFeatures * 4), split, NT - c);
+#pragma unroll
+                    for (int j = 0; j < kTogether; ++j)
+                        if (slot0 + c + j * split < slot1) store(slot0 + c + j * split, v[j] * scale);
                 }
                 tell_cluster(smem_addr(&pipe.freed), split, lane);
             } else if (wide) results_sync();  // the next tile starts with the first buffer again
@@ -451,6 +491,7 @@ struct TcOuter {
     void *out;
     long long out_group, out_f, out_c;
     int split;
+    bool follows;
     int *status;
 };
 
@@ -477,8 +518,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     constexpr bool PAIRED = S::kPaired;
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
+    let_next_launch_start();
     if (tid == 0) pipe_init(pipe, stages, PAIRED, split);
     if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), 2 * NT);
+    wait_for_launch_before();
     tc_fence_before();
     __syncthreads();
     if (PAIRED || split > 1) cluster_sync();
@@ -592,6 +635,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             const int quad = warp & 3, f = f0 + quad * 32 + lane, mine = tid - 128;
             uint16_t *out = (uint16_t *)a.out + g * a.out_group;
             const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT;
+            const uint32_t own_partial = partial + (quad * 32 + lane) * 4;
             const bool none = s0 == s1;
             const bool wide = a.out_f == 1 && a.i % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
 #pragma unroll 1
@@ -609,7 +653,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 if (split > 1) {
 #pragma unroll
                     for (int x = 0; x < 32; ++x)
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(partial + ((c + x) * kTcFeatures + quad * 32 + lane) * 4), "f"(v[x]) : "memory");
+                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(own_partial + (c + x) * (kTcFeatures * 4)), "f"(v[x]) : "memory");
                 } else if (wide) {
                     const uint32_t at = staging + (c >> 5 & 1) * (32 * kOutPitch);
 #pragma unroll
@@ -634,10 +678,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 tell_cluster(smem_addr(&pipe.partials), split, lane);
                 mbar_wait(smem_addr(&pipe.partials), turn & 1, gave_up, a.status);
                 fence_cluster();
-                for (int c = part; c < cols && c0 + c < a.j; c += split) {
-                    float v = 0.0f;
-                    for (int p = 0; p < split; ++p) v += load_peer(partial + (c * kTcFeatures + quad * 32 + lane) * 4, p);
-                    if (f < a.i) out[f * a.out_f + (c0 + c) * a.out_c] = to_16(v, a.bf16);
+                for (int c = part; c < cols && c0 + c < a.j; c += kTogether * split) {
+                    float v[kTogether] = {};
+                    add_partials(v, own_partial + c * (kTcFeatures * 4), split, cols - c);
+#pragma unroll
+                    for (int j = 0; j < kTogether; ++j) {
+                        const int cc = c + j * split;
+                        if (f < a.i && cc < cols && c0 + cc < a.j) out[f * a.out_f + (c0 + cc) * a.out_c] = to_16(v[j], a.bf16);
+                    }
                 }
                 tell_cluster(smem_addr(&pipe.freed), split, lane);
             } else if (wide) results_sync();

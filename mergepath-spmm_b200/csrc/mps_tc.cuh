@@ -221,14 +221,16 @@ __device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
     mbar_arrive_cluster(remote);
 }
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
-// Waits for the launch before this one on the stream, where this one was allowed to start ahead of its end.
+// Launches of one call follow one another with programmatic serialization: every kernel lets the next one start at once (its
+// blocks take the SMs that fall free, its set-up overlaps the end of this one) and waits for the launch before it, and with it
+// all earlier ones, before it touches memory.  Nothing where a launch was an ordinary one.
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
     uint32_t remote;
     float v;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote) : "memory");
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
     return v;
 }
 

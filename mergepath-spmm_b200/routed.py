@@ -98,12 +98,12 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, n_groups: in
     dev = logits.device
     _check(dev, ("logits", logits, logits.dtype, (rows, experts)), ("bias", bias, torch.float32, (experts,)))
     spec = _spec(experts, top_k, score, n_groups, top_groups, group_top, renormalise, scale)
-    ids = torch.empty((rows, top_k), dtype=torch.int32, device=dev)
-    weights = torch.empty((rows, top_k), dtype=torch.float32, device=dev)
-    groups = None
-    if group:
-        groups = Groups(torch.empty(experts + 1, dtype=torch.int32, device=dev), torch.empty(rows * top_k, dtype=torch.int32, device=dev),
-                        torch.empty((rows, top_k), dtype=torch.int32, device=dev))
+    # one allocation: five take longer than the kernels of a small batch
+    k = max(top_k, 0)  # what is wrong with it the entry point says
+    n, shape, pitch = rows * k, (rows, k), (k, 1)
+    buf = torch.empty(4 * n + experts + 1 if group else 2 * n, dtype=torch.int32, device=dev)
+    ids, weights = buf.as_strided(shape, pitch, 0), buf.view(torch.float32).as_strided(shape, pitch, n)
+    groups = Groups(buf.as_strided((experts + 1,), (1,), 4 * n), buf.as_strided((n,), (1,), 2 * n), buf.as_strided(shape, pitch, 3 * n)) if group else None
     ptr, row, slot = groups or (None, None, None)
     _call(dev, stream, "mps_route", rows, C.byref(spec), _dtype(logits), _ptr(logits), _ptr(bias), _ptr(ids), _ptr(weights), _ptr(ptr), _ptr(row), _ptr(slot))
     return ids, weights, groups
