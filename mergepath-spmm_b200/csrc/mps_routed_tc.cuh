@@ -92,21 +92,73 @@ __device__ __forceinline__ void tell_cluster(uint32_t bar, int split, int lane) 
     if (lane < split) mbar_arrive_at(bar, lane);
 }
 
-// The parts of all blocks, in their order, for columns a `split` apart (kTogether of them, those below `columns`): the loads of
-// a block's part are in flight together, one by one they took 13 us for 32 columns.
-constexpr int kTogether = 8;
-__device__ __forceinline__ void add_partials(float (&v)[kTogether], uint32_t addr, int split, int columns) {
-    for (int p = 0; p < split; p += 2) {  // split is 1 or even
-        float w[2][kTogether];
+// Where the parts of a tile's sums meet: block o of the cluster adds up the o-th of `split` equal runs of columns, in the order
+// of the blocks.  Every block writes its part of a run into block o's shared memory (reading the others' from there took a
+// microsecond a round: 13 us for 32 columns).
+struct Meeting {
+    uint32_t buffer;  // [blocks][columns of a run][features]
+    int split, part, run;
+    __device__ __forceinline__ uint32_t at(int block, int column) const { return buffer + (block * run + column % run) * (kTcFeatures * 4); }
+    // eight columns from c (a multiple of eight) of one feature; start: the buffer holds something to start from where this
+    // block adds up
+    __device__ __forceinline__ void give(int c, int feature, const float *v, bool start) const {
+        const int owner = c / run;
+        const uint32_t to = at(part, c) + feature * 4;
+        if (owner == part) {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+            for (int j = 0; j < 8; ++j) store_shared_f32(to + j * (kTcFeatures * 4), start ? v[j] + load_shared_f32(to + j * (kTcFeatures * 4)) : v[j]);
+        } else {
+            const uint32_t remote = in_block(to, owner);
 #pragma unroll
-            for (int j = 0; j < kTogether; ++j)
-                w[q][j] = j * split < columns && p + q < split ? load_peer(addr + j * split * (kTcFeatures * 4), p + q) : 0.0f;
+            for (int j = 0; j < 8; ++j) store_cluster_f32(remote + j * (kTcFeatures * 4), v[j]);
+        }
+    }
+    __device__ __forceinline__ float sum(int column, int feature) const {
+        float v = 0.0f;
+        for (int p = 0; p < split; ++p) v += load_shared_f32(at(p, column) + feature * 4);
+        return v;
+    }
+    __device__ __forceinline__ void sum8(int column, int feature, float (&v)[8]) const {
 #pragma unroll
-        for (int q = 0; q < 2; ++q)
+        for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+        for (int p = 0; p < split; ++p) {
+            const uint32_t from = at(p, column) + feature * 4;
+            const float4 x = load_shared_float4(from), y = load_shared_float4(from + 16);
+            v[0] += x.x, v[1] += x.y, v[2] += x.z, v[3] += x.w, v[4] += y.x, v[5] += y.y, v[6] += y.z, v[7] += y.w;
+        }
+    }
+};
+
+__device__ __forceinline__ uint4 pack_16(const float (&v)[8], float scale, bool bf16) {
+    uint32_t w[4];
 #pragma unroll
-            for (int j = 0; j < kTogether; ++j) v[j] += w[q][j];
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)to_16(v[2 * i] * scale, bf16) | (uint32_t)to_16(v[2 * i + 1] * scale, bf16) << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// v[j] += <u of column c + j, the feature's row of that column's matrix> over `ranks` (a multiple of eight): u in shared memory (64
+// floats a column), m[j] the matrices' addresses, `stride` elements between ranks.
+template <bool BF16>
+__device__ __forceinline__ void add_low_rank(float (&v)[4], const uint32_t (&u)[4], const uint16_t *const (&m)[4], int ranks, long long stride) {
+    for (int r = 0; r < ranks; r += 8) {
+        uint32_t w[4][4];
+        if (stride == 1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4 *>(w[j]) = *reinterpret_cast<const uint4 *>(m[j] + r);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[j][i] = m[j][(r + 2 * i) * stride] | (uint32_t)m[j][(r + 2 * i + 1) * stride] << 16;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float4 x = load_shared_float4(u[j] + (r + 4 * h) * 4);
+                const float2 p = from_16x2<BF16>(w[j][2 * h]), q = from_16x2<BF16>(w[j][2 * h + 1]);
+                v[j] = fmaf(x.w, q.y, fmaf(x.z, q.x, fmaf(x.y, p.y, fmaf(x.x, p.x, v[j]))));
+            }
     }
 }
 
@@ -231,7 +283,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     };
     const bool loads_rows = warp >= 8 && a.gather;
     if (loads_rows) fetch_rows(worker);
-    const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);  // where loads are reported
+    const uint32_t full0 = PAIRED ? in_block(smem_addr(&pipe.full[0]), 0) : smem_addr(&pipe.full[0]);  // where loads are reported
     RingAt pos;  // this warp's place in the ring
 
     int turn = 0;  // tiles done so far
@@ -328,79 +380,81 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     }
                 }
             };
-            const uint32_t own_partial = partial + (quad * 32 + lane) * 4;  // this thread's feature, columns kTcFeatures * 4 bytes apart
+            const Meeting meeting = {partial, split, part, NT / split};
+            const int feature = quad * 32 + lane;
             if (reduce) {
                 mbar_wait(smem_addr(&pipe.freed), (turn & 1) ^ 1, gave_up, a.status);
                 if (a.ids) {
-                    // the columns this block stores start from u times the adapter's matrix: four columns' loads in flight, the
-                    // matrices asked for before the wait for u
+                    // The columns this block adds up start from u times the adapter's matrix.  The matrices are asked for before
+                    // the wait for u; u goes through shared memory, 64 of the rank at a time; four columns' loads are in flight.
+                    const int first_slot = slot0 + part * meeting.run, own = min(max(slot1 - first_slot, 0), meeting.run);
+                    int id[2];  // of the columns lane and lane + 32
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        id[h] = lane + 32 * h < own ? a.ids[first_slot + lane + 32 * h] : -1;
+                        if (id[h] >= a.delta_adapters) {
+                            atomicOr(a.status, kStatusBadIndex);
+                            id[h] = -1;
+                        }
+                    }
+                    const int fc = min(f, a.n - 1);
+                    auto matrix = [&](int c) {  // of column c; some adapter's where it has none
+                        const int i = __shfl_sync(0xffffffffu, c < 32 ? id[0] : id[1], c & 31);
+                        return a.delta_m + max(i, 0) * a.delta_group + fc * a.delta_f;
+                    };
                     if (turn == 0) {
-                        for (int c = part; slot0 + c < slot1; c += split) {
-                            const int id = a.ids[slot0 + c];
-                            if ((unsigned)id < (unsigned)a.delta_adapters && f < a.n)
-                                for (int r = 0; r < a.delta_rank; r += a.delta_r == 1 ? 64 : 1)
-                                    asm volatile("prefetch.global.L2 [%0];" ::"l"(a.delta_m + id * a.delta_group + f * a.delta_f + r * a.delta_r));
+                        for (int c = 0; c < own; ++c) {
+                            const uint16_t *m = matrix(c);
+                            for (int r = 0; r < a.delta_rank; r += a.delta_r == 1 ? 64 : 1) asm volatile("prefetch.global.L2 [%0];" ::"l"(m + r * a.delta_r));
                         }
                         if (a.ahead) wait_for_launch_before();
                     }
-                    for (int c = part; slot0 + c < slot1; c += 4 * split) {
-                        const float *u[4];
-                        const uint16_t *m[4];
-                        float v[4] = {};
-                        bool live[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int slot = slot0 + c + j * split;
-                            int id = slot < slot1 ? a.ids[slot] : -1;
-                            if (id >= a.delta_adapters) {
-                                atomicOr(a.status, kStatusBadIndex);
-                                id = -1;
-                            }
-                            live[j] = id >= 0 && f < a.n;
-                            u[j] = a.delta_u + (long long)(live[j] ? slot : 0) * a.delta_rank;
-                            m[j] = a.delta_m + (live[j] ? id * a.delta_group + f * a.delta_f : 0);
+                    for (int r0 = 0; r0 < a.delta_rank; r0 += 64) {
+                        const int ranks = min(64, a.delta_rank - r0);  // multiples of eight here
+                        for (int i = mine * 4; i < own * ranks; i += 128 * 4) {
+                            const int c = i / ranks, r = i - c * ranks;
+                            const float4 q = *reinterpret_cast<const float4 *>(a.delta_u + (long long)(first_slot + c) * a.delta_rank + r0 + r);
+                            asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(staging + (c * 64 + r) * 4), "f"(q.x), "f"(q.y), "f"(q.z), "f"(q.w)
+                                         : "memory");
                         }
-                        for (int r = 0; r < a.delta_rank; r += 8) {  // the rank is a multiple of eight here
-                            uint16_t w[4][8];
+                        results_sync();
+                        for (int c = 0; c < own; c += 4) {
+                            const uint16_t *m[4];
+                            uint32_t u[4];
+                            float v[4] = {};
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                if (!live[j]) continue;
-                                if (a.delta_r == 1) *reinterpret_cast<uint4 *>(w[j]) = *reinterpret_cast<const uint4 *>(m[j] + r);
-                                else
-#pragma unroll
-                                    for (int i = 0; i < 8; ++i) w[j][i] = m[j][(r + i) * a.delta_r];
+                                const int cc = min(c + j, own - 1);
+                                m[j] = matrix(cc) + r0 * a.delta_r;
+                                u[j] = staging + cc * 64 * 4;
                             }
+                            if (a.bf16) add_low_rank<true>(v, u, m, ranks, a.delta_r);
+                            else add_low_rank<false>(v, u, m, ranks, a.delta_r);
 #pragma unroll
                             for (int j = 0; j < 4; ++j) {
-                                if (!live[j]) continue;
-                                const float4 p = *reinterpret_cast<const float4 *>(u[j] + r), q = *reinterpret_cast<const float4 *>(u[j] + r + 4);
-                                const float x[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
-#pragma unroll
-                                for (int i = 0; i < 8; ++i) v[j] = fmaf(x[i], from_16(w[j][i], a.bf16), v[j]);
+                                const int cc = c + j;
+                                const bool live = __shfl_sync(0xffffffffu, cc < 32 ? id[0] : id[1], cc & 31) >= 0;
+                                if (cc >= own) continue;
+                                const uint32_t to = meeting.at(part, cc) + feature * 4;
+                                const float have = r0 ? load_shared_f32(to) : 0.0f;
+                                store_shared_f32(to, live ? have + v[j] : have);  // whatever was read for a column without one stays out
                             }
                         }
-#pragma unroll
-                        for (int j = 0; j < 4; ++j)
-                            if (slot0 + c + j * split < slot1)
-                                asm volatile("st.shared.f32 [%0], %1;" ::"r"(own_partial + (c + j * split) * (kTcFeatures * 4)), "f"(v[j]) : "memory");
+                        results_sync();  // before the next ranks' u
                     }
                 }
             }
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
             tc_fence_after();
-            const bool wide = !reduce && !a.pair && a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
+            const bool rows_of_16 = !a.pair && a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0, wide = rows_of_16 && !reduce;
 #pragma unroll 1
             for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 32) {
                 float v[32];
                 tmem_load(tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + c0, v);
                 if (reduce) {
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const uint32_t at = own_partial + (c0 + j) * (kTcFeatures * 4);
-                        float have = 0.0f;
-                        if (a.ids && ((c0 + j) & (split - 1)) == part && slot0 + c0 + j < slot1) asm volatile("ld.shared.f32 %0, [%1];" : "=f"(have) : "r"(at) : "memory");
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(v[j] + have) : "memory");
-                    }
+                    for (int j = 0; j < 32; j += 8)
+                        if (slot0 + c0 + j < slot1) meeting.give(c0 + j, feature, v + j, a.ids);
                 } else if (wide) {
                     const uint32_t at = staging + (c0 >> 5 & 1) * (32 * kOutPitch);
 #pragma unroll
@@ -422,20 +476,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 }
             }
             tc_fence_before();
-            if (PAIRED) mbar_arrive_cluster(in_first(smem_addr(&pipe.tmem_empty[buf])));
+            if (PAIRED) mbar_arrive_at(smem_addr(&pipe.tmem_empty[buf]), 0);
             else mbar_arrive(smem_addr(&pipe.tmem_empty[buf]));
             if (reduce) {
                 // every block of the cluster adds up and stores its share of the columns
                 tell_cluster(smem_addr(&pipe.partials), split, lane);
                 mbar_wait(smem_addr(&pipe.partials), turn & 1, gave_up, a.status);
                 fence_cluster();
-                for (int c = part; slot0 + c < slot1; c += kTogether * split) {
-                    float v[kTogether] = {};
-                    add_partials(v, own_partial + c * (kTcFeatures * 4), split, NT - c);
-#pragma unroll
-                    for (int j = 0; j < kTogether; ++j)
-                        if (slot0 + c + j * split < slot1) store(slot0 + c + j * split, v[j] * scale);
-                }
+                const int first = part * meeting.run, own = min(max(slot1 - slot0 - first, 0), meeting.run);
+                if (rows_of_16) {
+                    const int fc = (mine & 15) * 8;
+                    for (int c = mine >> 4; c < own; c += 8) {
+                        float v[8];
+                        meeting.sum8(c, fc, v);
+                        const int r = out_row(slot0 + first + c);
+                        if (f0 + fc < a.n && r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = pack_16(v, scale, a.bf16);
+                    }
+                } else
+                    for (int c = 0; c < own; ++c) store(slot0 + first + c, meeting.sum(c, feature) * scale);
                 tell_cluster(smem_addr(&pipe.freed), split, lane);
             } else if (wide) results_sync();  // the next tile starts with the first buffer again
         }
@@ -533,7 +591,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     const long long n_tiles = (long long)a.n_groups * i_tiles * j_tiles;
     const long long worker = blockIdx.x / group_blocks, workers = gridDim.x / group_blocks;
     const bool gather = a.slot_row != nullptr;
-    const uint32_t full0 = PAIRED ? in_first(smem_addr(&pipe.full[0])) : smem_addr(&pipe.full[0]);
+    const uint32_t full0 = PAIRED ? in_block(smem_addr(&pipe.full[0]), 0) : smem_addr(&pipe.full[0]);
     RingAt pos;
     int turn = 0;
     for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
@@ -635,7 +693,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             const int quad = warp & 3, f = f0 + quad * 32 + lane, mine = tid - 128;
             uint16_t *out = (uint16_t *)a.out + g * a.out_group;
             const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT;
-            const uint32_t own_partial = partial + (quad * 32 + lane) * 4;
+            const Meeting meeting = {partial, split, part, cols / split};
+            const int feature = quad * 32 + lane;
             const bool none = s0 == s1;
             const bool wide = a.out_f == 1 && a.i % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
 #pragma unroll 1
@@ -652,8 +711,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
                 if (split > 1) {
 #pragma unroll
-                    for (int x = 0; x < 32; ++x)
-                        asm volatile("st.shared.f32 [%0], %1;" ::"r"(own_partial + (c + x) * (kTcFeatures * 4)), "f"(v[x]) : "memory");
+                    for (int x = 0; x < 32; x += 8) meeting.give(c + x, feature, v + x, false);
                 } else if (wide) {
                     const uint32_t at = staging + (c >> 5 & 1) * (32 * kOutPitch);
 #pragma unroll
@@ -672,20 +730,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
             }
             tc_fence_before();
-            if (PAIRED) mbar_arrive_cluster(in_first(smem_addr(&pipe.tmem_empty[buf])));
+            if (PAIRED) mbar_arrive_at(smem_addr(&pipe.tmem_empty[buf]), 0);
             else mbar_arrive(smem_addr(&pipe.tmem_empty[buf]));
             if (split > 1) {
                 tell_cluster(smem_addr(&pipe.partials), split, lane);
                 mbar_wait(smem_addr(&pipe.partials), turn & 1, gave_up, a.status);
                 fence_cluster();
-                for (int c = part; c < cols && c0 + c < a.j; c += kTogether * split) {
-                    float v[kTogether] = {};
-                    add_partials(v, own_partial + c * (kTcFeatures * 4), split, cols - c);
-#pragma unroll
-                    for (int j = 0; j < kTogether; ++j) {
-                        const int cc = c + j * split;
-                        if (f < a.i && cc < cols && c0 + cc < a.j) out[f * a.out_f + (c0 + cc) * a.out_c] = to_16(v[j], a.bf16);
-                    }
+                const int first = part * meeting.run, own = min(max(a.j - c0 - first, 0), meeting.run);
+                for (int c = 0; c < own; ++c) {
+                    const float v = meeting.sum(c, feature);
+                    if (f < a.i) out[f * a.out_f + (c0 + first + c) * a.out_c] = to_16(v, a.bf16);
                 }
                 tell_cluster(smem_addr(&pipe.freed), split, lane);
             } else if (wide) results_sync();

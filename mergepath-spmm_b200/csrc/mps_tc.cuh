@@ -186,6 +186,12 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
 __device__ __forceinline__ uint16_t to_16(float v, bool bf16) {
     return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
+// two values of a 32-bit word, the lower half first
+template <bool BF16>
+__device__ __forceinline__ float2 from_16x2(uint32_t v) {
+    if constexpr (BF16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+    else return __half22float2(__halves2half2(__ushort_as_half((uint16_t)v), __ushort_as_half((uint16_t)(v >> 16))));
+}
 __device__ __forceinline__ float from_16(uint16_t v, bool bf16) { return bf16 ? __bfloat162float(__ushort_as_bfloat16(v)) : __half2float(__ushort_as_half(v)); }
 
 __device__ __forceinline__ void store_shared_16(uint32_t addr, uint16_t v) { asm volatile("st.shared.u16 [%0], %1;" ::"r"(addr), "h"(v) : "memory"); }
@@ -205,20 +211,19 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// the address of block 0's variable of that address in this block
-__device__ __forceinline__ uint32_t in_first(uint32_t addr) {
+// the address of block `rank`'s variable of that address in this block, and a store to it
+__device__ __forceinline__ uint32_t in_block(uint32_t addr, uint32_t rank) {
     uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(addr));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
     return remote;
 }
+__device__ __forceinline__ void store_cluster_f32(uint32_t addr, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 // Arrives at a barrier of either block.  (With .release.cluster the arrival waits for the thread's writes to reach the cluster,
 // about a microsecond; it follows no writes here that the other block reads.)
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
 // the same at block `rank`'s barrier of that address
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar, uint32_t rank) {
-    uint32_t remote;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(bar), "r"(rank));
-    mbar_arrive_cluster(remote);
+    mbar_arrive_cluster(in_block(bar, rank));
 }
 __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cluster;" ::: "memory"); }
 // Launches of one call follow one another with programmatic serialization: every kernel lets the next one start at once (its
@@ -226,13 +231,17 @@ __device__ __forceinline__ void fence_cluster() { asm volatile("fence.acq_rel.cl
 // all earlier ones, before it touches memory.  Nothing where a launch was an ordinary one.
 __device__ __forceinline__ void wait_for_launch_before() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_launch_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ float load_peer(uint32_t addr, uint32_t rank) {
-    uint32_t remote;
+__device__ __forceinline__ float load_shared_f32(uint32_t addr) {
     float v;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(remote));
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
+__device__ __forceinline__ float4 load_shared_float4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void store_shared_f32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 
 // the products of one slice: `steps` (1..4) times 16 summed elements, the first overwriting the accumulator unless `add`
 template <bool PAIRED>
