@@ -274,7 +274,7 @@ __device__ __noinline__ int decide_exactly(const RouteArgs &a, const T *line, co
 // keys that decide it lie closer together than fp32 can tell is decided again on fp64 keys.  That keeps the choice the
 // definition's at a fraction of the cost of fp64 throughout.
 template <typename T, int VPL, bool SIGMOID>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_kernel(const RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
+__global__ void __launch_bounds__(32 * kRouteWarps, VPL <= 8 ? 8 : 1) route_kernel(const RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
                                                                 int *__restrict__ ids, float *__restrict__ weights) {
     extern __shared__ double s_cells[];
     mps::let_next_launch_start();

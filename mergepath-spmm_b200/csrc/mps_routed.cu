@@ -255,7 +255,7 @@ int split_of(long long tiles, int steps, int sms) {
 
 // How the rows of a product are cut: slots per tile and blocks per tile's sum, by an estimate of the time in SM cycles.  A step of
 // 64 summed elements takes the longest of its products (2 cycles a slot and 128 features), its bytes (64 a cycle and SM out of
-// L2) and its gathered rows (4.3 cycles each); a tile costs 1,500 cycles more where nothing overlaps its first loads and last
+// L2), its gathered rows (4.3 cycles each) and what its issue takes (330); a tile costs 1,500 cycles more where nothing overlaps its first loads and last
 // stores, 2,500 where a cluster adds its parts.  Measured: 32,768 slots of 32 groups, 2048 x 2048: 250 us with 256 slots per
 // tile; 32 slots of 64 groups, 1024 x 2048: 28 us with 32.
 struct Cut {
@@ -271,7 +271,7 @@ Cut best_cut(int slots, int groups, int features, int steps, bool gather, int sm
         const double per = slots / active, tiles_of_group = groups == 1 ? std::ceil(per / nt) : std::fmax(1.0, per / nt + 0.5);
         const double tiles = active * tiles_of_group * ((features + tile_f - 1) / tile_f);
         const double bytes = 128.0 * ((features < 128 ? features : 128) + loaded);
-        const double step = std::fmax(std::fmax(2.0 * nt + 20, bytes / 64), gather ? 4.3 * loaded : 0.0);
+        const double step = std::fmax(std::fmax(330.0, std::fmax(2.0 * nt + 20, bytes / 64)), gather ? 4.3 * loaded : 0.0);
         for (int split = 1; split <= (nt <= 64 ? nt / 8 : 1); split *= 2) {  // a block adds up eight columns at least
             if (split > 1 && steps < 2 * split) break;  // two slices each at least
             const double waves = std::ceil(tiles / (sms / (paired ? 2 : split)) - 0.05);

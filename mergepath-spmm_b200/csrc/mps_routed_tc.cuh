@@ -48,7 +48,7 @@ struct TcRows {
     int u_plane;              // rows between the hi and the lo plane of u
     int w_rows;               // rows of a matrix box (features, where they are its rows)
     bool w_shared, mn_major, gather, bf16, scatter, pair;  // pair: result stored as hi + lo planes of out
-    const float *group_scale;
+    const float *group_scale;  // pair: factor of a group's results (NULL: 1)
     void *out;
     long long out_plane;
     float *out_f32;           // pair: the result in fp32 too, by row (NULL: not wanted)
@@ -129,11 +129,21 @@ struct Meeting {
     }
 };
 
-__device__ __forceinline__ uint4 pack_16(const float (&v)[8], float scale, bool bf16) {
-    uint32_t w[4];
+__device__ __forceinline__ uint4 pack_16(const float (&v)[8], bool bf16) {
+    return bf16 ? make_uint4(to_16x2<true>(v[0], v[1]), to_16x2<true>(v[2], v[3]), to_16x2<true>(v[4], v[5]), to_16x2<true>(v[6], v[7]))
+                : make_uint4(to_16x2<false>(v[0], v[1]), to_16x2<false>(v[2], v[3]), to_16x2<false>(v[4], v[5]), to_16x2<false>(v[6], v[7]));
+}
+
+// 32 columns of one feature into 32 rows of shared memory, kOutPitch apart.  What the four result warps issue per tile is what a
+// short sum waits for, so the rounding takes two values an instruction and the type is no branch per value.
+template <bool BF16>
+__device__ __forceinline__ void spread_column(const float (&v)[32], uint32_t to) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)to_16(v[2 * i] * scale, bf16) | (uint32_t)to_16(v[2 * i + 1] * scale, bf16) << 16;
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < 32; j += 2) {
+        const uint32_t w = to_16x2<BF16>(v[j], v[j + 1]);
+        store_shared_16(to + j * kOutPitch, (uint16_t)w);
+        store_shared_16(to + (j + 1) * kOutPitch, (uint16_t)(w >> 16));
+    }
 }
 
 // v[j] += <u of column c + j, the feature's row of that column's matrix> over `ranks` (a multiple of eight): u in shared memory (64
@@ -173,16 +183,28 @@ struct TcShape {
     static constexpr int kColumns = 2 * NT;
     static constexpr int kReduce = NT <= 64 ? NT * kTcFeatures * 4 : 0;  // only small tiles are split
     static constexpr int kSplitStages = stages_for(kTcRing - kReduce, kStage);
-    static size_t bytes(int n_groups) { return 1024 + kTcRing + kOutTotal + (size_t)(3 * n_groups + 1) * sizeof(int); }
+    static size_t bytes(int n_groups) { return 1024 + kTcRing + kOutTotal + (size_t)(4 * n_groups + 2) * sizeof(int); }
 };
 
-// A cursor over the tiles of all groups: tile numbers only rise, so the group is found by walking on.
+// A cursor over the tiles of all groups: tile numbers only rise, so the group is found by walking on.  Where the matrix is shared
+// the whole tiles of every group come first and then the groups' rests: blocks take tiles in turn, and the short ones at the end
+// even out what the long ones leave (4096 rows of 8 adapters: 160 -> 152 us).  With a matrix per group a group's tiles stay
+// together, its rest counted among them, or the matrices would be read twice (32 groups: 257 -> 270 us).
 struct TcCursor {
-    const int *first, *lo, *hi;  // first tile of every group (n_groups + 1), its slots
-    int group, slot0, slot1;
+    const int *whole, *rest, *lo, *hi;  // whole tiles and rests before every group (n_groups + 1 each), its slots
+    int n_groups, group, slot0, slot1;
+    bool rests;
     __device__ __forceinline__ void seek(int tile, int nt) {
-        while (tile >= first[group + 1]) ++group;
-        slot0 = lo[group] + (tile - first[group]) * nt;
+        const int n_whole = whole[n_groups];
+        if (tile >= n_whole) {
+            if (!rests) group = 0;
+            rests = true;
+            while (tile - n_whole >= rest[group + 1]) ++group;
+            slot0 = lo[group] + (whole[group + 1] - whole[group]) * nt;
+        } else {
+            while (tile >= whole[group + 1]) ++group;
+            slot0 = lo[group] + (tile - whole[group]) * nt;
+        }
         slot1 = min(slot0 + nt, hi[group]);
     }
 };
@@ -192,11 +214,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     using S = TcShape<NT>;
     extern __shared__ uint8_t s_raw[];
     __shared__ TcPipe pipe;
-    __shared__ int s_sum[kTcThreads / 32];
+    __shared__ int s_sum[2][kTcThreads / 32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = (smem_addr(s_raw) + 1023) & ~1023u, staging = ring + kTcRing;
-    int *first = reinterpret_cast<int *>(s_raw + (ring - smem_addr(s_raw)) + kTcRing + kOutTotal);
-    int *lo = first + a.n_groups + 1, *hi = lo + a.n_groups;
+    int *whole = reinterpret_cast<int *>(s_raw + (ring - smem_addr(s_raw)) + kTcRing + kOutTotal);
+    int *rest = whole + a.n_groups + 1, *lo = rest + a.n_groups + 1, *hi = lo + a.n_groups;
     const int split = a.split, part = split > 1 ? (int)cluster_rank() : 0;
     const bool reduce = split > 1 || a.ids;  // results meet in shared memory before they are stored
     const int stages = reduce ? S::kSplitStages : S::kStages;
@@ -209,7 +231,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     // ---- tiles of the groups
     {
         constexpr int PER = (kMaxRowGroups + 1 + kTcThreads - 1) / kTcThreads;  // a list with the ungrouped rows has one group more
-        int tiles[PER], sum = 0;
+        int tiles[PER], sum = 0, sum_rest = 0;  // a whole tile counts 2, a rest 1
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int g = tid * PER + i;
@@ -219,28 +241,46 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 if (a.group_ptr) r = group_range(a.group_ptr, g, a.n_slots, a.status);
                 lo[g] = r.x;
                 hi[g] = r.y;
-                tiles[i] = (r.y - r.x + NT - 1) / NT;
+                const int n = r.y - r.x;
+                tiles[i] = a.w_shared ? n / NT * 2 + (n % NT ? 1 : 0) : (n + NT - 1) / NT * 2;
             }
-            sum += tiles[i];
+            sum += tiles[i] >> 1;
+            sum_rest += tiles[i] & 1;
         }
-        int scan = sum;
+        int scan = sum, scan_rest = sum_rest;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, scan, d);
-            if (lane >= d) scan += o;
+            const int o = __shfl_up_sync(0xffffffffu, scan, d), q = __shfl_up_sync(0xffffffffu, scan_rest, d);
+            if (lane >= d) {
+                scan += o;
+                scan_rest += q;
+            }
         }
-        if (lane == 31) s_sum[warp] = scan;
+        if (lane == 31) {
+            s_sum[0][warp] = scan;
+            s_sum[1][warp] = scan_rest;
+        }
         if (tid == 0) pipe_init(pipe, stages, PAIRED, split);
         if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), S::kColumns);
         __syncthreads();
-        for (int w = 0; w < warp; ++w) scan += s_sum[w];
-        int at = scan - sum;
+        for (int w = 0; w < warp; ++w) {
+            scan += s_sum[0][w];
+            scan_rest += s_sum[1][w];
+        }
+        int at = scan - sum, at_rest = scan_rest - sum_rest;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int g = tid * PER + i;
-            if (g < a.n_groups) first[g] = at;
-            at += tiles[i];
-            if (g == a.n_groups - 1) first[a.n_groups] = at;
+            if (g < a.n_groups) {
+                whole[g] = at;
+                rest[g] = at_rest;
+            }
+            at += tiles[i] >> 1;
+            at_rest += tiles[i] & 1;
+            if (g == a.n_groups - 1) {
+                whole[a.n_groups] = at;
+                rest[a.n_groups] = at_rest;
+            }
         }
         tc_fence_before();
         __syncthreads();
@@ -252,9 +292,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
     const int feature_tiles = (a.n + TILE_F - 1) / TILE_F, main_steps = (a.k + kTcDepth - 1) / kTcDepth;
     const int rank_steps = 2 * ((a.rank + kTcDepth - 1) / kTcDepth);
-    const long long n_tiles = (long long)first[a.n_groups] * feature_tiles;
+    const long long n_tiles = (long long)(whole[a.n_groups] + rest[a.n_groups]) * feature_tiles;
     const long long worker = blockIdx.x / group_blocks, workers = gridDim.x / group_blocks;
-    TcCursor cur = {first, lo, hi, 0, 0, 0};
+    TcCursor cur = {whole, rest, lo, hi, a.n_groups, 0, 0, 0, false};
 
     // steps of this block for a tile of group g
     auto range = [&](int g, int &s0, int &s1) {
@@ -359,7 +399,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             }
         } else if (warp >= 4 && warp < 8) {
             const int quad = warp & 3, f = f0 + quad * 32 + lane, mine = tid - 128;
-            const float scale = a.group_scale ? a.group_scale[g] : 1.0f;
+            const float scale = a.pair && a.group_scale ? a.group_scale[g] : 1.0f;
             uint16_t *out = (uint16_t *)a.out;
             auto out_row = [&](int slot) {  // where a slot's result goes, or -1
                 if (!a.scatter) return slot;
@@ -457,8 +497,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                         if (slot0 + c0 + j < slot1) meeting.give(c0 + j, feature, v + j, a.ids);
                 } else if (wide) {
                     const uint32_t at = staging + (c0 >> 5 & 1) * (32 * kOutPitch);
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) store_shared_16(at + j * kOutPitch + (quad * 32 + lane) * 2, to_16(v[j] * scale, a.bf16));
+                    if (a.bf16) spread_column<true>(v, at + feature * 2);
+                    else spread_column<false>(v, at + feature * 2);
                     results_sync();  // one per chunk is enough: the other buffer's readers have passed it too
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
@@ -490,7 +530,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                         float v[8];
                         meeting.sum8(c, fc, v);
                         const int r = out_row(slot0 + first + c);
-                        if (f0 + fc < a.n && r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = pack_16(v, scale, a.bf16);
+                        if (f0 + fc < a.n && r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = pack_16(v, a.bf16);
                     }
                 } else
                     for (int c = 0; c < own; ++c) store(slot0 + first + c, meeting.sum(c, feature) * scale);
@@ -714,8 +754,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     for (int x = 0; x < 32; x += 8) meeting.give(c + x, feature, v + x, false);
                 } else if (wide) {
                     const uint32_t at = staging + (c >> 5 & 1) * (32 * kOutPitch);
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) store_shared_16(at + x * kOutPitch + (quad * 32 + lane) * 2, to_16(v[x], a.bf16));
+                    if (a.bf16) spread_column<true>(v, at + feature * 2);
+                    else spread_column<false>(v, at + feature * 2);
                     results_sync();
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {

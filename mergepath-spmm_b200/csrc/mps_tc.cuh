@@ -186,6 +186,14 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
 __device__ __forceinline__ uint16_t to_16(float v, bool bf16) {
     return bf16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
+// two values rounded into one 32-bit word, the first below
+template <bool BF16>
+__device__ __forceinline__ uint32_t to_16x2(float a, float b) {
+    uint32_t r;
+    if constexpr (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
 // two values of a 32-bit word, the lower half first
 template <bool BF16>
 __device__ __forceinline__ float2 from_16x2(uint32_t v) {
