@@ -33,6 +33,6 @@ struct PerDevice {
 // Status word of the routing kernels on the current device (mps_route.cu): waits for the stream, returns it and clears it.
 int take_route_status(void *stream, int *status);
 // Rows listed by id as by mps_group_rows (device arrays), those without a valid id as a last group behind the others:
-// group_ptr has n_groups + 2 entries (mps_route.cu).  follows: the launch before on the stream is one of the same call.
-int list_rows_and_rest(int n_rows, int n_groups, const int32_t *ids, int32_t *group_ptr, int32_t *slot_row, bool follows, void *stream);
+// group_ptr has n_groups + 2 entries (mps_route.cu).
+int list_rows_and_rest(int n_rows, int n_groups, const int32_t *ids, int32_t *group_ptr, int32_t *slot_row, void *stream);
 }  // namespace mps

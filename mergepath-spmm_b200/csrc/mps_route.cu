@@ -654,8 +654,8 @@ int take_route_status(void *stream, int *status) {
     if (*status) RT_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
     return MPS_OK;
 }
-int list_rows_and_rest(int n_rows, int n_groups, const int32_t *ids, int32_t *group_ptr, int32_t *slot_row, bool follows, void *stream) {
-    return launch_group(n_rows, 1, n_groups, true, ids, group_ptr, slot_row, nullptr, follows, (cudaStream_t)stream);
+int list_rows_and_rest(int n_rows, int n_groups, const int32_t *ids, int32_t *group_ptr, int32_t *slot_row, void *stream) {
+    return launch_group(n_rows, 1, n_groups, true, ids, group_ptr, slot_row, nullptr, false, (cudaStream_t)stream);
 }
 }  // namespace mps
 

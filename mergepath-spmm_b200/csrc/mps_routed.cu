@@ -431,9 +431,12 @@ struct AdapterSpace {
     }
 };
 
+// Where a launch stands among those of its call: the first; or one that uses nothing of the one before it and runs beside that.
+enum Place { kFirst, kBeside };
+
 // u (two planes, slot order) = scale * rows of x times the adapters' matrices (mn_major: stored summed x rank); u_f32 (or NULL)
 // the same by row
-int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m, bool mn_major, void *u, float *u_f32, bool follows, int sms, cudaStream_t st) {
+int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m, bool mn_major, void *u, float *u_f32, Place place, int sms, cudaStream_t st) {
     TcRows a = {};
     a.bf16 = s.dtype == MPS_BF16;
     a.mn_major = mn_major;
@@ -446,7 +449,8 @@ int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m
     a.gather = a.pair = true;
     a.group_scale = s.scale;
     a.out = u;
-    a.follows = follows;
+    a.follows = place != kFirst;
+    a.apart = place == kBeside;
     a.out_plane = (long long)s.n_rows * s.rank;
     a.out_f32 = u_f32;
     if (int rc = tc_matrix(&a.w, &a, m, k, s.rank, s.n_adapters)) return rc;
@@ -490,7 +494,6 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cu
         a.ahead = ahead;
         return tc_rows(a, cut, x, s.n_rows, sms, st);
     }
-    if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, true, st)) return rc;
     a.group_ptr = ws.ptr;
     a.slot_row = ws.row;
     a.n_groups = s.n_adapters + 1;
@@ -534,7 +537,10 @@ int adapters(const AdapterShape &s, const void *x, const void *w, const void *a,
             mps::adapter_dots_kernel<<<grid, 256, 0, st>>>(s.k, s.rank, s.n_adapters, s.dtype == MPS_BF16, s.ids, s.scale, (const uint16_t *)x,
                                                            (const uint16_t *)a, (float *)ws.u, status);
             RD_CUDA(cudaGetLastError());
-        } else if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, false, sms, st)) return rc;
+        } else {
+            if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
+            if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, kBeside, sms, st)) return rc;
+        }
         return tc_adapter_wide(s, ws, cut, rows, s.k, s.n, x, w, ws.u, (const float *)ws.u, b, false, y, rows, sms, st);
     }
     float *u = (float *)ws.u;
@@ -551,8 +557,10 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
         Cut cut;
         if (int rc = sm_count(&sms)) return rc;
         const bool rows = by_rows(s, s.n, s.k, sms, &cut);
-        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, false, sms, st)) return rc;                               // scale * x A^T
-        if (int rc = tc_adapter_narrow(s, s.n, dy, b, true, ws.v, rows ? (float *)ws.v_f32 : nullptr, true, sms, st)) return rc;  // scale * dy B
+        if (!rows)
+            if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
+        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, rows ? kFirst : kBeside, sms, st)) return rc;             // scale * x A^T
+        if (int rc = tc_adapter_narrow(s, s.n, dy, b, true, ws.v, rows ? (float *)ws.v_f32 : nullptr, kBeside, sms, st)) return rc;  // scale * dy B
         if (int rc = tc_adapter_wide(s, ws, cut, rows, s.n, s.k, dy, w, ws.v, (const float *)ws.v_f32, a, true, dx, false, sms, st)) return rc;
         if (int rc = tc_adapter_outer(s, s.k, x, ws.v, da, 1, s.k, st)) return rc;
         return tc_adapter_outer(s, s.n, dy, ws.u, db, s.rank, 1, st);

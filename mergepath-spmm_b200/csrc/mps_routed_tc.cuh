@@ -58,6 +58,7 @@ struct TcRows {
     int delta_adapters, delta_rank;
     long long delta_group, delta_f, delta_r;
     bool ahead;               // only delta_u comes from the launch before this one
+    bool apart;               // nothing does: waited for at the end, for the launches behind
     int split;                // blocks of a cluster, each with its part of the sum (a power of two)
     bool follows;             // the launch before is one of the same call (host side)
     int *status;
@@ -178,7 +179,11 @@ template <int NT>
 struct TcShape {
     static constexpr bool kPaired = NT == 256;
     static constexpr int kRows = kPaired ? NT / 2 : NT;  // slots a block loads
-    static constexpr int kStage = kTcFeatures * 128 + kRows * 128;
+    static constexpr int kSlice = kTcFeatures * 128 + kRows * 128;  // bytes of a slice
+    // Slices per stage: waiting for a stage and handing it back take a thread about 200 ns, more than the products of a slice of
+    // few slots.
+    static constexpr int kSlices = NT <= 64 ? 2 : 1;
+    static constexpr int kStage = kSlices * kSlice;
     static constexpr int kStages = stages_for(kTcRing, kStage);
     static constexpr int kColumns = 2 * NT;
     static constexpr int kReduce = NT <= 64 ? NT * kTcFeatures * 4 : 0;  // only small tiles are split
@@ -227,7 +232,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
 
     let_next_launch_start();
-    if (!a.ahead) wait_for_launch_before();
+    if (warp == 0 && lane < 5) {
+        const CUtensorMap *maps[5] = {&a.w, &a.x, &a.x_run, &a.w2, &a.u};
+        if (lane < (a.rank ? 5 : 3)) tma_prefetch(maps[lane]);
+    }
+    if (!a.ahead && !a.apart) wait_for_launch_before();
     // ---- tiles of the groups
     {
         constexpr int PER = (kMaxRowGroups + 1 + kTcThreads - 1) / kTcThreads;  // a list with the ungrouped rows has one group more
@@ -338,21 +347,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (elect_one()) {
                 const int z = a.w_shared ? 0 : g;
                 const int halves = PAIRED || a.n - f0 > 64 ? 2 : 1;  // MN-major: boxes of 64 features (as many in both blocks)
-                const uint32_t w_bytes = a.mn_major ? halves * kBlock64 : a.w_rows * 128u;
-                for (int s = s0; s < s1; ++s, pos.next(stages)) {
-                    const int st = pos.stage;
-                    mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
-                    const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
-                    const bool second = s >= main_steps;
-                    const int e = s - main_steps, i0 = (second ? e >> 1 : s) * kTcDepth;
-                    if (half == 0) mbar_expect(bar, (PAIRED ? 2 : 1) * (w_bytes + S::kRows * 128u));
-                    const CUtensorMap *m = second ? &a.w2 : &a.w;
-                    if (a.mn_major)
-                        for (int h = 0; h < halves; ++h) tma_3d<PAIRED>(dst + h * kBlock64, m, f0 + h * 64, i0, second ? g : z, bar);
-                    else tma_3d<PAIRED>(dst, m, i0, f0, second ? g : z, bar);
-                    const int own = slot0 + half * columns / 2;
-                    if (second) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.u, i0, (e & 1) * a.u_plane + own, bar);
-                    else if (!a.gather) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);
+                const uint32_t w_bytes = a.mn_major ? halves * kBlock64 : a.w_rows * 128u, own = slot0 + half * columns / 2;
+                for (int s = s0; s < s1; s += S::kSlices, pos.next(stages)) {
+                    mbar_wait(smem_addr(&pipe.empty[pos.stage]), pos.parity ^ 1, gave_up, a.status);
+                    const uint32_t bar = full0 + pos.stage * 8;
+                    if (half == 0) mbar_expect(bar, min(S::kSlices, s1 - s) * (PAIRED ? 2 : 1) * (w_bytes + S::kRows * 128u));
+#pragma unroll
+                    for (int d = 0; d < S::kSlices; ++d) {
+                        if (d > 0 && s + d >= s1) break;
+                        const uint32_t dst = ring + pos.stage * S::kStage + d * S::kSlice;
+                        const bool second = s + d >= main_steps;
+                        const int e = s + d - main_steps, i0 = (second ? e >> 1 : s + d) * kTcDepth;
+                        const CUtensorMap *m = second ? &a.w2 : &a.w;
+                        if (a.mn_major)
+                            for (int h = 0; h < halves; ++h) tma_3d<PAIRED>(dst + h * kBlock64, m, f0 + h * 64, i0, second ? g : z, bar);
+                        else tma_3d<PAIRED>(dst, m, i0, f0, second ? g : z, bar);
+                        if (second) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.u, i0, (e & 1) * a.u_plane + own, bar);
+                        else if (!a.gather) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);
+                    }
                 }
             }
         } else if (warp == 1) {
@@ -362,14 +374,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, a.mn_major, false, TILE_F, columns);
                 const uint64_t a_step = operand_step(a.mn_major), b_step = operand_step(false);
                 const uint64_t a0 = operand(ring, a.mn_major), b0 = operand(ring + kTcFeatures * 128, false);
-                for (int s = s0; s < s1; ++s, pos.next(stages)) {
-                    const int st = pos.stage;
-                    mbar_wait(smem_addr(&pipe.full[st]), pos.parity, gave_up, a.status);
+                for (int s = s0; s < s1; s += S::kSlices, pos.next(stages)) {
+                    mbar_wait(smem_addr(&pipe.full[pos.stage]), pos.parity, gave_up, a.status);
                     tc_fence_after();
-                    const uint64_t da = operand_at(a0, st * S::kStage), db = operand_at(b0, st * S::kStage);
-                    const int left = s >= main_steps ? a.rank - ((s - main_steps) >> 1) * kTcDepth : a.k - s * kTcDepth;
-                    tc_slice<PAIRED>(d, da, db, a_step, b_step, idesc, min(4, (left + 15) >> 4), s > s0);
-                    tc_commit<PAIRED>(smem_addr(&pipe.empty[st]));
+#pragma unroll
+                    for (int d2 = 0; d2 < S::kSlices; ++d2) {
+                        if (d2 > 0 && s + d2 >= s1) break;
+                        const uint32_t from = pos.stage * S::kStage + d2 * S::kSlice;
+                        const int left = s + d2 >= main_steps ? a.rank - ((s + d2 - main_steps) >> 1) * kTcDepth : a.k - (s + d2) * kTcDepth;
+                        tc_slice<PAIRED>(d, operand_at(a0, from), operand_at(b0, from), a_step, b_step, idesc, min(4, (left + 15) >> 4), s > s0 || d2 > 0);
+                    }
+                    tc_commit<PAIRED>(smem_addr(&pipe.empty[pos.stage]));
                 }
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
@@ -379,22 +394,24 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             const int row0 = __shfl_sync(0xffffffffu, row, 0);
             const bool run = __all_sync(0xffffffffu, lane >= RPW || row == row0 + lane);
             fetch_rows(tile + workers);  // under way while this tile is loaded
-            for (int s = s0; s < s1; ++s, pos.next(stages)) {
-                const int st = pos.stage;
+            for (int s = s0; s < s1; s += S::kSlices, pos.next(stages)) {
                 // every use of a stage is waited for, also where nothing is loaded: a parity tells neighbouring uses apart only
-                mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
+                mbar_wait(smem_addr(&pipe.empty[pos.stage]), pos.parity ^ 1, gave_up, a.status);
                 __syncwarp();
-                if (s >= main_steps) continue;
-                const uint32_t dst = ring + st * S::kStage + kTcFeatures * 128 + (warp - 8) * RPW * 128;
-                if (run) {
-                    if (elect_one()) tma_2d<PAIRED>(dst, &a.x_run, s * kTcDepth, row0, full0 + st * 8);
-                    continue;
-                }
 #pragma unroll
-                for (int q = 0; q < RPW / 4; ++q) {
-                    const int r0 = __shfl_sync(0xffffffffu, row, 4 * q), r1 = __shfl_sync(0xffffffffu, row, 4 * q + 1);
-                    const int r2 = __shfl_sync(0xffffffffu, row, 4 * q + 2), r3 = __shfl_sync(0xffffffffu, row, 4 * q + 3);
-                    if (elect_one()) tma_rows<PAIRED>(dst + q * 512, &a.x, s * kTcDepth, r0, r1, r2, r3, full0 + st * 8);
+                for (int d = 0; d < S::kSlices; ++d) {
+                    if (s + d >= min(s1, main_steps)) break;
+                    const uint32_t dst = ring + pos.stage * S::kStage + d * S::kSlice + kTcFeatures * 128 + (warp - 8) * RPW * 128, bar = full0 + pos.stage * 8;
+                    if (run) {
+                        if (elect_one()) tma_2d<PAIRED>(dst, &a.x_run, (s + d) * kTcDepth, row0, bar);
+                        continue;
+                    }
+#pragma unroll
+                    for (int q = 0; q < RPW / 4; ++q) {
+                        const int r0 = __shfl_sync(0xffffffffu, row, 4 * q), r1 = __shfl_sync(0xffffffffu, row, 4 * q + 1);
+                        const int r2 = __shfl_sync(0xffffffffu, row, 4 * q + 2), r3 = __shfl_sync(0xffffffffu, row, 4 * q + 3);
+                        if (elect_one()) tma_rows<PAIRED>(dst + q * 512, &a.x, (s + d) * kTcDepth, r0, r1, r2, r3, bar);
+                    }
                 }
             }
         } else if (warp >= 4 && warp < 8) {
@@ -538,6 +555,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             } else if (wide) results_sync();  // the next tile starts with the first buffer again
         }
     }
+    if (a.apart) wait_for_launch_before();
     if (*gave_up) __nanosleep(1000000);  // copies in flight land before the block's memory is given back
     tc_fence_before();
     __syncthreads();
@@ -617,6 +635,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
     let_next_launch_start();
+    if (warp == 0 && lane < 4) {
+        const CUtensorMap *maps[4] = {&a.p_rows, &a.p_tile, &a.q_rows, &a.q_tile};
+        tma_prefetch(maps[lane]);
+    }
     if (tid == 0) pipe_init(pipe, stages, PAIRED, split);
     if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), 2 * NT);
     wait_for_launch_before();
