@@ -246,6 +246,8 @@ int launch_tc(const Args &args, long long blocks, int cluster, size_t smem, bool
     return MPS_OK;
 }
 
+int steps_of(int summed) { return (summed + mps::kTcDepth - 1) / mps::kTcDepth; }
+
 // Blocks that share a tile's sum: as many as leave no SM without work, but two slices each at least.
 int split_of(long long tiles, int steps, int sms) {
     int split = 1;
@@ -282,34 +284,54 @@ Cut best_cut(int slots, int groups, int features, int steps, bool gather, int sm
     return best;
 }
 
-template <int NT>
-int launch_tc_rows(const TcRows &a, int sms, cudaStream_t st) {
-    // a group ends in a part of a tile, so there are at most this many
-    const long long most = a.n_slots / NT + (a.n_groups < a.n_slots ? a.n_groups : a.n_slots);
-    const int tile_f = mps::kTcFeatures * (mps::TcShape<NT>::kPaired ? 2 : 1);
-    const long long tiles = most * ((a.n + tile_f - 1) / tile_f);
-    const int cluster = mps::TcShape<NT>::kPaired ? 2 : a.split;
-    const long long workers = sms / cluster;
-    return launch_tc<mps::tc_rows_kernel<NT>>(a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcShape<NT>::bytes(a.n_groups), a.follows, st);
+// Blocks for two products side by side, in proportion to their work; each at least a cluster, none more than it has tiles for.
+void share_blocks(int sms, int cluster, const long long (&tiles)[2], const double (&work)[2], long long (&blocks)[2]) {
+    const long long clusters = sms / cluster;
+    long long first = tiles[1] ? (long long)(clusters * work[0] / (work[0] + work[1]) + 0.5) : clusters;
+    if (tiles[1]) first = first < 1 ? 1 : first > clusters - 1 ? clusters - 1 : first;
+    blocks[0] = (tiles[0] < first ? tiles[0] : first) * cluster;
+    blocks[1] = (tiles[1] < clusters - first ? tiles[1] : clusters - first) * cluster;
 }
 
-// The rest of a filled in: what every use has in common.
-int tc_rows(TcRows a, const Cut &cut, const void *x, long long x_rows, int sms, cudaStream_t st) {
-    if (int rc = status_pointer(&a.status)) return rc;
-    a.split = cut.split;
+template <int NT, bool TWO>
+int launch_tc_rows(const mps::TcRowsLaunch &in, int sms, cudaStream_t st) {
+    mps::TcRowsLaunch l = in;
+    const int tile_f = mps::kTcFeatures * (mps::TcShape<NT>::kPaired ? 2 : 1), cluster = mps::TcShape<NT>::kPaired ? 2 : l.p[0].split;
+    long long tiles[2] = {}, blocks[2];
+    double work[2] = {};
+    for (int i = 0; i < (TWO ? 2 : 1); ++i) {
+        const TcRows &a = l.p[i];
+        const long long most = a.n_slots / NT + (a.n_groups < a.n_slots ? a.n_groups : a.n_slots);  // a group ends in a part of a tile
+        tiles[i] = most * ((a.n + tile_f - 1) / tile_f);
+        work[i] = (double)tiles[i] * a.k;
+        if (tiles[i] >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "routed product: %lld tiles", tiles[i]);
+    }
+    share_blocks(sms, cluster, tiles, work, blocks);
+    l.second = (int)blocks[0];
+    return launch_tc<mps::tc_rows_kernel<NT, TWO>>(l, blocks[0] + blocks[1], cluster, mps::TcShape<NT>::bytes(l.p[0].n_groups), l.p[0].follows, st);
+}
+
+// One product, or two of the same groups side by side (at most 64 slots per tile): what every use has in common filled in.  x_rows: rows of each x.
+int tc_rows(const TcRows *products, int n, const Cut &cut, const void *const *x, long long x_rows, int sms, cudaStream_t st) {
+    mps::TcRowsLaunch l = {};
     const int loaded = cut.nt == 256 ? mps::TcShape<256>::kRows : cut.nt;  // slots a block loads
-    if (int rc = tensor_map(&a.x, a.bf16, x, 2, a.k, x_rows, 1, a.gather ? 1 : loaded)) return rc;
-    if (a.gather)
-        if (int rc = tensor_map(&a.x_run, a.bf16, x, 2, a.k, x_rows, 1, loaded / 8)) return rc;
-    if (a.rank)
-        if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded)) return rc;
-    if (cut.nt == 32) return launch_tc_rows<32>(a, sms, st);
-    if (cut.nt == 64) return launch_tc_rows<64>(a, sms, st);
-    if (cut.nt == 128) return launch_tc_rows<128>(a, sms, st);
-    return launch_tc_rows<256>(a, sms, st);
+    for (int i = 0; i < n; ++i) {
+        TcRows &a = l.p[i];
+        a = products[i];
+        if (int rc = status_pointer(&a.status)) return rc;
+        a.split = cut.split;
+        if (int rc = tensor_map(&a.x, a.bf16, x[i], 2, a.k, x_rows, 1, a.gather ? 1 : loaded)) return rc;
+        if (a.gather)
+            if (int rc = tensor_map(&a.x_run, a.bf16, x[i], 2, a.k, x_rows, 1, loaded / 8)) return rc;
+        if (a.rank)
+            if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded)) return rc;
+    }
+    if (n == 2) return cut.nt == 32 ? launch_tc_rows<32, true>(l, sms, st) : launch_tc_rows<64, true>(l, sms, st);
+    if (cut.nt == 32) return launch_tc_rows<32, false>(l, sms, st);
+    if (cut.nt == 64) return launch_tc_rows<64, false>(l, sms, st);
+    if (cut.nt == 128) return launch_tc_rows<128, false>(l, sms, st);
+    return launch_tc_rows<256, false>(l, sms, st);
 }
-
-int steps_of(int summed) { return (summed + mps::kTcDepth - 1) / mps::kTcDepth; }
 
 // The matrices of a: stored features x summed (MN-major: summed x features), `groups` of them.
 int tc_matrix(CUtensorMap *map, TcRows *a, const void *w, int summed, int features, long long groups) {
@@ -318,30 +340,45 @@ int tc_matrix(CUtensorMap *map, TcRows *a, const void *w, int summed, int featur
                        : tensor_map(map, a->bf16, w, 3, summed, features, groups, a->w_rows);
 }
 
-template <int NT>
-int launch_tc_outer(TcOuter a, int sms, cudaStream_t st) {
-    const int cols = a.pair ? NT / 2 : NT;
+template <int NT, bool TWO>
+int launch_tc_outer(const mps::TcOuterLaunch &in, int sms, cudaStream_t st) {
+    mps::TcOuterLaunch l = in;
     const int tile_f = mps::kTcFeatures * (mps::TcOuterShape<NT>::kPaired ? 2 : 1);
-    const long long tiles = (long long)a.n_groups * ((a.i + tile_f - 1) / tile_f) * ((a.j + cols - 1) / cols);
-    const int steps = (a.n_slots / a.n_groups + mps::kTcDepth - 1) / mps::kTcDepth;  // of the mean group
-    a.split = NT <= 128 ? split_of(tiles, steps, sms) : 1;
-    const int cluster = mps::TcOuterShape<NT>::kPaired ? 2 : a.split;
-    const long long workers = sms / cluster;
-    return launch_tc<mps::tc_outer_kernel<NT>>(a, (tiles < workers ? tiles : workers) * cluster, cluster, mps::TcOuterShape<NT>::kBytes, a.follows, st);
+    long long tiles[2] = {}, blocks[2];
+    for (int i = 0; i < (TWO ? 2 : 1); ++i) {
+        const TcOuter &a = l.p[i];
+        const int cols = a.pair ? NT / 2 : NT;
+        tiles[i] = (long long)a.n_groups * ((a.i + tile_f - 1) / tile_f) * ((a.j + cols - 1) / cols);
+        if (tiles[i] >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "routed matrix gradient: %lld tiles", tiles[i]);
+    }
+    const TcOuter &a = l.p[0];
+    const int steps = steps_of(a.n_slots / a.n_groups);  // of the mean group
+    const int split = NT <= 128 ? split_of(tiles[0] + tiles[1], steps, sms) : 1, cluster = mps::TcOuterShape<NT>::kPaired ? 2 : split;
+    l.p[0].split = l.p[1].split = split;
+    const double work[2] = {(double)tiles[0], (double)tiles[1]};
+    share_blocks(sms, cluster, tiles, work, blocks);
+    l.second = (int)blocks[0];
+    return launch_tc<mps::tc_outer_kernel<NT, TWO>>(l, blocks[0] + blocks[1], cluster, mps::TcOuterShape<NT>::kBytes, a.follows, st);
 }
 
-// P: n_p_rows rows of a.i, by a.slot_row or in slot order; Q: rows of a.j in slot order (pair: two planes of them).
-int tc_outer(TcOuter a, const void *p, const void *q, cudaStream_t st) {
-    if (int rc = status_pointer(&a.status)) return rc;
+// One gradient by the matrices, or two of the same groups side by side (of pairs of planes).  P: n_p_rows rows of a.i, by a.slot_row or in slot order;
+// Q: rows of a.j in slot order (pair: two planes of them).
+int tc_outer(const TcOuter *products, int n, const void *const *p, const void *const *q, cudaStream_t st) {
+    mps::TcOuterLaunch l = {};
     int sms;
     if (int rc = sm_count(&sms)) return rc;
-    const unsigned long long q_rows = (a.pair ? 2ull : 1ull) * a.n_slots;
-    if (int rc = tensor_map(&a.p_rows, a.bf16, p, 2, a.i, a.n_p_rows, 1, 1)) return rc;
-    if (int rc = tensor_map(&a.p_tile, a.bf16, p, 2, a.i, a.n_p_rows, 1, mps::kTcDepth)) return rc;
-    if (int rc = tensor_map(&a.q_rows, a.bf16, q, 2, a.j, q_rows, 1, 1)) return rc;
-    if (int rc = tensor_map(&a.q_tile, a.bf16, q, 2, a.j, q_rows, 1, mps::kTcDepth)) return rc;
-    if (a.pair || a.j <= 128) return launch_tc_outer<128>(a, sms, st);
-    return launch_tc_outer<256>(a, sms, st);
+    for (int i = 0; i < n; ++i) {
+        TcOuter &a = l.p[i];
+        a = products[i];
+        if (int rc = status_pointer(&a.status)) return rc;
+        const unsigned long long q_rows = (a.pair ? 2ull : 1ull) * a.n_slots;
+        if (int rc = tensor_map(&a.p_rows, a.bf16, p[i], 2, a.i, a.n_p_rows, 1, 1)) return rc;
+        if (int rc = tensor_map(&a.p_tile, a.bf16, p[i], 2, a.i, a.n_p_rows, 1, mps::kTcDepth)) return rc;
+        if (int rc = tensor_map(&a.q_rows, a.bf16, q[i], 2, a.j, q_rows, 1, 1)) return rc;
+        if (int rc = tensor_map(&a.q_tile, a.bf16, q[i], 2, a.j, q_rows, 1, mps::kTcDepth)) return rc;
+    }
+    if (n == 2) return launch_tc_outer<128, true>(l, sms, st);
+    return l.p[0].j <= 128 ? launch_tc_outer<128, false>(l, sms, st) : launch_tc_outer<256, false>(l, sms, st);
 }
 
 // Whether tensor maps can describe the operands: a 16-bit type, row pitches and addresses in multiples of 16 bytes.
@@ -431,12 +468,9 @@ struct AdapterSpace {
     }
 };
 
-// Where a launch stands among those of its call: the first; or one that uses nothing of the one before it and runs beside that.
-enum Place { kFirst, kBeside };
-
-// u (two planes, slot order) = scale * rows of x times the adapters' matrices (mn_major: stored summed x rank); u_f32 (or NULL)
-// the same by row
-int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m, bool mn_major, void *u, float *u_f32, Place place, int sms, cudaStream_t st) {
+// The narrow product of rows of x with the adapters' matrices (mn_major: stored summed x rank): u (two planes, slot order) =
+// scale * x A; u_f32 (or NULL) the same by row.
+int tc_adapter_narrow(const AdapterShape &s, int k, const void *m, bool mn_major, void *u, float *u_f32, TcRows *out) {
     TcRows a = {};
     a.bf16 = s.dtype == MPS_BF16;
     a.mn_major = mn_major;
@@ -449,12 +483,11 @@ int tc_adapter_narrow(const AdapterShape &s, int k, const void *x, const void *m
     a.gather = a.pair = true;
     a.group_scale = s.scale;
     a.out = u;
-    a.follows = place != kFirst;
-    a.apart = place == kBeside;
     a.out_plane = (long long)s.n_rows * s.rank;
     a.out_f32 = u_f32;
     if (int rc = tc_matrix(&a.w, &a, m, k, s.rank, s.n_adapters)) return rc;
-    return tc_rows(a, best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(k), true, sms, 256), x, s.n_rows, sms, st);
+    *out = a;
+    return MPS_OK;
 }
 
 // Whether the shared matrix is read once for rows of any adapter, the low-rank part added in fp32 by the warps that store the
@@ -492,7 +525,7 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cu
         a.delta_f = mn_major ? 1 : s.rank;
         a.delta_r = mn_major ? n : 1;
         a.ahead = ahead;
-        return tc_rows(a, cut, x, s.n_rows, sms, st);
+        return tc_rows(&a, 1, cut, &x, s.n_rows, sms, st);
     }
     a.group_ptr = ws.ptr;
     a.slot_row = ws.row;
@@ -503,10 +536,10 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cu
     a.u_plane = s.n_rows;
     a.gather = a.scatter = true;
     if (int rc = tc_matrix(&a.w2, &a, m, s.rank, n, s.n_adapters)) return rc;
-    return tc_rows(a, cut, x, s.n_rows, sms, st);
+    return tc_rows(&a, 1, cut, &x, s.n_rows, sms, st);
 }
 
-int tc_adapter_outer(const AdapterShape &s, int features, const void *p, const void *q, void *out, long long out_f, long long out_c, cudaStream_t st) {
+TcOuter tc_adapter_outer(const AdapterShape &s, int features, void *out, long long out_f, long long out_c) {
     TcOuter a = {};
     a.bf16 = s.dtype == MPS_BF16;
     a.group_ptr = s.group_ptr;
@@ -520,7 +553,7 @@ int tc_adapter_outer(const AdapterShape &s, int features, const void *p, const v
     a.out_group = (long long)features * s.rank;
     a.out_f = out_f;
     a.out_c = out_c;
-    return tc_outer(a, p, q, st);
+    return a;
 }
 
 template <typename T>
@@ -539,7 +572,10 @@ int adapters(const AdapterShape &s, const void *x, const void *w, const void *a,
             RD_CUDA(cudaGetLastError());
         } else {
             if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
-            if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, kBeside, sms, st)) return rc;
+            TcRows narrow;
+            if (int rc = tc_adapter_narrow(s, s.k, a, false, ws.u, nullptr, &narrow)) return rc;
+            narrow.follows = narrow.apart = true;  // beside the listing
+            if (int rc = tc_rows(&narrow, 1, best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k), true, sms, 256), &x, s.n_rows, sms, st)) return rc;
         }
         return tc_adapter_wide(s, ws, cut, rows, s.k, s.n, x, w, ws.u, (const float *)ws.u, b, false, y, rows, sms, st);
     }
@@ -559,11 +595,17 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
         const bool rows = by_rows(s, s.n, s.k, sms, &cut);
         if (!rows)
             if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
-        if (int rc = tc_adapter_narrow(s, s.k, x, a, false, ws.u, nullptr, rows ? kFirst : kBeside, sms, st)) return rc;             // scale * x A^T
-        if (int rc = tc_adapter_narrow(s, s.n, dy, b, true, ws.v, rows ? (float *)ws.v_f32 : nullptr, kBeside, sms, st)) return rc;  // scale * dy B
+        TcRows narrow[2];  // side by side, and beside the listing: scale * x A^T and scale * dy B
+        if (int rc = tc_adapter_narrow(s, s.k, a, false, ws.u, nullptr, &narrow[0])) return rc;
+        if (int rc = tc_adapter_narrow(s, s.n, b, true, ws.v, rows ? (float *)ws.v_f32 : nullptr, &narrow[1])) return rc;
+        narrow[0].follows = narrow[0].apart = narrow[1].apart = !rows;
+        const void *const in[2] = {x, dy};
+        const Cut half = best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k > s.n ? s.k : s.n), true, sms / 2, 64);
+        if (int rc = tc_rows(narrow, 2, half, in, s.n_rows, sms, st)) return rc;
         if (int rc = tc_adapter_wide(s, ws, cut, rows, s.n, s.k, dy, w, ws.v, (const float *)ws.v_f32, a, true, dx, false, sms, st)) return rc;
-        if (int rc = tc_adapter_outer(s, s.k, x, ws.v, da, 1, s.k, st)) return rc;
-        return tc_adapter_outer(s, s.n, dy, ws.u, db, s.rank, 1, st);
+        const TcOuter outer[2] = {tc_adapter_outer(s, s.k, da, 1, s.k), tc_adapter_outer(s, s.n, db, s.rank, 1)};
+        const void *const q[2] = {ws.v, ws.u};
+        return tc_outer(outer, 2, in, q, st);
     }
     float *u = (float *)ws.u, *v = (float *)ws.v;
     if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
@@ -637,7 +679,7 @@ extern "C" int mps_routed_product(int32_t n_slots, int32_t n_rows, int32_t n_gro
         int sms;
         if (int rc = sm_count(&sms)) return rc;
         if (int rc = tc_matrix(&a.w, &a, d_w, summed, features, n_groups)) return rc;
-        return tc_rows(a, best_cut(n_slots, n_groups, features, steps_of(summed), a.gather, sms, 256), d_x, n_rows, sms, (cudaStream_t)stream);
+        return tc_rows(&a, 1, best_cut(n_slots, n_groups, features, steps_of(summed), a.gather, sms, 256), &d_x, n_rows, sms, (cudaStream_t)stream);
     }
     RowsArgs a = {};
     a.group_ptr = d_group_ptr;
@@ -675,7 +717,7 @@ extern "C" int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_group
         a.out_group = (long long)k * n;
         a.out_f = 1;
         a.out_c = k;
-        return tc_outer(a, d_x, d_dy, (cudaStream_t)stream);
+        return tc_outer(&a, 1, &d_x, &d_dy, (cudaStream_t)stream);
     }
     OuterArgs a = {};
     a.group_ptr = d_group_ptr;

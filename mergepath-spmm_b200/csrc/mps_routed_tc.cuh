@@ -64,6 +64,13 @@ struct TcRows {
     int *status;
 };
 
+// What a launch works on: one product or (TWO) two side by side, the second one from block `second` on, a multiple of the
+// cluster.  A kernel of its own: reading every argument by index cost the single product 5 percent.
+struct TcRowsLaunch {
+    TcRows p[2];
+    int second;
+};
+
 struct TcPipe {
     uint64_t full[12], empty[12], tmem_full[2], tmem_empty[2];  // of a pair's full and tmem_empty the first block's count
     uint64_t partials, freed;                                   // split: every block's part is in its shared memory / has been read
@@ -214,8 +221,32 @@ struct TcCursor {
     }
 };
 
-template <int NT>
-__global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_constant__ TcRows a) {
+// A worker's tiles: tiles of slots by tiles of features, the features fastest; counted up, a division each is 200 cycles.
+struct TileWalk {
+    int tile, feature, tiles, features, step_tile, step_feature;
+    __device__ __forceinline__ TileWalk(int tiles_, int features_, unsigned worker, unsigned workers)
+        : tile((int)(worker / (unsigned)features_)),
+          feature((int)(worker % (unsigned)features_)),
+          tiles(tiles_),
+          features(features_),
+          step_tile((int)(workers / (unsigned)features_)),
+          step_feature((int)(workers % (unsigned)features_)) {}
+    __device__ __forceinline__ bool more() const { return tile < tiles; }
+    __device__ __forceinline__ void next() {
+        tile += step_tile;
+        feature += step_feature;
+        if (feature >= features) {
+            feature -= features;
+            ++tile;
+        }
+    }
+};
+
+template <int NT, bool TWO>
+__global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_constant__ TcRowsLaunch launch) {
+    const bool is_second = TWO && (int)blockIdx.x >= launch.second;
+    const TcRows &a = launch.p[is_second];
+    const unsigned block = blockIdx.x - (is_second ? launch.second : 0), blocks = is_second ? gridDim.x - launch.second : TWO ? launch.second : gridDim.x;
     using S = TcShape<NT>;
     extern __shared__ uint8_t s_raw[];
     __shared__ TcPipe pipe;
@@ -234,7 +265,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     let_next_launch_start();
     if (warp == 0 && lane < 5) {
         const CUtensorMap *maps[5] = {&a.w, &a.x, &a.x_run, &a.w2, &a.u};
-        if (lane < (a.rank ? 5 : 3)) tma_prefetch(maps[lane]);
+        if (lane < 2 || (lane == 2 ? a.gather : a.rank > 0)) tma_prefetch(maps[lane]);
     }
     if (!a.ahead && !a.apart) wait_for_launch_before();
     // ---- tiles of the groups
@@ -299,17 +330,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     const uint32_t tmem = pipe.tmem;
     volatile int *gave_up = &pipe.gave_up;
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
-    const int feature_tiles = (a.n + TILE_F - 1) / TILE_F, main_steps = (a.k + kTcDepth - 1) / kTcDepth;
-    const int rank_steps = 2 * ((a.rank + kTcDepth - 1) / kTcDepth);
-    const long long n_tiles = (long long)(whole[a.n_groups] + rest[a.n_groups]) * feature_tiles;
-    const long long worker = blockIdx.x / group_blocks, workers = gridDim.x / group_blocks;
+    const int main_steps = (a.k + kTcDepth - 1) / kTcDepth, rank_steps = 2 * ((a.rank + kTcDepth - 1) / kTcDepth);
+    const int shift = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
+    TileWalk walk(whole[a.n_groups] + rest[a.n_groups], (a.n + TILE_F - 1) / TILE_F, block / group_blocks, blocks / group_blocks);
     TcCursor cur = {whole, rest, lo, hi, a.n_groups, 0, 0, 0, false};
 
     // steps of this block for a tile of group g
     auto range = [&](int g, int &s0, int &s1) {
         const int total = main_steps + (g < a.rank_groups ? rank_steps : 0);
-        s0 = (int)((long long)total * part / split);
-        s1 = (int)((long long)total * (part + 1) / split);
+        s0 = total * part >> shift;
+        s1 = total * (part + 1) >> shift;
     };
 
     // columns of a tile's products: only as many as there are slots, so that the last tile of a group costs what it holds
@@ -319,10 +349,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     constexpr int RPW = S::kRows / 8;
     int row = 0, next_row = 0;
     TcCursor ahead = cur;
-    auto fetch_rows = [&](long long tile) {
+    auto fetch_rows = [&](const TileWalk &w) {
         next_row = a.n_x_rows;  // out of range: zeros
-        if (tile >= n_tiles) return;
-        ahead.seek((int)(tile / feature_tiles), NT);
+        if (!w.more()) return;
+        ahead.seek(w.tile, NT);
         const int at = (warp - 8) * RPW + lane, slot = ahead.slot0 + half * columns_of(ahead) / 2 + at;
         if (lane < RPW && slot < ahead.slot1 && (!PAIRED || at < columns_of(ahead) / 2)) {
             const int r = a.slot_row[slot];
@@ -331,14 +361,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
         }
     };
     const bool loads_rows = warp >= 8 && a.gather;
-    if (loads_rows) fetch_rows(worker);
+    if (loads_rows) fetch_rows(walk);
     const uint32_t full0 = PAIRED ? in_block(smem_addr(&pipe.full[0]), 0) : smem_addr(&pipe.full[0]);  // where loads are reported
     RingAt pos;  // this warp's place in the ring
 
     int turn = 0;  // tiles done so far
-    for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
-        const int tt = (int)(tile / feature_tiles), f0 = (int)(tile - (long long)tt * feature_tiles) * TILE_F + half * kTcFeatures;
-        cur.seek(tt, NT);
+    for (; walk.more(); walk.next(), ++turn) {
+        const int f0 = walk.feature * TILE_F + half * kTcFeatures;
+        cur.seek(walk.tile, NT);
         const int g = cur.group, slot0 = cur.slot0, slot1 = cur.slot1, columns = columns_of(cur);
         int s0, s1;
         range(g, s0, s1);
@@ -393,7 +423,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             // neighbouring rows in order (a request's, listed by adapter) come as one box
             const int row0 = __shfl_sync(0xffffffffu, row, 0);
             const bool run = __all_sync(0xffffffffu, lane >= RPW || row == row0 + lane);
-            fetch_rows(tile + workers);  // under way while this tile is loaded
+            TileWalk then = walk;
+            then.next();
+            fetch_rows(then);  // under way while this tile is loaded
             for (int s = s0; s < s1; s += S::kSlices, pos.next(stages)) {
                 // every use of a stage is waited for, also where nothing is loaded: a parity tells neighbouring uses apart only
                 mbar_wait(smem_addr(&pipe.empty[pos.stage]), pos.parity ^ 1, gave_up, a.status);
@@ -506,8 +538,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             const bool rows_of_16 = !a.pair && a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0, wide = rows_of_16 && !reduce;
 #pragma unroll 1
             for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 32) {
-                float v[32];
-                tmem_load(tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + c0, v);
+                float v[32] = {};
+                if (s0 < s1) tmem_load(tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + c0, v);  // a block may have no part in a short sum
                 if (reduce) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 8)
@@ -611,6 +643,11 @@ struct TcOuter {
     int *status;
 };
 
+struct TcOuterLaunch {
+    TcOuter p[2];
+    int second;
+};
+
 template <int NT>
 struct TcOuterShape {
     static constexpr bool kPaired = NT == 256;
@@ -621,8 +658,11 @@ struct TcOuterShape {
     static constexpr size_t kBytes = 1024 + kTcRing + kOutTotal;
 };
 
-template <int NT>
-__global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_constant__ TcOuter a) {
+template <int NT, bool TWO>
+__global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_constant__ TcOuterLaunch launch) {
+    const bool is_second = TWO && (int)blockIdx.x >= launch.second;
+    const TcOuter &a = launch.p[is_second];
+    const int block = blockIdx.x - (is_second ? launch.second : 0), blocks = is_second ? gridDim.x - launch.second : TWO ? launch.second : gridDim.x;
     using S = TcOuterShape<NT>;
     extern __shared__ uint8_t s_raw[];
     __shared__ TcPipe pipe;
@@ -650,18 +690,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     volatile int *gave_up = &pipe.gave_up;
     const int cols = a.pair ? NT / 2 : NT;  // result columns per tile
     const int i_tiles = (a.i + TILE_F - 1) / TILE_F, j_tiles = (a.j + cols - 1) / cols;
-    const long long n_tiles = (long long)a.n_groups * i_tiles * j_tiles;
-    const long long worker = blockIdx.x / group_blocks, workers = gridDim.x / group_blocks;
+    const int per_group = i_tiles * j_tiles, n_tiles = a.n_groups * per_group;  // below 2^31 (host)
+    const int worker = block / group_blocks, workers = blocks / group_blocks, shift = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
     const bool gather = a.slot_row != nullptr;
     const uint32_t full0 = PAIRED ? in_block(smem_addr(&pipe.full[0]), 0) : smem_addr(&pipe.full[0]);
     RingAt pos;
     int turn = 0;
-    for (long long tile = worker; tile < n_tiles; tile += workers, ++turn) {
-        const int g = (int)(tile / ((long long)i_tiles * j_tiles)), rest = (int)(tile - (long long)g * i_tiles * j_tiles);
+    for (int tile = worker; tile < n_tiles; tile += workers, ++turn) {
+        const int g = tile / per_group, rest = tile - g * per_group;
         const int f0 = rest / j_tiles * TILE_F + half * kTcFeatures, c0 = rest % j_tiles * cols;
         const int2 slots = group_range(a.group_ptr, g, a.n_slots, a.status);
         const int total = (slots.y - slots.x + kTcDepth - 1) / kTcDepth;
-        const int s0 = (int)((long long)total * part / split), s1 = (int)((long long)total * (part + 1) / split);
+        const int s0 = (int)((long long)total * part >> shift), s1 = (int)((long long)total * (part + 1) >> shift);
         const int buf = turn & 1;
         const int p_blocks = PAIRED || a.i - f0 > 64 ? 2 : 1, q_blocks = a.pair || a.j - c0 > NT / 2 ? 2 : 1;
         const int q0 = c0 + half * q_blocks * 64;  // the columns this block loads

@@ -24,12 +24,6 @@ __device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-
 // one lane of a converged warp, in the form the compiler knows to be a single thread (products and their descriptors then stay
 // in uniform registers)
 __device__ __forceinline__ bool elect_one() {
@@ -51,18 +45,19 @@ struct RingAt {
     }
 };
 
-constexpr unsigned long long kWaitLimitNs = 2000000000ull;  // no wait of a working kernel comes near two seconds
+constexpr long long kWaitLimit = 1ll << 34;  // SM cycles, nine seconds: no wait of a working kernel comes near
 
-// Waits for the phase; after kWaitLimitNs (or once another thread of the block gave up) it records that and returns.  The
-// block then runs through its remaining steps without waiting, and its result counts as undefined.
+// Waits for the phase; after kWaitLimit (or once another thread of the block gave up) it records that and returns.  The block
+// then runs through its remaining steps without waiting, and its result counts as undefined.  Counted in the SM's own cycles,
+// which only rise; the global timer is read in two halves and may be set.
 __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatile int *gave_up, int *status) {
     if (mbar_try(bar, parity)) return;
-    const unsigned long long start = now_ns();
+    const long long start = clock64();
     for (;;) {
         for (int i = 0; i < 64; ++i)
             if (mbar_try(bar, parity)) return;
         if (*gave_up) return;
-        if (now_ns() - start > kWaitLimitNs) {
+        if (clock64() - start > kWaitLimit) {
             *gave_up = 1;
             atomicOr(status, kStatusTimeout);
             return;
