@@ -491,13 +491,13 @@ int tc_adapter_narrow(const AdapterShape &s, int k, const void *m, bool mn_major
 }
 
 // Whether the shared matrix is read once for rows of any adapter, the low-rank part added in fp32 by the warps that store the
-// results (about a quarter of an SM's 128 multiply-adds a cycle), or per adapter, the low-rank part summed on the tensor cores.
-// Measured at 4096 x 4096 in bf16: 64 rows of 24 adapters of rank 16 take ADAPT_A us by rows and ADAPT_B by adapter, 4096 rows
-// of 8 adapters of rank 64 ADAPT_C by adapter and ADAPT_D by rows.
-bool by_rows(const AdapterShape &s, int k, int n, int sms, Cut *cut) {
+// results (six multiply-adds a cycle and SM, 1.5 from matrices stored by rank, as measured), or per adapter, the low-rank part
+// summed on the tensor cores.  Measured at 4096 x 4096 in bf16, rank 16: 64 rows of 24 adapters 20 us by rows and 81 us by
+// adapter, 256 rows of 64 adapters 41 and 207, 1024 rows of 8 adapters 125 and 76; 4096 rows of 8 adapters of rank 64 1046 and 129.
+bool by_rows(const AdapterShape &s, int k, int n, bool by_rank, int sms, Cut *cut) {
     const Cut grouped = best_cut(s.n_rows, s.n_adapters + 1, n, steps_of(k) + 2 * steps_of(s.rank), true, sms, 256);
     const Cut rows = best_cut(s.n_rows, 1, n, steps_of(k), false, sms, 64);
-    const double low_rank = (double)s.n_rows * n * s.rank / (32.0 * sms);
+    const double low_rank = (double)s.n_rows * n * s.rank / ((by_rank ? 1.5 : 6.0) * sms);
     *cut = rows.cycles + low_rank < grouped.cycles ? rows : grouped;
     return rows.cycles + low_rank < grouped.cycles;
 }
@@ -564,7 +564,7 @@ int adapters(const AdapterShape &s, const void *x, const void *w, const void *a,
         Cut cut;
         if (int rc = sm_count(&sms)) return rc;
         if (int rc = status_pointer(&status)) return rc;
-        const bool rows = by_rows(s, s.k, s.n, sms, &cut);
+        const bool rows = by_rows(s, s.k, s.n, false, sms, &cut);
         if (rows) {
             const dim3 grid((unsigned)s.n_rows, (unsigned)((s.rank + 7) / 8));
             mps::adapter_dots_kernel<<<grid, 256, 0, st>>>(s.k, s.rank, s.n_adapters, s.dtype == MPS_BF16, s.ids, s.scale, (const uint16_t *)x,
@@ -592,7 +592,7 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
         int sms;
         Cut cut;
         if (int rc = sm_count(&sms)) return rc;
-        const bool rows = by_rows(s, s.n, s.k, sms, &cut);
+        const bool rows = by_rows(s, s.n, s.k, true, sms, &cut);
         if (!rows)
             if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
         TcRows narrow[2];  // side by side, and beside the listing: scale * x A^T and scale * dy B

@@ -798,7 +798,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             const Meeting meeting = {partial, split, part, cols / split};
             const int feature = quad * 32 + lane;
             const bool none = s0 == s1;
-            const bool wide = a.out_f == 1 && a.i % 8 == 0 && ((uintptr_t)a.out & 15) == 0;
+            const bool on_16 = ((uintptr_t)a.out & 15) == 0;
+            const bool wide = a.out_f == 1 && a.i % 8 == 0 && on_16, own_rows = a.out_c == 1 && a.j % 8 == 0 && on_16;  // rows of features / of columns
 #pragma unroll 1
             for (int c = 0; c < cols && c0 + c < a.j; c += 32) {
                 float v[32] = {};
@@ -824,6 +825,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                         const int cc = (mine >> 4) + 8 * x, fc = (mine & 15) * 8;
                         const uint4 q = load_shared_128(at + cc * kOutPitch + fc * 2);
                         if (c0 + c + cc < a.j && f0 + fc < a.i) *reinterpret_cast<uint4 *>(out + (c0 + c + cc) * a.out_c + f0 + fc) = q;
+                    }
+                } else if (own_rows) {
+#pragma unroll
+                    for (int x = 0; x < 32; x += 8) {
+                        const float w[8] = {v[x], v[x + 1], v[x + 2], v[x + 3], v[x + 4], v[x + 5], v[x + 6], v[x + 7]};
+                        if (f < a.i && c0 + c + x < a.j) *reinterpret_cast<uint4 *>(out + f * a.out_f + c0 + c + x) = pack_16(w, a.bf16);
                     }
                 } else {
 #pragma unroll

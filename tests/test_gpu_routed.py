@@ -75,6 +75,14 @@ def test_route(mps, cuda, dtype, rows, experts, top, kw):
     check_route(mps, logits, top, bias=bias, **kw)
 
 
+def test_route_without_rows(mps, cuda):
+    ids, weights, groups = mps.route(torch.empty(0, 40, device="cuda"), 3)
+    assert ids.shape == weights.shape == groups.slot.shape == (0, 3) and groups.row.shape == (0,) and groups.ptr.tolist() == [0] * 41
+    assert mps.route_backward(torch.empty(0, 40, device="cuda"), ids, weights).shape == (0, 40)
+    ids, weights, groups = mps.route(torch.randn(5, 40, device="cuda"), 3, group=False)
+    assert groups is None and ids.shape == (5, 3)
+
+
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("biased", [False, True])
 @pytest.mark.parametrize("n_groups", [1, 4])
@@ -225,6 +233,7 @@ PRODUCTS = [
     (64, 128, [1], 1, 0), (8, 8, [3, 0, 2], 1, 0), (64, 64, [0, 0, 5], 1, 3), (72, 136, [17, 1, 0, 33], 1, 2), (200, 328, [130, 64, 65, 1], 2, 6),
     (512, 256, [1, 1, 1, 1, 0, 1, 1, 2], 2, 0), (128, 1000, [300, 7], 1, 0), (1000, 72, [257, 255, 0, 16], 4, 8), (24, 2056, [40, 9], 1, 0),
     (1544, 384, [2, 9, 31, 0, 8, 8], 1, 0), (256, 512, [600, 128, 256, 40], 2, 8),
+    (64, 100, [300, 7, 40], 1, 0), (128, 3, [5, 1], 2, 0), (320, 136, [0] * 500 + [3] + [0] * 522 + [1], 1, 0), (64, 512, [2000, 700], 1, 4),
     (7, 5, [9, 0, 70], 1, 1), (33, 130, [65, 3], 2, 0), (1, 1, [2, 2], 1, 0), (4100, 12, [5, 70], 1, 0),
 ]
 
@@ -289,6 +298,36 @@ def test_product_without_slots(mps, cuda, dtype, k):
     out = torch.full((4, 16), SENTINEL, dtype=dtype, device="cuda")
     assert (mps.routed_product(x, w, g, out=out) == SENTINEL).all()
     assert not mps.routed_wgrad(x, torch.ones(4, 16, dtype=dtype, device="cuda"), g).any()
+    mps.routed_check()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_product_at_addresses_off_16_bytes(mps, cuda, dtype):
+    """Operands at addresses that no tensor map takes, and results at addresses that no 16-byte store takes."""
+    def shifted(t):
+        u = torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape)
+        return u.copy_(t)
+
+    gen, rng = gen_of(9), np.random.default_rng(9)
+    groups, (ptr, row, slot) = lists(counts_ids([40, 0, 300], 1, rng), 3)
+    x, w, dy = rand(gen, dtype, 340, 128), rand(gen, dtype, 3, 64, 128, scale=0.1), rand(gen, dtype, 340, 64)
+    y, dw = mps.routed_product(x, w, groups), mps.routed_wgrad(x, dy, groups)
+    out = shifted(torch.zeros_like(y))
+    assert torch.equal(mps.routed_product(x, w, groups, out=out), y)
+    assert torch.equal(mps.routed_wgrad(x, dy, groups, out=shifted(torch.zeros_like(dw))), dw)
+    want, mag = o.product(f64(x), f64(w), ptr, row, np.zeros(y.shape))
+    for a, b in ((shifted(x), w), (x, shifted(w))):
+        close(f64(mps.routed_product(a, b, groups)), want, dtype, 128, mag)
+    want, mag = o.wgrad(f64(x), f64(dy), ptr, row)
+    for a, b in ((shifted(x), dy), (x, shifted(dy))):
+        close(f64(mps.routed_wgrad(a, b, groups)), want, dtype, 300, mag)
+    a, b, scale = rand(gen, dtype, 3, 8, 128), rand(gen, dtype, 3, 64, 8), torch.ones(3, device="cuda")
+    ids = torch.from_numpy(rng.integers(-1, 3, 340).astype(np.int32)).cuda()
+    ag = mps.group_rows(ids, 3)
+    wide = mps.adapters(x, w[0], a, b, ids, ag, scale)
+    assert torch.equal(mps.adapters(x, w[0], a, b, ids, ag, scale, out=shifted(torch.zeros_like(wide))), wide)
+    ref = o.adapters(f64(x), f64(w[0]), f64(a), f64(b), ids.cpu().numpy(), np.ones(3))
+    close(f64(mps.adapters(x, w[0], a, shifted(b), ids, ag, scale)), ref[0], dtype, 128 + 8 + 2, ref[1], o.PAIR[dtype] * ref[2] + o.FLOOR[dtype] * ref[3])
     mps.routed_check()
 
 
@@ -360,7 +399,8 @@ ADAPTERS = [
     # rows, adapters, rank, k, n, order
     (1, 1, 8, 64, 64, "one"), (1, 5, 16, 256, 512, "none"), (64, 24, 16, 512, 256, "mixed"), (5, 70, 8, 128, 1000, "mixed"),
     (300, 3, 64, 200, 136, "runs"), (700, 6, 40, 512, 264, "runs"), (130, 2, 128, 72, 72, "mixed"), (257, 200, 24, 136, 640, "mixed"),
-    (90, 4, 8, 1000, 8, "runs"), (40, 3, 200, 64, 128, "mixed"), (33, 4, 3, 20, 30, "mixed"), (20, 2, 1, 7, 9, "mixed"), (50, 3, 12, 64, 64, "runs"),
+    (90, 4, 8, 1000, 8, "runs"), (40, 3, 200, 64, 128, "mixed"), (9, 3, 8, 64, 50, "mixed"), (1500, 3, 8, 64, 100, "mixed"), (40, 1024, 8, 64, 64, "mixed"),
+    (2600, 4, 16, 256, 512, "runs"), (2600, 4, 72, 128, 264, "mixed"), (3000, 1, 8, 64, 1024, "mixed"), (33, 4, 3, 20, 30, "mixed"), (20, 2, 1, 7, 9, "mixed"), (50, 3, 12, 64, 64, "runs"),
 ]
 
 
@@ -395,13 +435,14 @@ def test_adapters_and_gradients(mps, cuda, dtype, rows, n_adapters, rank, k, n, 
     mps.routed_check()
 
 
-def test_adapters_rows_do_not_meet(mps, cuda):
+@pytest.mark.parametrize("repeat", [30, 700])  # rows of any adapter in one tile; tiles of one adapter each
+def test_adapters_rows_do_not_meet(mps, cuda, repeat):
     """NaN in a row, in an adapter nobody asks for, or in one other rows ask for, stays with the rows concerned."""
     gen = gen_of(8)
-    ids = np.array([0, 1, -1, 2, 1, 0] * 30, dtype=np.int32)
+    ids = np.array([0, 1, -1, 2, 1, 0] * repeat, dtype=np.int32)
     d_ids = torch.from_numpy(ids).cuda()
     groups = mps.group_rows(d_ids, 4)
-    x, w = rand(gen, BF16, 180, 128), rand(gen, BF16, 256, 128)
+    x, w = rand(gen, BF16, len(ids), 128), rand(gen, BF16, 256, 128)
     a, b = rand(gen, BF16, 4, 16, 128), rand(gen, BF16, 4, 256, 16)
     a[3], b[3] = math.nan, math.inf
     y = mps.adapters(x, w, a, b, d_ids, groups)
@@ -414,7 +455,14 @@ def test_adapters_rows_do_not_meet(mps, cuda):
     x2 = x.clone()
     x2[3] = math.inf
     y3 = mps.adapters(x2, w, a, b, d_ids, groups)
-    assert torch.equal(y[torch.arange(180) != 3], y3[torch.arange(180) != 3]) and not torch.isfinite(y3[3]).any()
+    keep = torch.arange(len(ids)) != 3
+    assert torch.equal(y[keep], y3[keep]) and not torch.isfinite(y3[3]).any()
+    dy = rand(gen, BF16, len(ids), 256)
+    dx, da, db = mps.adapters_backward(dy, x, w, a, b, d_ids, groups)
+    assert torch.isfinite(dx).all() and torch.isfinite(da).all() and torch.isfinite(db).all()
+    dx2, da2, db2 = mps.adapters_backward(dy, x2, w, a, b, d_ids, groups)  # row 3 asks for adapter 2
+    assert torch.equal(dx, dx2) and torch.equal(da[[0, 1, 3]], da2[[0, 1, 3]]) and torch.equal(db[[0, 1, 3]], db2[[0, 1, 3]])
+    assert not torch.isfinite(da2[2]).all()
 
 
 def test_adapters_without_rows(mps, cuda):
