@@ -344,11 +344,14 @@ __global__ void __launch_bounds__(32 * kRouteWarps, VPL <= 8 ? 8 : 1) route_kern
 // Gradient by the logits, all of the row written.  With r = the chosen scores' shares and g = the weights' gradient:
 //   renormalised: dl_j = scale r_j (g_j - sum_i g_i r_i) (times 1 - s_j for a sigmoid), nothing for the others;
 //   softmax:      dl_e = scale p_e (g_e - sum_i g_i p_i);      sigmoid: dl_j = scale g_j s_j (1 - s_j).
-// An expert named twice gets both contributions, in the order of the choices.
+// One warp per row; the row is put together in shared memory, the chosen one after the other, so that an expert named twice gets
+// both contributions in the order of the choices.
 template <typename T, bool SIGMOID>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(RouteArgs a, const T *__restrict__ logits, const int *__restrict__ ids,
+__global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(const RouteArgs a, const T *__restrict__ logits, const int *__restrict__ ids,
                                                                          const float *__restrict__ d_weights, T *__restrict__ d_logits) {
+    extern __shared__ float s_rows[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float *cells = s_rows + (size_t)warp * a.n_experts;
     const bool dense = !SIGMOID && !a.renormalise;
     for (long long row = (long long)blockIdx.x * kRouteWarps + warp; row < a.n_rows; row += (long long)gridDim.x * kRouteWarps) {
         const T *line = logits + row * a.n_experts;
@@ -363,19 +366,24 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(RouteA
             if (id >= 0) g = d_weights[row * a.top_k + lane];
         }
         const float l = id >= 0 ? to_f32(line[id]) : -INFINITY;
-        float peak = 0.0f, total = 1.0f, own, common = 0.0f;
+        float own;
         if (dense) {
             float p = -INFINITY, t = 0.0f;
-            for (int e = lane; e < a.n_experts; e += 32) p = fmaxf(p, to_f32(line[e]));
-            peak = warp_max(p);
             for (int e = lane; e < a.n_experts; e += 32) {
                 const float v = to_f32(line[e]);
-                if (v != -INFINITY) t += expf(v - peak);
+                cells[e] = v;
+                p = v > p || v != v ? v : p;
             }
-            total = warp_sum(t);
-            const float share = l != -INFINITY ? expf(l - peak) / total : 0.0f;
-            own = a.scale * g * share;
-            common = warp_sum(own);
+            const float peak = warp_max(p);
+            for (int e = lane; e < a.n_experts; e += 32) {
+                const float v = cells[e], x = v != -INFINITY ? expf(v - peak) : 0.0f;
+                cells[e] = x;
+                t += x;
+            }
+            const float total = warp_sum(t);
+            own = l != -INFINITY ? a.scale * g * (expf(l - peak) / total) : 0.0f;
+            const float common = warp_sum(own);
+            for (int e = lane; e < a.n_experts; e += 32) cells[e] = total > 0.0f || total != total ? -(cells[e] / total) * common : 0.0f;
         } else {
             const float s = SIGMOID ? (id >= 0 ? sigmoid(l) : 0.0f) : 0.0f, slope = SIGMOID ? sigmoid(-l) : 1.0f;
             if (a.renormalise) {
@@ -387,21 +395,15 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_backward_kernel(RouteA
                 } else share = s / warp_sum(s);
                 own = a.scale * share * (g - warp_sum(g * share)) * (id >= 0 ? slope : 0.0f);
             } else own = id >= 0 ? a.scale * g * s * slope : 0.0f;
+            for (int e = lane; e < a.n_experts; e += 32) cells[e] = 0.0f;
         }
-        for (int e0 = 0; e0 < a.n_experts; e0 += 32) {
-            const int e = e0 + lane;
-            float d = 0.0f;
-            if (dense && e < a.n_experts) {
-                const float v = to_f32(line[e]);
-                d = v != -INFINITY ? -(expf(v - peak) / total) * common : 0.0f;
-            }
-            for (int j = 0; j < a.top_k; ++j) {
-                const int at = __shfl_sync(kAll, id, j);
-                const float c = __shfl_sync(kAll, own, j);
-                if (at == e) d += c;
-            }
-            if (e < a.n_experts) d_logits[row * a.n_experts + e] = mps::from_f32<T>(d);
+        __syncwarp();
+        for (int j = 0; j < a.top_k; ++j) {
+            if (lane == j && id >= 0) cells[id] += own;
+            __syncwarp();
         }
+        for (int e = lane; e < a.n_experts; e += 32) d_logits[row * a.n_experts + e] = mps::from_f32<T>(cells[e]);
+        __syncwarp();
     }
 }
 
@@ -700,8 +702,9 @@ static int launch_route_backward(const RouteArgs &a, bool sigmoid_score, const v
                                  cudaStream_t st) {
     const long long want = ((long long)a.n_rows + kRouteWarps - 1) / kRouteWarps;
     const unsigned blocks = (unsigned)(want < 148 * 16 ? want : 148 * 16);
-    if (sigmoid_score) route_backward_kernel<T, true><<<blocks, 32 * kRouteWarps, 0, st>>>(a, (const T *)logits, ids, d_weights, (T *)d_logits);
-    else route_backward_kernel<T, false><<<blocks, 32 * kRouteWarps, 0, st>>>(a, (const T *)logits, ids, d_weights, (T *)d_logits);
+    const size_t smem = (size_t)kRouteWarps * a.n_experts * sizeof(float);
+    if (sigmoid_score) route_backward_kernel<T, true><<<blocks, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, ids, d_weights, (T *)d_logits);
+    else route_backward_kernel<T, false><<<blocks, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, ids, d_weights, (T *)d_logits);
     RT_CUDA(cudaGetLastError());
     return MPS_OK;
 }
