@@ -341,6 +341,198 @@ __global__ void __launch_bounds__(32 * kRouteWarps, VPL <= 8 ? 8 : 1) route_kern
     }
 }
 
+// Many rows: eight lanes per row, four rows per warp, so that a pick's reductions serve four rows.  A lane holds a contiguous
+// eighth of the experts (a part of one group: 1, 2, 4 or 8 groups) as integers that order like the keys, the low five bits
+// replaced by the place in the lane: the lane's best is one integer maximum, equal keys go to the lower place by themselves, and
+// taking an expert out is a comparison with the value that won.  The five bits cost 2^-18 of a key, which the test for close
+// keys takes in; for 16-bit logits without a bias they are zeros.  16384 rows of 256 experts, top 8 of 4 of 8 groups:
+// OCTET_US us, WARP_US us with a warp per row (which keeps fewer rows, other group counts and more experts).
+constexpr int kOctetRows = 2048;  // from here on there are rows enough for 148 SMs
+
+template <typename T, int VPL, bool SIGMOID>
+__global__ void __launch_bounds__(32 * kRouteWarps) route_octet_kernel(const RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
+                                                                      int *__restrict__ ids, float *__restrict__ weights, bool vectors) {
+    extern __shared__ double s_cells[];
+    __shared__ int s_pick[kRouteWarps][4][kMaxTop];
+    mps::let_next_launch_start();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & 7, quad = lane >> 3;
+    double *cells = s_cells + (size_t)warp * (a.n_experts + (a.n_experts >> 5) + 1);
+    const int chunk = a.n_experts >> 3, first = sub * chunk, per_group = 8 / a.n_groups;  // lanes per group
+    const bool has_bias = bias != nullptr, grouped = a.n_groups > 1, need_score = has_bias || (grouped && a.group_top == 2);
+    const bool whole = sizeof(T) == 2 && !has_bias;  // the five bits lose nothing
+    auto row_max = [](float v) {
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) v = fmaxf(v, __shfl_xor_sync(kAll, v, d));
+        return v;
+    };
+    auto row_sum = [](float v) {
+#pragma unroll
+        for (int d = 1; d < 8; d <<= 1) v += __shfl_xor_sync(kAll, v, d);
+        return v;
+    };
+    auto key_of = [](unsigned packed) {  // the key, up to the five bits
+        const unsigned o = packed & ~31u;
+        return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
+    };
+    const long long rows_of_grid = (long long)gridDim.x * kRouteWarps * 4;
+    for (long long row0 = ((long long)blockIdx.x * kRouteWarps + warp) * 4; row0 < a.n_rows; row0 += rows_of_grid) {
+        const long long row = row0 + quad;
+        const bool live = row < a.n_rows;
+        const T *line = logits + (live ? row : 0) * a.n_experts;
+        float l[VPL];
+        if (vectors) {  // a lane's experts in 16-byte pieces
+            constexpr int N = mps::Pack<T>::N < VPL ? mps::Pack<T>::N : VPL;
+#pragma unroll
+            for (int i = 0; i < VPL; i += N) {
+                mps::Pack<T> p = {};
+                if (i < chunk) p = *reinterpret_cast<const mps::Pack<T> *>(line + first + i);
+#pragma unroll
+                for (int j = 0; j < N; ++j) l[i + j] = live && i < chunk ? to_f32(p.v[j]) : -INFINITY;
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) l[i] = live && i < chunk ? to_f32(line[first + i]) : -INFINITY;
+        }
+        bool nan = false;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            nan = nan || !(SIGMOID ? l[i] <= INFINITY : l[i] < INFINITY);
+            if (l[i] != l[i]) l[i] = -INFINITY;
+        }
+        nan = (__ballot_sync(kAll, nan) >> (quad * 8) & 0xff) != 0;
+        float peak = -INFINITY, total = 0.0f, total_w = 0.0f;
+        if (!SIGMOID && (need_score || !a.renormalise)) {
+#pragma unroll
+            for (int i = 0; i < VPL; ++i) peak = fmaxf(peak, l[i]);
+            peak = row_max(peak);
+            if (need_score) {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i)
+                    if (l[i] > -INFINITY) total += key_exp(l[i] - peak);
+                total = row_sum(total);
+            }
+            if (!a.renormalise) {  // the denominator of the weights
+#pragma unroll
+                for (int i = 0; i < VPL; ++i)
+                    if (l[i] > -INFINITY) total_w += expf(l[i] - peak);
+                total_w = row_sum(total_w);
+            }
+        }
+        // keys, and the lane's two largest group values
+        unsigned key[VPL];
+        float one = -INFINITY, two = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) {
+            const bool open = l[i] > -INFINITY;
+            float s = 0.0f;
+            if (need_score) s = SIGMOID ? key_sigmoid(l[i]) : key_div(key_exp(l[i] - peak), total);
+            const float k = has_bias ? s + (i < chunk ? bias[first + i] : 0.0f) : l[i];
+            const bool in = open && k > -INFINITY;
+            key[i] = in ? (ordered(k) & ~31u) | (31 - i) : 0u;
+            if (grouped) {
+                const float v = in ? (has_bias || !need_score ? k : s) : -INFINITY;
+                two = fmaxf(two, fminf(one, v));
+                one = fmaxf(one, v);
+            }
+        }
+        bool clear = true;
+        if (grouped) {
+            for (int d = 1; d < per_group; d <<= 1) {
+                const float o1 = __shfl_xor_sync(kAll, one, d), o2 = __shfl_xor_sync(kAll, two, d);
+                two = fmaxf(fmaxf(two, o2), fminf(one, o1));
+                one = fmaxf(one, o1);
+            }
+            const float rank = a.group_top == 2 && two > -INFINITY ? one + two : one;
+            int better = 0;
+            for (int d = per_group; d < 8; d += per_group) {  // every other group once
+                const float o = __shfl_xor_sync(kAll, rank, d);
+                if (o > rank || (o == rank && (sub ^ d) < sub)) ++better;
+            }
+            const bool kept = better < a.top_groups && rank > -INFINITY;
+            if (need_score) {  // logits compare exactly
+                const float last = -row_max(kept ? -rank : -INFINITY), next = row_max(kept ? -INFINITY : rank);
+                clear = !(next > -INFINITY) || !(last - next <= 2 * clearance<SIGMOID>(last));
+            }
+            if (!kept) {
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) key[i] = 0u;
+            }
+        }
+        // picks
+        unsigned best = 0u, prev = 0u;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i) best = max(best, key[i]);
+        int prev_at = -1;
+        for (int j = 0; j <= a.top_k; ++j) {  // one more than asked for: it must not lie close to the last
+            unsigned top = (best & ~31u) | (best ? 8 - sub : 0);  // the lower lane among equals
+#pragma unroll
+            for (int d = 1; d < 8; d <<= 1) top = max(top, __shfl_xor_sync(kAll, top, d));
+            const int owner = 8 - (int)(top & 31u);  // 8: none left in this row
+            const unsigned won = __shfl_sync(kAll, best, (quad << 3) | (owner & 7));
+            const int at = owner < 8 ? owner * chunk + 31 - (int)(won & 31u) : -1;
+            if (at >= 0 && prev_at >= 0 && !whole) {
+                const float p = key_of(prev), v = key_of(top);
+                const bool close = has_bias ? p - v <= clearance<SIGMOID>(v) + 8e-6f * fmaxf(fabsf(p), fabsf(v)) : (prev & ~31u) == (top & ~31u);
+                if (close) clear = clear && to_f32(line[prev_at]) == to_f32(line[at]) && (!has_bias || bias[prev_at] == bias[at]);
+            }
+            prev = top;
+            prev_at = at;
+            if (sub == 0 && j < a.top_k) s_pick[warp][quad][j] = at;
+            if (j == a.top_k || !__any_sync(kAll, at >= 0)) {
+                for (int r = j + 1; sub == 0 && r < a.top_k; ++r) s_pick[warp][quad][r] = -1;
+                break;
+            }
+            if (sub == owner) {
+                best = 0u;
+#pragma unroll
+                for (int i = 0; i < VPL; ++i) {
+                    key[i] = key[i] == won ? 0u : key[i];
+                    best = max(best, key[i]);
+                }
+            }
+        }
+        __syncwarp();
+        // rows that fp32 keys do not decide, by the whole warp
+        const unsigned unclear = __ballot_sync(kAll, live && !clear);
+        for (int q = 0; q < 4; ++q)
+            if (unclear >> (8 * q) & 0xff) {
+                const int mine = decide_exactly<T, VPL / 4, SIGMOID>(a, logits + (row0 + q) * a.n_experts, bias, cells, lane);
+                if (lane < a.top_k) s_pick[warp][q][lane] = mine;
+                __syncwarp();
+            }
+        // weights of the chosen, a lane every eighth
+        float lm[kMaxTop / 8], w[kMaxTop / 8], top = -INFINITY, sum = 0.0f;
+        int mine[kMaxTop / 8];
+#pragma unroll
+        for (int i = 0; i < kMaxTop / 8; ++i) {
+            const int j = sub + 8 * i;
+            mine[i] = j < a.top_k ? s_pick[warp][quad][j] : -1;
+            lm[i] = mine[i] >= 0 ? to_f32(line[mine[i]]) : -INFINITY;
+            top = fmaxf(top, lm[i]);
+        }
+        if (a.renormalise) top = row_max(top);
+#pragma unroll
+        for (int i = 0; i < kMaxTop / 8; ++i) {
+            w[i] = 0.0f;
+            if (mine[i] < 0) continue;
+            if (a.renormalise) w[i] = !SIGMOID || top < -30.0f ? expf(lm[i] - top) : sigmoid(lm[i]);
+            else w[i] = SIGMOID ? sigmoid(lm[i]) : expf(lm[i] - peak) / total_w;
+            sum += w[i];
+        }
+        if (a.renormalise) sum = row_sum(sum);
+#pragma unroll
+        for (int i = 0; i < kMaxTop / 8; ++i) {
+            const int j = sub + 8 * i;
+            if (live && j < a.top_k) {
+                ids[row * a.top_k + j] = mine[i];
+                const float v = a.renormalise ? w[i] / sum : w[i];
+                weights[row * a.top_k + j] = nan ? NAN : mine[i] >= 0 ? v * a.scale : 0.0f;
+            }
+        }
+        __syncwarp();
+    }
+}
+
 // Gradient by the logits, all of the row written.  With r = the chosen scores' shares and g = the weights' gradient:
 //   renormalised: dl_j = scale r_j (g_j - sum_i g_i r_i) (times 1 - s_j for a sigmoid), nothing for the others;
 //   softmax:      dl_e = scale p_e (g_e - sum_i g_i p_i);      sigmoid: dl_j = scale g_j s_j (1 - s_j).
@@ -609,6 +801,18 @@ int launch_route(const RouteArgs &a, const void *logits, const float *bias, int 
     const long long want = ((long long)a.n_rows + kRouteWarps - 1) / kRouteWarps;
     const unsigned blocks = (unsigned)(want < 148 * 8 ? want : 148 * 8);  // what is resident at once
     const int per_lane = (a.n_experts + 31) / 32;
+    if (a.n_rows >= kOctetRows && a.n_experts % 8 == 0 && a.n_experts <= 256 && a.n_groups <= 8 && 8 % a.n_groups == 0) {
+        const long long most = ((long long)a.n_rows + 4 * kRouteWarps - 1) / (4 * kRouteWarps);
+        const unsigned grid = (unsigned)(most < 148 * 8 ? most : 148 * 8);
+        const bool vectors = a.n_experts / 8 * sizeof(T) % 16 == 0 && ((uintptr_t)logits & 15) == 0;
+#define RT_LAUNCH(V) route_octet_kernel<T, V, SIGMOID><<<grid, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, bias, ids, weights, vectors)
+        if (a.n_experts <= 64) RT_LAUNCH(8);
+        else if (a.n_experts <= 128) RT_LAUNCH(16);
+        else RT_LAUNCH(32);
+#undef RT_LAUNCH
+        RT_CUDA(cudaGetLastError());
+        return MPS_OK;
+    }
 #define RT_LAUNCH(V) route_kernel<T, V, SIGMOID><<<blocks, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, bias, ids, weights)
     if (per_lane <= 1) RT_LAUNCH(1);
     else if (per_lane <= 2) RT_LAUNCH(2);

@@ -38,11 +38,15 @@ def _dtype(t) -> int:
     return d
 
 
-def _check(device, *named):
-    """Every (name, tensor, dtype, shape): a contiguous CUDA tensor on `device` of that dtype and shape (None: not given)."""
-    index = device.index
+def _is(t, dtype, shape, index) -> bool:
+    """A contiguous tensor of that dtype and shape on CUDA device `index`, or None (not given)."""
+    return t is None or (t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous())
+
+
+def _explain(device, *named):
+    """Raises for the first (name, tensor, dtype, shape) that is not what `_is` asks for."""
     for name, t, dtype, shape in named:
-        if t is None or (t.dtype is dtype and t.shape == shape and t.is_cuda and t.get_device() == index and t.is_contiguous()):
+        if _is(t, dtype, shape, device.index):
             continue
         if not t.is_cuda:
             raise ValueError(f"{name}: expected a CUDA tensor (there is no CPU path)")
@@ -76,12 +80,13 @@ def _call(device, stream, name, *args):
         capi.check(rc)
 
 
-def _matrix(name, t, dims=2):
-    if t.dim() != dims:
-        raise ValueError(f"{name}: expected {dims} dimensions, got {t.dim()}")
+def _shape(name, t, dims=2):
+    shape = t.shape
+    if len(shape) != dims:
+        raise ValueError(f"{name}: expected {dims} dimensions, got {len(shape)}")
     if not t.is_cuda:
         raise ValueError(f"{name}: expected a CUDA tensor (there is no CPU path)")
-    return t
+    return shape
 
 
 def _spec(n_experts, top_k, score, n_groups, top_groups, group_top, renormalise, scale):
@@ -94,9 +99,11 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, n_groups: in
           renormalise: bool = True, scale: float = 1.0, group: bool = True, stream=None):
     """(ids, weights, groups): the top_k experts of every row of `logits` (rows, experts) by score + bias among the best
     `top_groups` of `n_groups` expert groups, their weights (fp32), and the rows listed by expert (None with group=False)."""
-    rows, experts = _matrix("logits", logits).shape
+    rows, experts = _shape("logits", logits)
     dev = logits.device
-    _check(dev, ("logits", logits, logits.dtype, (rows, experts)), ("bias", bias, torch.float32, (experts,)))
+    at = dev.index
+    if not (_is(logits, logits.dtype, (rows, experts), at) and _is(bias, torch.float32, (experts,), at)):
+        _explain(dev, ("logits", logits, logits.dtype, (rows, experts)), ("bias", bias, torch.float32, (experts,)))
     spec = _spec(experts, top_k, score, n_groups, top_groups, group_top, renormalise, scale)
     # one allocation: five take longer than the kernels of a small batch
     k = max(top_k, 0)  # what is wrong with it the entry point says
@@ -111,11 +118,14 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, n_groups: in
 
 def route_backward(logits, ids, d_weights, *, score: str = "softmax", renormalise: bool = True, scale: float = 1.0, stream=None):
     """Gradient by the logits of route's weights for the choice `ids` and the weights' gradient (fp32)."""
-    rows, experts = _matrix("logits", logits).shape
+    rows, experts = _shape("logits", logits)
     dev = logits.device
-    top_k = _matrix("ids", ids).shape[1]
-    _check(dev, ("logits", logits, logits.dtype, (rows, experts)), ("ids", ids, torch.int32, (rows, top_k)),
-           ("d_weights", d_weights, torch.float32, (rows, top_k)))
+    top_k = _shape("ids", ids)[1]
+    at = dev.index
+    if not (_is(logits, logits.dtype, (rows, experts), at) and _is(ids, torch.int32, (rows, top_k), at)
+            and _is(d_weights, torch.float32, (rows, top_k), at)):
+        _explain(dev, ("logits", logits, logits.dtype, (rows, experts)), ("ids", ids, torch.int32, (rows, top_k)),
+               ("d_weights", d_weights, torch.float32, (rows, top_k)))
     spec = _spec(experts, top_k, score, 1, 1, 1, renormalise, scale)
     out = torch.empty_like(logits)
     _call(dev, stream, "mps_route_backward", rows, C.byref(spec), _dtype(logits), _ptr(logits), _ptr(ids), _ptr(d_weights), _ptr(out))
@@ -127,7 +137,9 @@ def group_rows(ids, n_groups: int, *, stream=None) -> Groups:
     dev = ids.device
     if ids.dim() not in (1, 2):
         raise ValueError(f"ids: expected 1 or 2 dimensions, got {ids.dim()}")
-    _check(dev, ("ids", ids, torch.int32, ids.shape))
+    at = dev.index
+    if not (_is(ids, torch.int32, ids.shape, at)):
+        _explain(dev, ("ids", ids, torch.int32, ids.shape))
     rows, per_row = ids.shape[0], 1 if ids.dim() == 1 else ids.shape[1]
     groups = Groups(torch.empty(max(n_groups, 0) + 1, dtype=torch.int32, device=dev), torch.empty(ids.numel(), dtype=torch.int32, device=dev),
                     torch.empty_like(ids))
@@ -138,13 +150,16 @@ def group_rows(ids, n_groups: int, *, stream=None) -> Groups:
 def routed_product(x, w, groups: Groups, *, gather: bool = True, transpose: bool = False, out=None, stream=None):
     """y[s] = x[groups.row[s]] @ w[g].T for the slots s of every group g (x[s] itself with gather=False); transpose=True
     multiplies by w[g] instead.  w (groups, n, k).  Rows of `out` behind the last slot in use are left as they were."""
-    n_groups, n, k = _matrix("w", w, 3).shape
+    n_groups, n, k = _shape("w", w, 3)
     inner, outer = (n, k) if transpose else (k, n)
-    dev, rows, slots = x.device, _matrix("x", x).shape[0], groups.row.numel()
+    dev, rows, slots = x.device, _shape("x", x)[0], groups.row.numel()
     if out is None:
         out = torch.empty((slots, outer), dtype=x.dtype, device=dev)
-    _check(dev, ("x", x, x.dtype, (rows, inner)), ("w", w, x.dtype, (n_groups, n, k)), ("groups.ptr", groups.ptr, torch.int32, (n_groups + 1,)),
-           ("groups.row", groups.row, torch.int32, (slots,)), ("out", out, x.dtype, (slots, outer)))
+    at = dev.index
+    if not (_is(x, x.dtype, (rows, inner), at) and _is(w, x.dtype, (n_groups, n, k), at) and _is(groups.ptr, torch.int32, (n_groups + 1,), at)
+            and _is(groups.row, torch.int32, (slots,), at) and _is(out, x.dtype, (slots, outer), at)):
+        _explain(dev, ("x", x, x.dtype, (rows, inner)), ("w", w, x.dtype, (n_groups, n, k)), ("groups.ptr", groups.ptr, torch.int32, (n_groups + 1,)),
+               ("groups.row", groups.row, torch.int32, (slots,)), ("out", out, x.dtype, (slots, outer)))
     _call(dev, stream, "mps_routed_product", slots, rows, n_groups, k, n, _dtype(x), int(transpose), _ptr(groups.ptr),
           _ptr(groups.row) if gather else None, _ptr(x), _ptr(w), _ptr(out))
     return out
@@ -154,11 +169,14 @@ def routed_wgrad(x, dy, groups: Groups, *, gather: bool = True, out=None, stream
     """dw[g] = sum over the slots s of g of outer(dy[s], x[groups.row[s]]) (x[s] with gather=False): (groups, n, k), zero for
     a group without slots."""
     dev, slots, n_groups = x.device, groups.row.numel(), groups.ptr.numel() - 1
-    (rows, k), n = _matrix("x", x).shape, _matrix("dy", dy).shape[1]
+    (rows, k), n = _shape("x", x), _shape("dy", dy)[1]
     if out is None:
         out = torch.empty((n_groups, n, k), dtype=x.dtype, device=dev)
-    _check(dev, ("x", x, x.dtype, (rows, k)), ("dy", dy, x.dtype, (slots, n)), ("groups.ptr", groups.ptr, torch.int32, (n_groups + 1,)),
-           ("groups.row", groups.row, torch.int32, (slots,)), ("out", out, x.dtype, (n_groups, n, k)))
+    at = dev.index
+    if not (_is(x, x.dtype, (rows, k), at) and _is(dy, x.dtype, (slots, n), at) and _is(groups.ptr, torch.int32, (n_groups + 1,), at)
+            and _is(groups.row, torch.int32, (slots,), at) and _is(out, x.dtype, (n_groups, n, k), at)):
+        _explain(dev, ("x", x, x.dtype, (rows, k)), ("dy", dy, x.dtype, (slots, n)), ("groups.ptr", groups.ptr, torch.int32, (n_groups + 1,)),
+               ("groups.row", groups.row, torch.int32, (slots,)), ("out", out, x.dtype, (n_groups, n, k)))
     _call(dev, stream, "mps_routed_wgrad", slots, rows, n_groups, k, n, _dtype(x), _ptr(groups.ptr), _ptr(groups.row) if gather else None,
           _ptr(x), _ptr(dy), _ptr(out))
     return out
@@ -166,22 +184,28 @@ def routed_wgrad(x, dy, groups: Groups, *, gather: bool = True, out=None, stream
 
 def routed_combine(rows, slot, weights=None, *, out=None, stream=None):
     """y[t] = sum over j of weights[t, j] * rows[slot[t, j]]; no term for a negative slot, weights None: 1 each."""
-    dev, (n_slots, dim), (n, per_row) = rows.device, _matrix("rows", rows).shape, _matrix("slot", slot).shape
+    dev, (n_slots, dim), (n, per_row) = rows.device, _shape("rows", rows), _shape("slot", slot)
     if out is None:
         out = torch.empty((n, dim), dtype=rows.dtype, device=dev)
-    _check(dev, ("rows", rows, rows.dtype, (n_slots, dim)), ("slot", slot, torch.int32, (n, per_row)), ("weights", weights, torch.float32, (n, per_row)),
-           ("out", out, rows.dtype, (n, dim)))
+    at = dev.index
+    if not (_is(rows, rows.dtype, (n_slots, dim), at) and _is(slot, torch.int32, (n, per_row), at) and _is(weights, torch.float32, (n, per_row), at)
+            and _is(out, rows.dtype, (n, dim), at)):
+        _explain(dev, ("rows", rows, rows.dtype, (n_slots, dim)), ("slot", slot, torch.int32, (n, per_row)), ("weights", weights, torch.float32, (n, per_row)),
+               ("out", out, rows.dtype, (n, dim)))
     _call(dev, stream, "mps_routed_combine", n, per_row, n_slots, dim, _dtype(rows), _ptr(slot), _ptr(weights), _ptr(rows), _ptr(out))
     return out
 
 
 def routed_combine_backward(dy, rows, slot, weights=None, *, out=None, stream=None):
     """(d_rows, d_weights) of routed_combine; `out` receives d_rows, whose rows that no slot names are left as they were."""
-    dev, (n_slots, dim), (n, per_row) = rows.device, _matrix("rows", rows).shape, _matrix("slot", slot).shape
+    dev, (n_slots, dim), (n, per_row) = rows.device, _shape("rows", rows), _shape("slot", slot)
     if out is None:
         out = torch.empty_like(rows)
-    _check(dev, ("dy", dy, rows.dtype, (n, dim)), ("rows", rows, rows.dtype, (n_slots, dim)), ("slot", slot, torch.int32, (n, per_row)),
-           ("weights", weights, torch.float32, (n, per_row)), ("out", out, rows.dtype, (n_slots, dim)))
+    at = dev.index
+    if not (_is(dy, rows.dtype, (n, dim), at) and _is(rows, rows.dtype, (n_slots, dim), at) and _is(slot, torch.int32, (n, per_row), at)
+            and _is(weights, torch.float32, (n, per_row), at) and _is(out, rows.dtype, (n_slots, dim), at)):
+        _explain(dev, ("dy", dy, rows.dtype, (n, dim)), ("rows", rows, rows.dtype, (n_slots, dim)), ("slot", slot, torch.int32, (n, per_row)),
+               ("weights", weights, torch.float32, (n, per_row)), ("out", out, rows.dtype, (n_slots, dim)))
     d_weights = torch.empty((n, per_row), dtype=torch.float32, device=dev)
     _call(dev, stream, "mps_routed_combine_backward", n, per_row, n_slots, dim, _dtype(rows), _ptr(slot), _ptr(weights), _ptr(dy), _ptr(rows), _ptr(out),
           _ptr(d_weights))
@@ -189,10 +213,15 @@ def routed_combine_backward(dy, rows, slot, weights=None, *, out=None, stream=No
 
 
 def _adapter_sizes(x, w, a, b, ids, groups, scale):
-    rows, (n, k), (n_adapters, rank) = _matrix("x", x).shape[0], _matrix("w", w).shape, _matrix("a", a, 3).shape[:2]
-    _check(x.device, ("x", x, x.dtype, (rows, k)), ("w", w, x.dtype, (n, k)), ("a", a, x.dtype, (n_adapters, rank, k)),
-           ("b", b, x.dtype, (n_adapters, n, rank)), ("ids", ids, torch.int32, (rows,)), ("groups.ptr", groups.ptr, torch.int32, (n_adapters + 1,)),
-           ("groups.row", groups.row, torch.int32, (rows,)), ("scale", scale, torch.float32, (n_adapters,)))
+    rows, (n, k), (n_adapters, rank) = _shape("x", x)[0], _shape("w", w), _shape("a", a, 3)[:2]
+    at = x.device.index
+    if not (_is(x, x.dtype, (rows, k), at) and _is(w, x.dtype, (n, k), at) and _is(a, x.dtype, (n_adapters, rank, k), at)
+            and _is(b, x.dtype, (n_adapters, n, rank), at) and _is(ids, torch.int32, (rows,), at)
+            and _is(groups.ptr, torch.int32, (n_adapters + 1,), at) and _is(groups.row, torch.int32, (rows,), at)
+            and _is(scale, torch.float32, (n_adapters,), at)):
+        _explain(x.device, ("x", x, x.dtype, (rows, k)), ("w", w, x.dtype, (n, k)), ("a", a, x.dtype, (n_adapters, rank, k)),
+               ("b", b, x.dtype, (n_adapters, n, rank)), ("ids", ids, torch.int32, (rows,)), ("groups.ptr", groups.ptr, torch.int32, (n_adapters + 1,)),
+               ("groups.row", groups.row, torch.int32, (rows,)), ("scale", scale, torch.float32, (n_adapters,)))
     return rows, k, n, n_adapters, rank
 
 
@@ -209,7 +238,9 @@ def adapters(x, w, a, b, ids, groups: Groups, scale=None, *, out=None, stream=No
     sizes = rows, k, n, _, _ = _adapter_sizes(x, w, a, b, ids, groups, scale)
     if out is None:
         out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
-    _check(x.device, ("out", out, x.dtype, (rows, n)))
+    at = x.device.index
+    if not (_is(out, x.dtype, (rows, n), at)):
+        _explain(x.device, ("out", out, x.dtype, (rows, n)))
     dtype = _dtype(x)
     ws = _adapter_workspace(x.device, sizes, dtype, False)
     if stream is not None:
@@ -222,7 +253,9 @@ def adapters(x, w, a, b, ids, groups: Groups, scale=None, *, out=None, stream=No
 def adapters_backward(dy, x, w, a, b, ids, groups: Groups, scale=None, *, stream=None):
     """(dx, da, db) of adapters; the shared projection and the scales are constants."""
     sizes = rows, k, n, _, _ = _adapter_sizes(x, w, a, b, ids, groups, scale)
-    _check(x.device, ("dy", dy, x.dtype, (rows, n)))
+    at = x.device.index
+    if not (_is(dy, x.dtype, (rows, n), at)):
+        _explain(x.device, ("dy", dy, x.dtype, (rows, n)))
     dx, da, db = torch.empty_like(x), torch.empty_like(a), torch.empty_like(b)
     dtype = _dtype(x)
     ws = _adapter_workspace(x.device, sizes, dtype, True)

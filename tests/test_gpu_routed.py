@@ -88,11 +88,13 @@ def test_route_without_rows(mps, cuda):
 @pytest.mark.parametrize("n_groups", [1, 4])
 def test_route_equal_logits_go_to_the_lowest_index(mps, cuda, score, biased, n_groups):
     gen = gen_of(5)
-    logits = torch.randint(-2, 3, (70, 64), generator=gen, device="cuda").float()
-    logits[0] = 0.0
-    logits[1, ::2] = -0.0
-    bias = torch.randint(0, 2, (64,), generator=gen, device="cuda").float() * 0.25 if biased else None
-    check_route(mps, logits, 9, score=score, bias=bias, n_groups=n_groups, top_groups=min(2, n_groups), group_top=2)
+    for rows in (70, 2060):  # a warp per row; eight lanes per row
+        logits = torch.randint(-2, 3, (rows, 64), generator=gen, device="cuda").float()
+        logits[0] = 0.0
+        logits[1, ::2] = -0.0
+        bias = torch.randint(0, 2, (64,), generator=gen, device="cuda").float() * 0.25 if biased else None
+        check_route(mps, logits, 9, score=score, bias=bias, n_groups=n_groups, top_groups=min(2, n_groups), group_top=2)
+        check_route(mps, logits.bfloat16(), 9, score=score, bias=bias, n_groups=n_groups, top_groups=min(2, n_groups), group_top=1)
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
@@ -107,12 +109,21 @@ def test_route_close_keys_are_told_apart(mps, cuda, score, group_top):
         ids, _, _ = mps.route(torch.from_numpy(logits[t:t + 1]).cuda(), 6, score=score, bias=bias, n_groups=4, top_groups=2, group_top=group_top)
         want, _ = o.route(logits[t:t + 1].astype(np.float64), 6, score, f64(bias), 4, 2, group_top)
         assert (ids.cpu().numpy() == want).all(), t
+        ids, _, _ = mps.route(torch.from_numpy(logits[t:t + 1]).cuda().repeat(2048, 1), 6, score=score, bias=bias, n_groups=4, top_groups=2,
+                              group_top=group_top)
+        assert (ids.cpu().numpy() == want).all(), t
+    close_logits = torch.from_numpy((3 + rng.random((2100, 64)) * 1e-5).astype(np.float32)).cuda()  # a few units in the last place apart
+    check_route(mps, close_logits, 10, score=score)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_route_not_a_number_and_infinite(mps, cuda, dtype, score):
-    logits = rand(gen_of(1), dtype, 12, 40)
+    for rows in (12, 2055):
+        not_a_number(mps, rand(gen_of(1), dtype, rows, 40), score)
+
+
+def not_a_number(mps, logits, score):
     logits[2, 5] = math.nan
     logits[3] = math.nan
     logits[5, :38] = -math.inf
