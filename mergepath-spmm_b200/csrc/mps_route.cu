@@ -85,13 +85,14 @@ __device__ __forceinline__ void warp_best(float &v, int &at) {
     at = (int)__reduce_min_sync(kAll, mine == top ? (unsigned)at : 0x7fffffffu);
     v = __uint_as_float(top & 0x80000000u ? top ^ 0x80000000u : ~top);
 }
-__device__ __forceinline__ void warp_best(double &v, int &at) {
-#pragma unroll
-    for (int d = 16; d; d >>= 1) {
-        const double ov = __shfl_xor_sync(kAll, v, d);
-        const int oa = __shfl_xor_sync(kAll, at, d);
-        if (ov > v || (ov == v && oa < at)) { v = ov; at = oa; }
-    }
+__device__ __forceinline__ void warp_best(double &v, int &at) {  // by the two halves of an integer that orders like the double
+    const long long bits = __double_as_longlong(v + 0.0);
+    const unsigned long long o = bits < 0 ? ~(unsigned long long)bits : (unsigned long long)bits | 1ull << 63;
+    const unsigned hi = (unsigned)(o >> 32), top_hi = __reduce_max_sync(kAll, hi);
+    const unsigned lo = hi == top_hi ? (unsigned)o : 0u, top_lo = __reduce_max_sync(kAll, lo);
+    at = (int)__reduce_min_sync(kAll, hi == top_hi && lo == top_lo ? (unsigned)at : 0x7fffffffu);
+    const unsigned long long top = (unsigned long long)top_hi << 32 | top_lo;
+    v = __longlong_as_double((long long)(top >> 63 ? top ^ 1ull << 63 : ~top));
 }
 
 // Sigmoid and exponential of the keys, which only have to order.  __expf is off by (2 + 1.173 |x|) 2^-23 of the result, which
@@ -250,7 +251,7 @@ __device__ __forceinline__ void row_keys(const float (&l)[VPL], const float (&b)
     }
 }
 
-// A row decided on fp64 keys: lane j returns the j-th expert.  Out of line, so that the few rows that need it do not cost the
+// A row decided exactly (logits as they are, scores in fp64): lane j returns the j-th expert.  Out of line, so that the few rows that need it do not cost the
 // others their registers.
 template <typename T, int VPL, bool SIGMOID>
 __device__ __noinline__ int decide_exactly(const RouteArgs &a, const T *line, const float *bias, double *cells, int lane) {
@@ -262,10 +263,17 @@ __device__ __noinline__ int decide_exactly(const RouteArgs &a, const T *line, co
         b[i] = bias && e < a.n_experts ? bias[e] : 0.0f;
         if (l[i] != l[i]) l[i] = -INFINITY;
     }
+    int mine;
+    if (!bias && (a.n_groups == 1 || a.group_top == 1)) {  // the logits themselves are compared
+        float key[VPL], value[VPL];
+        row_keys<float, VPL, SIGMOID>(l, b, false, false, key, value);
+        if (a.n_groups > 1) keep_groups<SIGMOID>(key, value, a, (float *)cells, lane);
+        choose<true, SIGMOID>(key, a, line, bias, lane, mine);
+        return mine;
+    }
     double key[VPL], value[VPL];
     row_keys<double, VPL, SIGMOID>(l, b, bias != nullptr, true, key, value);
     if (a.n_groups > 1) keep_groups<SIGMOID>(key, value, a, cells, lane);
-    int mine;
     choose<true, SIGMOID>(key, a, line, bias, lane, mine);
     return mine;
 }
@@ -344,13 +352,13 @@ __global__ void __launch_bounds__(32 * kRouteWarps, VPL <= 8 ? 8 : 1) route_kern
 // Many rows: eight lanes per row, four rows per warp, so that a pick's reductions serve four rows.  A lane holds a contiguous
 // eighth of the experts (a part of one group: 1, 2, 4 or 8 groups) as integers that order like the keys, the low five bits
 // replaced by the place in the lane: the lane's best is one integer maximum, equal keys go to the lower place by themselves, and
-// taking an expert out is a comparison with the value that won.  The five bits cost 2^-18 of a key, which the test for close
-// keys takes in; for 16-bit logits without a bias they are zeros.  16384 rows of 256 experts, top 8 of 4 of 8 groups:
-// OCTET_US us, WARP_US us with a warp per row (which keeps fewer rows, other group counts and more experts).
+// taking an expert out is a comparison with the value that won.  Keys that differ in the five bits only count as close (of
+// 16-bit logits without a bias they are zeros).  16384 rows of 256 experts, top 8 of 4 of 8 groups:
+// 30 us, 42 with a warp per row (which keeps fewer rows, other group counts and more experts).
 constexpr int kOctetRows = 2048;  // from here on there are rows enough for 148 SMs
 
 template <typename T, int VPL, bool SIGMOID>
-__global__ void __launch_bounds__(32 * kRouteWarps) route_octet_kernel(const RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
+__global__ void __launch_bounds__(32 * kRouteWarps, 6) route_octet_kernel(const RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
                                                                       int *__restrict__ ids, float *__restrict__ weights, bool vectors) {
     extern __shared__ double s_cells[];
     __shared__ int s_pick[kRouteWarps][4][kMaxTop];
@@ -472,7 +480,15 @@ __global__ void __launch_bounds__(32 * kRouteWarps) route_octet_kernel(const Rou
             const int at = owner < 8 ? owner * chunk + 31 - (int)(won & 31u) : -1;
             if (at >= 0 && prev_at >= 0 && !whole) {
                 const float p = key_of(prev), v = key_of(top);
-                const bool close = has_bias ? p - v <= clearance<SIGMOID>(v) + 8e-6f * fmaxf(fabsf(p), fabsf(v)) : (prev & ~31u) == (top & ~31u);
+                bool close = (prev & ~31u) == (top & ~31u);
+                if (has_bias && p - v <= clearance<SIGMOID>(v) + 8e-6f * fmaxf(fabsf(p), fabsf(v))) {  // within the five bits: by the whole keys
+                    auto whole_key = [&](int e) {
+                        const float x = to_f32(line[e]);
+                        return (SIGMOID ? key_sigmoid(x) : key_div(key_exp(x - peak), total)) + bias[e];
+                    };
+                    const float k = whole_key(at);
+                    close = close || whole_key(prev_at) - k <= clearance<SIGMOID>(k);
+                }
                 if (close) clear = clear && to_f32(line[prev_at]) == to_f32(line[at]) && (!has_bias || bias[prev_at] == bias[at]);
             }
             prev = top;
