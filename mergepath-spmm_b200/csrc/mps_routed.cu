@@ -324,7 +324,7 @@ int tc_rows(const TcRows *products, int n, const Cut &cut, const void *const *x,
         if (a.gather)
             if (int rc = tensor_map(&a.x_run, a.bf16, x[i], 2, a.k, x_rows, 1, loaded / 8)) return rc;
         if (a.rank)
-            if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded)) return rc;
+            if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded / 8)) return rc;
     }
     if (n == 2) return cut.nt == 32 ? launch_tc_rows<32, true>(l, sms, st) : launch_tc_rows<64, true>(l, sms, st);
     if (cut.nt == 32) return launch_tc_rows<32, false>(l, sms, st);

@@ -5,8 +5,9 @@
 // few rows meet each matrix and its bytes are what counts, 256 where the arithmetic does).  The matrices come by TMA in 64-deep
 // slices through a ring of stages, rows in slot order too; gathered rows by number, four per TMA instruction, issued by one
 // elected lane of each of eight warps: 0.29 us for 128 rows of a slice, about what the TMA unit gives (0.35 us from four warps,
-// 0.45 us as 16-byte asynchronous copies by 128 threads, 1.2 us from 32 diverged lanes of one warp).  Two accumulators in TMEM alternate, so a tile is stored while the next one is summed; results go through shared
-// memory, where 32 slots by 128 features become whole 256-byte rows.
+// 0.45 us as 16-byte asynchronous copies by 128 threads, 1.2 us from 32 diverged lanes of one warp).  Two accumulators in TMEM
+// alternate, so a tile is stored while the next one is summed; results go through shared memory, where 64 slots by 128 features
+// become whole 256-byte rows.
 //
 // A tile's sum may go on with a second product (`rank` > 0): the group's low-rank matrix times rows u that were computed before,
 // kept as hi + lo pairs of the 16-bit type (two planes), so that the intermediate's rounding (2^-16 in bf16, 2^-22 in fp16)
@@ -15,6 +16,9 @@
 // The widest tiles (NT = 256) belong to a pair of neighbouring blocks (cta_group::2): 256 features by 256 slots, each block
 // loading its 128 features and half of the slots, so that a block's slice is 32 KB instead of 48 and six of them are in flight.
 // Both blocks' loads arrive at the first one's barriers; it issues the products for both, and each stores the features it holds.
+//
+// Every warp that loads has something to load into every stage: the products of a slice wait for it, so it cannot fall behind
+// the ring.  A warp that only waited for a stage could be lapped, and a barrier's parity does not tell uses two apart.
 //
 // Few tiles with long sums are cut along the sum over the blocks of a cluster; the partial results meet in distributed shared
 // memory, added in the order of the blocks by the warps that store results, while the others are at the next tile.
@@ -33,7 +37,7 @@ constexpr int kTcFeatures = 128;
 constexpr int kTcDepth = 64;
 constexpr int kTcRing = 192 * 1024;            // shared memory of the stages
 constexpr int kOutPitch = kTcFeatures * 2 + 16;  // a result row in shared memory; the pad spreads 16-byte reads over the banks
-constexpr int kOutBytes = 2 * 32 * kOutPitch;    // two chunks of 32 rows
+constexpr int kOutBytes = 64 * kOutPitch;        // 64 rows at a time
 constexpr int kOutTotal = (kOutBytes + 1023) / 1024 * 1024;
 
 struct TcRows {
@@ -387,13 +391,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                         if (d > 0 && s + d >= s1) break;
                         const uint32_t dst = ring + pos.stage * S::kStage + d * S::kSlice;
                         const bool second = s + d >= main_steps;
-                        const int e = s + d - main_steps, i0 = (second ? e >> 1 : s + d) * kTcDepth;
+                        const int i0 = (second ? (s + d - main_steps) >> 1 : s + d) * kTcDepth;
                         const CUtensorMap *m = second ? &a.w2 : &a.w;
                         if (a.mn_major)
                             for (int h = 0; h < halves; ++h) tma_3d<PAIRED>(dst + h * kBlock64, m, f0 + h * 64, i0, second ? g : z, bar);
                         else tma_3d<PAIRED>(dst, m, i0, f0, second ? g : z, bar);
-                        if (second) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.u, i0, (e & 1) * a.u_plane + own, bar);
-                        else if (!a.gather) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);
+                        if (!a.gather) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);  // there is no second product then
                     }
                 }
             }
@@ -427,13 +430,18 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             then.next();
             fetch_rows(then);  // under way while this tile is loaded
             for (int s = s0; s < s1; s += S::kSlices, pos.next(stages)) {
-                // every use of a stage is waited for, also where nothing is loaded: a parity tells neighbouring uses apart only
                 mbar_wait(smem_addr(&pipe.empty[pos.stage]), pos.parity ^ 1, gave_up, a.status);
                 __syncwarp();
 #pragma unroll
                 for (int d = 0; d < S::kSlices; ++d) {
-                    if (s + d >= min(s1, main_steps)) break;
+                    if (s + d >= s1) break;
                     const uint32_t dst = ring + pos.stage * S::kStage + d * S::kSlice + kTcFeatures * 128 + (warp - 8) * RPW * 128, bar = full0 + pos.stage * 8;
+                    const int e = s + d - main_steps;
+                    if (e >= 0) {  // rows of the second product, in slot order
+                        const int line = (e & 1) * a.u_plane + slot0 + half * columns / 2 + (warp - 8) * RPW;
+                        if (elect_one()) tma_2d<PAIRED>(dst, &a.u, (e >> 1) * kTcDepth, line, bar);
+                        continue;
+                    }
                     if (run) {
                         if (elect_one()) tma_2d<PAIRED>(dst, &a.x_run, (s + d) * kTcDepth, row0, bar);
                         continue;
@@ -536,28 +544,43 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
             tc_fence_after();
             const bool rows_of_16 = !a.pair && a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0, wide = rows_of_16 && !reduce;
+            const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT;
+            if (wide) {
+                // 64 columns at a time: a result warp is alone on its scheduler, so two loads and 64 roundings in flight take little
+                // more time than half of them
 #pragma unroll 1
-            for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 32) {
-                float v[32] = {};
-                if (s0 < s1) tmem_load(tmem + ((uint32_t)(quad * 32) << 16) + buf * NT + c0, v);  // a block may have no part in a short sum
-                if (reduce) {
+                for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 64) {
+                    float v[2][32];
+                    tmem_start(lanes + c0, v[0]);
+                    if (NT > 32) tmem_start(lanes + c0 + 32, v[1]);
+                    tmem_wait(v[0]);
+                    if (NT > 32) tmem_wait(v[1]);
+                    results_sync();  // the rows before these have been read
 #pragma unroll
-                    for (int j = 0; j < 32; j += 8)
-                        if (slot0 + c0 + j < slot1) meeting.give(c0 + j, feature, v + j, a.ids);
-                } else if (wide) {
-                    const uint32_t at = staging + (c0 >> 5 & 1) * (32 * kOutPitch);
-                    if (a.bf16) spread_column<true>(v, at + feature * 2);
-                    else spread_column<false>(v, at + feature * 2);
-                    results_sync();  // one per chunk is enough: the other buffer's readers have passed it too
+                    for (int h = 0; h < (NT > 32 ? 2 : 1); ++h) {
+                        if (a.bf16) spread_column<true>(v[h], staging + h * 32 * kOutPitch + feature * 2);
+                        else spread_column<false>(v[h], staging + h * 32 * kOutPitch + feature * 2);
+                    }
+                    results_sync();
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
+                    for (int j = 0; j < (NT > 32 ? 8 : 4); ++j) {
                         const int c = (mine >> 4) + 8 * j, fc = (mine & 15) * 8;
-                        const uint4 q = load_shared_128(at + c * kOutPitch + fc * 2);
+                        const uint4 q = load_shared_128(staging + c * kOutPitch + fc * 2);
                         if (slot0 + c0 + c < slot1 && f0 + fc < a.n) {
                             const int r = out_row(slot0 + c0 + c);
                             if (r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = q;
                         }
                     }
+                }
+            } else
+#pragma unroll 1
+            for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 32) {
+                float v[32] = {};
+                if (s0 < s1) tmem_load(lanes + c0, v);  // a block may have no part in a short sum
+                if (reduce) {
+#pragma unroll
+                    for (int j = 0; j < 32; j += 8)
+                        if (slot0 + c0 + j < slot1) meeting.give(c0 + j, feature, v + j, a.ids);
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
@@ -584,7 +607,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 } else
                     for (int c = 0; c < own; ++c) store(slot0 + first + c, meeting.sum(c, feature) * scale);
                 tell_cluster(smem_addr(&pipe.freed), split, lane);
-            } else if (wide) results_sync();  // the next tile starts with the first buffer again
+            }
         }
     }
     if (a.apart) wait_for_launch_before();
@@ -696,6 +719,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     const uint32_t full0 = PAIRED ? in_block(smem_addr(&pipe.full[0]), 0) : smem_addr(&pipe.full[0]);
     RingAt pos;
     int turn = 0;
+    const int q_end = (a.pair ? 2 : 1) * a.n_slots;  // out of range of Q
     for (int tile = worker; tile < n_tiles; tile += workers, ++turn) {
         const int g = tile / per_group, rest = tile - g * per_group;
         const int f0 = rest / j_tiles * TILE_F + half * kTcFeatures, c0 = rest % j_tiles * cols;
@@ -707,16 +731,35 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
         const int q0 = c0 + half * q_blocks * 64;  // the columns this block loads
         if (warp == 0) {
             if (elect_one()) {
-                for (int s = s0; s < s1; ++s, pos.next(stages)) {
+                const int whole = min(s1, (slots.y - slots.x) / kTcDepth);  // the slices before this one are whole
+                const uint32_t bytes = (PAIRED ? 2 : 1) * (p_blocks + q_blocks) * kBlock64;
+                for (int s = s0; s < whole; ++s, pos.next(stages)) {
                     const int st = pos.stage, slot = slots.x + s * kTcDepth;
                     mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                     const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
-                    if (half == 0) mbar_expect(bar, (PAIRED ? 2 : 1) * (p_blocks + q_blocks) * kBlock64);
-                    if (slot + kTcDepth > slots.y) continue;  // part of a slice: by row number
+                    if (half == 0) mbar_expect(bar, bytes);
                     if (!gather)
                         for (int b = 0; b < p_blocks; ++b) tma_2d<PAIRED>(dst + b * kBlock64, &a.p_tile, f0 + b * 64, slot, bar);
                     for (int b = 0; b < q_blocks; ++b)
                         tma_2d<PAIRED>(dst + (2 + b) * kBlock64, &a.q_tile, a.pair ? c0 : q0 + b * 64, a.pair ? b * a.n_slots + slot : slot, bar);
+                }
+                if (max(s0, whole) < s1) {  // part of a slice: by row number, zeros behind the group's end
+                    const int st = pos.stage, slot = slots.x + (s1 - 1) * kTcDepth;
+                    mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
+                    const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
+                    if (half == 0) mbar_expect(bar, bytes);
+#pragma unroll 1
+                    for (int b = gather ? 2 : 0; b < 2 + q_blocks; ++b) {
+                        if (b >= p_blocks && b < 2) continue;
+                        const bool q = b >= 2;
+                        const int x = !q ? f0 + b * 64 : a.pair ? c0 : q0 + (b - 2) * 64, plane = q && a.pair ? (b - 2) * a.n_slots : 0;
+#pragma unroll 1
+                        for (int i = 0; i < kTcDepth; i += 4) {
+                            auto line = [&](int j) { return slot + i + j < slots.y ? plane + slot + i + j : q ? q_end : a.n_p_rows; };
+                            tma_rows<PAIRED>(dst + b * kBlock64 + i * 128, q ? &a.q_rows : &a.p_rows, x, line(0), line(1), line(2), line(3), bar);
+                        }
+                    }
+                    pos.next(stages);
                 }
             }
         } else if (warp == 1) {
@@ -735,14 +778,14 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
                 tc_commit<PAIRED>(smem_addr(&pipe.tmem_full[buf]));
             }
-        } else if (warp >= 8) {
+        } else if (warp >= 8 && gather) {
             // rows by number, an eighth of a slice's per warp.  The numbers are read eight slices ahead: a lane holds one of the
             // warp's eight of four neighbouring slices.
             auto fetch = [&](int s) {
                 const int slot = slots.x + (s + (lane >> 3)) * kTcDepth + (warp - 8) * 8 + (lane & 7);
                 int r = a.n_p_rows;  // out of range: zeros
                 if (s + (lane >> 3) < s1 && slot < slots.y) {
-                    r = gather ? a.slot_row[slot] : slot;
+                    r = a.slot_row[slot];
                     if ((unsigned)r >= (unsigned)a.n_p_rows) {
                         atomicOr(a.status, kStatusBadIndex);
                         r = a.n_p_rows;
@@ -750,7 +793,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 }
                 return r;
             };
-            const int q_end = (a.pair ? 2 : 1) * a.n_slots;  // out of range of Q
             int now = fetch(s0), next = fetch(s0 + 4);
             for (int s = s0; s < s1; ++s, pos.next(stages)) {
                 const int which = (s - s0) & 3;
@@ -758,37 +800,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     now = next;
                     next = fetch(s + 4);
                 }
-                const int st = pos.stage, slot = slots.x + s * kTcDepth;
-                const bool last = slot + kTcDepth > slots.y;
-                // every use of a stage is waited for, also where nothing is loaded: a parity tells neighbouring uses apart only
+                const int st = pos.stage;
                 mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                 __syncwarp();
                 const uint32_t dst = ring + st * S::kStage + (warp - 8) * 8 * 128, bar = full0 + st * 8;
-                if (gather || last) {
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int from = which * 8 + 4 * q;
-                        const int r0 = __shfl_sync(0xffffffffu, now, from), r1 = __shfl_sync(0xffffffffu, now, from + 1);
-                        const int r2 = __shfl_sync(0xffffffffu, now, from + 2), r3 = __shfl_sync(0xffffffffu, now, from + 3);
-                        if (elect_one()) {
-                            tma_rows<PAIRED>(dst + q * 512, &a.p_rows, f0, r0, r1, r2, r3, bar);
-                            if (p_blocks > 1) tma_rows<PAIRED>(dst + kBlock64 + q * 512, &a.p_rows, f0 + 64, r0, r1, r2, r3, bar);
-                        }
-                    }
-                }
-                if (last) {
-                    for (int q = 0; q < 2; ++q) {
-                        const int first = slot + (warp - 8) * 8 + 4 * q;
-                        for (int b = 0; b < q_blocks; ++b) {
-                            const int plane = a.pair ? b * a.n_slots : 0;
-                            auto line = [&](int i) { return first + i < slots.y ? plane + first + i : q_end; };
-                            if (elect_one())
-                                tma_rows<PAIRED>(dst + (2 + b) * kBlock64 + q * 512, &a.q_rows, a.pair ? c0 : q0 + b * 64, line(0), line(1), line(2), line(3), bar);
-                        }
+                for (int q = 0; q < 2; ++q) {
+                    const int from = which * 8 + 4 * q;
+                    const int r0 = __shfl_sync(0xffffffffu, now, from), r1 = __shfl_sync(0xffffffffu, now, from + 1);
+                    const int r2 = __shfl_sync(0xffffffffu, now, from + 2), r3 = __shfl_sync(0xffffffffu, now, from + 3);
+                    if (elect_one()) {
+                        tma_rows<PAIRED>(dst + q * 512, &a.p_rows, f0, r0, r1, r2, r3, bar);
+                        if (p_blocks > 1) tma_rows<PAIRED>(dst + kBlock64 + q * 512, &a.p_rows, f0 + 64, r0, r1, r2, r3, bar);
                     }
                 }
             }
-        } else if (warp >= 4) {
+        } else if (warp >= 4 && warp < 8) {
             if (split > 1) mbar_wait(smem_addr(&pipe.freed), (turn & 1) ^ 1, gave_up, a.status);
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
             tc_fence_after();
@@ -800,6 +827,40 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             const bool none = s0 == s1;
             const bool on_16 = ((uintptr_t)a.out & 15) == 0;
             const bool wide = a.out_f == 1 && a.i % 8 == 0 && on_16, own_rows = a.out_c == 1 && a.j % 8 == 0 && on_16;  // rows of features / of columns
+            if (wide && split == 1) {
+#pragma unroll 1
+                for (int c = 0; c < cols && c0 + c < a.j; c += 64) {
+                    float v[2][32] = {};
+                    if (!none) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) tmem_start(lanes + c + 32 * h, v[h]);
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) tmem_wait(v[h]);
+                        if (a.pair) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                float w[32];
+                                tmem_load(lanes + cols + c + 32 * h, w);
+#pragma unroll
+                                for (int x = 0; x < 32; ++x) v[h][x] += w[x];
+                            }
+                        }
+                    }
+                    results_sync();  // the rows before these have been read
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        if (a.bf16) spread_column<true>(v[h], staging + h * 32 * kOutPitch + feature * 2);
+                        else spread_column<false>(v[h], staging + h * 32 * kOutPitch + feature * 2);
+                    }
+                    results_sync();
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const int cc = (mine >> 4) + 8 * x, fc = (mine & 15) * 8;
+                        const uint4 q = load_shared_128(staging + cc * kOutPitch + fc * 2);
+                        if (c0 + c + cc < a.j && f0 + fc < a.i) *reinterpret_cast<uint4 *>(out + (c0 + c + cc) * a.out_c + f0 + fc) = q;
+                    }
+                }
+            } else
 #pragma unroll 1
             for (int c = 0; c < cols && c0 + c < a.j; c += 32) {
                 float v[32] = {};
@@ -815,17 +876,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 if (split > 1) {
 #pragma unroll
                     for (int x = 0; x < 32; x += 8) meeting.give(c + x, feature, v + x, false);
-                } else if (wide) {
-                    const uint32_t at = staging + (c >> 5 & 1) * (32 * kOutPitch);
-                    if (a.bf16) spread_column<true>(v, at + feature * 2);
-                    else spread_column<false>(v, at + feature * 2);
-                    results_sync();
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const int cc = (mine >> 4) + 8 * x, fc = (mine & 15) * 8;
-                        const uint4 q = load_shared_128(at + cc * kOutPitch + fc * 2);
-                        if (c0 + c + cc < a.j && f0 + fc < a.i) *reinterpret_cast<uint4 *>(out + (c0 + c + cc) * a.out_c + f0 + fc) = q;
-                    }
                 } else if (own_rows) {
 #pragma unroll
                     for (int x = 0; x < 32; x += 8) {
@@ -851,7 +901,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     if (f < a.i) out[f * a.out_f + (c0 + first + c) * a.out_c] = to_16(v, a.bf16);
                 }
                 tell_cluster(smem_addr(&pipe.freed), split, lane);
-            } else if (wide) results_sync();
+            }
         }
     }
     if (*gave_up) __nanosleep(1000000);

@@ -163,8 +163,8 @@ __device__ __forceinline__ uint32_t mma_desc(bool bf16, bool a_mn, bool b_mn, in
     return 1u << 4 | (uint32_t)bf16 << 7 | (uint32_t)bf16 << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
 
-// 32 consecutive columns of the calling warp's 32 TMEM lanes, one lane per thread
-__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+// 32 consecutive columns of the calling warp's 32 TMEM lanes, one lane per thread; there after tmem_wait
+__device__ __forceinline__ void tmem_start(uint32_t addr, float (&v)[32]) {
     uint32_t r[32];
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, "
@@ -173,9 +173,18 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
           "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
           "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+// The values pass through the wait, so that nothing uses them before it.
+__device__ __forceinline__ void tmem_wait(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
+}
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32]) {
+    tmem_start(addr, v);
+    tmem_wait(v);
 }
 
 __device__ __forceinline__ uint16_t to_16(float v, bool bf16) {
