@@ -43,17 +43,65 @@ bool known(int dtype) { return dtype == MPS_F32 || dtype == MPS_F16 || dtype == 
 
 // ---------------------------------------------------------------------------------------------- combine
 
-// y[t] = sum over j of weight[t, j] * rows[slot[t, j]].  Moves bytes only: a thread owns 16 bytes of a row of y (one element
-// where the row's pitch or a pointer is not a multiple of 16 bytes) and keeps the loads of all of the row's terms in flight.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) combine_kernel(int n_rows, int per_row, int n_slots, int dim, const int *__restrict__ slot_of,
+// 16 bytes of elements from any element's address p inside [lo, hi).  Where p is not on a 16-byte boundary two aligned loads are
+// shifted into place; at the edges of the buffer, where those would reach outside, the elements come one by one.
+template <typename T>
+__device__ __forceinline__ mps::Pack<T> load_any(const T *p, const T *lo, const T *hi) {
+    const uintptr_t at = (uintptr_t)p, m = at & 15, q = at - m;
+    mps::Pack<T> out;
+    if (m == 0) return *reinterpret_cast<const mps::Pack<T> *>(p);
+    if (q < (uintptr_t)lo || q + 32 > (uintptr_t)hi) {
+#pragma unroll
+        for (int i = 0; i < mps::Pack<T>::N; ++i) out.v[i] = p[i];
+        return out;
+    }
+    const uint4 x = *reinterpret_cast<const uint4 *>(q), y = *reinterpret_cast<const uint4 *>(q + 16);
+    uint32_t a[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+#pragma unroll
+    for (int i = 0; i < 6; ++i) a[i] = m & 8 ? a[i + 2] : a[i];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) a[i] = m & 4 ? a[i + 1] : a[i];
+    uint32_t *o = reinterpret_cast<uint32_t *>(&out);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = m & 2 ? __funnelshift_r(a[i], a[i + 1], 16) : a[i];
+    return out;
+}
+
+// A row of `dim` elements from dst in pieces: piece 0 up to dst's first 16-byte boundary, then whole 16 bytes, then what is left.
+template <typename T>
+struct Pieces {
+    static constexpr int N = mps::Pack<T>::N;
+    int head, dim;
+    __device__ __forceinline__ Pieces(const T *dst, int dim_) : head((int)((16 - ((uintptr_t)dst & 15)) & 15) / (int)sizeof(T)), dim(dim_) {}
+    __device__ __forceinline__ int start(int piece) const { return piece ? head + (piece - 1) * N : 0; }
+    __device__ __forceinline__ int count(int piece) const { return min(piece ? N : head, dim - start(piece)); }
+};
+// as many as any row can have
+template <typename T>
+int most_pieces(int dim, bool aligned) { return (dim + mps::Pack<T>::N - 1) / mps::Pack<T>::N + (aligned ? 0 : 1); }
+
+// y[t] = sum over j of weight[t, j] * rows[slot[t, j]].  Moves bytes only: a thread owns 16 bytes of a row of y and keeps the loads
+// of several of the row's terms in flight.  ALIGNED: every row starts on a 16-byte boundary; else the pieces lie on those of y
+// and the terms are shifted (14,210 rows of 8 terms of 549 fp16: ANY_US us, 139 element by element).
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256) combine_kernel(int n_rows, int per_row, int n_slots, int dim, int pieces, const int *__restrict__ slot_of,
                                                       const float *__restrict__ weights, const T *__restrict__ rows, T *__restrict__ y, int *status) {
     // blockIdx.x: rows (as many as fill 256 threads), blockIdx.y: stretches of a long row
-    const int per = dim / VEC, rows_here = per < 256 ? 256 / per : 1, local = per < 256 ? (int)threadIdx.x / per : 0;
-    const int c = ((int)threadIdx.x - local * per + (int)blockIdx.y * 256) * VEC;
-    if (local >= rows_here || c >= dim) return;
+    constexpr int N = mps::Pack<T>::N;
+    const int rows_here = pieces < 256 ? 256 / pieces : 1, local = pieces < 256 ? (int)threadIdx.x / pieces : 0;
+    const int piece = (int)threadIdx.x - local * pieces + (int)blockIdx.y * 256;
+    if (local >= rows_here || piece >= pieces) return;
+    const T *end = rows + (long long)n_slots * dim;
     for (long long t = (long long)blockIdx.x * rows_here + local; t < n_rows; t += (long long)gridDim.x * rows_here) {
-        float acc[VEC] = {};
+        T *dst = y + t * dim;
+        int from = piece * N, n = N;
+        if (!ALIGNED) {
+            const Pieces<T> p(dst, dim);
+            from = p.start(piece);
+            n = p.count(piece);
+            if (n <= 0) continue;
+        }
+        float acc[N] = {};
 #pragma unroll 4
         for (int j = 0; j < per_row; ++j) {
             const int s = slot_of[t * per_row + j];
@@ -63,29 +111,37 @@ __global__ void __launch_bounds__(256) combine_kernel(int n_rows, int per_row, i
                 continue;
             }
             const float w = weights ? weights[t * per_row + j] : 1.0f;
-            const T *src = rows + (long long)s * dim + c;
-            if constexpr (VEC > 1) {
-                const mps::Pack<T> p = *reinterpret_cast<const mps::Pack<T> *>(src);
+            const T *src = rows + (long long)s * dim + from;
+            if (ALIGNED || n == N) {
+                const mps::Pack<T> p = ALIGNED ? *reinterpret_cast<const mps::Pack<T> *>(src) : load_any(src, rows, end);
 #pragma unroll
-                for (int v = 0; v < VEC; ++v) acc[v] = fmaf(w, mps::to_f32(p.v[v]), acc[v]);
-            } else acc[0] = fmaf(w, mps::to_f32(*src), acc[0]);
+                for (int v = 0; v < N; ++v) acc[v] = fmaf(w, mps::to_f32(p.v[v]), acc[v]);
+            } else {
+#pragma unroll
+                for (int v = 0; v < N; ++v)
+                    if (v < n) acc[v] = fmaf(w, mps::to_f32(src[v]), acc[v]);
+            }
         }
-        if constexpr (VEC > 1) {
-            mps::Pack<T> p;
+        mps::Pack<T> p;
 #pragma unroll
-            for (int v = 0; v < VEC; ++v) p.v[v] = mps::from_f32<T>(acc[v]);
-            *reinterpret_cast<mps::Pack<T> *>(y + t * dim + c) = p;
-        } else y[t * dim + c] = mps::from_f32<T>(acc[0]);
+        for (int v = 0; v < N; ++v) p.v[v] = mps::from_f32<T>(acc[v]);
+        if (ALIGNED || n == N) *reinterpret_cast<mps::Pack<T> *>(dst + from) = p;
+        else
+#pragma unroll
+            for (int v = 0; v < N; ++v)
+                if (v < n) dst[from + v] = p.v[v];
     }
 }
 
 // d_rows[slot[t, j]] = weight[t, j] * dy[t] and d_weights[t, j] = <dy[t], rows[slot[t, j]]>, one warp per (t, j): rows is read
-// and d_rows written once, the repeated reads of dy[t] meet the cache.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) combine_backward_kernel(int n_rows, int per_row, int n_slots, int dim, const int *__restrict__ slot_of,
+// and d_rows written once, the repeated reads of dy[t] meet the cache.  ALIGNED as above, the pieces on d_rows' boundaries.
+template <typename T, bool ALIGNED>
+__global__ void __launch_bounds__(256) combine_backward_kernel(int n_rows, int per_row, int n_slots, int dim, int pieces, const int *__restrict__ slot_of,
                                                                const float *__restrict__ weights, const T *__restrict__ dy, const T *__restrict__ rows,
                                                                T *__restrict__ d_rows, float *__restrict__ d_weights, int *status) {
+    constexpr int N = mps::Pack<T>::N;
     const int lane = threadIdx.x & 31;
+    const T *end = rows + (long long)n_slots * dim, *dy_end = dy + (long long)n_rows * dim;
     for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < (long long)n_rows * per_row; i += (long long)gridDim.x * 8) {
         const long long t = i / per_row;
         int s = slot_of[i];
@@ -98,23 +154,27 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(int n_rows, int p
             const float w = weights ? weights[i] : 1.0f;
             const T *g = dy + t * dim, *src = rows + (long long)s * dim;
             T *dst = d_rows + (long long)s * dim;
+            const Pieces<T> cut(dst, dim);
 #pragma unroll 4
-            for (int c = lane * VEC; c < dim; c += 32 * VEC) {
-                if constexpr (VEC > 1) {
-                    const mps::Pack<T> p = *reinterpret_cast<const mps::Pack<T> *>(g + c);
+            for (int piece = lane; piece < pieces; piece += 32) {
+                const int from = ALIGNED ? piece * N : cut.start(piece), n = ALIGNED ? N : cut.count(piece);
+                if (ALIGNED || n == N) {
+                    const mps::Pack<T> p = ALIGNED ? *reinterpret_cast<const mps::Pack<T> *>(g + from) : load_any(g + from, dy, dy_end);
                     mps::Pack<T> q = {}, o;
-                    if (d_weights) q = *reinterpret_cast<const mps::Pack<T> *>(src + c);
+                    if (d_weights) q = ALIGNED ? *reinterpret_cast<const mps::Pack<T> *>(src + from) : load_any(src + from, rows, end);
 #pragma unroll
-                    for (int v = 0; v < VEC; ++v) {
+                    for (int v = 0; v < N; ++v) {
                         const float d = mps::to_f32(p.v[v]);
                         dot = fmaf(d, mps::to_f32(q.v[v]), dot);
                         o.v[v] = mps::from_f32<T>(w * d);
                     }
-                    *reinterpret_cast<mps::Pack<T> *>(dst + c) = o;
+                    *reinterpret_cast<mps::Pack<T> *>(dst + from) = o;
                 } else {
-                    const float d = mps::to_f32(g[c]);
-                    if (d_weights) dot = fmaf(d, mps::to_f32(src[c]), dot);
-                    dst[c] = mps::from_f32<T>(w * d);
+                    for (int v = 0; v < n; ++v) {
+                        const float d = mps::to_f32(g[from + v]);
+                        if (d_weights) dot = fmaf(d, mps::to_f32(src[from + v]), dot);
+                        dst[from + v] = mps::from_f32<T>(w * d);
+                    }
                 }
             }
         }
@@ -130,13 +190,12 @@ template <typename T>
 int launch_combine(int n_rows, int per_row, int n_slots, int dim, const int *slot_of, const float *weights, const void *rows, void *y, cudaStream_t st) {
     int *status;
     if (int rc = status_pointer(&status)) return rc;
-    constexpr int VEC = mps::Pack<T>::N;
-    const bool wide = dim % VEC == 0 && !misaligned(rows, 16) && !misaligned(y, 16);
-    const int per = wide ? dim / VEC : dim, rows_here = per < 256 ? 256 / per : 1;
+    const bool aligned = dim % mps::Pack<T>::N == 0 && !misaligned(rows, 16) && !misaligned(y, 16);
+    const int pieces = most_pieces<T>(dim, aligned), rows_here = pieces < 256 ? 256 / pieces : 1;
     const long long blocks = ((long long)n_rows + rows_here - 1) / rows_here;
-    const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20), (unsigned)((per + 255) / 256));
-    if (wide) combine_kernel<T, VEC><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)rows, (T *)y, status);
-    else combine_kernel<T, 1><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)rows, (T *)y, status);
+    const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20), (unsigned)((pieces + 255) / 256));
+    if (aligned) combine_kernel<T, true><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, pieces, slot_of, weights, (const T *)rows, (T *)y, status);
+    else combine_kernel<T, false><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, pieces, slot_of, weights, (const T *)rows, (T *)y, status);
     RD_CUDA(cudaGetLastError());
     return MPS_OK;
 }
@@ -146,16 +205,16 @@ int launch_combine_backward(int n_rows, int per_row, int n_slots, int dim, const
                             void *d_rows, float *d_weights, cudaStream_t st) {
     int *status;
     if (int rc = status_pointer(&status)) return rc;
-    constexpr int VEC = mps::Pack<T>::N;
-    const bool wide = dim % VEC == 0 && !misaligned(rows, 16) && !misaligned(dy, 16) && !misaligned(d_rows, 16);
+    const bool aligned = dim % mps::Pack<T>::N == 0 && !misaligned(rows, 16) && !misaligned(dy, 16) && !misaligned(d_rows, 16);
+    const int pieces = most_pieces<T>(dim, aligned);
     const long long blocks = ((long long)n_rows * per_row + 7) / 8;
     const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20);
-    if (wide)
-        combine_backward_kernel<T, VEC><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)dy, (const T *)rows, (T *)d_rows,
-                                                              d_weights, status);
+    if (aligned)
+        combine_backward_kernel<T, true><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, pieces, slot_of, weights, (const T *)dy, (const T *)rows,
+                                                               (T *)d_rows, d_weights, status);
     else
-        combine_backward_kernel<T, 1><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, slot_of, weights, (const T *)dy, (const T *)rows, (T *)d_rows,
-                                                            d_weights, status);
+        combine_backward_kernel<T, false><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, pieces, slot_of, weights, (const T *)dy, (const T *)rows,
+                                                                (T *)d_rows, d_weights, status);
     RD_CUDA(cudaGetLastError());
     return MPS_OK;
 }

@@ -827,23 +827,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             const bool none = s0 == s1;
             const bool on_16 = ((uintptr_t)a.out & 15) == 0;
             const bool wide = a.out_f == 1 && a.i % 8 == 0 && on_16, own_rows = a.out_c == 1 && a.j % 8 == 0 && on_16;  // rows of features / of columns
-            if (wide && split == 1) {
+            if (wide && split == 1 && none) {  // a group without slots
+                const int fc = (mine & 15) * 8;
+                for (int c = mine >> 4; c < cols && c0 + c < a.j; c += 8)
+                    if (f0 + fc < a.i) *reinterpret_cast<uint4 *>(out + (c0 + c) * a.out_c + f0 + fc) = make_uint4(0, 0, 0, 0);
+            } else if (wide && split == 1) {
 #pragma unroll 1
                 for (int c = 0; c < cols && c0 + c < a.j; c += 64) {
-                    float v[2][32] = {};
-                    if (!none) {
+                    float v[2][32];
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) tmem_start(lanes + c + 32 * h, v[h]);
+                    for (int h = 0; h < 2; ++h) tmem_start(lanes + c + 32 * h, v[h]);
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) tmem_wait(v[h]);
-                        if (a.pair) {
+                    for (int h = 0; h < 2; ++h) tmem_wait(v[h]);
+                    if (a.pair) {
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                float w[32];
-                                tmem_load(lanes + cols + c + 32 * h, w);
+                        for (int h = 0; h < 2; ++h) {
+                            float w[32];
+                            tmem_load(lanes + cols + c + 32 * h, w);
 #pragma unroll
-                                for (int x = 0; x < 32; ++x) v[h][x] += w[x];
-                            }
+                            for (int x = 0; x < 32; ++x) v[h][x] += w[x];
                         }
                     }
                     results_sync();  // the rows before these have been read

@@ -368,7 +368,7 @@ def test_product_offsets_beyond_31_bits(mps, cuda):
 # ---------------------------------------------------------------------------------------------- combine
 
 @pytest.mark.parametrize("dtype", [F32, F16, BF16])
-@pytest.mark.parametrize("rows,per,dim", [(1, 1, 1), (1, 8, 2048), (70, 2, 40), (33, 3, 37), (5, 5, 1000), (300, 1, 8), (9, 33, 264)])
+@pytest.mark.parametrize("rows,per,dim", [(1, 1, 1), (1, 8, 2048), (40, 8, 549), (3, 2, 4099), (21, 2, 7), (70, 2, 40), (33, 3, 37), (5, 5, 1000), (300, 1, 8), (9, 33, 264)])
 def test_combine_and_gradients(mps, cuda, dtype, rows, per, dim):
     rng, gen = np.random.default_rng(rows + dim), gen_of(dim)
     slots = rows * per + 3
