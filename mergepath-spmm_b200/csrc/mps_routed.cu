@@ -82,7 +82,7 @@ int most_pieces(int dim, bool aligned) { return (dim + mps::Pack<T>::N - 1) / mp
 
 // y[t] = sum over j of weight[t, j] * rows[slot[t, j]].  Moves bytes only: a thread owns 16 bytes of a row of y and keeps the loads
 // of several of the row's terms in flight.  ALIGNED: every row starts on a 16-byte boundary; else the pieces lie on those of y
-// and the terms are shifted (14,210 rows of 8 terms of 549 fp16: ANY_US us, 139 element by element).
+// and the terms are shifted (14,210 rows of 8 terms of 549 fp16: 61 us, 139 element by element).
 template <typename T, bool ALIGNED>
 __global__ void __launch_bounds__(256) combine_kernel(int n_rows, int per_row, int n_slots, int dim, int pieces, const int *__restrict__ slot_of,
                                                       const float *__restrict__ weights, const T *__restrict__ rows, T *__restrict__ y, int *status) {
@@ -133,18 +133,21 @@ __global__ void __launch_bounds__(256) combine_kernel(int n_rows, int per_row, i
     }
 }
 
-// d_rows[slot[t, j]] = weight[t, j] * dy[t] and d_weights[t, j] = <dy[t], rows[slot[t, j]]>, one warp per (t, j): rows is read
-// and d_rows written once, the repeated reads of dy[t] meet the cache.  ALIGNED as above, the pieces on d_rows' boundaries.
+// d_rows[slot[t, j]] = weight[t, j] * dy[t] and d_weights[t, j] = <dy[t], rows[slot[t, j]]>, `lanes` lanes (a power of two, as many
+// as a row has pieces, 32 at most) per (t, j): rows is read and d_rows written once, the repeated reads of dy[t] meet the cache.
+// ALIGNED as above, the pieces on d_rows' boundaries.
 template <typename T, bool ALIGNED>
-__global__ void __launch_bounds__(256) combine_backward_kernel(int n_rows, int per_row, int n_slots, int dim, int pieces, const int *__restrict__ slot_of,
-                                                               const float *__restrict__ weights, const T *__restrict__ dy, const T *__restrict__ rows,
-                                                               T *__restrict__ d_rows, float *__restrict__ d_weights, int *status) {
+__global__ void __launch_bounds__(256) combine_backward_kernel(int n_rows, int per_row, int n_slots, int dim, int pieces, int lanes,
+                                                               const int *__restrict__ slot_of, const float *__restrict__ weights, const T *__restrict__ dy,
+                                                               const T *__restrict__ rows, T *__restrict__ d_rows, float *__restrict__ d_weights, int *status) {
     constexpr int N = mps::Pack<T>::N;
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & (lanes - 1), per_warp = 32 / lanes;
     const T *end = rows + (long long)n_slots * dim, *dy_end = dy + (long long)n_rows * dim;
-    for (long long i = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); i < (long long)n_rows * per_row; i += (long long)gridDim.x * 8) {
-        const long long t = i / per_row;
-        int s = slot_of[i];
+    const long long pairs = (long long)n_rows * per_row;
+    // the lanes of a warp stay together for the sums: whole warps of pairs, some of them behind the last
+    for (long long i0 = ((long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * per_warp; i0 < pairs; i0 += (long long)gridDim.x * 8 * per_warp) {
+        const long long i = i0 + (threadIdx.x & 31) / lanes, t = i / per_row;
+        int s = i < pairs ? slot_of[i] : -1;
         if (s >= n_slots) {
             if (lane == 0) atomicOr(status, mps::kStatusBadIndex);
             s = -1;
@@ -156,7 +159,7 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(int n_rows, int p
             T *dst = d_rows + (long long)s * dim;
             const Pieces<T> cut(dst, dim);
 #pragma unroll 4
-            for (int piece = lane; piece < pieces; piece += 32) {
+            for (int piece = lane; piece < pieces; piece += lanes) {
                 const int from = ALIGNED ? piece * N : cut.start(piece), n = ALIGNED ? N : cut.count(piece);
                 if (ALIGNED || n == N) {
                     const mps::Pack<T> p = ALIGNED ? *reinterpret_cast<const mps::Pack<T> *>(g + from) : load_any(g + from, dy, dy_end);
@@ -179,9 +182,8 @@ __global__ void __launch_bounds__(256) combine_backward_kernel(int n_rows, int p
             }
         }
         if (d_weights) {
-#pragma unroll
-            for (int d = 16; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-            if (lane == 0) d_weights[i] = dot;
+            for (int d = lanes >> 1; d; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+            if (lane == 0 && i < pairs) d_weights[i] = dot;
         }
     }
 }
@@ -207,13 +209,15 @@ int launch_combine_backward(int n_rows, int per_row, int n_slots, int dim, const
     if (int rc = status_pointer(&status)) return rc;
     const bool aligned = dim % mps::Pack<T>::N == 0 && !misaligned(rows, 16) && !misaligned(dy, 16) && !misaligned(d_rows, 16);
     const int pieces = most_pieces<T>(dim, aligned);
-    const long long blocks = ((long long)n_rows * per_row + 7) / 8;
+    int lanes = 4;
+    while (lanes < 32 && lanes < pieces) lanes *= 2;
+    const long long blocks = ((long long)n_rows * per_row + 8 * (32 / lanes) - 1) / (8 * (32 / lanes));
     const unsigned grid = (unsigned)(blocks < (1 << 20) ? blocks : 1 << 20);
     if (aligned)
-        combine_backward_kernel<T, true><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, pieces, slot_of, weights, (const T *)dy, (const T *)rows,
+        combine_backward_kernel<T, true><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, pieces, lanes, slot_of, weights, (const T *)dy, (const T *)rows,
                                                                (T *)d_rows, d_weights, status);
     else
-        combine_backward_kernel<T, false><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, pieces, slot_of, weights, (const T *)dy, (const T *)rows,
+        combine_backward_kernel<T, false><<<grid, 256, 0, st>>>(n_rows, per_row, n_slots, dim, pieces, lanes, slot_of, weights, (const T *)dy, (const T *)rows,
                                                                 (T *)d_rows, d_weights, status);
     RD_CUDA(cudaGetLastError());
     return MPS_OK;
