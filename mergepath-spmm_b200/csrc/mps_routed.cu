@@ -339,7 +339,7 @@ Cut best_cut(int slots, int groups, int features, int steps, bool gather, int sm
         const double step = std::fmax(std::fmax(330.0, std::fmax(2.0 * nt + 20, bytes / 64)), gather ? 4.3 * loaded : 0.0);
         for (int split = 1; split <= (nt <= 64 ? nt / 8 : 1); split *= 2) {  // a block adds up eight columns at least
             if (split > 1 && steps < 2 * split) break;  // two slices each at least
-            const double waves = std::ceil(tiles / (sms / (paired ? 2 : split)) - 0.05);
+            const double waves = std::fmax(1.0, std::ceil(tiles / (sms / (paired ? 2 : split)) - 0.05));
             const double cycles = waves * (std::ceil((double)steps / split) * step + (split > 1 ? 2500 : 1500));
             if (cycles < best.cycles) best = {nt, split, cycles};
         }
