@@ -349,16 +349,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     // columns of a tile's products: only as many as there are slots, so that the last tile of a group costs what it holds
     auto columns_of = [](const TcCursor &c) { return PAIRED ? (c.slot1 - c.slot0 + 31) & ~31 : (c.slot1 - c.slot0 + 15) & ~15; };
 
-    // gathered rows: a warp loads an eighth of a slice's, a lane holding one row's number
+    // gathered rows: a warp loads an eighth of a slice's, a lane holding one row's number.  Of a group's last tile only as many as
+    // its products read, four at least (each warp has to load into every stage): a short tile's loads would take as long as a
+    // whole one's.
     constexpr int RPW = S::kRows / 8;
+    auto rows_per_warp = [&](int columns) { return min(RPW, ((PAIRED ? columns / 2 : columns) + 31) / 32 * 4); };
     int row = 0, next_row = 0;
     TcCursor ahead = cur;
     auto fetch_rows = [&](const TileWalk &w) {
         next_row = a.n_x_rows;  // out of range: zeros
         if (!w.more()) return;
         ahead.seek(w.tile, NT);
-        const int at = (warp - 8) * RPW + lane, slot = ahead.slot0 + half * columns_of(ahead) / 2 + at;
-        if (lane < RPW && slot < ahead.slot1 && (!PAIRED || at < columns_of(ahead) / 2)) {
+        const int columns = columns_of(ahead), mine = rows_per_warp(columns);
+        const int at = (warp - 8) * mine + lane, slot = ahead.slot0 + half * columns / 2 + at;
+        if (lane < mine && slot < ahead.slot1 && (!PAIRED || at < columns / 2)) {
             const int r = a.slot_row[slot];
             if ((unsigned)r < (unsigned)a.n_x_rows) next_row = r;
             else atomicOr(a.status, kStatusBadIndex);
@@ -382,10 +386,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 const int z = a.w_shared ? 0 : g;
                 const int halves = PAIRED || a.n - f0 > 64 ? 2 : 1;  // MN-major: boxes of 64 features (as many in both blocks)
                 const uint32_t w_bytes = a.mn_major ? halves * kBlock64 : a.w_rows * 128u, own = slot0 + half * columns / 2;
+                const uint32_t x_bytes = a.gather ? rows_per_warp(columns) * 1024u : S::kRows * 128u;
                 for (int s = s0; s < s1; s += S::kSlices, pos.next(stages)) {
                     mbar_wait(smem_addr(&pipe.empty[pos.stage]), pos.parity ^ 1, gave_up, a.status);
                     const uint32_t bar = full0 + pos.stage * 8;
-                    if (half == 0) mbar_expect(bar, min(S::kSlices, s1 - s) * (PAIRED ? 2 : 1) * (w_bytes + S::kRows * 128u));
+                    if (half == 0) {
+                        uint32_t bytes = 0;
+#pragma unroll
+                        for (int d = 0; d < S::kSlices; ++d)
+                            if (s + d < s1) bytes += w_bytes + (s + d < main_steps ? x_bytes : S::kRows * 128u);
+                        mbar_expect(bar, (PAIRED ? 2 : 1) * bytes);
+                    }
 #pragma unroll
                     for (int d = 0; d < S::kSlices; ++d) {
                         if (d > 0 && s + d >= s1) break;
@@ -425,7 +436,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             row = next_row;
             // neighbouring rows in order (a request's, listed by adapter) come as one box
             const int row0 = __shfl_sync(0xffffffffu, row, 0);
-            const bool run = __all_sync(0xffffffffu, lane >= RPW || row == row0 + lane);
+            const int n_rows = rows_per_warp(columns);
+            const bool run = n_rows == RPW && __all_sync(0xffffffffu, lane >= RPW || row == row0 + lane);
             TileWalk then = walk;
             then.next();
             fetch_rows(then);  // under way while this tile is loaded
@@ -435,22 +447,23 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
 #pragma unroll
                 for (int d = 0; d < S::kSlices; ++d) {
                     if (s + d >= s1) break;
-                    const uint32_t dst = ring + pos.stage * S::kStage + d * S::kSlice + kTcFeatures * 128 + (warp - 8) * RPW * 128, bar = full0 + pos.stage * 8;
+                    const uint32_t rows = ring + pos.stage * S::kStage + d * S::kSlice + kTcFeatures * 128, bar = full0 + pos.stage * 8;
                     const int e = s + d - main_steps;
                     if (e >= 0) {  // rows of the second product, in slot order
                         const int line = (e & 1) * a.u_plane + slot0 + half * columns / 2 + (warp - 8) * RPW;
-                        if (elect_one()) tma_2d<PAIRED>(dst, &a.u, (e >> 1) * kTcDepth, line, bar);
+                        if (elect_one()) tma_2d<PAIRED>(rows + (warp - 8) * RPW * 128, &a.u, (e >> 1) * kTcDepth, line, bar);
                         continue;
                     }
                     if (run) {
-                        if (elect_one()) tma_2d<PAIRED>(dst, &a.x_run, (s + d) * kTcDepth, row0, bar);
+                        if (elect_one()) tma_2d<PAIRED>(rows + (warp - 8) * RPW * 128, &a.x_run, (s + d) * kTcDepth, row0, bar);
                         continue;
                     }
 #pragma unroll
                     for (int q = 0; q < RPW / 4; ++q) {
+                        if (4 * q >= n_rows) break;
                         const int r0 = __shfl_sync(0xffffffffu, row, 4 * q), r1 = __shfl_sync(0xffffffffu, row, 4 * q + 1);
                         const int r2 = __shfl_sync(0xffffffffu, row, 4 * q + 2), r3 = __shfl_sync(0xffffffffu, row, 4 * q + 3);
-                        if (elect_one()) tma_rows<PAIRED>(dst + q * 512, &a.x, (s + d) * kTcDepth, r0, r1, r2, r3, bar);
+                        if (elect_one()) tma_rows<PAIRED>(rows + ((warp - 8) * n_rows + 4 * q) * 128, &a.x, (s + d) * kTcDepth, r0, r1, r2, r3, bar);
                     }
                 }
             }
