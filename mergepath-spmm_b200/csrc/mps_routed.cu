@@ -567,8 +567,9 @@ bool by_rows(const AdapterShape &s, int k, int n, bool by_rank, int sms, Cut *cu
 
 // out = x times the shared matrix plus u times the row's adapter matrix m; u_f32 by row (by_rows) or u in planes by slot.
 int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cut, bool rows, int k, int n, const void *x, const void *w, const void *u,
-                    const float *u_f32, const void *m, bool mn_major, void *out, bool ahead, int sms, cudaStream_t st) {
+                    const float *u_f32, const void *m, bool mn_major, void *out, bool ahead, bool next_after, int sms, cudaStream_t st) {
     TcRows a = {};
+    a.next_after = next_after;
     a.bf16 = s.dtype == MPS_BF16;
     a.mn_major = mn_major;
     a.n_slots = a.n_x_rows = s.n_rows;
@@ -611,7 +612,7 @@ TcOuter tc_adapter_outer(const AdapterShape &s, int features, void *out, long lo
     a.n_slots = a.n_p_rows = s.n_rows;
     a.i = features;
     a.j = s.rank;
-    a.pair = a.follows = true;
+    a.pair = a.follows = a.apart = true;  // beside the rows' gradient
     a.out = out;
     a.out_group = (long long)features * s.rank;
     a.out_f = out_f;
@@ -640,7 +641,7 @@ int adapters(const AdapterShape &s, const void *x, const void *w, const void *a,
             narrow.follows = narrow.apart = true;  // beside the listing
             if (int rc = tc_rows(&narrow, 1, best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k), true, sms, 256), &x, s.n_rows, sms, st)) return rc;
         }
-        return tc_adapter_wide(s, ws, cut, rows, s.k, s.n, x, w, ws.u, (const float *)ws.u, b, false, y, rows, sms, st);
+        return tc_adapter_wide(s, ws, cut, rows, s.k, s.n, x, w, ws.u, (const float *)ws.u, b, false, y, rows, false, sms, st);
     }
     float *u = (float *)ws.u;
     if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
@@ -665,7 +666,7 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
         const void *const in[2] = {x, dy};
         const Cut half = best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k > s.n ? s.k : s.n), true, sms / 2, 64);
         if (int rc = tc_rows(narrow, 2, half, in, s.n_rows, sms, st)) return rc;
-        if (int rc = tc_adapter_wide(s, ws, cut, rows, s.n, s.k, dy, w, ws.v, (const float *)ws.v_f32, a, true, dx, false, sms, st)) return rc;
+        if (int rc = tc_adapter_wide(s, ws, cut, rows, s.n, s.k, dy, w, ws.v, (const float *)ws.v_f32, a, true, dx, false, true, sms, st)) return rc;
         const TcOuter outer[2] = {tc_adapter_outer(s, s.k, da, 1, s.k), tc_adapter_outer(s, s.n, db, s.rank, 1)};
         const void *const q[2] = {ws.v, ws.u};
         return tc_outer(outer, 2, in, q, st);

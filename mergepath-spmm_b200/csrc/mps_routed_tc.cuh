@@ -38,6 +38,8 @@ constexpr int kTcDepth = 64;
 constexpr int kTcRing = 192 * 1024;            // shared memory of the stages
 constexpr int kOutPitch = kTcFeatures * 2 + 16;  // a result row in shared memory; the pad spreads 16-byte reads over the banks
 constexpr int kOutBytes = 64 * kOutPitch;        // 64 rows at a time
+constexpr int kF32Pitch = kTcFeatures * 4 + 16;  // 32 rows in fp32
+static_assert(32 * kF32Pitch <= kOutBytes);
 constexpr int kOutTotal = (kOutBytes + 1023) / 1024 * 1024;
 
 struct TcRows {
@@ -63,6 +65,7 @@ struct TcRows {
     long long delta_group, delta_f, delta_r;
     bool ahead;               // only delta_u comes from the launch before this one
     bool apart;               // nothing does: waited for at the end, for the launches behind
+    bool next_after;          // the launch behind starts once the one before has ended (it needs that one's results, not these)
     int split;                // blocks of a cluster, each with its part of the sum (a power of two)
     bool follows;             // the launch before is one of the same call (host side)
     int *status;
@@ -156,6 +159,33 @@ __device__ __forceinline__ void spread_column(const float (&v)[32], uint32_t to)
         store_shared_16(to + j * kOutPitch, (uint16_t)w);
         store_shared_16(to + (j + 1) * kOutPitch, (uint16_t)(w >> 16));
     }
+}
+
+// The same as hi + lo pairs, the lo rows `lo` bytes behind the hi rows.
+template <bool BF16>
+__device__ __forceinline__ void spread_pair(const float (&v)[32], uint32_t to, uint32_t lo) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 2) {
+        const uint32_t w = to_16x2<BF16>(v[j], v[j + 1]);
+        const float2 h = from_16x2<BF16>(w);
+        const uint32_t x = to_16x2<BF16>(v[j] - h.x, v[j + 1] - h.y);
+        store_shared_16(to + j * kOutPitch, (uint16_t)w);
+        store_shared_16(to + (j + 1) * kOutPitch, (uint16_t)(w >> 16));
+        store_shared_16(to + lo + j * kOutPitch, (uint16_t)x);
+        store_shared_16(to + lo + (j + 1) * kOutPitch, (uint16_t)(x >> 16));
+    }
+}
+
+__device__ __forceinline__ uint4 rest_of_16(const float (&v)[8], uint4 hi, bool bf16) {
+    const uint32_t w[4] = {hi.x, hi.y, hi.z, hi.w};
+    float lo[8];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const float2 h = bf16 ? from_16x2<true>(w[j]) : from_16x2<false>(w[j]);
+        lo[2 * j] = v[2 * j] - h.x;
+        lo[2 * j + 1] = v[2 * j + 1] - h.y;
+    }
+    return pack_16(lo, bf16);
 }
 
 // v[j] += <u of column c + j, the feature's row of that column's matrix> over `ranks` (a multiple of eight): u in shared memory (64
@@ -266,12 +296,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     constexpr bool PAIRED = S::kPaired;
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
 
-    let_next_launch_start();
+    if (!a.next_after) let_next_launch_start();
     if (warp == 0 && lane < 5) {
         const CUtensorMap *maps[5] = {&a.w, &a.x, &a.x_run, &a.w2, &a.u};
         if (lane < 2 || (lane == 2 ? a.gather : a.rank > 0)) tma_prefetch(maps[lane]);
     }
     if (!a.ahead && !a.apart) wait_for_launch_before();
+    if (a.next_after) let_next_launch_start();
     // ---- tiles of the groups
     {
         constexpr int PER = (kMaxRowGroups + 1 + kTcThreads - 1) / kTcThreads;  // a list with the ungrouped rows has one group more
@@ -479,16 +510,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             auto store = [&](int slot, float v) {
                 const int r = out_row(slot);
                 if (f >= a.n || r < 0) return;
-                const long long at = (long long)r * a.n + f;
-                const uint16_t h = to_16(v, a.bf16);
-                out[at] = h;
-                if (a.pair) {
-                    out[at + a.out_plane] = to_16(v - from_16(h, a.bf16), a.bf16);
-                    if (a.out_f32) {
-                        const int line = a.slot_row[slot];
-                        if ((unsigned)line < (unsigned)a.n_x_rows) a.out_f32[(long long)line * a.n + f] = v;
-                    }
-                }
+                out[(long long)r * a.n + f] = to_16(v, a.bf16);
+            };
+            // Where rows of results go is read ahead, a lane holding one of the 16 rows (of 64) that its warp stores: a load between
+            // two stores would wait for both.
+            auto line_ahead = [&](int c0) {
+                const int slot = slot0 + c0 + 2 * (warp - 4) + (lane & 1) + 8 * ((lane & 15) >> 1);
+                return slot < slot1 ? out_row(slot) : -1;
             };
             const Meeting meeting = {partial, split, part, NT / split};
             const int feature = quad * 32 + lane;
@@ -554,16 +582,52 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     }
                 }
             }
+            const bool rows_of_16 = a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0, wide = rows_of_16 && !reduce;  // pairs always are
+            int line = wide && !a.pair ? line_ahead(0) : 0;
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
             tc_fence_after();
-            const bool rows_of_16 = !a.pair && a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0, wide = rows_of_16 && !reduce;
             const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT;
-            if (wide) {
+            if (wide && a.pair) {
+#pragma unroll 1
+                for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 32) {
+                    float v[32];
+                    tmem_load(lanes + c0, v);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] *= scale;
+                    results_sync();  // the rows before these have been read
+                    if (a.bf16) spread_pair<true>(v, staging + feature * 2, 32 * kOutPitch);
+                    else spread_pair<false>(v, staging + feature * 2, 32 * kOutPitch);
+                    results_sync();
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const int c = (mine >> 4) + 8 * (j & 3), fc = (mine & 15) * 8;
+                        if (slot0 + c0 + c < slot1 && f0 + fc < a.n)
+                            *reinterpret_cast<uint4 *>(out + (j >> 2) * a.out_plane + (long long)(slot0 + c0 + c) * a.n + f0 + fc) =
+                                load_shared_128(staging + ((j >> 2) * 32 + c) * kOutPitch + fc * 2);
+                    }
+                    if (a.out_f32) {
+                        const int slot = slot0 + c0 + warp - 4 + 4 * (lane & 7);  // of the rows this warp stores
+                        const int at = slot < slot1 ? a.slot_row[slot] : -1;
+                        results_sync();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) store_shared_f32(staging + j * kF32Pitch + feature * 4, v[j]);
+                        results_sync();
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int to = __shfl_sync(0xffffffffu, at, j);
+                            if ((unsigned)to < (unsigned)a.n_x_rows && f0 + lane * 4 < a.n)
+                                *reinterpret_cast<float4 *>(a.out_f32 + (long long)to * a.n + f0 + lane * 4) =
+                                    load_shared_float4(staging + (warp - 4 + 4 * j) * kF32Pitch + lane * 16);
+                        }
+                    }
+                }
+            } else if (wide) {
                 // 64 columns at a time: a result warp is alone on its scheduler, so two loads and 64 roundings in flight take little
                 // more time than half of them
 #pragma unroll 1
                 for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 64) {
                     float v[2][32];
+                    if (c0) line = line_ahead(c0);
                     tmem_start(lanes + c0, v[0]);
                     if (NT > 32) tmem_start(lanes + c0 + 32, v[1]);
                     tmem_wait(v[0]);
@@ -579,10 +643,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     for (int j = 0; j < (NT > 32 ? 8 : 4); ++j) {
                         const int c = (mine >> 4) + 8 * j, fc = (mine & 15) * 8;
                         const uint4 q = load_shared_128(staging + c * kOutPitch + fc * 2);
-                        if (slot0 + c0 + c < slot1 && f0 + fc < a.n) {
-                            const int r = out_row(slot0 + c0 + c);
-                            if (r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = q;
-                        }
+                        const int r = __shfl_sync(0xffffffffu, line, 2 * j + (lane >> 4));
+                        if (r >= 0 && f0 + fc < a.n) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = q;
                     }
                 }
             } else
@@ -597,7 +659,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 } else {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
-                        if (slot0 + c0 + j < slot1) store(slot0 + c0 + j, v[j] * scale);
+                        if (slot0 + c0 + j < slot1) store(slot0 + c0 + j, v[j]);
                 }
             }
             tc_fence_before();
@@ -613,12 +675,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     const int fc = (mine & 15) * 8;
                     for (int c = mine >> 4; c < own; c += 8) {
                         float v[8];
+                        const int slot = slot0 + first + c, r = out_row(slot), by_row = a.out_f32 ? a.slot_row[slot] : -1;
                         meeting.sum8(c, fc, v);
-                        const int r = out_row(slot0 + first + c);
-                        if (f0 + fc < a.n && r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = pack_16(v, a.bf16);
+                        if (a.pair) {
+#pragma unroll
+                            for (int j = 0; j < 8; ++j) v[j] *= scale;
+                        }
+                        if (f0 + fc >= a.n || r < 0) continue;
+                        const uint4 hi = pack_16(v, a.bf16);
+                        uint16_t *to = out + (long long)r * a.n + f0 + fc;
+                        *reinterpret_cast<uint4 *>(to) = hi;
+                        if (a.pair) *reinterpret_cast<uint4 *>(to + a.out_plane) = rest_of_16(v, hi, a.bf16);
+                        if ((unsigned)by_row < (unsigned)a.n_x_rows) {
+                            float4 *line_f32 = reinterpret_cast<float4 *>(a.out_f32 + (long long)by_row * a.n + f0 + fc);
+                            line_f32[0] = make_float4(v[0], v[1], v[2], v[3]);
+                            line_f32[1] = make_float4(v[4], v[5], v[6], v[7]);
+                        }
                     }
                 } else
-                    for (int c = 0; c < own; ++c) store(slot0 + first + c, meeting.sum(c, feature) * scale);
+                    for (int c = 0; c < own; ++c) store(slot0 + first + c, meeting.sum(c, feature));
                 tell_cluster(smem_addr(&pipe.freed), split, lane);
             }
         }
@@ -676,6 +751,7 @@ struct TcOuter {
     long long out_group, out_f, out_c;
     int split;
     bool follows;
+    bool apart;                       // needs nothing of the launch before, which has waited for the one before itself
     int *status;
 };
 
@@ -717,7 +793,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     }
     if (tid == 0) pipe_init(pipe, stages, PAIRED, split);
     if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), 2 * NT);
-    wait_for_launch_before();
+    if (!a.apart) wait_for_launch_before();
     tc_fence_before();
     __syncthreads();
     if (PAIRED || split > 1) cluster_sync();
@@ -919,6 +995,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             }
         }
     }
+    if (a.apart) wait_for_launch_before();
     if (*gave_up) __nanosleep(1000000);
     tc_fence_before();
     __syncthreads();
