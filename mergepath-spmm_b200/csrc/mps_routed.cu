@@ -352,12 +352,14 @@ void share_blocks(int sms, int cluster, const long long (&tiles)[2], const doubl
     const long long clusters = sms / cluster;
     long long first = tiles[1] ? (long long)(clusters * work[0] / (work[0] + work[1]) + 0.5) : clusters;
     if (tiles[1]) first = first < 1 ? 1 : first > clusters - 1 ? clusters - 1 : first;
-    blocks[0] = (tiles[0] < first ? tiles[0] : first) * cluster;
-    blocks[1] = (tiles[1] < clusters - first ? tiles[1] : clusters - first) * cluster;
+    const long long second = tiles[1] < clusters - first ? tiles[1] : clusters - first;  // what one has no use for goes to the other
+    first = tiles[0] < clusters - second ? tiles[0] : clusters - second;
+    blocks[0] = first * cluster;
+    blocks[1] = second * cluster;
 }
 
 template <int NT, bool TWO>
-int launch_tc_rows(const mps::TcRowsLaunch &in, int sms, cudaStream_t st) {
+int launch_tc_rows(const mps::TcRowsLaunch &in, int sms, int *used, cudaStream_t st) {
     mps::TcRowsLaunch l = in;
     const int tile_f = mps::kTcFeatures * (mps::TcShape<NT>::kPaired ? 2 : 1), cluster = mps::TcShape<NT>::kPaired ? 2 : l.p[0].split;
     long long tiles[2] = {}, blocks[2];
@@ -371,11 +373,13 @@ int launch_tc_rows(const mps::TcRowsLaunch &in, int sms, cudaStream_t st) {
     }
     share_blocks(sms, cluster, tiles, work, blocks);
     l.second = (int)blocks[0];
+    if (used) *used = (int)(blocks[0] + blocks[1]);
     return launch_tc<mps::tc_rows_kernel<NT, TWO>>(l, blocks[0] + blocks[1], cluster, mps::TcShape<NT>::bytes(l.p[0].n_groups), l.p[0].follows, st);
 }
 
 // One product, or two of the same groups side by side (at most 64 slots per tile): what every use has in common filled in.  x_rows: rows of each x.
-int tc_rows(const TcRows *products, int n, const Cut &cut, const void *const *x, long long x_rows, int sms, cudaStream_t st) {
+// used (or NULL): the launch's blocks, each with an SM to itself.
+int tc_rows(const TcRows *products, int n, const Cut &cut, const void *const *x, long long x_rows, int sms, cudaStream_t st, int *used = nullptr) {
     mps::TcRowsLaunch l = {};
     const int loaded = cut.nt == 256 ? mps::TcShape<256>::kRows : cut.nt;  // slots a block loads
     for (int i = 0; i < n; ++i) {
@@ -389,11 +393,11 @@ int tc_rows(const TcRows *products, int n, const Cut &cut, const void *const *x,
         if (a.rank)
             if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded / 8)) return rc;
     }
-    if (n == 2) return cut.nt == 32 ? launch_tc_rows<32, true>(l, sms, st) : launch_tc_rows<64, true>(l, sms, st);
-    if (cut.nt == 32) return launch_tc_rows<32, false>(l, sms, st);
-    if (cut.nt == 64) return launch_tc_rows<64, false>(l, sms, st);
-    if (cut.nt == 128) return launch_tc_rows<128, false>(l, sms, st);
-    return launch_tc_rows<256, false>(l, sms, st);
+    if (n == 2) return cut.nt == 32 ? launch_tc_rows<32, true>(l, sms, used, st) : launch_tc_rows<64, true>(l, sms, used, st);
+    if (cut.nt == 32) return launch_tc_rows<32, false>(l, sms, used, st);
+    if (cut.nt == 64) return launch_tc_rows<64, false>(l, sms, used, st);
+    if (cut.nt == 128) return launch_tc_rows<128, false>(l, sms, used, st);
+    return launch_tc_rows<256, false>(l, sms, used, st);
 }
 
 // The matrices of a: stored features x summed (MN-major: summed x features), `groups` of them.
@@ -426,10 +430,8 @@ int launch_tc_outer(const mps::TcOuterLaunch &in, int sms, cudaStream_t st) {
 
 // One gradient by the matrices, or two of the same groups side by side (of pairs of planes).  P: n_p_rows rows of a.i, by a.slot_row or in slot order;
 // Q: rows of a.j in slot order (pair: two planes of them).
-int tc_outer(const TcOuter *products, int n, const void *const *p, const void *const *q, cudaStream_t st) {
+int tc_outer(const TcOuter *products, int n, const void *const *p, const void *const *q, int sms, cudaStream_t st) {
     mps::TcOuterLaunch l = {};
-    int sms;
-    if (int rc = sm_count(&sms)) return rc;
     for (int i = 0; i < n; ++i) {
         TcOuter &a = l.p[i];
         a = products[i];
@@ -565,11 +567,12 @@ bool by_rows(const AdapterShape &s, int k, int n, bool by_rank, int sms, Cut *cu
     return rows.cycles + low_rank < grouped.cycles;
 }
 
-// out = x times the shared matrix plus u times the row's adapter matrix m; u_f32 by row (by_rows) or u in planes by slot.
+// out = x times the shared matrix plus u times the row's adapter matrix m; u_f32 by row (by_rows) or u in planes by slot.  used
+// (or NULL): its blocks, where the launch behind it needs nothing of it and runs beside it.
 int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cut, bool rows, int k, int n, const void *x, const void *w, const void *u,
-                    const float *u_f32, const void *m, bool mn_major, void *out, bool ahead, bool next_after, int sms, cudaStream_t st) {
+                    const float *u_f32, const void *m, bool mn_major, void *out, bool ahead, int sms, cudaStream_t st, int *used = nullptr) {
     TcRows a = {};
-    a.next_after = next_after;
+    a.next_after = used != nullptr;
     a.bf16 = s.dtype == MPS_BF16;
     a.mn_major = mn_major;
     a.n_slots = a.n_x_rows = s.n_rows;
@@ -589,7 +592,7 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cu
         a.delta_f = mn_major ? 1 : s.rank;
         a.delta_r = mn_major ? n : 1;
         a.ahead = ahead;
-        return tc_rows(&a, 1, cut, &x, s.n_rows, sms, st);
+        return tc_rows(&a, 1, cut, &x, s.n_rows, sms, st, used);
     }
     a.group_ptr = ws.ptr;
     a.slot_row = ws.row;
@@ -600,7 +603,7 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cu
     a.u_plane = s.n_rows;
     a.gather = a.scatter = true;
     if (int rc = tc_matrix(&a.w2, &a, m, s.rank, n, s.n_adapters)) return rc;
-    return tc_rows(&a, 1, cut, &x, s.n_rows, sms, st);
+    return tc_rows(&a, 1, cut, &x, s.n_rows, sms, st, used);
 }
 
 TcOuter tc_adapter_outer(const AdapterShape &s, int features, void *out, long long out_f, long long out_c) {
@@ -641,7 +644,7 @@ int adapters(const AdapterShape &s, const void *x, const void *w, const void *a,
             narrow.follows = narrow.apart = true;  // beside the listing
             if (int rc = tc_rows(&narrow, 1, best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k), true, sms, 256), &x, s.n_rows, sms, st)) return rc;
         }
-        return tc_adapter_wide(s, ws, cut, rows, s.k, s.n, x, w, ws.u, (const float *)ws.u, b, false, y, rows, false, sms, st);
+        return tc_adapter_wide(s, ws, cut, rows, s.k, s.n, x, w, ws.u, (const float *)ws.u, b, false, y, rows, sms, st);
     }
     float *u = (float *)ws.u;
     if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
@@ -653,7 +656,7 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
                       void *workspace, cudaStream_t st) {
     const AdapterSpace ws(workspace, s.n_rows, s.n_adapters, s.rank, true);
     if (tc_widths(s.dtype, {s.k, s.n, s.rank}, {dy, x, w, a, b})) {
-        int sms;
+        int sms, used = 0;
         Cut cut;
         if (int rc = sm_count(&sms)) return rc;
         const bool rows = by_rows(s, s.n, s.k, true, sms, &cut);
@@ -666,10 +669,11 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
         const void *const in[2] = {x, dy};
         const Cut half = best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k > s.n ? s.k : s.n), true, sms / 2, 64);
         if (int rc = tc_rows(narrow, 2, half, in, s.n_rows, sms, st)) return rc;
-        if (int rc = tc_adapter_wide(s, ws, cut, rows, s.n, s.k, dy, w, ws.v, (const float *)ws.v_f32, a, true, dx, false, true, sms, st)) return rc;
+        if (int rc = tc_adapter_wide(s, ws, cut, rows, s.n, s.k, dy, w, ws.v, (const float *)ws.v_f32, a, true, dx, false, sms, st, &used)) return rc;
         const TcOuter outer[2] = {tc_adapter_outer(s, s.k, da, 1, s.k), tc_adapter_outer(s, s.n, db, s.rank, 1)};
         const void *const q[2] = {ws.v, ws.u};
-        return tc_outer(outer, 2, in, q, st);
+        // beside few blocks of that on the SMs they leave, else on each as it gets free
+        return tc_outer(outer, 2, in, q, used <= sms / 2 ? sms - used : sms, st);
     }
     float *u = (float *)ws.u, *v = (float *)ws.v;
     if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
@@ -768,6 +772,8 @@ extern "C" int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_group
     if (misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_x, size) || misaligned(d_dy, size) || misaligned(d_dw, size))
         return fail(MPS_ERR_ALIGN, "mps_routed_wgrad: a pointer is not aligned to its element size");
     if (n_slots > 0 && n_rows > 0 && tc_widths(dtype, {k, n}, {d_x, d_dy})) {
+        int sms;
+        if (int rc = sm_count(&sms)) return rc;
         TcOuter a = {};
         a.bf16 = dtype == MPS_BF16;
         a.group_ptr = d_group_ptr;
@@ -781,7 +787,7 @@ extern "C" int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_group
         a.out_group = (long long)k * n;
         a.out_f = 1;
         a.out_c = k;
-        return tc_outer(&a, 1, &d_x, &d_dy, (cudaStream_t)stream);
+        return tc_outer(&a, 1, &d_x, &d_dy, sms, (cudaStream_t)stream);
     }
     OuterArgs a = {};
     a.group_ptr = d_group_ptr;

@@ -11,11 +11,13 @@ constexpr int kPlainTile = 64, kPlainDepth = 16, kPlainThreads = 256;
 constexpr int kMaxRowGroups = 1024;  // groups a block scans at once
 
 // Start and end of group g inside [0, n_slots): whatever group_ptr holds, no slot outside the arrays is named.
-__device__ __forceinline__ int2 group_range(const int *group_ptr, int g, int n_slots, int *status) {
-    const int lo = group_ptr[g], hi = group_ptr[g + 1];
-    const int a = min(max(lo, 0), n_slots), b = min(max(hi, a), n_slots);
-    if (a != lo || b != hi) atomicOr(status, kStatusBadIndex);
+__device__ __forceinline__ int2 group_range(int2 ends, int n_slots, int *status) {
+    const int a = min(max(ends.x, 0), n_slots), b = min(max(ends.y, a), n_slots);
+    if (a != ends.x || b != ends.y) atomicOr(status, kStatusBadIndex);
     return make_int2(a, b);
+}
+__device__ __forceinline__ int2 group_range(const int *group_ptr, int g, int n_slots, int *status) {
+    return group_range(make_int2(group_ptr[g], group_ptr[g + 1]), n_slots, status);
 }
 
 // Group and slot range of tile number `tile` when every group is cut into tiles of `rows` slots.  Called by all THREADS

@@ -809,10 +809,13 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     RingAt pos;
     int turn = 0;
     const int q_end = (a.pair ? 2 : 1) * a.n_slots;  // out of range of Q
+    int2 ends = make_int2(0, 0);  // of the next tile's group: read a tile ahead
+    if (worker < n_tiles) ends = make_int2(a.group_ptr[worker / per_group], a.group_ptr[worker / per_group + 1]);
     for (int tile = worker; tile < n_tiles; tile += workers, ++turn) {
         const int g = tile / per_group, rest = tile - g * per_group;
+        const int2 slots = group_range(ends, a.n_slots, a.status);
+        if (tile + workers < n_tiles) ends = make_int2(a.group_ptr[(tile + workers) / per_group], a.group_ptr[(tile + workers) / per_group + 1]);
         const int f0 = rest / j_tiles * TILE_F + half * kTcFeatures, c0 = rest % j_tiles * cols;
-        const int2 slots = group_range(a.group_ptr, g, a.n_slots, a.status);
         const int total = (slots.y - slots.x + kTcDepth - 1) / kTcDepth;
         const int s0 = (int)((long long)total * part >> shift), s1 = (int)((long long)total * (part + 1) >> shift);
         const int buf = turn & 1;
@@ -832,18 +835,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     for (int b = 0; b < q_blocks; ++b)
                         tma_2d<PAIRED>(dst + (2 + b) * kBlock64, &a.q_tile, a.pair ? c0 : q0 + b * 64, a.pair ? b * a.n_slots + slot : slot, bar);
                 }
-                if (max(s0, whole) < s1) {  // part of a slice: by row number, zeros behind the group's end
+                if (max(s0, whole) < s1) {  // part of a slice: by row number, zeros behind the group's end up to what the products read
                     const int st = pos.stage, slot = slots.x + (s1 - 1) * kTcDepth;
                     mbar_wait(smem_addr(&pipe.empty[st]), pos.parity ^ 1, gave_up, a.status);
                     const uint32_t bar = full0 + st * 8, dst = ring + st * S::kStage;
-                    if (half == 0) mbar_expect(bar, bytes);
+                    const int n_read = min(kTcDepth, (slots.y - slot + 15) & ~15);
+                    if (half == 0) mbar_expect(bar, (PAIRED ? 2 : 1) * 128 * (p_blocks * (gather ? kTcDepth : n_read) + q_blocks * n_read));
 #pragma unroll 1
                     for (int b = gather ? 2 : 0; b < 2 + q_blocks; ++b) {
                         if (b >= p_blocks && b < 2) continue;
                         const bool q = b >= 2;
                         const int x = !q ? f0 + b * 64 : a.pair ? c0 : q0 + (b - 2) * 64, plane = q && a.pair ? (b - 2) * a.n_slots : 0;
 #pragma unroll 1
-                        for (int i = 0; i < kTcDepth; i += 4) {
+                        for (int i = 0; i < n_read; i += 4) {
                             auto line = [&](int j) { return slot + i + j < slots.y ? plane + slot + i + j : q ? q_end : a.n_p_rows; };
                             tma_rows<PAIRED>(dst + b * kBlock64 + i * 128, q ? &a.q_rows : &a.p_rows, x, line(0), line(1), line(2), line(3), bar);
                         }
