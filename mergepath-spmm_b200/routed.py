@@ -3,7 +3,8 @@
 The routing is kept as the rows listed by group (`Groups`): `ptr` is the row_ptr over groups, `row` the col_idx (the input row
 in every slot), `slot` the slot of every (row, choice).  Thin wrappers of the mps_route* / mps_routed_* / mps_adapters* entry
 points of include/mps.h over torch CUDA tensors (float32, float16 or bfloat16); no reference counterpart.  Gradients are
-functions of their own.  Nothing synchronises; `routed_check()` waits and reports what the device met out of range.
+functions of their own.  `stream` is where a call runs and what it returns belongs to.  Nothing synchronises; `routed_check()`
+waits and reports what the device met out of range.
 """
 from __future__ import annotations
 
@@ -70,6 +71,8 @@ _raw_stream = getattr(getattr(torch, "_C", None), "_cuda_getCurrentRawStream", N
 def _call(device, stream, name, *args):
     """The entry point on `device` and `stream` (default: torch's current stream of that device)."""
     fn = getattr(capi.lib(), name)
+    if stream is not None and stream.device != device:
+        raise ValueError(f"stream: on {stream.device}, expected {device}")
     handle = _raw_stream(device.index) if stream is None else stream.cuda_stream
     if device.index == torch.cuda.current_device():
         rc = fn(*args, handle)
@@ -78,6 +81,14 @@ def _call(device, stream, name, *args):
             rc = fn(*args, handle)
     if rc:
         capi.check(rc)
+
+
+def _new(stream, shape, dtype, device):
+    """Memory of the stream that is going to write it: work of another one may still be under way on what that one has freed."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def _shape(name, t, dims=2):
@@ -108,7 +119,7 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, n_groups: in
     # one allocation: five take longer than the kernels of a small batch
     k = max(top_k, 0)  # what is wrong with it the entry point says
     n, shape, pitch = rows * k, (rows, k), (k, 1)
-    buf = torch.empty(4 * n + experts + 1 if group else 2 * n, dtype=torch.int32, device=dev)
+    buf = _new(stream, 4 * n + experts + 1 if group else 2 * n, torch.int32, dev)
     ids, weights = buf.as_strided(shape, pitch, 0), buf.view(torch.float32).as_strided(shape, pitch, n)
     groups = Groups(buf.as_strided((experts + 1,), (1,), 4 * n), buf.as_strided((n,), (1,), 2 * n), buf.as_strided(shape, pitch, 3 * n)) if group else None
     ptr, row, slot = groups or (None, None, None)
@@ -127,7 +138,7 @@ def route_backward(logits, ids, d_weights, *, score: str = "softmax", renormalis
         _explain(dev, ("logits", logits, logits.dtype, (rows, experts)), ("ids", ids, torch.int32, (rows, top_k)),
                ("d_weights", d_weights, torch.float32, (rows, top_k)))
     spec = _spec(experts, top_k, score, 1, 1, 1, renormalise, scale)
-    out = torch.empty_like(logits)
+    out = _new(stream, logits.shape, logits.dtype, dev)
     _call(dev, stream, "mps_route_backward", rows, C.byref(spec), _dtype(logits), _ptr(logits), _ptr(ids), _ptr(d_weights), _ptr(out))
     return out
 
@@ -141,8 +152,7 @@ def group_rows(ids, n_groups: int, *, stream=None) -> Groups:
     if not (_is(ids, torch.int32, ids.shape, at)):
         _explain(dev, ("ids", ids, torch.int32, ids.shape))
     rows, per_row = ids.shape[0], 1 if ids.dim() == 1 else ids.shape[1]
-    groups = Groups(torch.empty(max(n_groups, 0) + 1, dtype=torch.int32, device=dev), torch.empty(ids.numel(), dtype=torch.int32, device=dev),
-                    torch.empty_like(ids))
+    groups = Groups(*(_new(stream, shape, torch.int32, dev) for shape in (max(n_groups, 0) + 1, ids.numel(), ids.shape)))
     _call(dev, stream, "mps_group_rows", rows, per_row, n_groups, _ptr(ids), _ptr(groups.ptr), _ptr(groups.row), _ptr(groups.slot))
     return groups
 
@@ -154,7 +164,7 @@ def routed_product(x, w, groups: Groups, *, gather: bool = True, transpose: bool
     inner, outer = (n, k) if transpose else (k, n)
     dev, rows, slots = x.device, _shape("x", x)[0], groups.row.numel()
     if out is None:
-        out = torch.empty((slots, outer), dtype=x.dtype, device=dev)
+        out = _new(stream, (slots, outer), x.dtype, dev)
     at = dev.index
     if not (_is(x, x.dtype, (rows, inner), at) and _is(w, x.dtype, (n_groups, n, k), at) and _is(groups.ptr, torch.int32, (n_groups + 1,), at)
             and _is(groups.row, torch.int32, (slots,), at) and _is(out, x.dtype, (slots, outer), at)):
@@ -171,7 +181,7 @@ def routed_wgrad(x, dy, groups: Groups, *, gather: bool = True, out=None, stream
     dev, slots, n_groups = x.device, groups.row.numel(), groups.ptr.numel() - 1
     (rows, k), n = _shape("x", x), _shape("dy", dy)[1]
     if out is None:
-        out = torch.empty((n_groups, n, k), dtype=x.dtype, device=dev)
+        out = _new(stream, (n_groups, n, k), x.dtype, dev)
     at = dev.index
     if not (_is(x, x.dtype, (rows, k), at) and _is(dy, x.dtype, (slots, n), at) and _is(groups.ptr, torch.int32, (n_groups + 1,), at)
             and _is(groups.row, torch.int32, (slots,), at) and _is(out, x.dtype, (n_groups, n, k), at)):
@@ -186,7 +196,7 @@ def routed_combine(rows, slot, weights=None, *, out=None, stream=None):
     """y[t] = sum over j of weights[t, j] * rows[slot[t, j]]; no term for a negative slot, weights None: 1 each."""
     dev, (n_slots, dim), (n, per_row) = rows.device, _shape("rows", rows), _shape("slot", slot)
     if out is None:
-        out = torch.empty((n, dim), dtype=rows.dtype, device=dev)
+        out = _new(stream, (n, dim), rows.dtype, dev)
     at = dev.index
     if not (_is(rows, rows.dtype, (n_slots, dim), at) and _is(slot, torch.int32, (n, per_row), at) and _is(weights, torch.float32, (n, per_row), at)
             and _is(out, rows.dtype, (n, dim), at)):
@@ -200,13 +210,13 @@ def routed_combine_backward(dy, rows, slot, weights=None, *, out=None, stream=No
     """(d_rows, d_weights) of routed_combine; `out` receives d_rows, whose rows that no slot names are left as they were."""
     dev, (n_slots, dim), (n, per_row) = rows.device, _shape("rows", rows), _shape("slot", slot)
     if out is None:
-        out = torch.empty_like(rows)
+        out = _new(stream, rows.shape, rows.dtype, dev)
     at = dev.index
     if not (_is(dy, rows.dtype, (n, dim), at) and _is(rows, rows.dtype, (n_slots, dim), at) and _is(slot, torch.int32, (n, per_row), at)
             and _is(weights, torch.float32, (n, per_row), at) and _is(out, rows.dtype, (n_slots, dim), at)):
         _explain(dev, ("dy", dy, rows.dtype, (n, dim)), ("rows", rows, rows.dtype, (n_slots, dim)), ("slot", slot, torch.int32, (n, per_row)),
                ("weights", weights, torch.float32, (n, per_row)), ("out", out, rows.dtype, (n_slots, dim)))
-    d_weights = torch.empty((n, per_row), dtype=torch.float32, device=dev)
+    d_weights = _new(stream, (n, per_row), torch.float32, dev)
     _call(dev, stream, "mps_routed_combine_backward", n, per_row, n_slots, dim, _dtype(rows), _ptr(slot), _ptr(weights), _ptr(dy), _ptr(rows), _ptr(out),
           _ptr(d_weights))
     return out, d_weights
@@ -225,11 +235,11 @@ def _adapter_sizes(x, w, a, b, ids, groups, scale):
     return rows, k, n, n_adapters, rank
 
 
-def _adapter_workspace(device, sizes, dtype, backward):
+def _adapter_workspace(stream, device, sizes, dtype, backward):
     need = capi.lib().mps_adapters_workspace(*sizes, dtype, int(backward))
     if need < 0:
         capi.check(int(need))
-    return torch.empty(need, dtype=torch.uint8, device=device)
+    return _new(stream, need, torch.uint8, device)
 
 
 def adapters(x, w, a, b, ids, groups: Groups, scale=None, *, out=None, stream=None):
@@ -237,14 +247,12 @@ def adapters(x, w, a, b, ids, groups: Groups, scale=None, *, out=None, stream=No
     w (n, k), a (adapters, rank, k), b (adapters, n, rank), groups = group_rows(ids, adapters), scale fp32 or None (1)."""
     sizes = rows, k, n, _, _ = _adapter_sizes(x, w, a, b, ids, groups, scale)
     if out is None:
-        out = torch.empty((rows, n), dtype=x.dtype, device=x.device)
+        out = _new(stream, (rows, n), x.dtype, x.device)
     at = x.device.index
     if not (_is(out, x.dtype, (rows, n), at)):
         _explain(x.device, ("out", out, x.dtype, (rows, n)))
     dtype = _dtype(x)
-    ws = _adapter_workspace(x.device, sizes, dtype, False)
-    if stream is not None:
-        ws.record_stream(stream)
+    ws = _adapter_workspace(stream, x.device, sizes, dtype, False)
     _call(x.device, stream, "mps_adapters", *sizes, dtype, _ptr(ids), _ptr(groups.ptr), _ptr(groups.row), _ptr(scale), _ptr(x), _ptr(w), _ptr(a), _ptr(b),
           _ptr(out), _ptr(ws), ws.numel())
     return out
@@ -256,11 +264,9 @@ def adapters_backward(dy, x, w, a, b, ids, groups: Groups, scale=None, *, stream
     at = x.device.index
     if not (_is(dy, x.dtype, (rows, n), at)):
         _explain(x.device, ("dy", dy, x.dtype, (rows, n)))
-    dx, da, db = torch.empty_like(x), torch.empty_like(a), torch.empty_like(b)
+    dx, da, db = (_new(stream, t.shape, t.dtype, t.device) for t in (x, a, b))
     dtype = _dtype(x)
-    ws = _adapter_workspace(x.device, sizes, dtype, True)
-    if stream is not None:
-        ws.record_stream(stream)
+    ws = _adapter_workspace(stream, x.device, sizes, dtype, True)
     _call(x.device, stream, "mps_adapters_backward", *sizes, dtype, _ptr(ids), _ptr(groups.ptr), _ptr(groups.row), _ptr(scale), _ptr(dy), _ptr(x), _ptr(w),
           _ptr(a), _ptr(b), _ptr(dx), _ptr(da), _ptr(db), _ptr(ws), ws.numel())
     return dx, da, db

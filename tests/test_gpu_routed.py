@@ -597,6 +597,61 @@ def test_stream_argument(mps, cuda):
     assert torch.equal(out, want[-4])
 
 
+@pytest.mark.parametrize("name", ["route", "route_backward", "group_rows", "product", "wgrad", "combine", "combine_backward", "adapters", "adapters_backward"])
+def test_results_on_another_stream_are_memory_of_that_stream(mps, cuda, name):
+    """The current stream is still going to write what it has freed; a call on another stream must not be given that."""
+    gen = gen_of(11)
+    x, dy, w = rand(gen, torch.bfloat16, 300, 64), rand(gen, torch.bfloat16, 600, 96), rand(gen, torch.bfloat16, 6, 96, 64)
+    logits, weights = rand(gen, torch.float32, 300, 6), rand(gen, torch.float32, 300, 2)
+    ids, _, groups = mps.route(logits, 2)
+    one = ids[:, 0].contiguous()
+    ag, a, b = mps.group_rows(one, 6), rand(gen, torch.bfloat16, 6, 8, 64), rand(gen, torch.bfloat16, 6, 96, 8)
+
+    def call(s):
+        if name == "route":
+            ids_, weights_, groups_ = mps.route(logits, 2, stream=s)
+            return (ids_, weights_, *groups_)
+        if name == "route_backward":
+            return (mps.route_backward(logits, ids, weights, stream=s),)
+        if name == "group_rows":
+            return tuple(mps.group_rows(ids, 6, stream=s))
+        if name == "product":
+            return (mps.routed_product(x, w, groups, stream=s),)
+        if name == "wgrad":
+            return (mps.routed_wgrad(x, dy, groups, stream=s),)
+        if name == "combine":
+            return (mps.routed_combine(dy, groups.slot, weights, stream=s),)
+        if name == "combine_backward":
+            return mps.routed_combine_backward(dy[:300], dy, groups.slot, weights, stream=s)
+        if name == "adapters":
+            return (mps.adapters(x, w[0], a, b, one, ag, stream=s),)
+        return mps.adapters_backward(dy[:300], x, w[0], a, b, one, ag, stream=s)
+
+    want = call(None)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    torch.cuda._sleep(100_000_000)  # about 50 ms
+    size = 4 * 600 + 7 if name == "route" else 0  # route's results share one allocation
+    freed = [torch.empty(max(t.numel() * t.element_size(), 4 * size), dtype=torch.uint8, device="cuda") for t in want for _ in range(4)]
+    for t in freed:
+        t.fill_(3)
+    del freed, t
+    got = call(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, w_) for g, w_ in zip(got, want))
+
+
+def test_stream_of_another_device_is_refused(mps, cuda):
+    class Elsewhere:
+        device, cuda_stream = torch.device("cuda", 99), 0
+
+    slot = torch.zeros(4, 1, dtype=torch.int32, device="cuda")
+    rows = torch.ones(4, 8, device="cuda")
+    with pytest.raises(ValueError, match="stream: on cuda:99, expected cuda:0"):
+        mps.routed_combine(rows, slot, out=torch.empty_like(rows), stream=Elsewhere())
+
+
 def test_captured_and_replayed_on_new_inputs(mps, cuda):
     """Two graphs over the same inputs, replayed at once on two streams, after the inputs were changed in place."""
     t, other = everything_inputs(4), everything_inputs(5)
