@@ -9,6 +9,7 @@ waits and reports what the device met out of range.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple
 
 from . import capi
@@ -83,12 +84,20 @@ def _call(device, stream, name, *args):
         capi.check(rc)
 
 
-def _new(stream, shape, dtype, device):
-    """Memory of the stream that is going to write it: work of another one may still be under way on what that one has freed."""
+def _new(stream, like, shape, dtype=None):
+    """Memory of the stream that is going to write it: work of another one may still be under way on what that one has freed.
+    By `new_empty` on the device of `like`: `torch.empty` with a dtype and a device takes a microsecond longer."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape) if dtype is None else like.new_empty(shape, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return like.new_empty(shape, dtype=dtype)
+
+
+def _like(stream, t):
+    if stream is None:
+        return torch.empty_like(t)
+    with torch.cuda.stream(stream):
+        return torch.empty_like(t)
 
 
 def _shape(name, t, dims=2):
@@ -116,13 +125,16 @@ def route(logits, top_k: int, *, score: str = "softmax", bias=None, n_groups: in
     if not (_is(logits, logits.dtype, (rows, experts), at) and _is(bias, torch.float32, (experts,), at)):
         _explain(dev, ("logits", logits, logits.dtype, (rows, experts)), ("bias", bias, torch.float32, (experts,)))
     spec = _spec(experts, top_k, score, n_groups, top_groups, group_top, renormalise, scale)
-    # one allocation: five take longer than the kernels of a small batch
+    # one allocation and few views: five of each take longer than the kernels of a small batch
     k = max(top_k, 0)  # what is wrong with it the entry point says
-    n, shape, pitch = rows * k, (rows, k), (k, 1)
-    buf = _new(stream, 4 * n + experts + 1 if group else 2 * n, torch.int32, dev)
-    ids, weights = buf.as_strided(shape, pitch, 0), buf.view(torch.float32).as_strided(shape, pitch, n)
-    groups = Groups(buf.as_strided((experts + 1,), (1,), 4 * n), buf.as_strided((n,), (1,), 2 * n), buf.as_strided(shape, pitch, 3 * n)) if group else None
-    ptr, row, slot = groups or (None, None, None)
+    n = rows * k
+    if group:
+        by_row, row, ptr = _new(stream, logits, 4 * n + experts + 1, torch.int32).split_with_sizes((3 * n, n, experts + 1))
+        ids, weights, slot = by_row.view(3, rows, k).unbind(0)
+        groups = Groups(ptr, row, slot)
+    else:
+        (ids, weights), ptr, row, slot, groups = _new(stream, logits, (2, rows, k), torch.int32).unbind(0), None, None, None, None
+    weights = weights.view(torch.float32)
     _call(dev, stream, "mps_route", rows, C.byref(spec), _dtype(logits), _ptr(logits), _ptr(bias), _ptr(ids), _ptr(weights), _ptr(ptr), _ptr(row), _ptr(slot))
     return ids, weights, groups
 
@@ -138,7 +150,7 @@ def route_backward(logits, ids, d_weights, *, score: str = "softmax", renormalis
         _explain(dev, ("logits", logits, logits.dtype, (rows, experts)), ("ids", ids, torch.int32, (rows, top_k)),
                ("d_weights", d_weights, torch.float32, (rows, top_k)))
     spec = _spec(experts, top_k, score, 1, 1, 1, renormalise, scale)
-    out = _new(stream, logits.shape, logits.dtype, dev)
+    out = _like(stream, logits)
     _call(dev, stream, "mps_route_backward", rows, C.byref(spec), _dtype(logits), _ptr(logits), _ptr(ids), _ptr(d_weights), _ptr(out))
     return out
 
@@ -152,7 +164,7 @@ def group_rows(ids, n_groups: int, *, stream=None) -> Groups:
     if not (_is(ids, torch.int32, ids.shape, at)):
         _explain(dev, ("ids", ids, torch.int32, ids.shape))
     rows, per_row = ids.shape[0], 1 if ids.dim() == 1 else ids.shape[1]
-    groups = Groups(*(_new(stream, shape, torch.int32, dev) for shape in (max(n_groups, 0) + 1, ids.numel(), ids.shape)))
+    groups = Groups(_new(stream, ids, max(n_groups, 0) + 1), _new(stream, ids, ids.numel()), _like(stream, ids))
     _call(dev, stream, "mps_group_rows", rows, per_row, n_groups, _ptr(ids), _ptr(groups.ptr), _ptr(groups.row), _ptr(groups.slot))
     return groups
 
@@ -164,7 +176,7 @@ def routed_product(x, w, groups: Groups, *, gather: bool = True, transpose: bool
     inner, outer = (n, k) if transpose else (k, n)
     dev, rows, slots = x.device, _shape("x", x)[0], groups.row.numel()
     if out is None:
-        out = _new(stream, (slots, outer), x.dtype, dev)
+        out = _new(stream, x, (slots, outer))
     at = dev.index
     if not (_is(x, x.dtype, (rows, inner), at) and _is(w, x.dtype, (n_groups, n, k), at) and _is(groups.ptr, torch.int32, (n_groups + 1,), at)
             and _is(groups.row, torch.int32, (slots,), at) and _is(out, x.dtype, (slots, outer), at)):
@@ -181,7 +193,7 @@ def routed_wgrad(x, dy, groups: Groups, *, gather: bool = True, out=None, stream
     dev, slots, n_groups = x.device, groups.row.numel(), groups.ptr.numel() - 1
     (rows, k), n = _shape("x", x), _shape("dy", dy)[1]
     if out is None:
-        out = _new(stream, (n_groups, n, k), x.dtype, dev)
+        out = _new(stream, x, (n_groups, n, k))
     at = dev.index
     if not (_is(x, x.dtype, (rows, k), at) and _is(dy, x.dtype, (slots, n), at) and _is(groups.ptr, torch.int32, (n_groups + 1,), at)
             and _is(groups.row, torch.int32, (slots,), at) and _is(out, x.dtype, (n_groups, n, k), at)):
@@ -196,7 +208,7 @@ def routed_combine(rows, slot, weights=None, *, out=None, stream=None):
     """y[t] = sum over j of weights[t, j] * rows[slot[t, j]]; no term for a negative slot, weights None: 1 each."""
     dev, (n_slots, dim), (n, per_row) = rows.device, _shape("rows", rows), _shape("slot", slot)
     if out is None:
-        out = _new(stream, (n, dim), rows.dtype, dev)
+        out = _new(stream, rows, (n, dim))
     at = dev.index
     if not (_is(rows, rows.dtype, (n_slots, dim), at) and _is(slot, torch.int32, (n, per_row), at) and _is(weights, torch.float32, (n, per_row), at)
             and _is(out, rows.dtype, (n, dim), at)):
@@ -210,13 +222,13 @@ def routed_combine_backward(dy, rows, slot, weights=None, *, out=None, stream=No
     """(d_rows, d_weights) of routed_combine; `out` receives d_rows, whose rows that no slot names are left as they were."""
     dev, (n_slots, dim), (n, per_row) = rows.device, _shape("rows", rows), _shape("slot", slot)
     if out is None:
-        out = _new(stream, rows.shape, rows.dtype, dev)
+        out = _like(stream, rows)
     at = dev.index
     if not (_is(dy, rows.dtype, (n, dim), at) and _is(rows, rows.dtype, (n_slots, dim), at) and _is(slot, torch.int32, (n, per_row), at)
             and _is(weights, torch.float32, (n, per_row), at) and _is(out, rows.dtype, (n_slots, dim), at)):
         _explain(dev, ("dy", dy, rows.dtype, (n, dim)), ("rows", rows, rows.dtype, (n_slots, dim)), ("slot", slot, torch.int32, (n, per_row)),
                ("weights", weights, torch.float32, (n, per_row)), ("out", out, rows.dtype, (n_slots, dim)))
-    d_weights = _new(stream, (n, per_row), torch.float32, dev)
+    d_weights = _new(stream, rows, (n, per_row), torch.float32)
     _call(dev, stream, "mps_routed_combine_backward", n, per_row, n_slots, dim, _dtype(rows), _ptr(slot), _ptr(weights), _ptr(dy), _ptr(rows), _ptr(out),
           _ptr(d_weights))
     return out, d_weights
@@ -235,11 +247,12 @@ def _adapter_sizes(x, w, a, b, ids, groups, scale):
     return rows, k, n, n_adapters, rank
 
 
-def _adapter_workspace(stream, device, sizes, dtype, backward):
-    need = capi.lib().mps_adapters_workspace(*sizes, dtype, int(backward))
+@functools.lru_cache(maxsize=64)
+def _workspace_bytes(*sizes) -> int:
+    need = capi.lib().mps_adapters_workspace(*sizes)
     if need < 0:
         capi.check(int(need))
-    return _new(stream, need, torch.uint8, device)
+    return need
 
 
 def adapters(x, w, a, b, ids, groups: Groups, scale=None, *, out=None, stream=None):
@@ -247,12 +260,12 @@ def adapters(x, w, a, b, ids, groups: Groups, scale=None, *, out=None, stream=No
     w (n, k), a (adapters, rank, k), b (adapters, n, rank), groups = group_rows(ids, adapters), scale fp32 or None (1)."""
     sizes = rows, k, n, _, _ = _adapter_sizes(x, w, a, b, ids, groups, scale)
     if out is None:
-        out = _new(stream, (rows, n), x.dtype, x.device)
+        out = _new(stream, x, (rows, n))
     at = x.device.index
     if not (_is(out, x.dtype, (rows, n), at)):
         _explain(x.device, ("out", out, x.dtype, (rows, n)))
     dtype = _dtype(x)
-    ws = _adapter_workspace(stream, x.device, sizes, dtype, False)
+    ws = _new(stream, x, _workspace_bytes(*sizes, dtype, 0), torch.uint8)
     _call(x.device, stream, "mps_adapters", *sizes, dtype, _ptr(ids), _ptr(groups.ptr), _ptr(groups.row), _ptr(scale), _ptr(x), _ptr(w), _ptr(a), _ptr(b),
           _ptr(out), _ptr(ws), ws.numel())
     return out
@@ -264,9 +277,9 @@ def adapters_backward(dy, x, w, a, b, ids, groups: Groups, scale=None, *, stream
     at = x.device.index
     if not (_is(dy, x.dtype, (rows, n), at)):
         _explain(x.device, ("dy", dy, x.dtype, (rows, n)))
-    dx, da, db = (_new(stream, t.shape, t.dtype, t.device) for t in (x, a, b))
+    dx, da, db = _like(stream, x), _like(stream, a), _like(stream, b)
     dtype = _dtype(x)
-    ws = _adapter_workspace(stream, x.device, sizes, dtype, True)
+    ws = _new(stream, x, _workspace_bytes(*sizes, dtype, 1), torch.uint8)
     _call(x.device, stream, "mps_adapters_backward", *sizes, dtype, _ptr(ids), _ptr(groups.ptr), _ptr(groups.row), _ptr(scale), _ptr(dy), _ptr(x), _ptr(w),
           _ptr(a), _ptr(b), _ptr(dx), _ptr(da), _ptr(db), _ptr(ws), ws.numel())
     return dx, da, db
