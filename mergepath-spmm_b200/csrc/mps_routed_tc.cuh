@@ -232,20 +232,22 @@ struct TcShape {
     static size_t bytes(int n_groups) { return 1024 + kTcRing + kOutTotal + (size_t)(4 * n_groups + 2) * sizeof(int); }
 };
 
-// A cursor over the tiles of all groups: tile numbers only rise, so the group is found by walking on.  Where the matrix is shared
+// A cursor over the tiles of all groups that have slots (a few rows of many experts leave most without, and a walk past those
+// costs 40 ns each: 32 slots of 256 matrices of 2048 x 1024 40 -> 28 us): tile numbers only rise, so the group is found by walking on.  Where the matrix is shared
 // the whole tiles of every group come first and then the groups' rests: blocks take tiles in turn, and the short ones at the end
 // even out what the long ones leave (4096 rows of 8 adapters: 160 -> 152 us).  With a matrix per group a group's tiles stay
 // together, its rest counted among them, or the matrices would be read twice (32 groups: 257 -> 270 us).
 struct TcCursor {
-    const int *whole, *rest, *lo, *hi;  // whole tiles and rests before every group (n_groups + 1 each), its slots
+    const int *whole, *rest, *lo, *hi;  // whole tiles before every group and (rests before it | its number << 16), n_groups + 1 each; its slots
     int n_groups, group, slot0, slot1;
     bool rests;
+    __device__ __forceinline__ int number() const { return rest[group] >> 16; }
     __device__ __forceinline__ void seek(int tile, int nt) {
         const int n_whole = whole[n_groups];
         if (tile >= n_whole) {
             if (!rests) group = 0;
             rests = true;
-            while (tile - n_whole >= rest[group + 1]) ++group;
+            while (tile - n_whole >= (rest[group + 1] & 0xffff)) ++group;
             slot0 = lo[group] + (whole[group + 1] - whole[group]) * nt;
         } else {
             while (tile >= whole[group + 1]) ++group;
@@ -284,7 +286,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     using S = TcShape<NT>;
     extern __shared__ uint8_t s_raw[];
     __shared__ TcPipe pipe;
-    __shared__ int s_sum[2][kTcThreads / 32];
+    __shared__ int s_sum[3][kTcThreads / 32], s_active;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = (smem_addr(s_raw) + 1023) & ~1023u, staging = ring + kTcRing;
     int *whole = reinterpret_cast<int *>(s_raw + (ring - smem_addr(s_raw)) + kTcRing + kOutTotal);
@@ -306,55 +308,60 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     // ---- tiles of the groups
     {
         constexpr int PER = (kMaxRowGroups + 1 + kTcThreads - 1) / kTcThreads;  // a list with the ungrouped rows has one group more
-        int tiles[PER], sum = 0, sum_rest = 0;  // a whole tile counts 2, a rest 1
+        int2 slots[PER];
+        int tiles[PER], sum = 0, sum_rest = 0, active = 0;  // a whole tile counts 2, a rest 1
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int g = tid * PER + i;
             tiles[i] = 0;
             if (g < a.n_groups) {
-                int2 r = make_int2(0, a.n_slots);
-                if (a.group_ptr) r = group_range(a.group_ptr, g, a.n_slots, a.status);
-                lo[g] = r.x;
-                hi[g] = r.y;
-                const int n = r.y - r.x;
+                slots[i] = make_int2(0, a.n_slots);
+                if (a.group_ptr) slots[i] = group_range(a.group_ptr, g, a.n_slots, a.status);
+                const int n = slots[i].y - slots[i].x;
                 tiles[i] = a.w_shared ? n / NT * 2 + (n % NT ? 1 : 0) : (n + NT - 1) / NT * 2;
             }
             sum += tiles[i] >> 1;
             sum_rest += tiles[i] & 1;
+            active += tiles[i] > 0;
         }
-        int scan = sum, scan_rest = sum_rest;
+        int scan = sum, scan_rest = sum_rest, scan_active = active;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
-            const int o = __shfl_up_sync(0xffffffffu, scan, d), q = __shfl_up_sync(0xffffffffu, scan_rest, d);
+            const int o = __shfl_up_sync(0xffffffffu, scan, d), q = __shfl_up_sync(0xffffffffu, scan_rest, d), n = __shfl_up_sync(0xffffffffu, scan_active, d);
             if (lane >= d) {
                 scan += o;
                 scan_rest += q;
+                scan_active += n;
             }
         }
         if (lane == 31) {
             s_sum[0][warp] = scan;
             s_sum[1][warp] = scan_rest;
+            s_sum[2][warp] = scan_active;
         }
         if (tid == 0) pipe_init(pipe, stages, PAIRED, split);
         if (warp == 1) tmem_alloc<PAIRED>(smem_addr(&pipe.tmem), S::kColumns);
         __syncthreads();
-        for (int w = 0; w < warp; ++w) {
-            scan += s_sum[0][w];
-            scan_rest += s_sum[1][w];
-        }
-        int at = scan - sum, at_rest = scan_rest - sum_rest;
+        const bool before = lane < warp;
+        int at = scan - sum + __reduce_add_sync(0xffffffffu, before ? s_sum[0][lane] : 0);
+        int at_rest = scan_rest - sum_rest + __reduce_add_sync(0xffffffffu, before ? s_sum[1][lane] : 0);
+        int to = scan_active - active + __reduce_add_sync(0xffffffffu, before ? s_sum[2][lane] : 0);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
             const int g = tid * PER + i;
-            if (g < a.n_groups) {
-                whole[g] = at;
-                rest[g] = at_rest;
+            if (tiles[i] > 0) {
+                whole[to] = at;
+                rest[to] = at_rest | g << 16;
+                lo[to] = slots[i].x;
+                hi[to] = slots[i].y;
+                ++to;
             }
             at += tiles[i] >> 1;
             at_rest += tiles[i] & 1;
             if (g == a.n_groups - 1) {
-                whole[a.n_groups] = at;
-                rest[a.n_groups] = at_rest;
+                whole[to] = at;
+                rest[to] = at_rest;
+                s_active = to;
             }
         }
         tc_fence_before();
@@ -367,8 +374,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
     const int main_steps = (a.k + kTcDepth - 1) / kTcDepth, rank_steps = 2 * ((a.rank + kTcDepth - 1) / kTcDepth);
     const int shift = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
-    TileWalk walk(whole[a.n_groups] + rest[a.n_groups], (a.n + TILE_F - 1) / TILE_F, block / group_blocks, blocks / group_blocks);
-    TcCursor cur = {whole, rest, lo, hi, a.n_groups, 0, 0, 0, false};
+    const int n_active = s_active;
+    TileWalk walk(whole[n_active] + (rest[n_active] & 0xffff), (a.n + TILE_F - 1) / TILE_F, block / group_blocks, blocks / group_blocks);
+    TcCursor cur = {whole, rest, lo, hi, n_active, 0, 0, 0, false};
 
     // steps of this block for a tile of group g
     auto range = [&](int g, int &s0, int &s1) {
@@ -408,7 +416,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     for (; walk.more(); walk.next(), ++turn) {
         const int f0 = walk.feature * TILE_F + half * kTcFeatures;
         cur.seek(walk.tile, NT);
-        const int g = cur.group, slot0 = cur.slot0, slot1 = cur.slot1, columns = columns_of(cur);
+        const int g = cur.number(), slot0 = cur.slot0, slot1 = cur.slot1, columns = columns_of(cur);
         int s0, s1;
         range(g, s0, s1);
         const int buf = turn & 1;
