@@ -233,10 +233,11 @@ struct TcShape {
 };
 
 // A cursor over the tiles of all groups that have slots (a few rows of many experts leave most without, and a walk past those
-// costs 40 ns each: 32 slots of 256 matrices of 2048 x 1024 40 -> 28 us): tile numbers only rise, so the group is found by walking on.  Where the matrix is shared
-// the whole tiles of every group come first and then the groups' rests: blocks take tiles in turn, and the short ones at the end
-// even out what the long ones leave (4096 rows of 8 adapters: 160 -> 152 us).  With a matrix per group a group's tiles stay
-// together, its rest counted among them, or the matrices would be read twice (32 groups: 257 -> 270 us).
+// costs 40 ns each: 32 slots of 256 matrices of 2048 x 1024 40 -> 28 us).  Tile numbers only rise, so the group is found by
+// walking on.  Where the matrix is shared the whole tiles of every group come first and then the groups' rests: blocks take tiles
+// in turn, and the short ones at the end even out what the long ones leave (4096 rows of 8 adapters: 160 -> 152 us).  With a
+// matrix per group a group's tiles stay together, its rest counted among them, or the matrices would be read twice (32 groups:
+// 257 -> 270 us).
 struct TcCursor {
     const int *whole, *rest, *lo, *hi;  // whole tiles before every group and (rests before it | its number << 16), n_groups + 1 each; its slots
     int n_groups, group, slot0, slot1;

@@ -281,6 +281,13 @@ def test_product_and_gradients(mps, cuda, dtype, k, n, counts, per_row, padded):
     mps.routed_check()
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("k,n,counts", [(128, 512, [0] * 1000 + [700] + [0] * 20 + [40, 0, 0]), (256, 72, [5] + [0] * 1022 + [70]), (64, 320, [0] * 40 + [9] + [0] * 60)])
+def test_product_of_few_groups_of_many(mps, cuda, dtype, k, n, counts):
+    """Groups without slots, in every place and for narrow and wide tiles: passed over by the products, zeros in the gradient."""
+    test_product_and_gradients(mps, cuda, dtype, k, n, counts, 1, 0)
+
+
 @pytest.mark.parametrize("dtype,k,n", [(BF16, 256, 192), (F16, 72, 40), (F32, 30, 20)])
 def test_product_rows_do_not_meet(mps, cuda, dtype, k, n):
     """A row of NaN or infinity reaches its own slots and its own group's matrix gradient only."""
@@ -443,6 +450,25 @@ def test_adapters_and_gradients(mps, cuda, dtype, rows, n_adapters, rank, k, n, 
         close(f64(g), want[0], dtype, t, want[1], o.PAIR[dtype] * want[2] + o.FLOOR[dtype] * want[3])
     ones = torch.ones(n_adapters, device="cuda")
     assert torch.equal(mps.adapters(x, w, a, b, d_ids, groups), mps.adapters(x, w, a, b, d_ids, groups, ones))
+    mps.routed_check()
+
+
+@pytest.mark.parametrize("rows", [9, 1500])
+def test_few_adapters_of_many(mps, cuda, rows):
+    gen = gen_of(rows)
+    ids = np.array([3, 700, 1023, -1, 700], np.int32)[np.random.default_rng(rows).integers(0, 5, rows)]
+    n_adapters, rank, k, n = 1024, 16, 128, 192
+    d_ids = torch.from_numpy(ids).cuda()
+    groups = mps.group_rows(d_ids, n_adapters)
+    x, w, dy = rand(gen, BF16, rows, k), rand(gen, BF16, n, k, scale=k ** -0.5), rand(gen, BF16, rows, n, scale=0.1)
+    a, b = rand(gen, BF16, n_adapters, rank, k, scale=k ** -0.5), rand(gen, BF16, n_adapters, n, rank, scale=rank ** -0.5)
+    scale = torch.rand(n_adapters, generator=gen, device="cuda") + 0.5
+    want = o.adapters(f64(x), f64(w), f64(a), f64(b), ids, f64(scale))
+    close(f64(mps.adapters(x, w, a, b, d_ids, groups, scale)), want[0], BF16, k + rank + 2, want[1], o.PAIR[BF16] * want[2] + o.FLOOR[BF16] * want[3])
+    got = mps.adapters_backward(dy, x, w, a, b, d_ids, groups, scale)
+    terms = (n + rank + 2, n + rows + 2, k + rows + 2)
+    for g, want, t in zip(got, o.adapters_grad(f64(dy), f64(x), f64(w), f64(a), f64(b), ids, f64(scale)), terms):
+        close(f64(g), want[0], BF16, t, want[1], o.PAIR[BF16] * want[2] + o.FLOOR[BF16] * want[3])
     mps.routed_check()
 
 
