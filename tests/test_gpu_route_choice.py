@@ -1,0 +1,91 @@
+"""The router's choice where it is hard to tell, against the 64-bit definition: equal keys at the last place, and keys in one bucket
+of the packed form."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+import routed_oracle as o
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+FEW, MANY = 40, 2061  # a warp per row; eight lanes per row (from 2048 rows on)
+
+
+def ids_of(mps, logits, top, **kw):
+    ids = mps.route(logits, top, group=False, **kw)[0]
+    mps.routed_check()
+    return ids.cpu().numpy()
+
+
+def same_choice(mps, logits, top, **kw):
+    """As the definition has it, and the same whether the rows come at once or a few at a time."""
+    want, _ = o.route(logits.detach().cpu().double().numpy(), top, kw.get("score", "softmax"), None if kw.get("bias") is None else kw["bias"].cpu().double().numpy(),
+                      kw.get("n_groups", 1), kw.get("top_groups", 1), kw.get("group_top", 1))
+    got = ids_of(mps, logits, top, **kw)
+    bad = np.argwhere((got != want).any(1)).ravel()
+    assert not bad.size, (bad.size, bad[:4], got[bad[:4]], want[bad[:4]])
+
+
+@pytest.mark.parametrize("rows", [FEW, MANY])
+@pytest.mark.parametrize("experts", [24, 64, 200])
+@pytest.mark.parametrize("places", [(0, 1, 2), (0, 9, 18), (5, 3, 20), (2, 0, 1)])
+def test_equal_logits_before_a_larger_one(mps, cuda, rows, experts, places):
+    """Two equal logits, and one a unit in the last place above them, asked for the best one and the best two."""
+    logits = torch.rand(rows, experts, generator=torch.Generator(device="cuda").manual_seed(experts), device="cuda") - 3
+    first, second, third = places
+    logits[:, first] = logits[:, second] = 1.0
+    logits[:, third] = float(np.nextafter(np.float32(1.0), np.float32(2.0)))
+    for top in (1, 2):
+        same_choice(mps, logits, top)
+        same_choice(mps, -logits, top)  # negative keys
+        same_choice(mps, logits, top, n_groups=8, top_groups=8, score="sigmoid")
+
+
+@pytest.mark.parametrize("rows", [FEW, MANY])
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("equals", [2, 3, 7])
+def test_equal_keys_at_the_last_place(mps, cuda, rows, dtype, score, equals):
+    """Keys that fp32 cannot tell apart: several experts of equal logit and bias, and later ones whose score is larger or smaller
+    by less than fp32 resolves."""
+    logits = torch.full((rows, 64), -40.0, dtype=dtype, device="cuda")
+    base = 20.0 if score == "sigmoid" else 0.0  # a sigmoid of 20 and more is 1 in fp32
+    logits[:, 4:4 + equals] = base
+    logits[::2, 30] = base + 0.125
+    logits[1::2, 30] = base - 0.125
+    logits[::3, 50] = base + 0.25
+    if score == "softmax":
+        logits[:, 63] = 60.0  # the others' scores are below 1e-22: nothing beside the bias
+    bias = torch.zeros(64, device="cuda")
+    bias[4:51] = 1.0
+    for top in (1, 2, 3, equals, equals + 1, equals + 2):
+        same_choice(mps, logits, top, score=score, bias=bias)
+        same_choice(mps, logits, top, score=score, bias=bias, n_groups=4, top_groups=4)
+
+
+@pytest.mark.parametrize("rows", [FEW * 8, 4096])
+@pytest.mark.parametrize("top", [1, 2])
+def test_keys_beside_a_bucket_edge(mps, cuda, rows, top):
+    """Keys around a number whose last five bits are zeros: the best is just above it, one just below, and one further down with a
+    lower index.  Their distance is a few units of fp32's last place, which is what the scores' errors are."""
+    rng = np.random.default_rng(rows + top)
+    experts = 32
+    bias = (1.0 - rng.random(experts) * 0.5).astype(np.float32)
+    logits = np.full((rows, experts), -9.0)
+    edge = 1 + 2.0 ** -18 * rng.integers(20000, 40000, rows)  # multiples of 32 units of [1, 2)
+
+    def put(e, key):
+        logits[:, e] = np.log((key - bias[e]) / (1 - (key - bias[e])))
+
+    unit = 2.0 ** -23
+    put(0, edge - (20 + 10 * rng.random(rows)) * unit)
+    put(1, edge + rng.normal(size=rows) * 2 * unit)
+    put(2, edge + rng.normal(size=rows) * 2 * unit)
+    if top == 2:
+        put(3, edge + 0.01)
+    order = np.concatenate([rng.permutation(4), np.arange(4, experts)])
+    for at in (np.arange(experts), order):
+        same_choice(mps, torch.from_numpy(np.ascontiguousarray(logits[:, at], dtype=np.float32)).cuda(), top, score="sigmoid", bias=torch.from_numpy(bias[at]).cuda())
