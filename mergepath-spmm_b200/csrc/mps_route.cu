@@ -112,6 +112,11 @@ __device__ __forceinline__ double key_div(double x, double y) { return x / y; }
 // that for two keys.
 template <bool SIGMOID>
 __device__ __forceinline__ float clearance(float key) { return (SIGMOID ? 1e-6f : 6e-6f) + 2.5e-7f * fabsf(key); }
+// How far a group's fp32 rank may be off: half of that for each of the keys it is made of, which may cancel, and the sum's rounding.
+template <bool SIGMOID>
+__device__ __forceinline__ float rank_error(float one, float two, bool both) {
+    return 0.5f * clearance<SIGMOID>(one) + (both ? 0.5f * clearance<SIGMOID>(two) + 6e-8f * fabsf(one + two) : 0.0f);
+}
 
 // Keeps the experts of the best groups: key of the others becomes -inf.  `cells` is this warp's shared row of n_experts
 // (+ padding) values.  Returns false where fp32 cannot tell the last group kept from the first one dropped.
@@ -144,23 +149,24 @@ __device__ __forceinline__ bool keep_groups(F (&key)[VPL], const F (&value)[VPL]
         two = two > low ? two : low;
     }
     F rank = one;
-    if (a.group_top == 2 && two > neg_inf<F>()) rank = one + two;
+    const bool both = a.group_top == 2 && two > neg_inf<F>();
+    if (both) rank = one + two;
     if (g >= a.n_groups || lane % parts) rank = neg_inf<F>();
+    const F own = rank;
     unsigned kept = 0;
-    F last = neg_inf<F>();
     for (int j = 0; j < a.top_groups; ++j) {
         F best = rank;
         int at = lane;
         warp_best(best, at);
         if (!(best > neg_inf<F>())) break;
         kept |= 1u << (at / parts);
-        last = best;
         if (lane == at) rank = neg_inf<F>();
     }
     bool clear = true;
     if (sizeof(F) == 4) {
-        const float next = (float)warp_max(rank);
-        clear = !((float)last - next <= 2 * clearance<SIGMOID>((float)last)) || !(next > -INFINITY);
+        const float off = rank_error<SIGMOID>((float)one, (float)two, both);
+        const float least = -warp_max(rank != own ? off - (float)own : -INFINITY), most = warp_max(rank > neg_inf<F>() ? (float)rank + off : -INFINITY);
+        clear = least > most;
     }
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
@@ -452,7 +458,8 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 6) route_octet_kernel(const 
                 two = fmaxf(fmaxf(two, o2), fminf(one, o1));
                 one = fmaxf(one, o1);
             }
-            const float rank = a.group_top == 2 && two > -INFINITY ? one + two : one;
+            const bool both = a.group_top == 2 && two > -INFINITY;
+            const float rank = both ? one + two : one;
             int better = 0;
             for (int d = per_group; d < 8; d += per_group) {  // every other group once
                 const float o = __shfl_xor_sync(kAll, rank, d);
@@ -460,8 +467,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 6) route_octet_kernel(const 
             }
             const bool kept = better < a.top_groups && rank > -INFINITY;
             if (need_score) {  // logits compare exactly
-                const float last = -row_max(kept ? -rank : -INFINITY), next = row_max(kept ? -INFINITY : rank);
-                clear = !(next > -INFINITY) || !(last - next <= 2 * clearance<SIGMOID>(last));
+                const float off = rank_error<SIGMOID>(one, two, both);
+                const float least = -row_max(kept ? off - rank : -INFINITY), most = row_max(!kept && rank > -INFINITY ? rank + off : -INFINITY);
+                clear = least > most;
             }
             if (!kept) {
 #pragma unroll

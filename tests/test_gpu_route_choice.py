@@ -1,5 +1,5 @@
-"""The router's choice where it is hard to tell, against the 64-bit definition: equal keys at the last place, and keys in one bucket
-of the packed form."""
+"""The router's choice where it is hard to tell, against the 64-bit definition: equal keys at the last place, keys in one bucket
+of the packed form, and group ranks whose two keys cancel."""
 import math
 
 import numpy as np
@@ -89,3 +89,19 @@ def test_keys_beside_a_bucket_edge(mps, cuda, rows, top):
     order = np.concatenate([rng.permutation(4), np.arange(4, experts)])
     for at in (np.arange(experts), order):
         same_choice(mps, torch.from_numpy(np.ascontiguousarray(logits[:, at], dtype=np.float32)).cuda(), top, score="sigmoid", bias=torch.from_numpy(bias[at]).cuda())
+
+
+@pytest.mark.parametrize("rows", [FEW * 10, MANY])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("size", [1000.0, 3e5])
+def test_group_ranks_whose_keys_cancel(mps, cuda, rows, score, size):
+    """Groups of two experts with biases of +size and -size: the ranks are sums of the two scores, far finer than either key."""
+    rng = np.random.default_rng(int(size))
+    logits = rng.normal(size=(rows, 16)).astype(np.float32)
+    if score == "sigmoid":  # neighbouring groups' sums of scores within the rounding of a key of one another
+        s = 1 / (1 + np.exp(-logits.astype(np.float64)))
+        want = np.clip(s[:, 0] + s[:, 1] - s[:, 2] + rng.normal(size=rows) * size * 2.0 ** -24, 1e-3, 1 - 1e-3)
+        logits[:, 3] = np.log(want / (1 - want))
+    bias = np.tile([size, -size], 8).astype(np.float32)
+    same_choice(mps, torch.from_numpy(logits).cuda(), 2, score=score, bias=torch.from_numpy(bias).cuda(), n_groups=8, top_groups=1, group_top=2)
+    same_choice(mps, torch.from_numpy(logits).cuda(), 3, score=score, bias=torch.from_numpy(bias).cuda(), n_groups=8, top_groups=4, group_top=2)
