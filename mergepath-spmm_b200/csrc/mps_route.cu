@@ -166,7 +166,10 @@ __device__ __forceinline__ bool keep_groups(F (&key)[VPL], const F (&value)[VPL]
     if (sizeof(F) == 4) {
         const float off = rank_error<SIGMOID>((float)one, (float)two, both);
         const float least = -warp_max(rank != own ? off - (float)own : -INFINITY), most = warp_max(rank > neg_inf<F>() ? (float)rank + off : -INFINITY);
-        clear = least > most;
+        // the sum of two keys of the type's lowest or largest value has left fp32, though neither key has
+        const bool beyond = (float)one > -INFINITY && !(fabsf((float)own) < INFINITY) && g < a.n_groups && lane % parts == 0;
+        const bool none_beyond = !__any_sync(kAll, beyond);
+        clear = least > most && none_beyond;
     }
 #pragma unroll
     for (int i = 0; i < VPL; ++i) {
@@ -469,7 +472,9 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 6) route_octet_kernel(const 
             if (need_score) {  // logits compare exactly
                 const float off = rank_error<SIGMOID>(one, two, both);
                 const float least = -row_max(kept ? off - rank : -INFINITY), most = row_max(!kept && rank > -INFINITY ? rank + off : -INFINITY);
-                clear = least > most;
+                const bool beyond = one > -INFINITY && !(fabsf(rank) < INFINITY);  // see keep_groups
+                const unsigned lanes_beyond = __ballot_sync(kAll, beyond);  // by all lanes: rows differ in what they compare
+                clear = least > most && !(lanes_beyond >> (quad * 8) & 0xff);
             }
             if (!kept) {
 #pragma unroll

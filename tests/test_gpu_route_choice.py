@@ -1,5 +1,5 @@
 """The router's choice where it is hard to tell, against the 64-bit definition: equal keys at the last place, keys in one bucket
-of the packed form, and group ranks whose two keys cancel."""
+of the packed form, and group ranks whose two keys cancel or leave fp32's range."""
 import math
 
 import numpy as np
@@ -105,3 +105,24 @@ def test_group_ranks_whose_keys_cancel(mps, cuda, rows, score, size):
     bias = np.tile([size, -size], 8).astype(np.float32)
     same_choice(mps, torch.from_numpy(logits).cuda(), 2, score=score, bias=torch.from_numpy(bias).cuda(), n_groups=8, top_groups=1, group_top=2)
     same_choice(mps, torch.from_numpy(logits).cuda(), 3, score=score, bias=torch.from_numpy(bias).cuda(), n_groups=8, top_groups=4, group_top=2)
+
+
+@pytest.mark.parametrize("rows", [FEW, MANY])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("value", [torch.finfo(F32).min, torch.finfo(F32).max])
+def test_group_ranks_beyond_the_type(mps, cuda, rows, score, value):
+    """Experts masked (or forced) by a bias of the type's lowest (largest) value: the sum of two such keys has left fp32, the group
+    has not left the choice."""
+    logits = torch.randn(rows, 32, generator=torch.Generator(device="cuda").manual_seed(3), device="cuda")
+    for masked in (slice(0, 16), slice(8, 32), slice(0, 32), slice(8, 30)):
+        bias = torch.zeros(32, device="cuda")
+        bias[masked] = value
+        for n_groups, top_groups in ((4, 2), (4, 3), (8, 5), (2, 1)):
+            same_choice(mps, logits, 6, score=score, bias=bias, n_groups=n_groups, top_groups=top_groups, group_top=2)
+
+
+MANY_FORMS = [
+    # experts, groups, top_groups, group_top, top: every width of the eight-lane form, its groups, and choices in each of its lanes' places
+    (8, 1, 1, 1, 8), (64, 2, 1, 2, 17), (72, 1, 1, 1, 9), (72, 4, 2, 2, 24), (128, 1, 1, 1, 1), (128, 2, 1, 1, 16), (128, 4, 3, 2, 32), (128, 8, 4, 2, 8),
+    (136, 8, 2, 1, 12), (200, 2, 2, 2, 32), (200, 1, 1, 1, 16), (256, 1, 1, 1, 8), (256, 2, 1, 2, 1), (256, 4, 2, 1, 16), (256, 8, 4, 2, 8), (256, 8, 3, 2, 32),
+]
