@@ -1,5 +1,5 @@
-"""The router's choice where it is hard to tell, against the 64-bit definition: equal keys at the last place, keys in one bucket
-of the packed form, and group ranks whose two keys cancel or leave fp32's range."""
+"""The router's choice where it is hard to tell (equal keys at the last place, keys in one bucket of the packed form, group ranks
+whose two keys cancel or leave fp32's range), and every form of the kernel for many rows, against the 64-bit definition."""
 import math
 
 import numpy as np
@@ -126,3 +126,41 @@ MANY_FORMS = [
     (8, 1, 1, 1, 8), (64, 2, 1, 2, 17), (72, 1, 1, 1, 9), (72, 4, 2, 2, 24), (128, 1, 1, 1, 1), (128, 2, 1, 1, 16), (128, 4, 3, 2, 32), (128, 8, 4, 2, 8),
     (136, 8, 2, 1, 12), (200, 2, 2, 2, 32), (200, 1, 1, 1, 16), (256, 1, 1, 1, 8), (256, 2, 1, 2, 1), (256, 4, 2, 1, 16), (256, 8, 4, 2, 8), (256, 8, 3, 2, 32),
 ]
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("experts,n_groups,top_groups,group_top,top", MANY_FORMS)
+def test_many_rows(mps, cuda, dtype, experts, n_groups, top_groups, group_top, top):
+    from test_gpu_routed import check_route
+    gen = torch.Generator(device="cuda").manual_seed(experts + top)
+    rows = MANY
+    logits = (torch.randn(rows, experts, generator=gen, device="cuda") * 1.5).to(dtype)
+    bias = torch.randn(experts, generator=gen, device="cuda") * 0.05
+    groups = dict(n_groups=n_groups, top_groups=top_groups, group_top=group_top)
+    check_route(mps, logits, top, score="sigmoid", bias=bias, scale=2.5, **groups)
+    check_route(mps, logits, top, renormalise=False, **groups)
+    logits[:, torch.rand(experts, generator=gen, device="cuda") < 0.4] = -math.inf  # masked experts, and rows with none left
+    logits[::3] = -math.inf
+    logits[1::7, : max(1, experts // 2)] = torch.finfo(dtype).min
+    flat = torch.empty(rows * experts + 1, dtype=dtype, device="cuda")  # the same rows off 16 bytes
+    shifted = flat[1:].view(rows, experts)
+    shifted.copy_(logits)
+    for score, b, renormalise in (("softmax", bias, True), ("sigmoid", None, False)):
+        ids, weights = check_route(mps, logits, top, score=score, bias=b, renormalise=renormalise, **groups)
+        again, same, _ = mps.route(shifted, top, score=score, bias=b, renormalise=renormalise, **groups)
+        assert torch.equal(ids, again) and torch.equal(weights, same)
+        few = torch.cat([mps.route(part, top, score=score, bias=b, renormalise=renormalise, group=False, **groups)[0] for part in logits.split(1000)])
+        assert torch.equal(ids, few)
+
+
+@pytest.mark.parametrize("experts,n_groups,top", [(128, 1, 9), (128, 8, 9), (256, 1, 20), (256, 4, 20)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("biased", [False, True])
+def test_many_rows_of_equal_and_close_keys(mps, cuda, experts, n_groups, top, score, biased):
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    equal = torch.randint(-2, 3, (MANY, experts), generator=gen, device="cuda").float()
+    close = 3 + torch.rand(MANY, experts, generator=gen, device="cuda") * 1e-5  # a few units in the last place apart
+    bias = torch.randint(0, 2, (experts,), generator=gen, device="cuda").float() * 0.25 if biased else None
+    for logits in (equal, equal.bfloat16(), close):
+        for group_top in (1, 2):
+            same_choice(mps, logits, top, score=score, bias=bias, n_groups=n_groups, top_groups=max(1, n_groups // 2), group_top=group_top)
