@@ -459,8 +459,8 @@ MPS_API int mps_routed_combine_backward(int32_t n_rows, int32_t per_row, int32_t
  *   y[t, :] = x[t, :] W^T + scale[a] (x[t, :] A[a]^T) B[a]^T,  a = ids[t]; a row with a negative id gets the projection alone.
  * d_x n_rows x k, d_w n x k, d_a n_adapters x rank x k, d_b n_adapters x n x rank, d_scale n_adapters fp32 (NULL: 1), d_y
  * n_rows x n.  d_group_ptr and d_slot_row list the rows by adapter (mps_group_rows of d_ids, per_row 1).  n_adapters <= 1024,
- * rank <= 4096.  With 16-bit types the intermediate scale * x A^T is kept to twice their digits; in fp16 it has to stay inside
- * fp16's range (65504).  d_workspace: mps_adapters_workspace bytes (a negative return is an error), 256-byte aligned, for this call
+ * rank <= 4096.  The intermediate scale * x A^T is kept in fp32; with 16-bit types the second product may read it as the sum of two
+ * tf32 values (2^-21 of it at most are lost).  A group's rows may be listed in any order.  d_workspace: mps_adapters_workspace bytes (a negative return is an error), 256-byte aligned, for this call
  * alone while it runs. */
 MPS_API int64_t mps_adapters_workspace(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, int backward);
 MPS_API int mps_adapters(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, const int32_t *d_ids,
@@ -468,7 +468,9 @@ MPS_API int mps_adapters(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapter
                  const void *d_a, const void *d_b, void *d_y, void *d_workspace, int64_t workspace_bytes, void *stream);
 
 /* Its gradients by x, A and B (the shared projection and the scales are constants), each written whole:
- *   dx = dy W + scale (dy B) A,   dA[a] = scale sum (dy B)^T x,   dB[a] = scale sum dy^T (x A^T)   over the rows of a. */
+ *   dx = dy W + scale (dy B) A,   dA[a] = scale sum (dy B)^T x,   dB[a] = scale sum dy^T (x A^T)   over the rows of a.
+ * With 16-bit types dA and dB may read the intermediates scale * dy B and scale * x A^T as two values of the type (2^-16 of each lost
+ * in bf16; 2^-22 in fp16, or 2^-40 of the adapter's largest where that is more). */
 MPS_API int mps_adapters_backward(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, const int32_t *d_ids,
                           const int32_t *d_group_ptr, const int32_t *d_slot_row, const float *d_scale, const void *d_dy,
                           const void *d_x, const void *d_w, const void *d_a, const void *d_b, void *d_dx, void *d_da, void *d_db,

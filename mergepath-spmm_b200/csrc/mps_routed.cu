@@ -5,6 +5,7 @@
 
 #include <cmath>
 #include <initializer_list>
+#include <type_traits>
 
 #include "mps_internal.h"
 #include "mps_routed_plain.cuh"
@@ -257,8 +258,8 @@ int sm_count(int *n) {
     return MPS_OK;
 }
 
-// Tensor map of `dims` sizes (innermost first, rows packed) of a 16-bit type, read in boxes of 64 elements by box_rows.
-int tensor_map(CUtensorMap *map, bool bf16, const void *base, int dims, unsigned long long d0, unsigned long long d1, unsigned long long d2, int box_rows) {
+// Tensor map of `dims` sizes (innermost first, rows packed) of one of the types, read in boxes of 128 bytes by box_rows.
+int tensor_map(CUtensorMap *map, int dtype, const void *base, int dims, unsigned long long d0, unsigned long long d1, unsigned long long d2, int box_rows) {
     typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
                                const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
     static const Encode encode = [] {
@@ -268,9 +269,11 @@ int tensor_map(CUtensorMap *map, bool bf16, const void *base, int dims, unsigned
         return (Encode)fn;
     }();
     if (!encode) return fail(MPS_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-    const cuuint64_t size[3] = {d0, d1, d2}, pitch[2] = {d0 * 2, d0 * d1 * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
-    const CUresult rc = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, dims, const_cast<void *>(base), size, pitch,
+    const unsigned bytes = (unsigned)size_of(dtype);
+    const cuuint64_t size[3] = {d0, d1, d2}, pitch[2] = {d0 * bytes, d0 * d1 * bytes};
+    const cuuint32_t box[3] = {128 / bytes, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    const CUtensorMapDataType type = dtype == MPS_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : dtype == MPS_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult rc = encode(map, type, dims, const_cast<void *>(base), size, pitch,
                                box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (rc != CUDA_SUCCESS) return fail(MPS_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %llu x %llu x %llu", (int)rc, d0, d1, d2);
@@ -358,7 +361,9 @@ void share_blocks(int sms, int cluster, const long long (&tiles)[2], const doubl
     blocks[1] = second * cluster;
 }
 
-template <int NT, bool TWO>
+int type_of(bool bf16) { return bf16 ? MPS_BF16 : MPS_F16; }
+
+template <int NT, bool TWO, bool RANK = false>
 int launch_tc_rows(const mps::TcRowsLaunch &in, int sms, int *used, cudaStream_t st) {
     mps::TcRowsLaunch l = in;
     const int tile_f = mps::kTcFeatures * (mps::TcShape<NT>::kPaired ? 2 : 1), cluster = mps::TcShape<NT>::kPaired ? 2 : l.p[0].split;
@@ -374,7 +379,7 @@ int launch_tc_rows(const mps::TcRowsLaunch &in, int sms, int *used, cudaStream_t
     share_blocks(sms, cluster, tiles, work, blocks);
     l.second = (int)blocks[0];
     if (used) *used = (int)(blocks[0] + blocks[1]);
-    return launch_tc<mps::tc_rows_kernel<NT, TWO>>(l, blocks[0] + blocks[1], cluster, mps::TcShape<NT>::bytes(l.p[0].n_groups), l.p[0].follows, st);
+    return launch_tc<mps::tc_rows_kernel<NT, TWO, RANK>>(l, blocks[0] + blocks[1], cluster, mps::TcShape<NT>::bytes(l.p[0].n_groups), l.p[0].follows, st);
 }
 
 // One product, or two of the same groups side by side (at most 64 slots per tile): what every use has in common filled in.  x_rows: rows of each x.
@@ -387,13 +392,22 @@ int tc_rows(const TcRows *products, int n, const Cut &cut, const void *const *x,
         a = products[i];
         if (int rc = status_pointer(&a.status)) return rc;
         a.split = cut.split;
-        if (int rc = tensor_map(&a.x, a.bf16, x[i], 2, a.k, x_rows, 1, a.gather ? 1 : loaded)) return rc;
+        if (int rc = tensor_map(&a.x, type_of(a.bf16), x[i], 2, a.k, x_rows, 1, a.gather ? 1 : loaded)) return rc;
         if (a.gather)
-            if (int rc = tensor_map(&a.x_run, a.bf16, x[i], 2, a.k, x_rows, 1, loaded / 8)) return rc;
-        if (a.rank)
-            if (int rc = tensor_map(&a.u, a.bf16, a.u_base, 2, a.rank, 2ull * a.u_plane, 1, loaded / 8)) return rc;
+            if (int rc = tensor_map(&a.x_run, type_of(a.bf16), x[i], 2, a.k, x_rows, 1, loaded / 8)) return rc;
+        if (a.rank) {
+            if (int rc = tensor_map(&a.u, MPS_F32, a.u_base, 2, a.rank, 2ull * x_rows, 1, 1)) return rc;
+            if (int rc = tensor_map(&a.u_run, MPS_F32, a.u_base, 2, a.rank, 2ull * x_rows, 1, loaded / 8)) return rc;
+            if (int rc = tensor_map(&a.w2, MPS_F32, a.w2_base, 3, a.rank, a.n, a.rank_groups, a.w_rows)) return rc;
+        }
     }
     if (n == 2) return cut.nt == 32 ? launch_tc_rows<32, true>(l, sms, used, st) : launch_tc_rows<64, true>(l, sms, used, st);
+    if (l.p[0].rank) {
+        if (cut.nt == 32) return launch_tc_rows<32, false, true>(l, sms, used, st);
+        if (cut.nt == 64) return launch_tc_rows<64, false, true>(l, sms, used, st);
+        if (cut.nt == 128) return launch_tc_rows<128, false, true>(l, sms, used, st);
+        return launch_tc_rows<256, false, true>(l, sms, used, st);
+    }
     if (cut.nt == 32) return launch_tc_rows<32, false>(l, sms, used, st);
     if (cut.nt == 64) return launch_tc_rows<64, false>(l, sms, used, st);
     if (cut.nt == 128) return launch_tc_rows<128, false>(l, sms, used, st);
@@ -403,8 +417,8 @@ int tc_rows(const TcRows *products, int n, const Cut &cut, const void *const *x,
 // The matrices of a: stored features x summed (MN-major: summed x features), `groups` of them.
 int tc_matrix(CUtensorMap *map, TcRows *a, const void *w, int summed, int features, long long groups) {
     a->w_rows = features < mps::kTcFeatures ? (features + 7) / 8 * 8 : mps::kTcFeatures;
-    return a->mn_major ? tensor_map(map, a->bf16, w, 3, features, summed, groups, mps::kTcDepth)
-                       : tensor_map(map, a->bf16, w, 3, summed, features, groups, a->w_rows);
+    return a->mn_major ? tensor_map(map, type_of(a->bf16), w, 3, features, summed, groups, mps::kTcDepth)
+                       : tensor_map(map, type_of(a->bf16), w, 3, summed, features, groups, a->w_rows);
 }
 
 template <int NT, bool TWO>
@@ -437,10 +451,10 @@ int tc_outer(const TcOuter *products, int n, const void *const *p, const void *c
         a = products[i];
         if (int rc = status_pointer(&a.status)) return rc;
         const unsigned long long q_rows = (a.pair ? 2ull : 1ull) * a.n_slots;
-        if (int rc = tensor_map(&a.p_rows, a.bf16, p[i], 2, a.i, a.n_p_rows, 1, 1)) return rc;
-        if (int rc = tensor_map(&a.p_tile, a.bf16, p[i], 2, a.i, a.n_p_rows, 1, mps::kTcDepth)) return rc;
-        if (int rc = tensor_map(&a.q_rows, a.bf16, q[i], 2, a.j, q_rows, 1, 1)) return rc;
-        if (int rc = tensor_map(&a.q_tile, a.bf16, q[i], 2, a.j, q_rows, 1, mps::kTcDepth)) return rc;
+        if (int rc = tensor_map(&a.p_rows, type_of(a.bf16), p[i], 2, a.i, a.n_p_rows, 1, 1)) return rc;
+        if (int rc = tensor_map(&a.p_tile, type_of(a.bf16), p[i], 2, a.i, a.n_p_rows, 1, mps::kTcDepth)) return rc;
+        if (int rc = tensor_map(&a.q_rows, type_of(a.bf16), q[i], 2, a.j, q_rows, 1, 1)) return rc;
+        if (int rc = tensor_map(&a.q_tile, type_of(a.bf16), q[i], 2, a.j, q_rows, 1, mps::kTcDepth)) return rc;
     }
     if (n == 2) return launch_tc_outer<128, true>(l, sms, st);
     return l.p[0].j <= 128 ? launch_tc_outer<128, false>(l, sms, st) : launch_tc_outer<256, false>(l, sms, st);
@@ -511,31 +525,60 @@ int adapter_wide(const AdapterShape &s, int k, int n, const void *x, const void 
     return launch_plain_rows<T, T, true>(a, x, w, m, out, st);
 }
 
-// Workspace: the two intermediates (fp32 by row, or hi and lo planes by slot: 4 bytes a value either way), the gradient's second
-// one in fp32 as well, then the rows listed with those that ask for no adapter behind the others.
+// Whether the shared matrix is read once for rows of any adapter, the low-rank part added in fp32 by the warps that store the
+// results (six multiply-adds a cycle and SM, 1.5 from matrices stored by rank, as measured), or per adapter, the low-rank part
+// summed on the tensor cores.  Measured at 4096 x 4096 in bf16, rank 16: 64 rows of 24 adapters 20 us by rows and 81 us by
+// adapter, 256 rows of 64 adapters 41 and 207, 1024 rows of 8 adapters 125 and 76; 4096 rows of 8 adapters of rank 64 1046 and 129.
+// Made for the SMs of a B200 whatever the device has free, so that a call decides as its workspace's size was decided.
+bool by_rows(const AdapterShape &s, int k, int n, bool by_rank, Cut *cut) {
+    constexpr int sms = 148;
+    const Cut grouped = best_cut(s.n_rows, s.n_adapters + 1, n, steps_of(k) + 2 * ((s.rank + mps::kRankDepth - 1) / mps::kRankDepth), true, sms, 256);
+    const Cut rows = best_cut(s.n_rows, 1, n, steps_of(k), false, sms, 64);
+    const double low_rank = (double)s.n_rows * n * s.rank / ((by_rank ? 1.5 : 6.0) * sms);
+    *cut = rows.cycles + low_rank < grouped.cycles ? rows : grouped;
+    return rows.cycles + low_rank < grouped.cycles;
+}
+
+// Workspace.  The intermediates in fp32, by row; where rows are tiled by adapter the one that the wide product reads as two planes
+// of tf32 values, and the adapters' matrices in fp32 with the rank contiguous; for the matrix gradients both intermediates as two
+// planes of the type in slot order with their exponents, and the magnitudes these come from; then the rows listed with those that
+// ask for no adapter behind the others.  Where no tensor map describes the operands the first two are all.
 struct AdapterSpace {
-    char *u, *v, *v_f32;
-    int *ptr, *row;
+    float *u, *v, *wide, *m;
+    uint16_t *u_planes, *v_planes;
+    unsigned *u_maxima, *v_maxima;
+    int *u_exponents, *v_exponents, *ptr, *row;
+    bool rows;  // see by_rows
+    Cut cut;
     int64_t bytes;
-    AdapterSpace(void *base, int n_rows, int n_adapters, int rank, bool backward) {
+    AdapterSpace(void *base, const AdapterShape &s, bool backward) {
         char *at = (char *)base;
-        auto take = [&](int64_t size) {
-            char *p = at;
-            at += (size + 255) / 256 * 256;
-            return p;
+        auto take = [&](auto *&p, bool wanted, int64_t count) {
+            p = wanted ? (std::remove_reference_t<decltype(p)>)at : nullptr;
+            if (wanted) at += (count * (int64_t)sizeof(*p) + 255) / 256 * 256;
         };
-        u = take((int64_t)n_rows * rank * 4);
-        v = backward ? take((int64_t)n_rows * rank * 4) : nullptr;
-        v_f32 = backward ? take((int64_t)n_rows * rank * 4) : nullptr;
-        ptr = (int *)take(4ll * (n_adapters + 2));
-        row = (int *)take(4ll * n_rows);
+        const int64_t values = (int64_t)s.n_rows * s.rank;
+        const bool tc = s.dtype != MPS_F32 && s.k % 8 == 0 && s.rank % 8 == 0 && (!backward || s.n % 8 == 0);
+        const int summed = backward ? s.n : s.k, features = backward ? s.k : s.n;  // of the wide product
+        rows = by_rows(s, summed, features, backward, &cut);
+        take(u, true, values);
+        take(v, backward, values);
+        take(wide, tc && !rows, 2 * values);
+        take(m, tc && !rows, (int64_t)s.n_adapters * features * s.rank);
+        for (int i = 0; i < 2; ++i) {
+            take(i ? v_planes : u_planes, tc && backward, 2 * values);
+            take(i ? v_maxima : u_maxima, tc && backward, (int64_t)s.n_rows * ((s.rank + 31) / 32));
+            take(i ? v_exponents : u_exponents, tc && backward, (int64_t)s.n_adapters * ((s.rank + 63) / 64));
+        }
+        take(ptr, tc && !rows, s.n_adapters + 2);
+        take(row, tc && !rows, s.n_rows);
         bytes = at - (char *)base;
     }
 };
 
-// The narrow product of rows of x with the adapters' matrices (mn_major: stored summed x rank): u (two planes, slot order) =
-// scale * x A; u_f32 (or NULL) the same by row.
-int tc_adapter_narrow(const AdapterShape &s, int k, const void *m, bool mn_major, void *u, float *u_f32, TcRows *out) {
+// The narrow product of rows of x with the adapters' matrices (mn_major: stored summed x rank): scale * x A by row, in fp32 (u), as
+// planes of tf32 values and with its largest magnitudes, each where not NULL.
+int tc_adapter_narrow(const AdapterShape &s, int k, const void *m, bool mn_major, float *u, float *u_tf32, unsigned *maxima, TcRows *out) {
     TcRows a = {};
     a.bf16 = s.dtype == MPS_BF16;
     a.mn_major = mn_major;
@@ -545,32 +588,57 @@ int tc_adapter_narrow(const AdapterShape &s, int k, const void *m, bool mn_major
     a.n_slots = a.n_x_rows = s.n_rows;
     a.k = k;
     a.n = s.rank;
-    a.gather = a.pair = true;
+    a.gather = true;
     a.group_scale = s.scale;
-    a.out = u;
-    a.out_plane = (long long)s.n_rows * s.rank;
-    a.out_f32 = u_f32;
+    a.out_f32 = u;
+    a.out_tf32 = u_tf32;
+    a.maxima = maxima;
     if (int rc = tc_matrix(&a.w, &a, m, k, s.rank, s.n_adapters)) return rc;
     *out = a;
     return MPS_OK;
 }
 
-// Whether the shared matrix is read once for rows of any adapter, the low-rank part added in fp32 by the warps that store the
-// results (six multiply-adds a cycle and SM, 1.5 from matrices stored by rank, as measured), or per adapter, the low-rank part
-// summed on the tensor cores.  Measured at 4096 x 4096 in bf16, rank 16: 64 rows of 24 adapters 20 us by rows and 81 us by
-// adapter, 256 rows of 64 adapters 41 and 207, 1024 rows of 8 adapters 125 and 76; 4096 rows of 8 adapters of rank 64 1046 and 129.
-bool by_rows(const AdapterShape &s, int k, int n, bool by_rank, int sms, Cut *cut) {
-    const Cut grouped = best_cut(s.n_rows, s.n_adapters + 1, n, steps_of(k) + 2 * steps_of(s.rank), true, sms, 256);
-    const Cut rows = best_cut(s.n_rows, 1, n, steps_of(k), false, sms, 64);
-    const double low_rank = (double)s.n_rows * n * s.rank / ((by_rank ? 1.5 : 6.0) * sms);
-    *cut = rows.cycles + low_rank < grouped.cycles ? rows : grouped;
-    return rows.cycles + low_rank < grouped.cycles;
+// What the products behind the narrow one read, see adapter_prepare_kernel.  m (or NULL): the wide product's adapter matrices.
+int tc_adapter_prepare(const AdapterShape &s, const AdapterSpace &ws, const void *m, bool by_rank, int features, bool backward, int span, int sms, cudaStream_t st) {
+    mps::PrepareArgs a = {};
+    a.group_ptr = s.group_ptr;
+    a.slot_row = s.slot_row;
+    a.n_groups = s.n_adapters;
+    a.n_slots = a.n_rows = s.n_rows;
+    a.rank = s.rank;
+    a.m = (const uint16_t *)m;
+    a.m_f32 = ws.m;
+    a.features = features;
+    a.by_rank = by_rank;
+    if (backward) {
+        a.values[0] = ws.u, a.values[1] = ws.v;
+        a.planes[0] = ws.u_planes, a.planes[1] = ws.v_planes;
+        if (s.dtype == MPS_F16) {  // bf16 has fp32's range
+            a.maxima[0] = ws.u_maxima, a.maxima[1] = ws.v_maxima;
+            a.exponents[0] = ws.u_exponents, a.exponents[1] = ws.v_exponents;
+        }
+        a.span = span;
+    }
+    if (int rc = status_pointer(&a.status)) return rc;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(2 * sms);
+    cfg.blockDim = dim3(256);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (s.dtype == MPS_BF16) RD_CUDA(cudaLaunchKernelEx(&cfg, mps::adapter_prepare_kernel<true>, a));
+    else RD_CUDA(cudaLaunchKernelEx(&cfg, mps::adapter_prepare_kernel<false>, a));
+    return MPS_OK;
 }
 
-// out = x times the shared matrix plus u times the row's adapter matrix m; u_f32 by row (by_rows) or u in planes by slot.  used
-// (or NULL): its blocks, where the launch behind it needs nothing of it and runs beside it.
-int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cut, bool rows, int k, int n, const void *x, const void *w, const void *u,
-                    const float *u_f32, const void *m, bool mn_major, void *out, bool ahead, int sms, cudaStream_t st, int *used = nullptr) {
+// out = x times the shared matrix plus u times the row's adapter matrix m: of rows of any adapter (ws.rows), with u by row, or by
+// adapter with the planes and matrices of the workspace.  used (or NULL): its blocks, where the launch behind it needs nothing of
+// it and runs beside it.
+int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, int k, int n, const void *x, const void *w, const float *u, const void *m, bool mn_major,
+                    void *out, bool ahead, int sms, cudaStream_t st, int *used = nullptr) {
     TcRows a = {};
     a.next_after = used != nullptr;
     a.bf16 = s.dtype == MPS_BF16;
@@ -581,10 +649,10 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cu
     a.w_shared = a.follows = true;
     a.out = out;
     if (int rc = tc_matrix(&a.w, &a, w, k, n, 1)) return rc;
-    if (rows) {
+    if (ws.rows) {
         a.n_groups = 1;
         a.ids = s.ids;
-        a.delta_u = u_f32;
+        a.delta_u = u;
         a.delta_m = (const uint16_t *)m;
         a.delta_adapters = s.n_adapters;
         a.delta_rank = s.rank;
@@ -592,21 +660,20 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, const Cut &cu
         a.delta_f = mn_major ? 1 : s.rank;
         a.delta_r = mn_major ? n : 1;
         a.ahead = ahead;
-        return tc_rows(&a, 1, cut, &x, s.n_rows, sms, st, used);
+        return tc_rows(&a, 1, ws.cut, &x, s.n_rows, sms, st, used);
     }
     a.group_ptr = ws.ptr;
     a.slot_row = ws.row;
     a.n_groups = s.n_adapters + 1;
     a.rank = s.rank;
     a.rank_groups = s.n_adapters;
-    a.u_base = u;
-    a.u_plane = s.n_rows;
+    a.u_base = ws.wide;
+    a.w2_base = ws.m;
     a.gather = a.scatter = true;
-    if (int rc = tc_matrix(&a.w2, &a, m, s.rank, n, s.n_adapters)) return rc;
-    return tc_rows(&a, 1, cut, &x, s.n_rows, sms, st, used);
+    return tc_rows(&a, 1, ws.cut, &x, s.n_rows, sms, st, used);
 }
 
-TcOuter tc_adapter_outer(const AdapterShape &s, int features, void *out, long long out_f, long long out_c) {
+TcOuter tc_adapter_outer(const AdapterShape &s, int features, const int *exponents, void *out, long long out_f, long long out_c) {
     TcOuter a = {};
     a.bf16 = s.dtype == MPS_BF16;
     a.group_ptr = s.group_ptr;
@@ -616,6 +683,7 @@ TcOuter tc_adapter_outer(const AdapterShape &s, int features, void *out, long lo
     a.i = features;
     a.j = s.rank;
     a.pair = a.follows = a.apart = true;  // beside the rows' gradient
+    a.exponents = exponents;
     a.out = out;
     a.out_group = (long long)features * s.rank;
     a.out_f = out_f;
@@ -625,60 +693,58 @@ TcOuter tc_adapter_outer(const AdapterShape &s, int features, void *out, long lo
 
 template <typename T>
 int adapters(const AdapterShape &s, const void *x, const void *w, const void *a, const void *b, void *y, void *workspace, cudaStream_t st) {
-    const AdapterSpace ws(workspace, s.n_rows, s.n_adapters, s.rank, false);
+    const AdapterSpace ws(workspace, s, false);
     if (tc_widths(s.dtype, {s.k, s.rank}, {x, w, a, b})) {
         int sms, *status;
-        Cut cut;
         if (int rc = sm_count(&sms)) return rc;
         if (int rc = status_pointer(&status)) return rc;
-        const bool rows = by_rows(s, s.k, s.n, false, sms, &cut);
-        if (rows) {
+        if (ws.rows) {
             const dim3 grid((unsigned)s.n_rows, (unsigned)((s.rank + 7) / 8));
             mps::adapter_dots_kernel<<<grid, 256, 0, st>>>(s.k, s.rank, s.n_adapters, s.dtype == MPS_BF16, s.ids, s.scale, (const uint16_t *)x,
-                                                           (const uint16_t *)a, (float *)ws.u, status);
+                                                           (const uint16_t *)a, ws.u, status);
             RD_CUDA(cudaGetLastError());
         } else {
             if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
             TcRows narrow;
-            if (int rc = tc_adapter_narrow(s, s.k, a, false, ws.u, nullptr, &narrow)) return rc;
+            if (int rc = tc_adapter_narrow(s, s.k, a, false, nullptr, ws.wide, nullptr, &narrow)) return rc;
             narrow.follows = narrow.apart = true;  // beside the listing
             if (int rc = tc_rows(&narrow, 1, best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k), true, sms, 256), &x, s.n_rows, sms, st)) return rc;
+            if (int rc = tc_adapter_prepare(s, ws, b, false, s.n, false, 0, sms, st)) return rc;
         }
-        return tc_adapter_wide(s, ws, cut, rows, s.k, s.n, x, w, ws.u, (const float *)ws.u, b, false, y, rows, sms, st);
+        return tc_adapter_wide(s, ws, s.k, s.n, x, w, ws.u, b, false, y, ws.rows, sms, st);
     }
-    float *u = (float *)ws.u;
-    if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
-    return adapter_wide<T>(s, s.k, s.n, x, w, 1, s.k, u, b, 1, s.rank, y, st);
+    if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, ws.u, st)) return rc;
+    return adapter_wide<T>(s, s.k, s.n, x, w, 1, s.k, ws.u, b, 1, s.rank, y, st);
 }
 
 template <typename T>
 int adapters_backward(const AdapterShape &s, const void *dy, const void *x, const void *w, const void *a, const void *b, void *dx, void *da, void *db,
                       void *workspace, cudaStream_t st) {
-    const AdapterSpace ws(workspace, s.n_rows, s.n_adapters, s.rank, true);
+    const AdapterSpace ws(workspace, s, true);
     if (tc_widths(s.dtype, {s.k, s.n, s.rank}, {dy, x, w, a, b})) {
         int sms, used = 0;
-        Cut cut;
         if (int rc = sm_count(&sms)) return rc;
-        const bool rows = by_rows(s, s.n, s.k, true, sms, &cut);
-        if (!rows)
+        if (!ws.rows)
             if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
+        const bool scaled = s.dtype == MPS_F16;
         TcRows narrow[2];  // side by side, and beside the listing: scale * x A^T and scale * dy B
-        if (int rc = tc_adapter_narrow(s, s.k, a, false, ws.u, nullptr, &narrow[0])) return rc;
-        if (int rc = tc_adapter_narrow(s, s.n, b, true, ws.v, rows ? (float *)ws.v_f32 : nullptr, &narrow[1])) return rc;
-        narrow[0].follows = narrow[0].apart = narrow[1].apart = !rows;
+        if (int rc = tc_adapter_narrow(s, s.k, a, false, ws.u, nullptr, scaled ? ws.u_maxima : nullptr, &narrow[0])) return rc;
+        if (int rc = tc_adapter_narrow(s, s.n, b, true, ws.v, ws.wide, scaled ? ws.v_maxima : nullptr, &narrow[1])) return rc;
+        narrow[0].follows = narrow[0].apart = narrow[1].apart = !ws.rows;
         const void *const in[2] = {x, dy};
         const Cut half = best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k > s.n ? s.k : s.n), true, sms / 2, 64);
         if (int rc = tc_rows(narrow, 2, half, in, s.n_rows, sms, st)) return rc;
-        if (int rc = tc_adapter_wide(s, ws, cut, rows, s.n, s.k, dy, w, ws.v, (const float *)ws.v_f32, a, true, dx, false, sms, st, &used)) return rc;
-        const TcOuter outer[2] = {tc_adapter_outer(s, s.k, da, 1, s.k), tc_adapter_outer(s, s.n, db, s.rank, 1)};
-        const void *const q[2] = {ws.v, ws.u};
+        if (int rc = tc_adapter_prepare(s, ws, ws.rows ? nullptr : a, true, s.k, true, half.split > 1 ? 2 : mps::kSpan, sms, st)) return rc;
+        if (int rc = tc_adapter_wide(s, ws, s.n, s.k, dy, w, ws.v, a, true, dx, false, sms, st, &used)) return rc;
+        const TcOuter outer[2] = {tc_adapter_outer(s, s.k, scaled ? ws.v_exponents : nullptr, da, 1, s.k),
+                                  tc_adapter_outer(s, s.n, scaled ? ws.u_exponents : nullptr, db, s.rank, 1)};
+        const void *const q[2] = {ws.v_planes, ws.u_planes};
         // beside few blocks of that on the SMs they leave, else on each as it gets free
         return tc_outer(outer, 2, in, q, used <= sms / 2 ? sms - used : sms, st);
     }
-    float *u = (float *)ws.u, *v = (float *)ws.v;
-    if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, u, st)) return rc;
-    if (int rc = adapter_narrow<T>(s, s.n, dy, b, s.rank, 1, v, st)) return rc;
-    if (int rc = adapter_wide<T>(s, s.n, s.k, dy, w, s.k, 1, v, a, s.k, 1, dx, st)) return rc;
+    if (int rc = adapter_narrow<T>(s, s.k, x, a, 1, s.k, ws.u, st)) return rc;
+    if (int rc = adapter_narrow<T>(s, s.n, dy, b, s.rank, 1, ws.v, st)) return rc;
+    if (int rc = adapter_wide<T>(s, s.n, s.k, dy, w, s.k, 1, ws.v, a, s.k, 1, dx, st)) return rc;
     OuterArgs o = {};
     o.group_ptr = s.group_ptr;
     o.slot_row = s.slot_row;
@@ -687,24 +753,29 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
     o.p_by_row = o.q_by_row = true;
     o.i = s.rank;
     o.j = s.k;
-    if (int rc = launch_plain_outer<float, T, T>(o, v, x, da, st)) return rc;
+    if (int rc = launch_plain_outer<float, T, T>(o, ws.v, x, da, st)) return rc;
     o.i = s.n;
     o.j = s.rank;
-    return launch_plain_outer<T, float, T>(o, dy, u, db, st);
+    return launch_plain_outer<T, float, T>(o, dy, ws.u, db, st);
 }
 
-int check_adapters(const char *who, const AdapterShape &s, const void *workspace, int64_t bytes, bool backward) {
+int check_adapter_sizes(const char *who, const AdapterShape &s) {
     if (s.n_rows < 0 || s.k < 1 || s.n < 1 || s.n_adapters < 1 || s.rank < 1)
         return fail(MPS_ERR_ARG, "%s: %d rows, k = %d, n = %d, %d adapters of rank %d", who, s.n_rows, s.k, s.n, s.n_adapters, s.rank);
     if (!known(s.dtype)) return fail(MPS_ERR_ARG, "%s: unknown dtype %d", who, s.dtype);
     if (s.n_adapters > mps::kMaxRowGroups) return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d adapters", who, mps::kMaxRowGroups);
     if (s.k > 1 << 21 || s.n > 1 << 21 || s.rank > 1 << 12) return fail(MPS_ERR_UNSUPPORTED, "%s: k and n may be up to %d, the rank up to %d", who, 1 << 21, 1 << 12);
     if (s.n_rows >= 1 << 30) return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d rows", who, (1 << 30) - 1);
+    return MPS_OK;
+}
+
+int check_adapters(const char *who, const AdapterShape &s, const void *workspace, int64_t bytes, bool backward) {
+    if (int rc = check_adapter_sizes(who, s)) return rc;
     if (!s.group_ptr || (s.n_rows > 0 && (!s.ids || !s.slot_row))) return fail(MPS_ERR_ARG, "%s: NULL pointer", who);
     if (misaligned(s.ids, 4) || misaligned(s.group_ptr, 4) || misaligned(s.slot_row, 4) || misaligned(s.scale, 4))
         return fail(MPS_ERR_ALIGN, "%s: a pointer is not aligned to its element size", who);
     if (s.n_rows > 0) {
-        const int64_t need = AdapterSpace(nullptr, s.n_rows, s.n_adapters, s.rank, backward).bytes;
+        const int64_t need = AdapterSpace(nullptr, s, backward).bytes;
         if (!workspace || bytes < need) return fail(MPS_ERR_ARG, "%s: the workspace needs %lld bytes, %lld given", who, (long long)need, (long long)bytes);
         if (misaligned(workspace, 256)) return fail(MPS_ERR_ALIGN, "%s: the workspace must be 256-byte aligned", who);
     }
@@ -832,9 +903,9 @@ extern "C" int mps_routed_combine_backward(int32_t n_rows, int32_t per_row, int3
 }
 
 extern "C" int64_t mps_adapters_workspace(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, int backward) {
-    if (n_rows < 0 || k < 1 || n < 1 || n_adapters < 1 || rank < 1 || !known(dtype))
-        return fail(MPS_ERR_ARG, "mps_adapters_workspace: %d rows, k = %d, n = %d, %d adapters of rank %d, dtype %d", n_rows, k, n, n_adapters, rank, dtype);
-    return AdapterSpace(nullptr, n_rows, n_adapters, rank, backward != 0).bytes;
+    const AdapterShape s = {n_rows, k, n, n_adapters, rank, dtype, nullptr, nullptr, nullptr, nullptr};
+    if (int rc = check_adapter_sizes("mps_adapters_workspace", s)) return rc;
+    return n_rows == 0 ? 0 : AdapterSpace(nullptr, s, backward != 0).bytes;
 }
 
 extern "C" int mps_adapters(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, const int32_t *d_ids,

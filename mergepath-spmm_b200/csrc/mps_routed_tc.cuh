@@ -9,9 +9,10 @@
 // alternate, so a tile is stored while the next one is summed; results go through shared memory, where 64 slots by 128 features
 // become whole 256-byte rows.
 //
-// A tile's sum may go on with a second product (`rank` > 0): the group's low-rank matrix times rows u that were computed before,
-// kept as hi + lo pairs of the 16-bit type (two planes), so that the intermediate's rounding (2^-16 in bf16, 2^-22 in fp16)
-// stays below the result's.
+// A tile's sum may go on with a second product (RANK): the group's low-rank matrix times rows u that were computed before.  u is
+// kept as two planes of tf32 values, whose sum has fp32's range and is off by 2^-21 of u at most, and the matrix, exactly, in fp32
+// (adapter_prepare_kernel).  A pair of fp16 values instead has no digits left below 2^-24 and ends at 65504, and intermediates
+// next to nothing are what training starts from (the second matrix begins at zero).
 //
 // The widest tiles (NT = 256) belong to a pair of neighbouring blocks (cta_group::2): 256 features by 256 slots, each block
 // loading its 128 features and half of the slots, so that a block's slice is 32 KB instead of 48 and six of them are in flight.
@@ -35,6 +36,7 @@ namespace mps {
 constexpr int kTcThreads = 512;  // warps: 0 TMA, 1 products, 2-3 none, 4-7 results (TMEM lanes go by warp number mod 4), 8-15 row loads
 constexpr int kTcFeatures = 128;
 constexpr int kTcDepth = 64;
+constexpr int kRankDepth = 32;                 // of the rank in a slice of the second product, whose elements are 32-bit
 constexpr int kTcRing = 192 * 1024;            // shared memory of the stages
 constexpr int kOutPitch = kTcFeatures * 2 + 16;  // a result row in shared memory; the pad spreads 16-byte reads over the banks
 constexpr int kOutBytes = 64 * kOutPitch;        // 64 rows at a time
@@ -43,21 +45,20 @@ static_assert(32 * kF32Pitch <= kOutBytes);
 constexpr int kOutTotal = (kOutBytes + 1023) / 1024 * 1024;
 
 struct TcRows {
-    CUtensorMap w, x, w2, u;  // matrices {i, f, group} or {f, i, group}; rows {i, row}; the low-rank pair's matrix and rows
-    CUtensorMap x_run;        // gathered rows: as many neighbouring ones as a warp loads
+    CUtensorMap w, x, w2, u;  // matrices {i, f, group} or {f, i, group}; rows {i, row}; the second product's {rank, f, group}, {rank, row}
+    CUtensorMap x_run, u_run; // gathered rows: as many neighbouring ones as a warp loads
     const int *group_ptr;     // NULL: one group of all slots
     const int *slot_row;      // row behind a slot; NULL: the slot itself
     int n_groups, n_slots, n_x_rows;
     int k, n;                 // summed index, result features
     int rank, rank_groups;    // depth of the second product; groups that have one (the first rank_groups)
-    const void *u_base;       // rows of the second product (host side)
-    int u_plane;              // rows between the hi and the lo plane of u
+    const float *u_base, *w2_base;  // its rows, two planes of n_x_rows, and matrices (host side)
     int w_rows;               // rows of a matrix box (features, where they are its rows)
-    bool w_shared, mn_major, gather, bf16, scatter, pair;  // pair: result stored as hi + lo planes of out
-    const float *group_scale;  // pair: factor of a group's results (NULL: 1)
+    bool w_shared, mn_major, gather, bf16, scatter;
     void *out;
-    long long out_plane;
-    float *out_f32;           // pair: the result in fp32 too, by row (NULL: not wanted)
+    float *out_f32, *out_tf32;  // instead of out: the result in fp32, by row, and as two planes of tf32 values (NULL: not wanted)
+    const float *group_scale;   // factor of a group's results then (NULL: 1)
+    unsigned *maxima;           // the largest finite magnitudes of them, see finite_bits (NULL: not wanted)
     const int *ids;           // delta: adapter of a row,
     const float *delta_u;     //   the rows' intermediates (by row, delta_rank each),
     const uint16_t *delta_m;  //   the adapters' matrices with their strides by adapter, feature and rank index
@@ -81,6 +82,7 @@ struct TcRowsLaunch {
 struct TcPipe {
     uint64_t full[12], empty[12], tmem_full[2], tmem_empty[2];  // of a pair's full and tmem_empty the first block's count
     uint64_t partials, freed;                                   // split: every block's part is in its shared memory / has been read
+    uint64_t summed;                                            // the products before a tile's second one are done
     uint32_t tmem;
     int gave_up;
 };
@@ -96,6 +98,7 @@ __device__ __forceinline__ void pipe_init(TcPipe &pipe, int stages, bool paired,
     }
     mbar_init(smem_addr(&pipe.partials), 4 * split);  // a lane of each of the four result warps of every block
     mbar_init(smem_addr(&pipe.freed), 4 * split);
+    mbar_init(smem_addr(&pipe.summed), 1);
     pipe.gave_up = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
@@ -161,31 +164,21 @@ __device__ __forceinline__ void spread_column(const float (&v)[32], uint32_t to)
     }
 }
 
-// The same as hi + lo pairs, the lo rows `lo` bytes behind the hi rows.
-template <bool BF16>
-__device__ __forceinline__ void spread_pair(const float (&v)[32], uint32_t to, uint32_t lo) {
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-        const uint32_t w = to_16x2<BF16>(v[j], v[j + 1]);
-        const float2 h = from_16x2<BF16>(w);
-        const uint32_t x = to_16x2<BF16>(v[j] - h.x, v[j + 1] - h.y);
-        store_shared_16(to + j * kOutPitch, (uint16_t)w);
-        store_shared_16(to + (j + 1) * kOutPitch, (uint16_t)(w >> 16));
-        store_shared_16(to + lo + j * kOutPitch, (uint16_t)x);
-        store_shared_16(to + lo + (j + 1) * kOutPitch, (uint16_t)(x >> 16));
+// Four values of an fp32 result, at `at` of out_f32 and of both planes of out_tf32.
+__device__ __forceinline__ void store_f32(const TcRows &a, long long at, float4 v) {
+    if (a.out_f32) *reinterpret_cast<float4 *>(a.out_f32 + at) = v;
+    if (a.out_tf32) {
+        *reinterpret_cast<float4 *>(a.out_tf32 + at) = make_float4(tf32_first(v.x), tf32_first(v.y), tf32_first(v.z), tf32_first(v.w));
+        *reinterpret_cast<float4 *>(a.out_tf32 + (long long)a.n_x_rows * a.n + at) = make_float4(tf32_second(v.x), tf32_second(v.y), tf32_second(v.z), tf32_second(v.w));
     }
 }
 
-__device__ __forceinline__ uint4 rest_of_16(const float (&v)[8], uint4 hi, bool bf16) {
-    const uint32_t w[4] = {hi.x, hi.y, hi.z, hi.w};
-    float lo[8];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const float2 h = bf16 ? from_16x2<true>(w[j]) : from_16x2<false>(w[j]);
-        lo[2 * j] = v[2 * j] - h.x;
-        lo[2 * j + 1] = v[2 * j + 1] - h.y;
-    }
-    return pack_16(lo, bf16);
+// Largest finite magnitudes of an fp32 result, for who scales it: of every 32 features and `span` slots of a group, counted from its
+// first, an entry at [feature / 32][first of the slots].  span: kSpan, or 2 where the blocks of a cluster share a tile.
+constexpr int kSpan = 32;
+__device__ __forceinline__ unsigned finite_bits(float v) {
+    const unsigned bits = __float_as_uint(v) & 0x7fffffffu;
+    return bits < 0x7f800000u ? bits : 0u;
 }
 
 // v[j] += <u of column c + j, the feature's row of that column's matrix> over `ranks` (a multiple of eight): u in shared memory (64
@@ -279,7 +272,8 @@ struct TileWalk {
     }
 };
 
-template <int NT, bool TWO>
+// RANK: with a second product.  Forms of their own, so that it costs the others nothing.
+template <int NT, bool TWO, bool RANK>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_constant__ TcRowsLaunch launch) {
     const bool is_second = TWO && (int)blockIdx.x >= launch.second;
     const TcRows &a = launch.p[is_second];
@@ -300,9 +294,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     const int half = PAIRED ? (int)cluster_rank() : 0, group_blocks = PAIRED ? 2 : split;
 
     if (!a.next_after) let_next_launch_start();
-    if (warp == 0 && lane < 5) {
-        const CUtensorMap *maps[5] = {&a.w, &a.x, &a.x_run, &a.w2, &a.u};
-        if (lane < 2 || (lane == 2 ? a.gather : a.rank > 0)) tma_prefetch(maps[lane]);
+    if (warp == 0 && lane < (RANK ? 6 : 3)) {
+        const CUtensorMap *maps[6] = {&a.w, &a.x, &a.x_run, &a.w2, &a.u, &a.u_run};
+        if (lane != 2 || a.gather) tma_prefetch(maps[lane]);
     }
     if (!a.ahead && !a.apart) wait_for_launch_before();
     if (a.next_after) let_next_launch_start();
@@ -373,7 +367,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     const uint32_t tmem = pipe.tmem;
     volatile int *gave_up = &pipe.gave_up;
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
-    const int main_steps = (a.k + kTcDepth - 1) / kTcDepth, rank_steps = 2 * ((a.rank + kTcDepth - 1) / kTcDepth);
+    const int main_steps = (a.k + kTcDepth - 1) / kTcDepth, rank_steps = RANK ? 2 * ((a.rank + kRankDepth - 1) / kRankDepth) : 0;  // of each plane in turn
     const int shift = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
     const int n_active = s_active;
     TileWalk walk(whole[n_active] + (rest[n_active] & 0xffff), (a.n + TILE_F - 1) / TILE_F, block / group_blocks, blocks / group_blocks);
@@ -381,7 +375,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
 
     // steps of this block for a tile of group g
     auto range = [&](int g, int &s0, int &s1) {
-        const int total = main_steps + (g < a.rank_groups ? rank_steps : 0);
+        const int total = main_steps + (RANK && g < a.rank_groups ? rank_steps : 0);
         s0 = total * part >> shift;
         s1 = total * (part + 1) >> shift;
     };
@@ -412,6 +406,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     if (loads_rows) fetch_rows(walk);
     const uint32_t full0 = PAIRED ? in_block(smem_addr(&pipe.full[0]), 0) : smem_addr(&pipe.full[0]);  // where loads are reported
     RingAt pos;  // this warp's place in the ring
+    uint32_t summed_parity = 0;
 
     int turn = 0;  // tiles done so far
     for (; walk.more(); walk.next(), ++turn) {
@@ -434,20 +429,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                         uint32_t bytes = 0;
 #pragma unroll
                         for (int d = 0; d < S::kSlices; ++d)
-                            if (s + d < s1) bytes += w_bytes + (s + d < main_steps ? x_bytes : S::kRows * 128u);
+                            if (s + d < s1) bytes += (!RANK || s + d < main_steps ? w_bytes : a.w_rows * 128u) + x_bytes;
                         mbar_expect(bar, (PAIRED ? 2 : 1) * bytes);
                     }
 #pragma unroll
                     for (int d = 0; d < S::kSlices; ++d) {
                         if (d > 0 && s + d >= s1) break;
                         const uint32_t dst = ring + pos.stage * S::kStage + d * S::kSlice;
-                        const bool second = s + d >= main_steps;
-                        const int i0 = (second ? (s + d - main_steps) >> 1 : s + d) * kTcDepth;
-                        const CUtensorMap *m = second ? &a.w2 : &a.w;
+                        if (RANK && s + d >= main_steps) {
+                            tma_3d<PAIRED>(dst, &a.w2, ((s + d - main_steps) >> 1) * kRankDepth, f0, g, bar);
+                            continue;
+                        }
+                        const int i0 = (s + d) * kTcDepth;
                         if (a.mn_major)
-                            for (int h = 0; h < halves; ++h) tma_3d<PAIRED>(dst + h * kBlock64, m, f0 + h * 64, i0, second ? g : z, bar);
-                        else tma_3d<PAIRED>(dst, m, i0, f0, second ? g : z, bar);
-                        if (!a.gather) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);  // there is no second product then
+                            for (int h = 0; h < halves; ++h) tma_3d<PAIRED>(dst + h * kBlock64, &a.w, f0 + h * 64, i0, z, bar);
+                        else tma_3d<PAIRED>(dst, &a.w, i0, f0, z, bar);
+                        if (!a.gather) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);
                     }
                 }
             }
@@ -457,7 +454,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 tc_fence_after();
                 const uint32_t d = tmem + buf * NT, idesc = mma_desc(a.bf16, a.mn_major, false, TILE_F, columns);
                 const uint64_t a_step = operand_step(a.mn_major), b_step = operand_step(false);
-                const uint64_t a0 = operand(ring, a.mn_major), b0 = operand(ring + kTcFeatures * 128, false);
+                const uint64_t a0 = operand(ring, a.mn_major), b0 = operand(ring + kTcFeatures * 128, false), m0 = operand(ring, false);
                 for (int s = s0; s < s1; s += S::kSlices, pos.next(stages)) {
                     mbar_wait(smem_addr(&pipe.full[pos.stage]), pos.parity, gave_up, a.status);
                     tc_fence_after();
@@ -465,8 +462,20 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     for (int d2 = 0; d2 < S::kSlices; ++d2) {
                         if (d2 > 0 && s + d2 >= s1) break;
                         const uint32_t from = pos.stage * S::kStage + d2 * S::kSlice;
-                        const int left = s + d2 >= main_steps ? a.rank - ((s + d2 - main_steps) >> 1) * kTcDepth : a.k - (s + d2) * kTcDepth;
-                        tc_slice<PAIRED>(d, operand_at(a0, from), operand_at(b0, from), a_step, b_step, idesc, min(4, (left + 15) >> 4), s > s0 || d2 > 0);
+                        const bool add = s > s0 || d2 > 0;
+                        const int e = s + d2 - main_steps;
+                        if (!RANK || e < 0) {
+                            tc_slice<PAIRED>(d, operand_at(a0, from), operand_at(b0, from), a_step, b_step, idesc, min(4, (a.k - (s + d2) * kTcDepth + 15) >> 4), add);
+                            continue;
+                        }
+                        if (e == 0 && add) {  // products of another kind follow those before only once they are done
+                            tc_commit<PAIRED>(smem_addr(&pipe.summed));
+                            mbar_wait(smem_addr(&pipe.summed), summed_parity, gave_up, a.status);
+                            summed_parity ^= 1;
+                            tc_fence_after();
+                        }
+                        tc_slice<PAIRED, true>(d, operand_at(m0, from), operand_at(b0, from), b_step, b_step, mma_desc_tf32(TILE_F, columns),
+                                               min(4, (a.rank - (e >> 1) * kRankDepth + 7) >> 3), add);
                     }
                     tc_commit<PAIRED>(smem_addr(&pipe.empty[pos.stage]));
                 }
@@ -488,28 +497,29 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 for (int d = 0; d < S::kSlices; ++d) {
                     if (s + d >= s1) break;
                     const uint32_t rows = ring + pos.stage * S::kStage + d * S::kSlice + kTcFeatures * 128, bar = full0 + pos.stage * 8;
-                    const int e = s + d - main_steps;
-                    if (e >= 0) {  // rows of the second product, in slot order
-                        const int line = (e & 1) * a.u_plane + slot0 + half * columns / 2 + (warp - 8) * RPW;
-                        if (elect_one()) tma_2d<PAIRED>(rows + (warp - 8) * RPW * 128, &a.u, (e >> 1) * kTcDepth, line, bar);
-                        continue;
-                    }
-                    if (run) {
-                        if (elect_one()) tma_2d<PAIRED>(rows + (warp - 8) * RPW * 128, &a.x_run, (s + d) * kTcDepth, row0, bar);
-                        continue;
-                    }
+                    auto load = [&](const CUtensorMap *one, const CUtensorMap *several, int i0, int plane) {
+                        if (run) {
+                            if (elect_one()) tma_2d<PAIRED>(rows + (warp - 8) * RPW * 128, several, i0, plane + row0, bar);
+                            return;
+                        }
 #pragma unroll
-                    for (int q = 0; q < RPW / 4; ++q) {
-                        if (4 * q >= n_rows) break;
-                        const int r0 = __shfl_sync(0xffffffffu, row, 4 * q), r1 = __shfl_sync(0xffffffffu, row, 4 * q + 1);
-                        const int r2 = __shfl_sync(0xffffffffu, row, 4 * q + 2), r3 = __shfl_sync(0xffffffffu, row, 4 * q + 3);
-                        if (elect_one()) tma_rows<PAIRED>(rows + ((warp - 8) * n_rows + 4 * q) * 128, &a.x, (s + d) * kTcDepth, r0, r1, r2, r3, bar);
-                    }
+                        for (int q = 0; q < RPW / 4; ++q) {
+                            if (4 * q >= n_rows) break;
+                            const int r0 = __shfl_sync(0xffffffffu, row, 4 * q), r1 = __shfl_sync(0xffffffffu, row, 4 * q + 1);
+                            const int r2 = __shfl_sync(0xffffffffu, row, 4 * q + 2), r3 = __shfl_sync(0xffffffffu, row, 4 * q + 3);
+                            if (elect_one())
+                                tma_rows<PAIRED>(rows + ((warp - 8) * n_rows + 4 * q) * 128, one, i0, plane + r0, plane + r1, plane + r2, plane + r3, bar);
+                        }
+                    };
+                    const int e = s + d - main_steps;
+                    if (!RANK || e < 0) load(&a.x, &a.x_run, (s + d) * kTcDepth, 0);
+                    else load(&a.u, &a.u_run, (e >> 1) * kRankDepth, e & 1 ? a.n_x_rows : 0);  // the same rows of one plane of u
                 }
             }
         } else if (warp >= 4 && warp < 8) {
             const int quad = warp & 3, f = f0 + quad * 32 + lane, mine = tid - 128;
-            const float scale = a.pair && a.group_scale ? a.group_scale[g] : 1.0f;
+            const bool f32 = a.out == nullptr;
+            const float scale = f32 && a.group_scale ? a.group_scale[g] : 1.0f;
             uint16_t *out = (uint16_t *)a.out;
             auto out_row = [&](int slot) {  // where a slot's result goes, or -1
                 if (!a.scatter) return slot;
@@ -591,43 +601,37 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     }
                 }
             }
-            const bool rows_of_16 = a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0, wide = rows_of_16 && !reduce;  // pairs always are
-            int line = wide && !a.pair ? line_ahead(0) : 0;
+            const bool rows_of_16 = a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0, wide = rows_of_16 && !reduce;  // fp32 results always are
+            int line = wide && !f32 ? line_ahead(0) : 0;
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
             tc_fence_after();
             const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT;
-            if (wide && a.pair) {
+            if (wide && f32) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 32) {
                     float v[32];
+                    const int slot = slot0 + c0 + warp - 4 + 4 * (lane & 7);  // of the rows this warp stores
+                    const int at = slot < slot1 ? a.slot_row[slot] : -1;
                     tmem_load(lanes + c0, v);
+                    unsigned largest = 0;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] *= scale;
+                    for (int j = 0; j < 32; ++j) {
+                        v[j] *= scale;
+                        if (f < a.n && slot0 + c0 + j < slot1) largest = max(largest, finite_bits(v[j]));
+                    }
+                    if (a.maxima) {
+                        largest = __reduce_max_sync(0xffffffffu, largest);
+                        if (lane == 0 && f < a.n) a.maxima[(long long)(f >> 5) * a.n_slots + slot0 + c0] = largest;
+                    }
                     results_sync();  // the rows before these have been read
-                    if (a.bf16) spread_pair<true>(v, staging + feature * 2, 32 * kOutPitch);
-                    else spread_pair<false>(v, staging + feature * 2, 32 * kOutPitch);
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) store_shared_f32(staging + j * kF32Pitch + feature * 4, v[j]);
                     results_sync();
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int c = (mine >> 4) + 8 * (j & 3), fc = (mine & 15) * 8;
-                        if (slot0 + c0 + c < slot1 && f0 + fc < a.n)
-                            *reinterpret_cast<uint4 *>(out + (j >> 2) * a.out_plane + (long long)(slot0 + c0 + c) * a.n + f0 + fc) =
-                                load_shared_128(staging + ((j >> 2) * 32 + c) * kOutPitch + fc * 2);
-                    }
-                    if (a.out_f32) {
-                        const int slot = slot0 + c0 + warp - 4 + 4 * (lane & 7);  // of the rows this warp stores
-                        const int at = slot < slot1 ? a.slot_row[slot] : -1;
-                        results_sync();
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) store_shared_f32(staging + j * kF32Pitch + feature * 4, v[j]);
-                        results_sync();
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int to = __shfl_sync(0xffffffffu, at, j);
-                            if ((unsigned)to < (unsigned)a.n_x_rows && f0 + lane * 4 < a.n)
-                                *reinterpret_cast<float4 *>(a.out_f32 + (long long)to * a.n + f0 + lane * 4) =
-                                    load_shared_float4(staging + (warp - 4 + 4 * j) * kF32Pitch + lane * 16);
-                        }
+                        const int to = __shfl_sync(0xffffffffu, at, j);
+                        if ((unsigned)to < (unsigned)a.n_x_rows && f0 + lane * 4 < a.n)
+                            store_f32(a, (long long)to * a.n + f0 + lane * 4, load_shared_float4(staging + (warp - 4 + 4 * j) * kF32Pitch + lane * 16));
                     }
                 }
             } else if (wide) {
@@ -682,24 +686,31 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 const int first = part * meeting.run, own = min(max(slot1 - slot0 - first, 0), meeting.run);
                 if (rows_of_16) {
                     const int fc = (mine & 15) * 8;
-                    for (int c = mine >> 4; c < own; c += 8) {
+                    for (int c0 = 2 * (warp - 4); c0 < own; c0 += 8) {
+                        const int c = c0 + (lane >> 4);  // a half warp per column; a run is a multiple of eight, so it has this one
                         float v[8];
-                        const int slot = slot0 + first + c, r = out_row(slot), by_row = a.out_f32 ? a.slot_row[slot] : -1;
+                        const int slot = slot0 + first + c;
+                        const bool live = c < own && f0 + fc < a.n;
+                        const int r = !live ? -1 : f32 ? a.slot_row[slot] : out_row(slot);
                         meeting.sum8(c, fc, v);
-                        if (a.pair) {
+                        if (f32) {
+                            unsigned largest = 0;
 #pragma unroll
-                            for (int j = 0; j < 8; ++j) v[j] *= scale;
-                        }
-                        if (f0 + fc >= a.n || r < 0) continue;
-                        const uint4 hi = pack_16(v, a.bf16);
-                        uint16_t *to = out + (long long)r * a.n + f0 + fc;
-                        *reinterpret_cast<uint4 *>(to) = hi;
-                        if (a.pair) *reinterpret_cast<uint4 *>(to + a.out_plane) = rest_of_16(v, hi, a.bf16);
-                        if ((unsigned)by_row < (unsigned)a.n_x_rows) {
-                            float4 *line_f32 = reinterpret_cast<float4 *>(a.out_f32 + (long long)by_row * a.n + f0 + fc);
-                            line_f32[0] = make_float4(v[0], v[1], v[2], v[3]);
-                            line_f32[1] = make_float4(v[4], v[5], v[6], v[7]);
-                        }
+                            for (int j = 0; j < 8; ++j) {
+                                v[j] *= scale;
+                                if (live) largest = max(largest, finite_bits(v[j]));
+                            }
+                            if (a.maxima) {  // of four lanes' features and both columns
+                                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+                                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+                                largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 16));
+                                if ((lane & 19) == 0 && f0 + fc < a.n) a.maxima[(long long)((f0 + fc) >> 5) * a.n_slots + slot0 + first + c0] = largest;
+                            }
+                            if ((unsigned)r < (unsigned)a.n_x_rows) {
+                                store_f32(a, (long long)r * a.n + f0 + fc, make_float4(v[0], v[1], v[2], v[3]));
+                                store_f32(a, (long long)r * a.n + f0 + fc + 4, make_float4(v[4], v[5], v[6], v[7]));
+                            }
+                        } else if (r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = pack_16(v, a.bf16);
                     }
                 } else
                     for (int c = 0; c < own; ++c) store(slot0 + first + c, meeting.sum(c, feature));
@@ -745,17 +756,183 @@ __global__ void __launch_bounds__(256) adapter_dots_kernel(int k, int rank, int 
     if (lane == 0) u[(long long)row * rank + r] = scale ? sum * scale[id] : sum;
 }
 
+// What the adapters' products read in another form than it came in.  First the matrices of the groups that have slots, in fp32 with
+// the rank contiguous (exact, and what a tf32 product reads by TMA); they are beside the launch before.  Behind that launch, for the
+// matrix gradients, its two fp32 results as hi + lo planes of the 16-bit type in slot order (off by 2^-16 of a value in bf16,
+// 2^-22 in fp16; of an infinite value lo is zero).  fp16 has not fp32's range: there a group's values of 64 columns are multiplied
+// by the power of two that brings the largest of them, out of `maxima`, just below 2^15, so that what fp16 rounds away is 2^-40 of
+// that largest at most.  Bytes bound it: 2 read and 4 written per element of a matrix (8 matrices of 4096 x 64: 12 MB, on the SMs
+// that the narrow product leaves), 4 and 4 per value.
+struct PrepareArgs {
+    const int *group_ptr, *slot_row;
+    int n_groups, n_slots, n_rows, rank;
+    bool bf16;
+    const uint16_t *m;        // matrices by group, features x rank (by_rank: rank x features); NULL: none
+    float *m_f32;
+    int features;
+    bool by_rank;
+    const float *values[2];   // by row; NULL: none
+    uint16_t *planes[2];
+    const unsigned *maxima[2];  // NULL: not scaled
+    int *exponents[2];
+    int span;
+    int *status;
+};
+
+template <bool BF16>
+__device__ __forceinline__ void split_16(float4 v, uint2 &hi, uint2 &lo) {
+    hi = make_uint2(to_16x2<BF16>(v.x, v.y), to_16x2<BF16>(v.z, v.w));
+    const float2 h = from_16x2<BF16>(hi.x), q = from_16x2<BF16>(hi.y);
+    auto rest = [](float x, float first) { return fabsf(first) < INFINITY ? x - first : 0.0f; };
+    lo = make_uint2(to_16x2<BF16>(rest(v.x, h.x), rest(v.y, h.y)), to_16x2<BF16>(rest(v.z, q.x), rest(v.w, q.y)));
+}
+
+template <bool BF16>
+__global__ void __launch_bounds__(256) adapter_prepare_kernel(const PrepareArgs a) {
+    constexpr int N = 4;  // loads in flight
+    __shared__ int s_ptr[kMaxRowGroups + 1];
+    __shared__ uint16_t s_active[kMaxRowGroups];
+    __shared__ int s_count[8];
+    let_next_launch_start();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    for (int g = tid; g <= a.n_groups; g += 256) s_ptr[g] = a.group_ptr[g];
+    __syncthreads();
+    auto range = [&](int g) { return group_range(make_int2(s_ptr[g], s_ptr[g + 1]), a.n_slots, a.status); };
+    if (a.m) {
+        int n_active = 0;  // groups with slots, in order
+        for (int g0 = 0; g0 < a.n_groups; g0 += 256) {
+            const int g = g0 + tid;
+            bool active = false;
+            if (g < a.n_groups) {
+                const int2 slots = range(g);
+                active = slots.x < slots.y;
+            }
+            const unsigned lanes = __ballot_sync(0xffffffffu, active);
+            if (lane == 0) s_count[warp] = __popc(lanes);
+            __syncthreads();
+            int at = n_active + __popc(lanes & ((1u << lane) - 1));
+            for (int w = 0; w < 8; ++w) {
+                if (w < warp) at += s_count[w];
+                n_active += s_count[w];
+            }
+            if (active) s_active[at] = (uint16_t)g;
+            __syncthreads();
+        }
+        const long long size = (long long)a.features * a.rank, per = size / 8, all = n_active * per, step = (long long)gridDim.x * 256;
+        for (long long i0 = (long long)blockIdx.x * 256 + tid; i0 < all; i0 += N * step) {
+            uint32_t w[N][4];
+            long long to[N];
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                const long long i = i0 + n * step;
+                to[n] = -1;
+                if (i >= all) continue;
+                const int which = (int)(i / per);
+                const long long first = s_active[which] * size, rest = i - which * per;
+                if (a.by_rank) {  // eight ranks of a feature, neighbouring threads at neighbouring features
+                    const int r = (int)(rest / a.features) * 8, f = (int)(rest - (long long)(r / 8) * a.features);
+                    const uint16_t *q = a.m + first + (long long)r * a.features + f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) w[n][j] = q[(long long)(2 * j) * a.features] | (uint32_t)q[(long long)(2 * j + 1) * a.features] << 16;
+                    to[n] = first + (long long)f * a.rank + r;
+                } else {
+                    const uint4 q = *reinterpret_cast<const uint4 *>(a.m + first + rest * 8);
+                    w[n][0] = q.x, w[n][1] = q.y, w[n][2] = q.z, w[n][3] = q.w;
+                    to[n] = first + rest * 8;
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+                if (to[n] < 0) continue;
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const float2 x = from_16x2<BF16>(w[n][2 * j]), y = from_16x2<BF16>(w[n][2 * j + 1]);
+                    *reinterpret_cast<float4 *>(a.m_f32 + to[n] + 4 * j) = make_float4(x.x, x.y, y.x, y.y);
+                }
+            }
+        }
+    }
+    // a warp per 32 slots of either result, cut where groups end
+    const int used = min(max(s_ptr[a.n_groups], 0), a.n_slots), runs = a.values[0] ? (used + 31) / 32 : 0, blocks_of_rank = (a.rank + 63) / 64;
+    const int step = gridDim.x * 8;
+    int run = blockIdx.x * 8 + warp;
+    // Who has nothing to split makes room for the next launch's blocks; one stays, so that what waits for this launch waits for the
+    // one before, too.
+    if (blockIdx.x > 0 && blockIdx.x * 8 >= 2 * runs) return;
+    auto row_of = [&](int n) {  // the row of this lane's slot
+        const int slot = (n >= runs ? n - runs : n) * 32 + lane, row = n < 2 * runs && slot < used ? a.slot_row[slot] : -1;
+        return (unsigned)row < (unsigned)a.n_rows ? row : -1;
+    };
+    int row = row_of(run);
+    wait_for_launch_before();
+    for (; run < 2 * runs; run += step, row = row_of(run)) {
+        const int which = run >= runs, first = (which ? run - runs : run) * 32, end = min(first + 32, used);
+        const float *values = a.values[which];
+        const unsigned *maxima = a.maxima[which];
+        int s = first;
+        while (s < end) {
+            int g = 0, above = a.n_groups;  // the last group that starts at s or before it
+            while (above - g > 1) {
+                const int mid = (g + above) >> 1;
+                if (s_ptr[mid] <= s) g = mid;
+                else above = mid;
+            }
+            const int2 slots = range(g);
+            const int stop = max(min(end, slots.y), s + 1);
+            for (int j = 0; j < blocks_of_rank; ++j) {
+                const int pieces = min(64, a.rank - 64 * j) / 4, count = (stop - s) * pieces;
+                float4 v[N];
+                auto load = [&](int i0) {
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        const int i = i0 + 32 * n, r = __shfl_sync(0xffffffffu, row, (s - first + i / pieces) & 31);
+                        v[n] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                        if (i < count && r >= 0) v[n] = __ldcg(reinterpret_cast<const float4 *>(values + (long long)r * a.rank + 64 * j + i % pieces * 4));
+                    }
+                };
+                load(lane);
+                float scale = 1.0f;
+                if (maxima) {
+                    unsigned largest = 0;
+                    for (int b = 2 * j; b < 2 * j + 2 && b * 32 < a.rank; ++b)
+                        for (int i = slots.x + lane * a.span; i < slots.y; i += 32 * a.span) largest = max(largest, __ldcg(maxima + (long long)b * a.n_slots + i));
+                    largest = __reduce_max_sync(0xffffffffu, largest);
+                    const int exponent = largest ? min(268 - (int)(largest >> 23), 253) : 127;  // 2^e .. 2^(e+1) to 2^14 .. 2^15; one
+                    scale = __uint_as_float((uint32_t)exponent << 23);
+                    if (s == slots.x && lane == 0) a.exponents[which][(long long)g * blocks_of_rank + j] = exponent;
+                }
+                for (int i0 = 0; i0 < count; i0 += 32 * N) {
+                    if (i0) load(i0 + lane);
+#pragma unroll
+                    for (int n = 0; n < N; ++n) {
+                        const int i = i0 + lane + 32 * n;
+                        if (i >= count) continue;
+                        uint2 hi, lo;
+                        split_16<BF16>(make_float4(v[n].x * scale, v[n].y * scale, v[n].z * scale, v[n].w * scale), hi, lo);
+                        uint16_t *to = a.planes[which] + (long long)(s + i / pieces) * a.rank + 64 * j + i % pieces * 4;
+                        *reinterpret_cast<uint2 *>(to) = hi;
+                        *reinterpret_cast<uint2 *>(to + (long long)a.n_slots * a.rank) = lo;
+                    }
+                }
+            }
+            s = stop;
+        }
+    }
+}
+
 // tc_outer_kernel: out[g][f, c] = sum over the slots s of group g of P[.., f] Q[s, c] - the gradient by a group's matrix.  The
 // summed index is the slot, so both operands lie across it (MN-major): a stage holds 64 slots of 128 features of P and of up
 // to NT columns of Q in blocks of 64.  Whole slices of rows in slot order come as a box per block; gathered rows and the last
 // slice of a group by row number, those behind the group's end named out of range: zeros, whatever lies there.
-// With `pair` a block of columns of Q is a hi and a lo plane, added up when the result is stored.
+// With `pair` a block of columns of Q is a hi and a lo plane, added up when the result is stored, and each group's values have been
+// multiplied by a power of two (adapter_prepare_kernel): the result is by its inverse.
 struct TcOuter {
     CUtensorMap p_rows, p_tile, q_rows, q_tile;  // boxes of one row / of 64
     const int *group_ptr, *slot_row;  // slot_row: rows of P (NULL: in slot order)
     int n_groups, n_slots, n_p_rows;
     int i, j;                         // features of P, columns of Q
     bool bf16, pair;                  // pair: Q is two planes of n_slots rows
+    const int *exponents;             //   and the exponent field of the power of two by [group][column / 64] (NULL: one)
     void *out;
     long long out_group, out_f, out_c;
     int split;
@@ -941,6 +1118,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             const Meeting meeting = {partial, split, part, cols / split};
             const int feature = quad * 32 + lane;
             const bool none = s0 == s1;
+            float inverse = 1.0f;
+            if (a.exponents && slots.x < slots.y) inverse = __uint_as_float((uint32_t)(254 - __ldcg(a.exponents + (long long)g * ((a.j + 63) / 64) + (c0 >> 6))) << 23);
+            // an infinite sum of hi values is the result, whatever an infinite factor made of the lo ones
+            auto join = [&](float hi, float lo) { return (fabsf(hi) < INFINITY ? hi + lo : hi) * inverse; };
             if (wide && split == 1) {
 #pragma unroll 1
                 for (int c = 0; c < cols && c0 + c < a.j; c += 64) {
@@ -955,7 +1136,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                             float w[32];
                             tmem_load(lanes + cols + c + 32 * h, w);
 #pragma unroll
-                            for (int x = 0; x < 32; ++x) v[h][x] += w[x];
+                            for (int x = 0; x < 32; ++x) v[h][x] = join(v[h][x], w[x]);
                         }
                     }
                     results_sync();  // the rows before these have been read
@@ -982,7 +1163,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                         float w[32];
                         tmem_load(lanes + cols + c, w);
 #pragma unroll
-                        for (int x = 0; x < 32; ++x) v[x] += w[x];
+                        for (int x = 0; x < 32; ++x) v[x] = join(v[x], w[x]);
                     }
                 }
                 if (split > 1) {

@@ -2,6 +2,7 @@
 #pragma once
 #include <cuda.h>
 #include <cuda_runtime.h>
+#include <math.h>
 #include <stdint.h>
 
 #include "mps_types.cuh"
@@ -65,8 +66,8 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatil
     }
 }
 
-// ---- TMA: boxes of 64 elements (128 bytes, 128-byte swizzle) by some rows.  The x coordinate is a multiple of 64 elements
-// throughout, so every copy starts on a 128-byte multiple of its row.
+// ---- TMA: boxes of 64 elements of a 16-bit type or 32 of fp32 (128 bytes, 128-byte swizzle) by some rows.  The x coordinate is a
+// multiple of as many throughout, so every copy starts on a 128-byte multiple of its row.
 // PAIRED: the barrier may be the other block's.
 template <bool PAIRED>
 __device__ __forceinline__ void tma_2d(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar) {
@@ -131,11 +132,22 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
                      : "memory");
     else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-template <bool PAIRED>
+// TF32: 32-bit operands with ten bits of fraction, eight summed elements at a time; else a 16-bit type, sixteen
+template <bool PAIRED, bool TF32>
 __device__ __forceinline__ void tc_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    if constexpr (PAIRED)
+    if constexpr (PAIRED && TF32)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+            "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+    else if constexpr (PAIRED)
         asm volatile(
             "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+            "r"(idesc), "r"((uint32_t)add)
+            : "memory");
+    else if constexpr (TF32)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
             "r"(idesc), "r"((uint32_t)add)
             : "memory");
     else
@@ -162,6 +174,8 @@ __device__ __forceinline__ uint64_t operand_at(uint64_t first, uint32_t bytes) {
 __device__ __forceinline__ uint32_t mma_desc(bool bf16, bool a_mn, bool b_mn, int m, int n) {
     return 1u << 4 | (uint32_t)bf16 << 7 | (uint32_t)bf16 << 10 | (uint32_t)a_mn << 15 | (uint32_t)b_mn << 16 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24;
 }
+// the same of two tf32 operands, their summed index contiguous
+__device__ __forceinline__ uint32_t mma_desc_tf32(int m, int n) { return 1u << 4 | 2u << 7 | 2u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(m >> 4) << 24; }
 
 // 32 consecutive columns of the calling warp's 32 TMEM lanes, one lane per thread; there after tmem_wait
 __device__ __forceinline__ void tmem_start(uint32_t addr, float (&v)[32]) {
@@ -255,14 +269,23 @@ __device__ __forceinline__ float4 load_shared_float4(uint32_t addr) {
 }
 __device__ __forceinline__ void store_shared_f32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 
-// the products of one slice: `steps` (1..4) times 16 summed elements, the first overwriting the accumulator unless `add`
-template <bool PAIRED>
+// An fp32 value as the sum of two tf32 values, off by 2^-21 of it at most: its first eleven bits, and what is left rounded to
+// eleven.  The second has the first's sign and is no zero unless the value is one, so that an infinite factor gives the infinity
+// that the value would; of an infinite value it is next to nothing.
+__device__ __forceinline__ float tf32_first(float v) { return v != v ? v : __uint_as_float(__float_as_uint(v) & 0xffffe000u); }
+__device__ __forceinline__ float tf32_second(float v) {
+    const uint32_t rest = fabsf(v) < INFINITY ? (__float_as_uint(fabsf(v - tf32_first(v))) + 0x1000u) & 0xffffe000u : 0u;
+    return v == 0.0f ? 0.0f : copysignf(__uint_as_float(rest < 0x00800000u ? 0x00800000u : rest), v);
+}
+
+// the products of one slice: `steps` (1..4) times 32 bytes of summed elements, the first overwriting the accumulator unless `add`
+template <bool PAIRED, bool TF32 = false>
 __device__ __forceinline__ void tc_slice(uint32_t d, uint64_t a, uint64_t b, uint64_t a_step, uint64_t b_step, uint32_t idesc, int steps, bool add) {
     if (steps == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) tc_mma<PAIRED>(d, a + i * a_step, b + i * b_step, idesc, add || i > 0);
+        for (int i = 0; i < 4; ++i) tc_mma<PAIRED, TF32>(d, a + i * a_step, b + i * b_step, idesc, add || i > 0);
     } else {
-        for (int i = 0; i < steps; ++i) tc_mma<PAIRED>(d, a + i * a_step, b + i * b_step, idesc, add || i > 0);
+        for (int i = 0; i < steps; ++i) tc_mma<PAIRED, TF32>(d, a + i * a_step, b + i * b_step, idesc, add || i > 0);
     }
 }
 
