@@ -433,7 +433,7 @@ MPS_API int mps_group_rows(int32_t n_rows, int32_t per_row, int32_t n_groups, co
 /* y[s, :] = x[slot_row[s], :] * W[g]^T for the slots s of every group g: d_x n_rows x k, d_w n_groups x n x k, d_y n_slots x n.
  * transpose != 0: y[s, :] = x[slot_row[s], :] * W[g] with d_x n_rows x n and d_y n_slots x k - the gradient by the rows.
  * d_slot_row == NULL: x has a row per slot (n_rows >= n_slots).  Rows of d_y outside the groups are left as they were.
- * n_groups <= 1024; k and n up to 2^21. */
+ * n_groups <= 1024; k and n up to 2^21; n_slots and n_rows up to 2^31 - 1025. */
 MPS_API int mps_routed_product(int32_t n_slots, int32_t n_rows, int32_t n_groups, int32_t k, int32_t n, int dtype, int transpose,
                        const int32_t *d_group_ptr, const int32_t *d_slot_row, const void *d_x, const void *d_w, void *d_y, void *stream);
 
@@ -444,7 +444,7 @@ MPS_API int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_groups, 
 
 /* y[t, :] = sum over j of weights[t, j] * rows[slot_of[t, j], :] (d_weights NULL: 1 each; no term for a slot below 0):
  * mps_spmm with the routing as A, for a fixed number of terms per row, without a plan.  d_rows n_slots x dim, d_y n_rows x dim.
- * Summed in the order of j. */
+ * Summed in the order of j.  dim up to 2^24. */
 MPS_API int mps_routed_combine(int32_t n_rows, int32_t per_row, int32_t n_slots, int32_t dim, int dtype, const int32_t *d_slot_of,
                        const float *d_weights, const void *d_rows, void *d_y, void *stream);
 

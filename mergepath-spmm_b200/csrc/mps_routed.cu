@@ -476,6 +476,8 @@ int check_product(const char *who, int n_slots, int n_rows, int n_groups, int k,
     if (!known(dtype)) return fail(MPS_ERR_ARG, "%s: unknown dtype %d", who, dtype);
     if (n_groups > mps::kMaxRowGroups) return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d groups", who, mps::kMaxRowGroups);
     if (k > 1 << 21 || n > 1 << 21) return fail(MPS_ERR_UNSUPPORTED, "%s: k and n may be up to %d", who, 1 << 21);
+    constexpr int most = INT32_MAX - 1024;  // the end of a tile or slice that starts before the last one is still a 32-bit number
+    if (n_slots > most || n_rows > most) return fail(MPS_ERR_UNSUPPORTED, "%s: at most %d slots and rows", who, most);
     return MPS_OK;
 }
 
@@ -876,6 +878,7 @@ static int check_combine(const char *who, int n_rows, int per_row, int n_slots, 
     if (n_rows < 0 || per_row < 1 || n_slots < 0 || dim < 1) return fail(MPS_ERR_ARG, "%s: %d rows of %d terms, %d slots, dim %d", who, n_rows, per_row, n_slots, dim);
     if (!known(dtype)) return fail(MPS_ERR_ARG, "%s: unknown dtype %d", who, dtype);
     if ((long long)n_rows * per_row >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "%s: rows * per_row does not fit 31 bits", who);
+    if (dim > 1 << 24) return fail(MPS_ERR_UNSUPPORTED, "%s: dim may be up to %d", who, 1 << 24);  // stretches of a row are the grid's y
     return MPS_OK;
 }
 
