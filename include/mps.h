@@ -387,7 +387,8 @@ MPS_API int mps_multi_get_c(mps_multi *m, void *host_C, int32_t from_gpu);
  *
  * All of these launch asynchronously on `stream`, allocate nothing, keep nothing between calls, may be captured into a graph,
  * and run side by side on different streams.  Types are MPS_F32, MPS_F16 and MPS_BF16 (weights, biases and scales always
- * fp32); every sum is kept in fp32 and rounded once.  Arrays are contiguous; results do not depend on the run.  The device
+ * fp32); every sum is kept in fp32 and rounded once.  Arrays are contiguous; a result that shares memory with an operand is refused
+ * (but mps_routed_combine_backward may write d_drows over d_rows); results do not depend on the run.  The device
  * checks what it indexes by: a bad id, slot or group offset is skipped (no access outside the arrays, what it named is
  * undefined) and reported by mps_routed_check. */
 

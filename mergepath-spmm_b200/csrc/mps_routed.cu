@@ -40,6 +40,26 @@ int status_pointer(int **p) {
 
 bool misaligned(const void *p, size_t size) { return ((uintptr_t)p & (size - 1)) != 0; }
 size_t size_of(int dtype) { return dtype == MPS_F32 ? 4 : 2; }
+
+struct Span {
+    const void *at;
+    long long elements;
+};
+// Whether a result shares memory with an operand (or a result named after it), which other blocks may still have to read.
+bool overlap(int dtype, std::initializer_list<Span> results, std::initializer_list<Span> operands) {
+    const uintptr_t size = size_of(dtype);
+    auto meet = [&](const Span &a, const Span &b) {
+        const uintptr_t p = (uintptr_t)a.at, q = (uintptr_t)b.at;
+        return p && q && a.elements > 0 && b.elements > 0 && p < q + (uintptr_t)b.elements * size && q < p + (uintptr_t)a.elements * size;
+    };
+    for (const Span *r = results.begin(); r != results.end(); ++r) {
+        for (const Span &o : operands)
+            if (meet(*r, o)) return true;
+        for (const Span *q = r + 1; q != results.end(); ++q)
+            if (meet(*r, *q)) return true;
+    }
+    return false;
+}
 bool known(int dtype) { return dtype == MPS_F32 || dtype == MPS_F16 || dtype == MPS_BF16; }
 
 // ---------------------------------------------------------------------------------------------- combine
@@ -804,6 +824,8 @@ extern "C" int mps_routed_product(int32_t n_slots, int32_t n_rows, int32_t n_gro
     if (misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_x, size) || misaligned(d_w, size) || misaligned(d_y, size))
         return fail(MPS_ERR_ALIGN, "mps_routed_product: a pointer is not aligned to its element size");
     const int summed = transpose ? n : k, features = transpose ? k : n;
+    if (overlap(dtype, {{d_y, (long long)n_slots * features}}, {{d_x, (long long)n_rows * summed}, {d_w, (long long)n_groups * k * n}}))
+        return fail(MPS_ERR_ARG, "mps_routed_product: the result overlaps an operand");
     if (n_rows > 0 && tc_widths(dtype, {k, summed}, {d_x, d_w})) {
         TcRows a = {};
         a.bf16 = dtype == MPS_BF16;
@@ -844,6 +866,8 @@ extern "C" int mps_routed_wgrad(int32_t n_slots, int32_t n_rows, int32_t n_group
     const size_t size = size_of(dtype);
     if (misaligned(d_group_ptr, 4) || misaligned(d_slot_row, 4) || misaligned(d_x, size) || misaligned(d_dy, size) || misaligned(d_dw, size))
         return fail(MPS_ERR_ALIGN, "mps_routed_wgrad: a pointer is not aligned to its element size");
+    if (overlap(dtype, {{d_dw, (long long)n_groups * k * n}}, {{d_x, (long long)n_rows * k}, {d_dy, (long long)n_slots * n}}))
+        return fail(MPS_ERR_ARG, "mps_routed_wgrad: the result overlaps an operand");
     if (n_slots > 0 && n_rows > 0 && tc_widths(dtype, {k, n}, {d_x, d_dy})) {
         int sms;
         if (int rc = sm_count(&sms)) return rc;
@@ -890,6 +914,8 @@ extern "C" int mps_routed_combine(int32_t n_rows, int32_t per_row, int32_t n_slo
     const size_t size = size_of(dtype);
     if (misaligned(d_slot_of, 4) || misaligned(d_weights, 4) || misaligned(d_rows, size) || misaligned(d_y, size))
         return fail(MPS_ERR_ALIGN, "mps_routed_combine: a pointer is not aligned to its element size");
+    if (overlap(dtype, {{d_y, (long long)n_rows * dim}}, {{d_rows, (long long)n_slots * dim}}))
+        return fail(MPS_ERR_ARG, "mps_routed_combine: the result overlaps an operand");
     RD_BY_TYPE(dtype, launch_combine<T>(n_rows, per_row, n_slots, dim, d_slot_of, d_weights, d_rows, d_y, (cudaStream_t)stream));
 }
 
@@ -902,6 +928,8 @@ extern "C" int mps_routed_combine_backward(int32_t n_rows, int32_t per_row, int3
     if (misaligned(d_slot_of, 4) || misaligned(d_weights, 4) || misaligned(d_dweights, 4) || misaligned(d_dy, size) || misaligned(d_rows, size) ||
         misaligned(d_drows, size))
         return fail(MPS_ERR_ALIGN, "mps_routed_combine_backward: a pointer is not aligned to its element size");
+    if (overlap(dtype, {{d_drows, (long long)n_slots * dim}}, {{d_dy, (long long)n_rows * dim}, {d_rows == d_drows ? nullptr : d_rows, (long long)n_slots * dim}}))
+        return fail(MPS_ERR_ARG, "mps_routed_combine_backward: the result overlaps an operand");
     RD_BY_TYPE(dtype, launch_combine_backward<T>(n_rows, per_row, n_slots, dim, d_slot_of, d_weights, d_dy, d_rows, d_drows, d_dweights, (cudaStream_t)stream));
 }
 
@@ -921,6 +949,10 @@ extern "C" int mps_adapters(int32_t n_rows, int32_t k, int32_t n, int32_t n_adap
     const size_t size = size_of(dtype);
     if (misaligned(d_x, size) || misaligned(d_w, size) || misaligned(d_a, size) || misaligned(d_b, size) || misaligned(d_y, size))
         return fail(MPS_ERR_ALIGN, "mps_adapters: a pointer is not aligned to its element size");
+    const long long matrix = (long long)n_adapters * rank, space = (workspace_bytes + (int64_t)size - 1) / (int64_t)size;
+    if (overlap(dtype, {{d_y, (long long)n_rows * n}, {d_workspace, space}},
+                {{d_x, (long long)n_rows * k}, {d_w, (long long)n * k}, {d_a, matrix * k}, {d_b, matrix * n}}))
+        return fail(MPS_ERR_ARG, "mps_adapters: the result or the workspace overlaps an operand");
     RD_BY_TYPE(dtype, adapters<T>(s, d_x, d_w, d_a, d_b, d_y, d_workspace, (cudaStream_t)stream));
 }
 
@@ -935,6 +967,10 @@ extern "C" int mps_adapters_backward(int32_t n_rows, int32_t k, int32_t n, int32
     if (misaligned(d_dy, size) || misaligned(d_x, size) || misaligned(d_w, size) || misaligned(d_a, size) || misaligned(d_b, size) ||
         misaligned(d_dx, size) || misaligned(d_da, size) || misaligned(d_db, size))
         return fail(MPS_ERR_ALIGN, "mps_adapters_backward: a pointer is not aligned to its element size");
+    const long long matrix = (long long)n_adapters * rank, space = n_rows ? (workspace_bytes + (int64_t)size - 1) / (int64_t)size : 0;
+    if (overlap(dtype, {{d_dx, (long long)n_rows * k}, {d_da, matrix * k}, {d_db, matrix * n}, {d_workspace, space}},
+                {{d_dy, (long long)n_rows * n}, {d_x, (long long)n_rows * k}, {d_w, (long long)n * k}, {d_a, matrix * k}, {d_b, matrix * n}}))
+        return fail(MPS_ERR_ARG, "mps_adapters_backward: a result or the workspace overlaps an operand");
     if (n_rows == 0) {  // no rows: the adapters' gradients are zero
         const size_t bytes = (size_t)n_adapters * rank * size;
         RD_CUDA(cudaMemsetAsync(d_da, 0, bytes * k, (cudaStream_t)stream));

@@ -37,3 +37,42 @@ def test_workspace_of_sizes_the_adapters_refuse(mps):
     for backward in (0, 1):  # what a call needs grows with the call, and a call without rows needs nothing
         sizes = [L.mps_adapters_workspace(rows, 256, 512, 8, 16, 2, backward) for rows in (0, 1, 64, 4096)]
         assert sizes[0] == 0 and sizes[1] > 0 and sizes[1] < sizes[2] < sizes[3]
+
+
+def test_results_over_what_is_read(mps):
+    """A result that lies over an operand would be read after it was written."""
+    L, c = mps.capi.lib(), mps.capi
+    x, w, y = P, P << 1, P << 2
+    size = 2
+
+    def product(x, w, y, transpose=0):
+        return L.mps_routed_product(8, 4, 2, 16, 32, 2, transpose, P, P, x, w, y, None)
+
+    for rc in (product(x, w, x), product(x, w, x + (4 * 16 - 1) * size // 2 * 2), product(x, w, w), product(x, w, w - 16), product(x, w, x, 1)):
+        code(mps, rc, c.ERR_ARG, "overlap")
+    for rc in (L.mps_routed_wgrad(8, 4, 2, 16, 32, 2, P, P, x, w, x, None), L.mps_routed_wgrad(8, 4, 2, 16, 32, 2, P, P, x, w, w + 2, None)):
+        code(mps, rc, c.ERR_ARG, "overlap")
+    code(mps, L.mps_routed_combine(4, 2, 8, 16, 2, P, P, x, x, None), c.ERR_ARG, "overlap")
+    code(mps, L.mps_routed_combine(4, 2, 8, 16, 2, P, P, x, x - 2, None), c.ERR_ARG, "overlap")
+    code(mps, L.mps_routed_combine_backward(4, 2, 8, 16, 2, P, P, x, w, x, P, None), c.ERR_ARG, "overlap")
+    code(mps, L.mps_routed_combine_backward(4, 2, 8, 16, 2, P, P, x, w, w + 2, P, None), c.ERR_ARG, "overlap")  # in place, but shifted
+
+    need = L.mps_adapters_workspace(16, 64, 64, 4, 8, 2, 1)
+    at = {name: P * (i + 1) for i, name in enumerate(("dy", "x", "w", "a", "b", "y", "dx", "da", "db", "ws"))}
+
+    def forward(**change):
+        t = {**at, **change}
+        return L.mps_adapters(16, 64, 64, 4, 8, 2, P, P, P, None, t["x"], t["w"], t["a"], t["b"], t["y"], t["ws"], need, None)
+
+    def backward(**change):
+        t = {**at, **change}
+        return L.mps_adapters_backward(16, 64, 64, 4, 8, 2, P, P, P, None, t["dy"], t["x"], t["w"], t["a"], t["b"], t["dx"], t["da"], t["db"], t["ws"], need, None)
+
+    for operand in ("x", "w", "a", "b"):
+        code(mps, forward(y=at[operand]), c.ERR_ARG, "overlap")
+        for result in ("dx", "da", "db"):
+            code(mps, backward(**{result: at[operand]}), c.ERR_ARG, "overlap")
+    code(mps, backward(dx=at["dy"]), c.ERR_ARG, "overlap")
+    code(mps, forward(ws=at["x"]), c.ERR_ARG, "overlap")
+    code(mps, backward(ws=at["dx"]), c.ERR_ARG, "overlap")
+    code(mps, backward(da=at["db"]), c.ERR_ARG, "overlap")
