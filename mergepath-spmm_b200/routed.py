@@ -286,7 +286,11 @@ def adapters_backward(dy, x, w, a, b, ids, groups: Groups, scale=None, *, stream
 
 
 def routed_check(device=None, stream=None) -> None:
-    """Waits for the stream and raises if a routed operator on the device met an index out of range or gave up a wait since
-    the last check."""
-    with torch.cuda.device(torch.cuda.current_device() if device is None else device):
-        capi.check(capi.lib().mps_routed_check((torch.cuda.current_stream() if stream is None else stream).cuda_stream))
+    """Waits for the stream and raises if a routed operator on the device (default: the stream's, or the current one) met an index
+    out of range or gave up a wait since the last check."""
+    if device is None:
+        device = torch.device("cuda", torch.cuda.current_device()) if stream is None else stream.device
+    device = torch.device("cuda", device) if isinstance(device, int) else torch.device(device)
+    if device.index is None:
+        device = torch.device(device.type, torch.cuda.current_device())
+    _call(device, stream, "mps_routed_check")
