@@ -30,6 +30,7 @@ namespace {
     } while (0)
 
 __device__ int g_status;
+__global__ void clear_status(int bits) { atomicAnd(&g_status, ~bits); }
 
 constexpr int kMaxExperts = 1024;   // 32 keys per lane
 constexpr int kMaxTop = 32;         // one chosen expert per lane
@@ -891,10 +892,13 @@ bool misaligned(const void *p, size_t size) { return ((uintptr_t)p & (size - 1))
 namespace mps {
 int take_route_status(void *stream, int *status) {
     cudaStream_t st = (cudaStream_t)stream;
-    static const int zero = 0;
     RT_CUDA(cudaMemcpyFromSymbolAsync(status, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
     RT_CUDA(cudaStreamSynchronize(st));
-    if (*status) RT_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+    if (*status) {  // see mps_routed_check
+        clear_status<<<1, 1, 0, st>>>(*status);
+        RT_CUDA(cudaGetLastError());
+        RT_CUDA(cudaStreamSynchronize(st));
+    }
     return MPS_OK;
 }
 int list_rows_and_rest(int n_rows, int n_groups, const int32_t *ids, int32_t *group_ptr, int32_t *slot_row, void *stream) {

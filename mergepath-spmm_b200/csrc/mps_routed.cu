@@ -27,6 +27,7 @@ namespace {
     } while (0)
 
 __device__ int g_status;
+__global__ void clear_status(int bits) { atomicAnd(&g_status, ~bits); }
 
 int status_pointer(int **p) {
     static mps::PerDevice<int *> known;
@@ -983,10 +984,13 @@ extern "C" int mps_adapters_backward(int32_t n_rows, int32_t k, int32_t n, int32
 extern "C" int mps_routed_check(void *stream) {
     cudaStream_t st = (cudaStream_t)stream;
     int routed = 0, route = 0;
-    static const int zero = 0;
     RD_CUDA(cudaMemcpyFromSymbolAsync(&routed, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
     RD_CUDA(cudaStreamSynchronize(st));
-    if (routed) RD_CUDA(cudaMemcpyToSymbolAsync(g_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, st));
+    if (routed) {  // what was read and nothing else: another stream may have reported something since; done when this returns
+        clear_status<<<1, 1, 0, st>>>(routed);
+        RD_CUDA(cudaGetLastError());
+        RD_CUDA(cudaStreamSynchronize(st));
+    }
     if (int rc = mps::take_route_status(st, &route)) return rc;
     const int status = routed | route;
     if (status & mps::kStatusTimeout) return fail(MPS_ERR_DEVICE, "mps_routed_check: a kernel gave up a wait");
