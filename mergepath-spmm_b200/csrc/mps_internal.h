@@ -30,6 +30,8 @@ struct PerDevice {
     }
 };
 
+// SMs of the current device (mps_route.cu).
+int sm_count(int *n);
 // Status word of the routing kernels on the current device (mps_route.cu): waits for the stream, returns it and clears it.
 int take_route_status(void *stream, int *status);
 // Rows listed by id as by mps_group_rows (device arrays), those without a valid id as a last group behind the others:

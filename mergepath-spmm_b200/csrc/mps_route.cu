@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(32 * kRouteWarps, VPL <= 8 ? 8 : 1) route_kern
 // 16-bit logits without a bias they are zeros); behind the last place every key is compared with the last pick until they are
 // too far down for the five bits to matter.  16384 rows of 256 experts, top 8 of 4 of 8 groups:
 // 30 us, 42 with a warp per row (which keeps fewer rows, other group counts and more experts).
-constexpr int kOctetRows = 2048;  // from here on there are rows enough for 148 SMs
+constexpr int kOctetRows = 2048;  // from here on there are rows enough for a B200's 148 SMs
 
 template <typename T, int VPL, bool SIGMOID>
 __global__ void __launch_bounds__(32 * kRouteWarps, 6) route_octet_kernel(const RouteArgs a, const T *__restrict__ logits, const float *__restrict__ bias,
@@ -833,17 +833,30 @@ int launch_group(long long n_pairs, int per_row, int n_groups, bool rest, const 
     return MPS_OK;
 }
 
+// Blocks for `want` blocks' worth of rows: no more than the device has room for at once, each then walks over its share.
+template <typename Kernel>
+int resident_blocks(Kernel kernel, long long want, size_t smem, unsigned *blocks) {
+    int sms, per_sm = 1;
+    if (int rc = mps::sm_count(&sms)) return rc;
+    if (want > sms) RT_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, 32 * kRouteWarps, smem));
+    const long long room = (long long)sms * per_sm;
+    *blocks = (unsigned)(want < room ? want : room);
+    return MPS_OK;
+}
+
 template <typename T, bool SIGMOID>
 int launch_route(const RouteArgs &a, const void *logits, const float *bias, int *ids, float *weights, cudaStream_t st) {
     const size_t smem = (size_t)kRouteWarps * (a.n_experts + (a.n_experts >> 5) + 1) * sizeof(double);
-    const long long want = ((long long)a.n_rows + kRouteWarps - 1) / kRouteWarps;
-    const unsigned blocks = (unsigned)(want < 148 * 8 ? want : 148 * 8);  // what is resident at once
     const int per_lane = (a.n_experts + 31) / 32;
     if (a.n_rows >= kOctetRows && a.n_experts % 8 == 0 && a.n_experts <= 256 && a.n_groups <= 8 && 8 % a.n_groups == 0) {
-        const long long most = ((long long)a.n_rows + 4 * kRouteWarps - 1) / (4 * kRouteWarps);
-        const unsigned grid = (unsigned)(most < 148 * 8 ? most : 148 * 8);
+        const long long want = ((long long)a.n_rows + 4 * kRouteWarps - 1) / (4 * kRouteWarps);
+        unsigned grid;
         const bool vectors = a.n_experts / 8 * sizeof(T) % 16 == 0 && ((uintptr_t)logits & 15) == 0;
-#define RT_LAUNCH(V) route_octet_kernel<T, V, SIGMOID><<<grid, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, bias, ids, weights, vectors)
+#define RT_LAUNCH(V)                                                                                                                          \
+    do {                                                                                                                                      \
+        if (int rc = resident_blocks(route_octet_kernel<T, V, SIGMOID>, want, smem, &grid)) return rc;                                        \
+        route_octet_kernel<T, V, SIGMOID><<<grid, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, bias, ids, weights, vectors);           \
+    } while (0)
         if (a.n_experts <= 64) RT_LAUNCH(8);
         else if (a.n_experts <= 128) RT_LAUNCH(16);
         else RT_LAUNCH(32);
@@ -851,7 +864,13 @@ int launch_route(const RouteArgs &a, const void *logits, const float *bias, int 
         RT_CUDA(cudaGetLastError());
         return MPS_OK;
     }
-#define RT_LAUNCH(V) route_kernel<T, V, SIGMOID><<<blocks, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, bias, ids, weights)
+    const long long want = ((long long)a.n_rows + kRouteWarps - 1) / kRouteWarps;
+    unsigned blocks;
+#define RT_LAUNCH(V)                                                                                                       \
+    do {                                                                                                                   \
+        if (int rc = resident_blocks(route_kernel<T, V, SIGMOID>, want, smem, &blocks)) return rc;                         \
+        route_kernel<T, V, SIGMOID><<<blocks, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, bias, ids, weights);     \
+    } while (0)
     if (per_lane <= 1) RT_LAUNCH(1);
     else if (per_lane <= 2) RT_LAUNCH(2);
     else if (per_lane <= 4) RT_LAUNCH(4);
@@ -890,6 +909,15 @@ bool misaligned(const void *p, size_t size) { return ((uintptr_t)p & (size - 1))
 }  // namespace
 
 namespace mps {
+int sm_count(int *n) {
+    static PerDevice<int> known;
+    int dev = 0;
+    RT_CUDA(cudaGetDevice(&dev));
+    if ((*n = known.get(dev))) return MPS_OK;
+    RT_CUDA(cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev));
+    known.put(dev, *n);
+    return MPS_OK;
+}
 int take_route_status(void *stream, int *status) {
     cudaStream_t st = (cudaStream_t)stream;
     RT_CUDA(cudaMemcpyFromSymbolAsync(status, g_status, sizeof(int), 0, cudaMemcpyDeviceToHost, st));
@@ -946,8 +974,10 @@ template <typename T>
 static int launch_route_backward(const RouteArgs &a, bool sigmoid_score, const void *logits, const int *ids, const float *d_weights, void *d_logits,
                                  cudaStream_t st) {
     const long long want = ((long long)a.n_rows + kRouteWarps - 1) / kRouteWarps;
-    const unsigned blocks = (unsigned)(want < 148 * 16 ? want : 148 * 16);
     const size_t smem = (size_t)kRouteWarps * a.n_experts * sizeof(float);
+    unsigned blocks;
+    if (int rc = sigmoid_score ? resident_blocks(route_backward_kernel<T, true>, want, smem, &blocks) : resident_blocks(route_backward_kernel<T, false>, want, smem, &blocks))
+        return rc;
     if (sigmoid_score) route_backward_kernel<T, true><<<blocks, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, ids, d_weights, (T *)d_logits);
     else route_backward_kernel<T, false><<<blocks, 32 * kRouteWarps, smem, st>>>(a, (const T *)logits, ids, d_weights, (T *)d_logits);
     RT_CUDA(cudaGetLastError());

@@ -13,6 +13,7 @@
 #include "mps_types.cuh"
 
 using mps::fail;
+using mps::sm_count;
 using mps::OuterArgs;
 using mps::RowsArgs;
 using mps::TcOuter;
@@ -268,16 +269,6 @@ int launch_plain_outer(OuterArgs a, const void *p, const void *q, void *out, cud
 }
 
 // ---- tensor cores
-
-int sm_count(int *n) {
-    static mps::PerDevice<int> known;
-    int dev = 0;
-    RD_CUDA(cudaGetDevice(&dev));
-    if ((*n = known.get(dev))) return MPS_OK;
-    RD_CUDA(cudaDeviceGetAttribute(n, cudaDevAttrMultiProcessorCount, dev));
-    known.put(dev, *n);
-    return MPS_OK;
-}
 
 // Tensor map of `dims` sizes (innermost first, rows packed) of one of the types, read in boxes of 128 bytes by box_rows.
 int tensor_map(CUtensorMap *map, int dtype, const void *base, int dims, unsigned long long d0, unsigned long long d1, unsigned long long d2, int box_rows) {
