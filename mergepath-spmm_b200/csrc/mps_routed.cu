@@ -292,10 +292,9 @@ int tensor_map(CUtensorMap *map, int dtype, const void *base, int dims, unsigned
     return MPS_OK;
 }
 
-// A launch of `blocks` blocks in clusters; `follows`: the launch before it on the stream is one of the same call, and this one may
-// start before that has ended.
-template <auto Kernel, typename Args>
-int launch_tc(const Args &args, long long blocks, int cluster, size_t smem, bool follows, cudaStream_t st) {
+// Lets the kernel have the device's shared memory, once per device.
+template <auto Kernel>
+int allow_smem() {
     static mps::PerDevice<int> allowed;  // shared memory the kernel may ask for
     int dev = 0;
     RD_CUDA(cudaGetDevice(&dev));
@@ -307,6 +306,42 @@ int launch_tc(const Args &args, long long blocks, int cluster, size_t smem, bool
         RD_CUDA(cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, most - (int)at.sharedSizeBytes));
         allowed.put(dev, most);
     }
+    return MPS_OK;
+}
+
+// Clusters of that size that the device runs at once, one block per SM.  Fewer than SMs / size: a cluster lies in one GPC (a B200
+// runs 33 of four and 15 of eight).  Tiles are dealt out by block number, so a cluster that starts behind another doubles the time.
+template <auto Kernel>
+int clusters_at_once(int cluster, size_t smem, int sms, int *n) {
+    static mps::PerDevice<int> known[4];  // of 1, 2, 4 and 8 blocks
+    const int which = cluster == 1 ? 0 : cluster == 2 ? 1 : cluster == 4 ? 2 : 3;
+    int dev = 0;
+    RD_CUDA(cudaGetDevice(&dev));
+    if ((*n = known[which].get(dev)) == 0) {
+        if (int rc = allow_smem<Kernel>()) return rc;
+        cudaLaunchAttribute attr;
+        attr.id = cudaLaunchAttributeClusterDimension;
+        attr.val.clusterDim.x = cluster;
+        attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(cluster);
+        cfg.blockDim = dim3(mps::kTcThreads);
+        cfg.dynamicSmemBytes = smem;
+        cfg.attrs = &attr;
+        cfg.numAttrs = 1;
+        RD_CUDA(cudaOccupancyMaxActiveClusters(n, Kernel, &cfg));
+        if (*n < 1) *n = 1;
+        known[which].put(dev, *n);
+    }
+    if (*n > sms / cluster) *n = sms / cluster;  // of those left to this launch
+    return MPS_OK;
+}
+
+// A launch of `blocks` blocks in clusters; `follows`: the launch before it on the stream is one of the same call, and this one may
+// start before that has ended.
+template <auto Kernel, typename Args>
+int launch_tc(const Args &args, long long blocks, int cluster, size_t smem, bool follows, cudaStream_t st) {
+    if (int rc = allow_smem<Kernel>()) return rc;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
@@ -363,8 +398,7 @@ Cut best_cut(int slots, int groups, int features, int steps, bool gather, int sm
 }
 
 // Blocks for two products side by side, in proportion to their work; each at least a cluster, none more than it has tiles for.
-void share_blocks(int sms, int cluster, const long long (&tiles)[2], const double (&work)[2], long long (&blocks)[2]) {
-    const long long clusters = sms / cluster;
+void share_blocks(long long clusters, int cluster, const long long (&tiles)[2], const double (&work)[2], long long (&blocks)[2]) {
     long long first = tiles[1] ? (long long)(clusters * work[0] / (work[0] + work[1]) + 0.5) : clusters;
     if (tiles[1]) first = first < 1 ? 1 : first > clusters - 1 ? clusters - 1 : first;
     const long long second = tiles[1] < clusters - first ? tiles[1] : clusters - first;  // what one has no use for goes to the other
@@ -388,10 +422,13 @@ int launch_tc_rows(const mps::TcRowsLaunch &in, int sms, int *used, cudaStream_t
         work[i] = (double)tiles[i] * a.k;
         if (tiles[i] >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "routed product: %lld tiles", tiles[i]);
     }
-    share_blocks(sms, cluster, tiles, work, blocks);
+    const size_t smem = mps::TcShape<NT>::bytes(l.p[0].n_groups);
+    int clusters;
+    if (int rc = clusters_at_once<mps::tc_rows_kernel<NT, TWO, RANK>>(cluster, smem, sms, &clusters)) return rc;
+    share_blocks(clusters, cluster, tiles, work, blocks);
     l.second = (int)blocks[0];
     if (used) *used = (int)(blocks[0] + blocks[1]);
-    return launch_tc<mps::tc_rows_kernel<NT, TWO, RANK>>(l, blocks[0] + blocks[1], cluster, mps::TcShape<NT>::bytes(l.p[0].n_groups), l.p[0].follows, st);
+    return launch_tc<mps::tc_rows_kernel<NT, TWO, RANK>>(l, blocks[0] + blocks[1], cluster, smem, l.p[0].follows, st);
 }
 
 // One product, or two of the same groups side by side (at most 64 slots per tile): what every use has in common filled in.  x_rows: rows of each x.
@@ -449,7 +486,9 @@ int launch_tc_outer(const mps::TcOuterLaunch &in, int sms, cudaStream_t st) {
     const int split = NT <= 128 ? split_of(tiles[0] + tiles[1], steps, sms) : 1, cluster = mps::TcOuterShape<NT>::kPaired ? 2 : split;
     l.p[0].split = l.p[1].split = split;
     const double work[2] = {(double)tiles[0], (double)tiles[1]};
-    share_blocks(sms, cluster, tiles, work, blocks);
+    int clusters;
+    if (int rc = clusters_at_once<mps::tc_outer_kernel<NT, TWO>>(cluster, mps::TcOuterShape<NT>::kBytes, sms, &clusters)) return rc;
+    share_blocks(clusters, cluster, tiles, work, blocks);
     l.second = (int)blocks[0];
     return launch_tc<mps::tc_outer_kernel<NT, TWO>>(l, blocks[0] + blocks[1], cluster, mps::TcOuterShape<NT>::kBytes, a.follows, st);
 }
