@@ -409,7 +409,7 @@ void share_blocks(long long clusters, int cluster, const long long (&tiles)[2], 
 
 int type_of(bool bf16) { return bf16 ? MPS_BF16 : MPS_F16; }
 
-template <int NT, bool TWO, bool RANK = false>
+template <int NT, mps::TcUse USE, bool TWO = false>
 int launch_tc_rows(const mps::TcRowsLaunch &in, int sms, int *used, cudaStream_t st) {
     mps::TcRowsLaunch l = in;
     const int tile_f = mps::kTcFeatures * (mps::TcShape<NT>::kPaired ? 2 : 1), cluster = mps::TcShape<NT>::kPaired ? 2 : l.p[0].split;
@@ -424,15 +424,23 @@ int launch_tc_rows(const mps::TcRowsLaunch &in, int sms, int *used, cudaStream_t
     }
     const size_t smem = mps::TcShape<NT>::bytes(l.p[0].n_groups);
     int clusters;
-    if (int rc = clusters_at_once<mps::tc_rows_kernel<NT, TWO, RANK>>(cluster, smem, sms, &clusters)) return rc;
+    if (int rc = clusters_at_once<mps::tc_rows_kernel<NT, USE, TWO>>(cluster, smem, sms, &clusters)) return rc;
     share_blocks(clusters, cluster, tiles, work, blocks);
     l.second = (int)blocks[0];
     if (used) *used = (int)(blocks[0] + blocks[1]);
-    return launch_tc<mps::tc_rows_kernel<NT, TWO, RANK>>(l, blocks[0] + blocks[1], cluster, smem, l.p[0].follows, st);
+    return launch_tc<mps::tc_rows_kernel<NT, USE, TWO>>(l, blocks[0] + blocks[1], cluster, smem, l.p[0].follows, st);
 }
 
-// One product, or two of the same groups side by side (at most 64 slots per tile): what every use has in common filled in.  x_rows: rows of each x.
-// used (or NULL): the launch's blocks, each with an SM to itself.
+// The matrices of a: stored features x summed (MN-major: summed x features), `groups` of them.
+int tc_matrix(CUtensorMap *map, TcRows *a, const void *w, int summed, int features, long long groups) {
+    a->w_rows = features < mps::kTcFeatures ? (features + 7) / 8 * 8 : mps::kTcFeatures;
+    return a->mn_major ? tensor_map(map, type_of(a->bf16), w, 3, features, summed, groups, mps::kTcDepth)
+                       : tensor_map(map, type_of(a->bf16), w, 3, summed, features, groups, a->w_rows);
+}
+
+// One product, or two narrow ones of the same groups side by side (at most 64 slots per tile): what every use has in common filled in.
+// x_rows: rows of each x.  used (or NULL): the launch's blocks, each with an SM to itself.
+template <mps::TcUse USE>
 int tc_rows(const TcRows *products, int n, const Cut &cut, const void *const *x, long long x_rows, int sms, cudaStream_t st, int *used = nullptr) {
     mps::TcRowsLaunch l = {};
     const int loaded = cut.nt == 256 ? mps::TcShape<256>::kRows : cut.nt;  // slots a block loads
@@ -445,29 +453,23 @@ int tc_rows(const TcRows *products, int n, const Cut &cut, const void *const *x,
         if (a.gather)
             if (int rc = tensor_map(&a.x_run, type_of(a.bf16), x[i], 2, a.k, x_rows, 1, loaded / 8)) return rc;
         if (a.rank) {
-            if (int rc = tensor_map(&a.u, MPS_F32, a.u_base, 2, a.rank, 2ull * x_rows, 1, 1)) return rc;
-            if (int rc = tensor_map(&a.u_run, MPS_F32, a.u_base, 2, a.rank, 2ull * x_rows, 1, loaded / 8)) return rc;
-            if (int rc = tensor_map(&a.w2, MPS_F32, a.w2_base, 3, a.rank, a.n, a.rank_groups, a.w_rows)) return rc;
+            const int type = a.bf16 ? MPS_BF16 : MPS_F32;
+            if (int rc = tensor_map(&a.u, type, a.u_base, 2, a.rank, 2ull * x_rows, 1, 1)) return rc;
+            if (int rc = tensor_map(&a.u_run, type, a.u_base, 2, a.rank, 2ull * x_rows, 1, loaded / 8)) return rc;
+            if (a.bf16) {
+                if (int rc = tc_matrix(&a.w2, &a, a.w2_base, a.rank, a.n, a.rank_groups)) return rc;
+            } else if (int rc = tensor_map(&a.w2, MPS_F32, a.w2_base, 3, a.rank, a.n, a.rank_groups, a.w_rows)) return rc;
         }
     }
-    if (n == 2) return cut.nt == 32 ? launch_tc_rows<32, true>(l, sms, used, st) : launch_tc_rows<64, true>(l, sms, used, st);
-    if (l.p[0].rank) {
-        if (cut.nt == 32) return launch_tc_rows<32, false, true>(l, sms, used, st);
-        if (cut.nt == 64) return launch_tc_rows<64, false, true>(l, sms, used, st);
-        if (cut.nt == 128) return launch_tc_rows<128, false, true>(l, sms, used, st);
-        return launch_tc_rows<256, false, true>(l, sms, used, st);
+    if constexpr (USE == mps::kNarrow)
+        if (n == 2) return cut.nt == 32 ? launch_tc_rows<32, USE, true>(l, sms, used, st) : launch_tc_rows<64, USE, true>(l, sms, used, st);
+    if (cut.nt == 32) return launch_tc_rows<32, USE>(l, sms, used, st);
+    if constexpr (USE == mps::kByRow) return launch_tc_rows<64, USE>(l, sms, used, st);
+    else {
+        if (cut.nt == 64) return launch_tc_rows<64, USE>(l, sms, used, st);
+        if (cut.nt == 128) return launch_tc_rows<128, USE>(l, sms, used, st);
+        return launch_tc_rows<256, USE>(l, sms, used, st);
     }
-    if (cut.nt == 32) return launch_tc_rows<32, false>(l, sms, used, st);
-    if (cut.nt == 64) return launch_tc_rows<64, false>(l, sms, used, st);
-    if (cut.nt == 128) return launch_tc_rows<128, false>(l, sms, used, st);
-    return launch_tc_rows<256, false>(l, sms, used, st);
-}
-
-// The matrices of a: stored features x summed (MN-major: summed x features), `groups` of them.
-int tc_matrix(CUtensorMap *map, TcRows *a, const void *w, int summed, int features, long long groups) {
-    a->w_rows = features < mps::kTcFeatures ? (features + 7) / 8 * 8 : mps::kTcFeatures;
-    return a->mn_major ? tensor_map(map, type_of(a->bf16), w, 3, features, summed, groups, mps::kTcDepth)
-                       : tensor_map(map, type_of(a->bf16), w, 3, summed, features, groups, a->w_rows);
 }
 
 template <int NT, bool TWO>
@@ -477,7 +479,7 @@ int launch_tc_outer(const mps::TcOuterLaunch &in, int sms, cudaStream_t st) {
     long long tiles[2] = {}, blocks[2];
     for (int i = 0; i < (TWO ? 2 : 1); ++i) {
         const TcOuter &a = l.p[i];
-        const int cols = a.pair ? NT / 2 : NT;
+        const int cols = TWO ? NT / 2 : NT;
         tiles[i] = (long long)a.n_groups * ((a.i + tile_f - 1) / tile_f) * ((a.j + cols - 1) / cols);
         if (tiles[i] >= 1LL << 31) return fail(MPS_ERR_UNSUPPORTED, "routed matrix gradient: %lld tiles", tiles[i]);
     }
@@ -501,7 +503,7 @@ int tc_outer(const TcOuter *products, int n, const void *const *p, const void *c
         TcOuter &a = l.p[i];
         a = products[i];
         if (int rc = status_pointer(&a.status)) return rc;
-        const unsigned long long q_rows = (a.pair ? 2ull : 1ull) * a.n_slots;
+        const unsigned long long q_rows = n * (unsigned long long)a.n_slots;
         if (int rc = tensor_map(&a.p_rows, type_of(a.bf16), p[i], 2, a.i, a.n_p_rows, 1, 1)) return rc;
         if (int rc = tensor_map(&a.p_tile, type_of(a.bf16), p[i], 2, a.i, a.n_p_rows, 1, mps::kTcDepth)) return rc;
         if (int rc = tensor_map(&a.q_rows, type_of(a.bf16), q[i], 2, a.j, q_rows, 1, 1)) return rc;
@@ -585,20 +587,21 @@ int adapter_wide(const AdapterShape &s, int k, int n, const void *x, const void 
 // Made for the SMs of a B200 whatever the device has free, so that a call decides as its workspace's size was decided.
 bool by_rows(const AdapterShape &s, int k, int n, bool by_rank, Cut *cut) {
     constexpr int sms = 148;
-    const Cut grouped = best_cut(s.n_rows, s.n_adapters + 1, n, steps_of(k) + 2 * ((s.rank + mps::kRankDepth - 1) / mps::kRankDepth), true, sms, 256);
+    const Cut grouped = best_cut(s.n_rows, s.n_adapters + 1, n, steps_of(k) + 2 * steps_of(s.rank), true, sms, 256);
     const Cut rows = best_cut(s.n_rows, 1, n, steps_of(k), false, sms, 64);
     const double low_rank = (double)s.n_rows * n * s.rank / ((by_rank ? 1.5 : 6.0) * sms);
     *cut = rows.cycles + low_rank < grouped.cycles ? rows : grouped;
     return rows.cycles + low_rank < grouped.cycles;
 }
 
-// Workspace.  The intermediates in fp32, by row; where rows are tiled by adapter the one that the wide product reads as two planes
-// of tf32 values, and the adapters' matrices in fp32 with the rank contiguous; for the matrix gradients both intermediates as two
-// planes of the type in slot order with their exponents, and the magnitudes these come from; then the rows listed with those that
-// ask for no adapter behind the others.  Where no tensor map describes the operands the first two are all.
+// Workspace.  The intermediates in fp32, by row; where rows are tiled by adapter the one that the wide product reads in two planes,
+// by row, and in fp16 the adapters' matrices in fp32 with the rank contiguous; for the matrix gradients both intermediates in two
+// planes of the type in slot order, in fp16 with their exponents and the magnitudes that these come from; then the rows listed with
+// those that ask for no adapter behind the others.  Where no tensor map describes the operands the first two are all.
 struct AdapterSpace {
-    float *u, *v, *wide, *m;
-    uint16_t *u_planes, *v_planes;
+    float *u, *v, *m;
+    char *wide;
+    uint16_t *u_slots, *v_slots;
     unsigned *u_maxima, *v_maxima;
     int *u_exponents, *v_exponents, *ptr, *row;
     bool rows;  // see by_rows
@@ -611,17 +614,17 @@ struct AdapterSpace {
             if (wanted) at += (count * (int64_t)sizeof(*p) + 255) / 256 * 256;
         };
         const int64_t values = (int64_t)s.n_rows * s.rank;
-        const bool tc = s.dtype != MPS_F32 && s.k % 8 == 0 && s.rank % 8 == 0 && (!backward || s.n % 8 == 0);
+        const bool tc = s.dtype != MPS_F32 && s.k % 8 == 0 && s.rank % 8 == 0 && (!backward || s.n % 8 == 0), fp16 = s.dtype == MPS_F16;
         const int summed = backward ? s.n : s.k, features = backward ? s.k : s.n;  // of the wide product
         rows = by_rows(s, summed, features, backward, &cut);
         take(u, true, values);
         take(v, backward, values);
-        take(wide, tc && !rows, 2 * values);
-        take(m, tc && !rows, (int64_t)s.n_adapters * features * s.rank);
+        take(wide, tc && !rows, 2 * values * (fp16 ? 4 : 2));
+        take(m, tc && !rows && fp16, (int64_t)s.n_adapters * features * s.rank);
         for (int i = 0; i < 2; ++i) {
-            take(i ? v_planes : u_planes, tc && backward, 2 * values);
-            take(i ? v_maxima : u_maxima, tc && backward, (int64_t)s.n_rows * ((s.rank + 31) / 32));
-            take(i ? v_exponents : u_exponents, tc && backward, (int64_t)s.n_adapters * ((s.rank + 63) / 64));
+            take(i ? v_slots : u_slots, tc && backward, 2 * values);
+            take(i ? v_maxima : u_maxima, tc && backward && fp16, (int64_t)s.n_rows * ((s.rank + 31) / 32));
+            take(i ? v_exponents : u_exponents, tc && backward && fp16, (int64_t)s.n_adapters * ((s.rank + 63) / 64));
         }
         take(ptr, tc && !rows, s.n_adapters + 2);
         take(row, tc && !rows, s.n_rows);
@@ -629,29 +632,23 @@ struct AdapterSpace {
     }
 };
 
-// The narrow product of rows of x with the adapters' matrices (mn_major: stored summed x rank): scale * x A by row, in fp32 (u), as
-// planes of tf32 values and with its largest magnitudes, each where not NULL.
-int tc_adapter_narrow(const AdapterShape &s, int k, const void *m, bool mn_major, float *u, float *u_tf32, unsigned *maxima, TcRows *out) {
-    TcRows a = {};
-    a.bf16 = s.dtype == MPS_BF16;
-    a.mn_major = mn_major;
-    a.group_ptr = s.group_ptr;
-    a.slot_row = s.slot_row;
-    a.n_groups = s.n_adapters;
-    a.n_slots = a.n_x_rows = s.n_rows;
-    a.k = k;
-    a.n = s.rank;
-    a.gather = true;
-    a.group_scale = s.scale;
-    a.out_f32 = u;
-    a.out_tf32 = u_tf32;
-    a.maxima = maxima;
-    if (int rc = tc_matrix(&a.w, &a, m, k, s.rank, s.n_adapters)) return rc;
-    *out = a;
-    return MPS_OK;
+// The narrow product of rows of x with the adapters' matrices (mn_major: stored summed x rank): scale * x A, stored as its out_...
+// pointers ask.
+int tc_adapter_narrow(const AdapterShape &s, int k, const void *m, bool mn_major, TcRows *a) {
+    a->bf16 = s.dtype == MPS_BF16;
+    a->mn_major = mn_major;
+    a->group_ptr = s.group_ptr;
+    a->slot_row = s.slot_row;
+    a->n_groups = s.n_adapters;
+    a->n_slots = a->n_x_rows = s.n_rows;
+    a->k = k;
+    a->n = s.rank;
+    a->gather = true;
+    a->group_scale = s.scale;
+    return tc_matrix(&a->w, a, m, k, s.rank, s.n_adapters);
 }
 
-// What the products behind the narrow one read, see adapter_prepare_kernel.  m (or NULL): the wide product's adapter matrices.
+// What the products behind the narrow one read in fp16, see adapter_prepare_kernel.  m (or NULL): the wide product's adapter matrices.
 int tc_adapter_prepare(const AdapterShape &s, const AdapterSpace &ws, const void *m, bool by_rank, int features, bool backward, int span, int sms, cudaStream_t st) {
     mps::PrepareArgs a = {};
     a.group_ptr = s.group_ptr;
@@ -663,13 +660,15 @@ int tc_adapter_prepare(const AdapterShape &s, const AdapterSpace &ws, const void
     a.m_f32 = ws.m;
     a.features = features;
     a.by_rank = by_rank;
+    a.run = 1;
     if (backward) {
+        // as many slots per warp as a group has on average: a warp takes one group after the other, about a microsecond each, and
+        // reads what a large one's exponent comes from again for every run of its slots
+        while (a.run < 32 && 2 * a.run * s.n_adapters <= s.n_rows) a.run *= 2;
         a.values[0] = ws.u, a.values[1] = ws.v;
-        a.planes[0] = ws.u_planes, a.planes[1] = ws.v_planes;
-        if (s.dtype == MPS_F16) {  // bf16 has fp32's range
-            a.maxima[0] = ws.u_maxima, a.maxima[1] = ws.v_maxima;
-            a.exponents[0] = ws.u_exponents, a.exponents[1] = ws.v_exponents;
-        }
+        a.planes[0] = ws.u_slots, a.planes[1] = ws.v_slots;
+        a.maxima[0] = ws.u_maxima, a.maxima[1] = ws.v_maxima;
+        a.exponents[0] = ws.u_exponents, a.exponents[1] = ws.v_exponents;
         a.span = span;
     }
     if (int rc = status_pointer(&a.status)) return rc;
@@ -682,8 +681,7 @@ int tc_adapter_prepare(const AdapterShape &s, const AdapterSpace &ws, const void
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
-    if (s.dtype == MPS_BF16) RD_CUDA(cudaLaunchKernelEx(&cfg, mps::adapter_prepare_kernel<true>, a));
-    else RD_CUDA(cudaLaunchKernelEx(&cfg, mps::adapter_prepare_kernel<false>, a));
+    RD_CUDA(cudaLaunchKernelEx(&cfg, mps::adapter_prepare_kernel, a));
     return MPS_OK;
 }
 
@@ -699,7 +697,7 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, int k, int n,
     a.n_slots = a.n_x_rows = s.n_rows;
     a.k = k;
     a.n = n;
-    a.w_shared = a.follows = true;
+    a.follows = true;
     a.out = out;
     if (int rc = tc_matrix(&a.w, &a, w, k, n, 1)) return rc;
     if (ws.rows) {
@@ -713,7 +711,7 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, int k, int n,
         a.delta_f = mn_major ? 1 : s.rank;
         a.delta_r = mn_major ? n : 1;
         a.ahead = ahead;
-        return tc_rows(&a, 1, ws.cut, &x, s.n_rows, sms, st, used);
+        return tc_rows<mps::kByRow>(&a, 1, ws.cut, &x, s.n_rows, sms, st, used);
     }
     a.group_ptr = ws.ptr;
     a.slot_row = ws.row;
@@ -721,9 +719,9 @@ int tc_adapter_wide(const AdapterShape &s, const AdapterSpace &ws, int k, int n,
     a.rank = s.rank;
     a.rank_groups = s.n_adapters;
     a.u_base = ws.wide;
-    a.w2_base = ws.m;
-    a.gather = a.scatter = true;
-    return tc_rows(&a, 1, ws.cut, &x, s.n_rows, sms, st, used);
+    a.w2_base = a.bf16 ? m : ws.m;
+    a.gather = true;
+    return a.bf16 ? tc_rows<mps::kWide16>(&a, 1, ws.cut, &x, s.n_rows, sms, st, used) : tc_rows<mps::kWideTf32>(&a, 1, ws.cut, &x, s.n_rows, sms, st, used);
 }
 
 TcOuter tc_adapter_outer(const AdapterShape &s, int features, const int *exponents, void *out, long long out_f, long long out_c) {
@@ -735,7 +733,7 @@ TcOuter tc_adapter_outer(const AdapterShape &s, int features, const int *exponen
     a.n_slots = a.n_p_rows = s.n_rows;
     a.i = features;
     a.j = s.rank;
-    a.pair = a.follows = a.apart = true;  // beside the rows' gradient
+    a.follows = a.apart = true;  // beside the rows' gradient
     a.exponents = exponents;
     a.out = out;
     a.out_group = (long long)features * s.rank;
@@ -758,11 +756,13 @@ int adapters(const AdapterShape &s, const void *x, const void *w, const void *a,
             RD_CUDA(cudaGetLastError());
         } else {
             if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
-            TcRows narrow;
-            if (int rc = tc_adapter_narrow(s, s.k, a, false, nullptr, ws.wide, nullptr, &narrow)) return rc;
+            TcRows narrow = {};
+            if (int rc = tc_adapter_narrow(s, s.k, a, false, &narrow)) return rc;
+            narrow.out_wide = ws.wide;
             narrow.follows = narrow.apart = true;  // beside the listing
-            if (int rc = tc_rows(&narrow, 1, best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k), true, sms, 256), &x, s.n_rows, sms, st)) return rc;
-            if (int rc = tc_adapter_prepare(s, ws, b, false, s.n, false, 0, sms, st)) return rc;
+            if (int rc = tc_rows<mps::kNarrow>(&narrow, 1, best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k), true, sms, 256), &x, s.n_rows, sms, st)) return rc;
+            if (s.dtype == MPS_F16)
+                if (int rc = tc_adapter_prepare(s, ws, b, false, s.n, false, 0, sms, st)) return rc;
         }
         return tc_adapter_wide(s, ws, s.k, s.n, x, w, ws.u, b, false, y, ws.rows, sms, st);
     }
@@ -779,19 +779,28 @@ int adapters_backward(const AdapterShape &s, const void *dy, const void *x, cons
         if (int rc = sm_count(&sms)) return rc;
         if (!ws.rows)
             if (int rc = mps::list_rows_and_rest(s.n_rows, s.n_adapters, s.ids, ws.ptr, ws.row, st)) return rc;
-        const bool scaled = s.dtype == MPS_F16;
-        TcRows narrow[2];  // side by side, and beside the listing: scale * x A^T and scale * dy B
-        if (int rc = tc_adapter_narrow(s, s.k, a, false, ws.u, nullptr, scaled ? ws.u_maxima : nullptr, &narrow[0])) return rc;
-        if (int rc = tc_adapter_narrow(s, s.n, b, true, ws.v, ws.wide, scaled ? ws.v_maxima : nullptr, &narrow[1])) return rc;
+        const bool fp16 = s.dtype == MPS_F16;
+        TcRows narrow[2] = {};  // side by side, and beside the listing: scale * x A^T and scale * dy B
+        if (int rc = tc_adapter_narrow(s, s.k, a, false, &narrow[0])) return rc;
+        if (int rc = tc_adapter_narrow(s, s.n, b, true, &narrow[1])) return rc;
+        narrow[1].out_wide = ws.wide;
+        if (fp16) {  // split once all of an adapter's are there
+            narrow[0].out_f32 = ws.u, narrow[1].out_f32 = ws.v;
+            narrow[0].maxima = ws.u_maxima, narrow[1].maxima = ws.v_maxima;
+        } else {
+            narrow[0].out_slots = ws.u_slots, narrow[1].out_slots = ws.v_slots;
+            if (ws.rows) narrow[1].out_f32 = ws.v;
+        }
         narrow[0].follows = narrow[0].apart = narrow[1].apart = !ws.rows;
         const void *const in[2] = {x, dy};
         const Cut half = best_cut(s.n_rows, s.n_adapters, s.rank, steps_of(s.k > s.n ? s.k : s.n), true, sms / 2, 64);
-        if (int rc = tc_rows(narrow, 2, half, in, s.n_rows, sms, st)) return rc;
-        if (int rc = tc_adapter_prepare(s, ws, ws.rows ? nullptr : a, true, s.k, true, half.split > 1 ? 2 : mps::kSpan, sms, st)) return rc;
+        if (int rc = tc_rows<mps::kNarrow>(narrow, 2, half, in, s.n_rows, sms, st)) return rc;
+        if (fp16)
+            if (int rc = tc_adapter_prepare(s, ws, ws.rows ? nullptr : a, true, s.k, true, half.split > 1 ? 2 : mps::kSpan, sms, st)) return rc;
         if (int rc = tc_adapter_wide(s, ws, s.n, s.k, dy, w, ws.v, a, true, dx, false, sms, st, &used)) return rc;
-        const TcOuter outer[2] = {tc_adapter_outer(s, s.k, scaled ? ws.v_exponents : nullptr, da, 1, s.k),
-                                  tc_adapter_outer(s, s.n, scaled ? ws.u_exponents : nullptr, db, s.rank, 1)};
-        const void *const q[2] = {ws.v_planes, ws.u_planes};
+        const TcOuter outer[2] = {tc_adapter_outer(s, s.k, fp16 ? ws.v_exponents : nullptr, da, 1, s.k),
+                                  tc_adapter_outer(s, s.n, fp16 ? ws.u_exponents : nullptr, db, s.rank, 1)};
+        const void *const q[2] = {ws.v_slots, ws.u_slots};
         // beside few blocks of that on the SMs they leave, else on each as it gets free
         return tc_outer(outer, 2, in, q, used <= sms / 2 ? sms - used : sms, st);
     }
@@ -873,7 +882,7 @@ extern "C" int mps_routed_product(int32_t n_slots, int32_t n_rows, int32_t n_gro
         int sms;
         if (int rc = sm_count(&sms)) return rc;
         if (int rc = tc_matrix(&a.w, &a, d_w, summed, features, n_groups)) return rc;
-        return tc_rows(&a, 1, best_cut(n_slots, n_groups, features, steps_of(summed), a.gather, sms, 256), &d_x, n_rows, sms, (cudaStream_t)stream);
+        return tc_rows<mps::kProduct>(&a, 1, best_cut(n_slots, n_groups, features, steps_of(summed), a.gather, sms, 256), &d_x, n_rows, sms, (cudaStream_t)stream);
     }
     RowsArgs a = {};
     a.group_ptr = d_group_ptr;

@@ -9,10 +9,11 @@
 // alternate, so a tile is stored while the next one is summed; results go through shared memory, where 64 slots by 128 features
 // become whole 256-byte rows.
 //
-// A tile's sum may go on with a second product (RANK): the group's low-rank matrix times rows u that were computed before.  u is
-// kept as two planes of tf32 values, whose sum has fp32's range and is off by 2^-21 of u at most, and the matrix, exactly, in fp32
-// (adapter_prepare_kernel).  A pair of fp16 values instead has no digits left below 2^-24 and ends at 65504, and intermediates
-// next to nothing are what training starts from (the second matrix begins at zero).
+// A tile's sum may go on with a second product (RANK): the group's low-rank matrix times rows u that were computed before, in two
+// planes whose sum has fp32's range.  In bf16 they are bf16 values (off by 2^-16 of u at most) and meet the matrix as it is.  A pair
+// of fp16 values has no digits left below 2^-24 and ends at 65504, and intermediates next to nothing are what training starts from
+// (the second matrix begins at zero); so in fp16 they are tf32 values (2^-21), and the matrix, exactly, is in fp32
+// (adapter_prepare_kernel).
 //
 // The widest tiles (NT = 256) belong to a pair of neighbouring blocks (cta_group::2): 256 features by 256 slots, each block
 // loading its 128 features and half of the slots, so that a block's slice is 32 KB instead of 48 and six of them are in flight.
@@ -36,7 +37,16 @@ namespace mps {
 constexpr int kTcThreads = 512;  // warps: 0 TMA, 1 products, 2-3 none, 4-7 results (TMEM lanes go by warp number mod 4), 8-15 row loads
 constexpr int kTcFeatures = 128;
 constexpr int kTcDepth = 64;
-constexpr int kRankDepth = 32;                 // of the rank in a slice of the second product, whose elements are 32-bit
+// What a launch of the row products is for.  Each is a form of its own: a short launch waits for its code to arrive, so that what one
+// use needs costs the others a microsecond or two, and long ones their loops' registers (all in one form: 32,768 slots 303 us, of
+// their own 286; adapters of 4096 rows 165 and 153).
+enum TcUse {
+    kProduct,   // rows, gathered or not, times their group's matrix
+    kNarrow,    // gathered rows times narrow matrices, results in fp32 (or pairs that stand for it)
+    kByRow,     // rows in order times one matrix, plus u times the matrix of each row's own adapter, by the warps that store results
+    kWide16,    // rows listed by adapter times one matrix, plus a second product of the 16-bit type
+    kWideTf32,  // or of tf32
+};
 constexpr int kTcRing = 192 * 1024;            // shared memory of the stages
 constexpr int kOutPitch = kTcFeatures * 2 + 16;  // a result row in shared memory; the pad spreads 16-byte reads over the banks
 constexpr int kOutBytes = 64 * kOutPitch;        // 64 rows at a time
@@ -52,14 +62,16 @@ struct TcRows {
     int n_groups, n_slots, n_x_rows;
     int k, n;                 // summed index, result features
     int rank, rank_groups;    // depth of the second product; groups that have one (the first rank_groups)
-    const float *u_base, *w2_base;  // its rows, two planes of n_x_rows, and matrices (host side)
+    const void *u_base, *w2_base;  // its rows, two planes of n_x_rows, and matrices (host side)
     int w_rows;               // rows of a matrix box (features, where they are its rows)
-    bool w_shared, mn_major, gather, bf16, scatter;
+    bool mn_major, gather, bf16;
     void *out;
-    float *out_f32, *out_tf32;  // instead of out: the result in fp32, by row, and as two planes of tf32 values (NULL: not wanted)
+    float *out_f32;             // instead of out, each where not NULL: the result in fp32, by row,
+    void *out_wide;             //   as two planes by row for a second product,
+    uint16_t *out_slots;        //   as two planes of bf16 by slot,
+    unsigned *maxima;           //   and the largest finite magnitudes of it, see finite_bits
     const float *group_scale;   // factor of a group's results then (NULL: 1)
-    unsigned *maxima;           // the largest finite magnitudes of them, see finite_bits (NULL: not wanted)
-    const int *ids;           // delta: adapter of a row,
+    const int *ids;           // delta (kByRow): adapter of a row,
     const float *delta_u;     //   the rows' intermediates (by row, delta_rank each),
     const uint16_t *delta_m;  //   the adapters' matrices with their strides by adapter, feature and rank index
     int delta_adapters, delta_rank;
@@ -164,12 +176,28 @@ __device__ __forceinline__ void spread_column(const float (&v)[32], uint32_t to)
     }
 }
 
-// Four values of an fp32 result, at `at` of out_f32 and of both planes of out_tf32.
-__device__ __forceinline__ void store_f32(const TcRows &a, long long at, float4 v) {
-    if (a.out_f32) *reinterpret_cast<float4 *>(a.out_f32 + at) = v;
-    if (a.out_tf32) {
-        *reinterpret_cast<float4 *>(a.out_tf32 + at) = make_float4(tf32_first(v.x), tf32_first(v.y), tf32_first(v.z), tf32_first(v.w));
-        *reinterpret_cast<float4 *>(a.out_tf32 + (long long)a.n_x_rows * a.n + at) = make_float4(tf32_second(v.x), tf32_second(v.y), tf32_second(v.z), tf32_second(v.w));
+// Four values of an fp32 result from feature f, of a slot and its row (outside of x where the list is wrong: nothing by row).
+__device__ __forceinline__ void store_f32(const TcRows &a, int row, int slot, int f, float4 v) {
+    const bool by_row = (unsigned)row < (unsigned)a.n_x_rows;
+    const long long at = (long long)row * a.n + f, plane = (long long)a.n_x_rows * a.n;
+    if (a.out_f32 && by_row) *reinterpret_cast<float4 *>(a.out_f32 + at) = v;
+    if (a.bf16) {
+        uint2 first, second;
+        split_bf16(v, first, second);
+        if (a.out_wide && by_row) {
+            uint16_t *to = (uint16_t *)a.out_wide + at;
+            *reinterpret_cast<uint2 *>(to) = first;
+            *reinterpret_cast<uint2 *>(to + plane) = second;
+        }
+        if (a.out_slots) {
+            uint16_t *to = a.out_slots + (long long)slot * a.n + f;
+            *reinterpret_cast<uint2 *>(to) = first;
+            *reinterpret_cast<uint2 *>(to + (long long)a.n_slots * a.n) = second;
+        }
+    } else if (a.out_wide && by_row) {
+        float *to = (float *)a.out_wide + at;
+        *reinterpret_cast<float4 *>(to) = make_float4(tf32_first(v.x), tf32_first(v.y), tf32_first(v.z), tf32_first(v.w));
+        *reinterpret_cast<float4 *>(to + plane) = make_float4(tf32_second(v.x), tf32_second(v.y), tf32_second(v.z), tf32_second(v.w));
     }
 }
 
@@ -272,8 +300,7 @@ struct TileWalk {
     }
 };
 
-// RANK: with a second product.  Forms of their own, so that it costs the others nothing.
-template <int NT, bool TWO, bool RANK>
+template <int NT, TcUse USE, bool TWO>
 __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_constant__ TcRowsLaunch launch) {
     const bool is_second = TWO && (int)blockIdx.x >= launch.second;
     const TcRows &a = launch.p[is_second];
@@ -287,7 +314,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     int *whole = reinterpret_cast<int *>(s_raw + (ring - smem_addr(s_raw)) + kTcRing + kOutTotal);
     int *rest = whole + a.n_groups + 1, *lo = rest + a.n_groups + 1, *hi = lo + a.n_groups;
     const int split = a.split, part = split > 1 ? (int)cluster_rank() : 0;
-    const bool reduce = split > 1 || a.ids;  // results meet in shared memory before they are stored
+    constexpr bool RANK = USE == kWide16 || USE == kWideTf32, TF32 = USE == kWideTf32, F32 = USE == kNarrow, DELTA = USE == kByRow;
+    constexpr bool SHARED = RANK || DELTA;  // one matrix
+    const bool gather = USE == kProduct ? a.gather : !DELTA;
+    const bool reduce = DELTA || (S::kReduce > 0 && split > 1);  // results meet in shared memory before they are stored
     const int stages = reduce ? S::kSplitStages : S::kStages;
     const uint32_t partial = ring + (uint32_t)S::kSplitStages * S::kStage;
     constexpr bool PAIRED = S::kPaired;
@@ -296,7 +326,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     if (!a.next_after) let_next_launch_start();
     if (warp == 0 && lane < (RANK ? 6 : 3)) {
         const CUtensorMap *maps[6] = {&a.w, &a.x, &a.x_run, &a.w2, &a.u, &a.u_run};
-        if (lane != 2 || a.gather) tma_prefetch(maps[lane]);
+        if (lane != 2 || gather) tma_prefetch(maps[lane]);
     }
     if (!a.ahead && !a.apart) wait_for_launch_before();
     if (a.next_after) let_next_launch_start();
@@ -313,7 +343,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 slots[i] = make_int2(0, a.n_slots);
                 if (a.group_ptr) slots[i] = group_range(a.group_ptr, g, a.n_slots, a.status);
                 const int n = slots[i].y - slots[i].x;
-                tiles[i] = a.w_shared ? n / NT * 2 + (n % NT ? 1 : 0) : (n + NT - 1) / NT * 2;
+                tiles[i] = SHARED ? n / NT * 2 + (n % NT ? 1 : 0) : (n + NT - 1) / NT * 2;
             }
             sum += tiles[i] >> 1;
             sum_rest += tiles[i] & 1;
@@ -367,7 +397,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
     const uint32_t tmem = pipe.tmem;
     volatile int *gave_up = &pipe.gave_up;
     constexpr int TILE_F = PAIRED ? 2 * kTcFeatures : kTcFeatures;
-    const int main_steps = (a.k + kTcDepth - 1) / kTcDepth, rank_steps = RANK ? 2 * ((a.rank + kRankDepth - 1) / kRankDepth) : 0;  // of each plane in turn
+    constexpr int kRankDepth = TF32 ? 32 : 64;  // of the rank in a slice: 128 bytes
+    const int main_steps = (a.k + kTcDepth - 1) / kTcDepth;
+    const int rank_steps = RANK ? 2 * ((a.rank + kRankDepth - 1) / kRankDepth) : 0;  // of each plane in turn
     const int shift = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
     const int n_active = s_active;
     TileWalk walk(whole[n_active] + (rest[n_active] & 0xffff), (a.n + TILE_F - 1) / TILE_F, block / group_blocks, blocks / group_blocks);
@@ -402,7 +434,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             else atomicOr(a.status, kStatusBadIndex);
         }
     };
-    const bool loads_rows = warp >= 8 && a.gather;
+    const bool loads_rows = warp >= 8 && gather;
     if (loads_rows) fetch_rows(walk);
     const uint32_t full0 = PAIRED ? in_block(smem_addr(&pipe.full[0]), 0) : smem_addr(&pipe.full[0]);  // where loads are reported
     RingAt pos;  // this warp's place in the ring
@@ -418,10 +450,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
         const int buf = turn & 1;
         if (warp == 0) {
             if (elect_one()) {
-                const int z = a.w_shared ? 0 : g;
+                const int z = SHARED ? 0 : g;
                 const int halves = PAIRED || a.n - f0 > 64 ? 2 : 1;  // MN-major: boxes of 64 features (as many in both blocks)
                 const uint32_t w_bytes = a.mn_major ? halves * kBlock64 : a.w_rows * 128u, own = slot0 + half * columns / 2;
-                const uint32_t x_bytes = a.gather ? rows_per_warp(columns) * 1024u : S::kRows * 128u;
+                const uint32_t x_bytes = gather ? rows_per_warp(columns) * 1024u : S::kRows * 128u;
                 for (int s = s0; s < s1; s += S::kSlices, pos.next(stages)) {
                     mbar_wait(smem_addr(&pipe.empty[pos.stage]), pos.parity ^ 1, gave_up, a.status);
                     const uint32_t bar = full0 + pos.stage * 8;
@@ -429,22 +461,25 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                         uint32_t bytes = 0;
 #pragma unroll
                         for (int d = 0; d < S::kSlices; ++d)
-                            if (s + d < s1) bytes += (!RANK || s + d < main_steps ? w_bytes : a.w_rows * 128u) + x_bytes;
+                            if (s + d < s1) bytes += (!TF32 || s + d < main_steps ? w_bytes : a.w_rows * 128u) + x_bytes;
                         mbar_expect(bar, (PAIRED ? 2 : 1) * bytes);
                     }
 #pragma unroll
                     for (int d = 0; d < S::kSlices; ++d) {
                         if (d > 0 && s + d >= s1) break;
                         const uint32_t dst = ring + pos.stage * S::kStage + d * S::kSlice;
+                        auto load = [&](const CUtensorMap *map, bool mn_major, int i0, int number) {
+                            if (mn_major)
+                                for (int h = 0; h < halves; ++h) tma_3d<PAIRED>(dst + h * kBlock64, map, f0 + h * 64, i0, number, bar);
+                            else tma_3d<PAIRED>(dst, map, i0, f0, number, bar);
+                        };
                         if (RANK && s + d >= main_steps) {
-                            tma_3d<PAIRED>(dst, &a.w2, ((s + d - main_steps) >> 1) * kRankDepth, f0, g, bar);
+                            load(&a.w2, !TF32 && a.mn_major, ((s + d - main_steps) >> 1) * kRankDepth, g);
                             continue;
                         }
                         const int i0 = (s + d) * kTcDepth;
-                        if (a.mn_major)
-                            for (int h = 0; h < halves; ++h) tma_3d<PAIRED>(dst + h * kBlock64, &a.w, f0 + h * 64, i0, z, bar);
-                        else tma_3d<PAIRED>(dst, &a.w, i0, f0, z, bar);
-                        if (!a.gather) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);
+                        load(&a.w, a.mn_major, i0, z);
+                        if (!gather) tma_2d<PAIRED>(dst + kTcFeatures * 128, &a.x, i0, own, bar);
                     }
                 }
             }
@@ -464,8 +499,9 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                         const uint32_t from = pos.stage * S::kStage + d2 * S::kSlice;
                         const bool add = s > s0 || d2 > 0;
                         const int e = s + d2 - main_steps;
-                        if (!RANK || e < 0) {
-                            tc_slice<PAIRED>(d, operand_at(a0, from), operand_at(b0, from), a_step, b_step, idesc, min(4, (a.k - (s + d2) * kTcDepth + 15) >> 4), add);
+                        if (!TF32 || e < 0) {
+                            const int left = RANK && e >= 0 ? a.rank - (e >> 1) * kRankDepth : a.k - (s + d2) * kTcDepth;
+                            tc_slice<PAIRED>(d, operand_at(a0, from), operand_at(b0, from), a_step, b_step, idesc, min(4, (left + 15) >> 4), add);
                             continue;
                         }
                         if (e == 0 && add) {  // products of another kind follow those before only once they are done
@@ -518,11 +554,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             }
         } else if (warp >= 4 && warp < 8) {
             const int quad = warp & 3, f = f0 + quad * 32 + lane, mine = tid - 128;
-            const bool f32 = a.out == nullptr;
-            const float scale = f32 && a.group_scale ? a.group_scale[g] : 1.0f;
+            const float scale = F32 && a.group_scale ? a.group_scale[g] : 1.0f;
             uint16_t *out = (uint16_t *)a.out;
             auto out_row = [&](int slot) {  // where a slot's result goes, or -1
-                if (!a.scatter) return slot;
+                if (!RANK && !F32) return slot;
                 const int r = a.slot_row[slot];
                 return (unsigned)r < (unsigned)a.n_x_rows ? r : -1;
             };
@@ -541,7 +576,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             const int feature = quad * 32 + lane;
             if (reduce) {
                 mbar_wait(smem_addr(&pipe.freed), (turn & 1) ^ 1, gave_up, a.status);
-                if (a.ids) {
+                if constexpr (DELTA) {
                     // The columns this block adds up start from u times the adapter's matrix.  The matrices are asked for before
                     // the wait for u; u goes through shared memory, 64 of the rank at a time; four columns' loads are in flight.
                     const int first_slot = slot0 + part * meeting.run, own = min(max(slot1 - first_slot, 0), meeting.run);
@@ -601,17 +636,17 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     }
                 }
             }
-            const bool rows_of_16 = a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0, wide = rows_of_16 && !reduce;  // fp32 results always are
-            int line = wide && !f32 ? line_ahead(0) : 0;
+            const bool rows_of_16 = F32 || (a.n % 8 == 0 && ((uintptr_t)a.out & 15) == 0), wide = rows_of_16 && !reduce;
+            int line = wide && !F32 ? line_ahead(0) : 0;
             mbar_wait(smem_addr(&pipe.tmem_full[buf]), (turn >> 1) & 1, gave_up, a.status);
             tc_fence_after();
             const uint32_t lanes = tmem + ((uint32_t)(quad * 32) << 16) + buf * NT;
-            if (wide && f32) {
+            if (F32 && !reduce) {
 #pragma unroll 1
                 for (int c0 = 0; c0 < NT && slot0 + c0 < slot1; c0 += 32) {
                     float v[32];
                     const int slot = slot0 + c0 + warp - 4 + 4 * (lane & 7);  // of the rows this warp stores
-                    const int at = slot < slot1 ? a.slot_row[slot] : -1;
+                    const int at = slot < slot1 ? out_row(slot) : -1;
                     tmem_load(lanes + c0, v);
                     unsigned largest = 0;
 #pragma unroll
@@ -629,12 +664,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                     results_sync();
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        const int to = __shfl_sync(0xffffffffu, at, j);
-                        if ((unsigned)to < (unsigned)a.n_x_rows && f0 + lane * 4 < a.n)
-                            store_f32(a, (long long)to * a.n + f0 + lane * 4, load_shared_float4(staging + (warp - 4 + 4 * j) * kF32Pitch + lane * 16));
+                        const int to = __shfl_sync(0xffffffffu, at, j), from = slot0 + c0 + warp - 4 + 4 * j;
+                        if (from < slot1 && f0 + lane * 4 < a.n)
+                            store_f32(a, to, from, f0 + lane * 4, load_shared_float4(staging + (warp - 4 + 4 * j) * kF32Pitch + lane * 16));
                     }
                 }
-            } else if (wide) {
+            } else if (!F32 && wide) {
                 // 64 columns at a time: a result warp is alone on its scheduler, so two loads and 64 roundings in flight take little
                 // more time than half of them
 #pragma unroll 1
@@ -668,8 +703,8 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                 if (reduce) {
 #pragma unroll
                     for (int j = 0; j < 32; j += 8)
-                        if (slot0 + c0 + j < slot1) meeting.give(c0 + j, feature, v + j, a.ids);
-                } else {
+                        if (slot0 + c0 + j < slot1) meeting.give(c0 + j, feature, v + j, DELTA);
+                } else if (!F32) {
 #pragma unroll
                     for (int j = 0; j < 32; ++j)
                         if (slot0 + c0 + j < slot1) store(slot0 + c0 + j, v[j]);
@@ -679,21 +714,22 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
             if (PAIRED) mbar_arrive_at(smem_addr(&pipe.tmem_empty[buf]), 0);
             else mbar_arrive(smem_addr(&pipe.tmem_empty[buf]));
             if (reduce) {
-                // every block of the cluster adds up and stores its share of the columns
+                // every block of the cluster adds up and stores its share of the columns; their rows are looked up meanwhile
+                const int first = part * meeting.run, own = min(max(slot1 - slot0 - first, 0), meeting.run);
+                const int rows_here = rows_of_16 ? line_ahead(first) : -1;
                 tell_cluster(smem_addr(&pipe.partials), split, lane);
                 mbar_wait(smem_addr(&pipe.partials), turn & 1, gave_up, a.status);
                 fence_cluster();
-                const int first = part * meeting.run, own = min(max(slot1 - slot0 - first, 0), meeting.run);
                 if (rows_of_16) {
                     const int fc = (mine & 15) * 8;
-                    for (int c0 = 2 * (warp - 4); c0 < own; c0 += 8) {
-                        const int c = c0 + (lane >> 4);  // a half warp per column; a run is a multiple of eight, so it has this one
-                        float v[8];
-                        const int slot = slot0 + first + c;
+                    // a half warp per column; a run is a multiple of eight, so it has the second half's column even behind the last
+#pragma unroll 1
+                    for (int c0 = 2 * (warp - 4), i = lane >> 4; c0 < own; c0 += 8, i += 2) {
+                        const int c = c0 + (lane >> 4), slot = slot0 + first + c, r = __shfl_sync(0xffffffffu, rows_here, i);
                         const bool live = c < own && f0 + fc < a.n;
-                        const int r = !live ? -1 : f32 ? a.slot_row[slot] : out_row(slot);
+                        float v[8];
                         meeting.sum8(c, fc, v);
-                        if (f32) {
+                        if constexpr (F32) {
                             unsigned largest = 0;
 #pragma unroll
                             for (int j = 0; j < 8; ++j) {
@@ -706,11 +742,11 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_rows_kernel(const __grid_con
                                 largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 16));
                                 if ((lane & 19) == 0 && f0 + fc < a.n) a.maxima[(long long)((f0 + fc) >> 5) * a.n_slots + slot0 + first + c0] = largest;
                             }
-                            if ((unsigned)r < (unsigned)a.n_x_rows) {
-                                store_f32(a, (long long)r * a.n + f0 + fc, make_float4(v[0], v[1], v[2], v[3]));
-                                store_f32(a, (long long)r * a.n + f0 + fc + 4, make_float4(v[4], v[5], v[6], v[7]));
+                            if (live) {
+                                store_f32(a, r, slot, f0 + fc, make_float4(v[0], v[1], v[2], v[3]));
+                                store_f32(a, r, slot, f0 + fc + 4, make_float4(v[4], v[5], v[6], v[7]));
                             }
-                        } else if (r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = pack_16(v, a.bf16);
+                        } else if (live && r >= 0) *reinterpret_cast<uint4 *>(out + (long long)r * a.n + f0 + fc) = pack_16(v, a.bf16);
                     }
                 } else
                     for (int c = 0; c < own; ++c) store(slot0 + first + c, meeting.sum(c, feature));
@@ -756,38 +792,34 @@ __global__ void __launch_bounds__(256) adapter_dots_kernel(int k, int rank, int 
     if (lane == 0) u[(long long)row * rank + r] = scale ? sum * scale[id] : sum;
 }
 
-// What the adapters' products read in another form than it came in.  First the matrices of the groups that have slots, in fp32 with
+// What the adapters' products read in another form than it came in, in fp16.  First the matrices of the groups that have slots, in fp32 with
 // the rank contiguous (exact, and what a tf32 product reads by TMA); they are beside the launch before.  Behind that launch, for the
-// matrix gradients, its two fp32 results as hi + lo planes of the 16-bit type in slot order (off by 2^-16 of a value in bf16,
-// 2^-22 in fp16; of an infinite value lo is zero).  fp16 has not fp32's range: there a group's values of 64 columns are multiplied
-// by the power of two that brings the largest of them, out of `maxima`, just below 2^15, so that what fp16 rounds away is 2^-40 of
-// that largest at most.  Bytes bound it: 2 read and 4 written per element of a matrix (8 matrices of 4096 x 64: 12 MB, on the SMs
+// matrix gradients, its two fp32 results as hi + lo planes in slot order (off by 2^-22 of a value; of an infinite value lo is
+// zero).  fp16 has not fp32's range: a group's values of 64 columns are multiplied by the power of two that brings the largest of
+// them, out of `maxima`, just below 2^15, so that what fp16 rounds away is 2^-40 of that largest at most.  Bytes bound it: 2 read and 4 written per element of a matrix (8 matrices of 4096 x 64: 12 MB, on the SMs
 // that the narrow product leaves), 4 and 4 per value.
 struct PrepareArgs {
     const int *group_ptr, *slot_row;
     int n_groups, n_slots, n_rows, rank;
-    bool bf16;
     const uint16_t *m;        // matrices by group, features x rank (by_rank: rank x features); NULL: none
     float *m_f32;
     int features;
     bool by_rank;
     const float *values[2];   // by row; NULL: none
     uint16_t *planes[2];
-    const unsigned *maxima[2];  // NULL: not scaled
+    const unsigned *maxima[2];
     int *exponents[2];
-    int span;
+    int span, run;            // run: slots per warp, at most 32
     int *status;
 };
 
-template <bool BF16>
-__device__ __forceinline__ void split_16(float4 v, uint2 &hi, uint2 &lo) {
-    hi = make_uint2(to_16x2<BF16>(v.x, v.y), to_16x2<BF16>(v.z, v.w));
-    const float2 h = from_16x2<BF16>(hi.x), q = from_16x2<BF16>(hi.y);
+__device__ __forceinline__ void split_fp16(float4 v, uint2 &hi, uint2 &lo) {
+    hi = make_uint2(to_16x2<false>(v.x, v.y), to_16x2<false>(v.z, v.w));
+    const float2 h = from_16x2<false>(hi.x), q = from_16x2<false>(hi.y);
     auto rest = [](float x, float first) { return fabsf(first) < INFINITY ? x - first : 0.0f; };
-    lo = make_uint2(to_16x2<BF16>(rest(v.x, h.x), rest(v.y, h.y)), to_16x2<BF16>(rest(v.z, q.x), rest(v.w, q.y)));
+    lo = make_uint2(to_16x2<false>(rest(v.x, h.x), rest(v.y, h.y)), to_16x2<false>(rest(v.z, q.x), rest(v.w, q.y)));
 }
 
-template <bool BF16>
 __global__ void __launch_bounds__(256) adapter_prepare_kernel(const PrepareArgs a) {
     constexpr int N = 4;  // loads in flight
     __shared__ int s_ptr[kMaxRowGroups + 1];
@@ -846,27 +878,27 @@ __global__ void __launch_bounds__(256) adapter_prepare_kernel(const PrepareArgs 
                 if (to[n] < 0) continue;
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    const float2 x = from_16x2<BF16>(w[n][2 * j]), y = from_16x2<BF16>(w[n][2 * j + 1]);
+                    const float2 x = from_16x2<false>(w[n][2 * j]), y = from_16x2<false>(w[n][2 * j + 1]);
                     *reinterpret_cast<float4 *>(a.m_f32 + to[n] + 4 * j) = make_float4(x.x, x.y, y.x, y.y);
                 }
             }
         }
     }
-    // a warp per 32 slots of either result, cut where groups end
-    const int used = min(max(s_ptr[a.n_groups], 0), a.n_slots), runs = a.values[0] ? (used + 31) / 32 : 0, blocks_of_rank = (a.rank + 63) / 64;
+    // a warp per run of slots of either result, cut where groups end
+    const int used = min(max(s_ptr[a.n_groups], 0), a.n_slots), runs = a.values[0] ? (used + a.run - 1) / a.run : 0, blocks_of_rank = (a.rank + 63) / 64;
     const int step = gridDim.x * 8;
     int run = blockIdx.x * 8 + warp;
     // Who has nothing to split makes room for the next launch's blocks; one stays, so that what waits for this launch waits for the
     // one before, too.
-    if (blockIdx.x > 0 && blockIdx.x * 8 >= 2 * runs) return;
+    if (blockIdx.x > 0 && (long long)blockIdx.x * 8 >= 2ll * runs) return;
     auto row_of = [&](int n) {  // the row of this lane's slot
-        const int slot = (n >= runs ? n - runs : n) * 32 + lane, row = n < 2 * runs && slot < used ? a.slot_row[slot] : -1;
+        const int slot = (n >= runs ? n - runs : n) * a.run + lane, row = n < 2 * runs && lane < a.run && slot < used ? a.slot_row[slot] : -1;
         return (unsigned)row < (unsigned)a.n_rows ? row : -1;
     };
     int row = row_of(run);
     wait_for_launch_before();
     for (; run < 2 * runs; run += step, row = row_of(run)) {
-        const int which = run >= runs, first = (which ? run - runs : run) * 32, end = min(first + 32, used);
+        const int which = run >= runs, first = (which ? run - runs : run) * a.run, end = min(first + a.run, used);
         const float *values = a.values[which];
         const unsigned *maxima = a.maxima[which];
         int s = first;
@@ -891,16 +923,13 @@ __global__ void __launch_bounds__(256) adapter_prepare_kernel(const PrepareArgs 
                     }
                 };
                 load(lane);
-                float scale = 1.0f;
-                if (maxima) {
-                    unsigned largest = 0;
-                    for (int b = 2 * j; b < 2 * j + 2 && b * 32 < a.rank; ++b)
-                        for (int i = slots.x + lane * a.span; i < slots.y; i += 32 * a.span) largest = max(largest, __ldcg(maxima + (long long)b * a.n_slots + i));
-                    largest = __reduce_max_sync(0xffffffffu, largest);
-                    const int exponent = largest ? min(268 - (int)(largest >> 23), 253) : 127;  // 2^e .. 2^(e+1) to 2^14 .. 2^15; one
-                    scale = __uint_as_float((uint32_t)exponent << 23);
-                    if (s == slots.x && lane == 0) a.exponents[which][(long long)g * blocks_of_rank + j] = exponent;
-                }
+                unsigned largest = 0;
+                for (int b = 2 * j; b < 2 * j + 2 && b * 32 < a.rank; ++b)
+                    for (int i = slots.x + lane * a.span; i < slots.y; i += 32 * a.span) largest = max(largest, __ldcg(maxima + (long long)b * a.n_slots + i));
+                largest = __reduce_max_sync(0xffffffffu, largest);
+                const int exponent = largest ? min(268 - (int)(largest >> 23), 253) : 127;  // 2^e .. 2^(e+1) to 2^14 .. 2^15; one
+                const float scale = __uint_as_float((uint32_t)exponent << 23);
+                if (s == slots.x && lane == 0) a.exponents[which][(long long)g * blocks_of_rank + j] = exponent;
                 for (int i0 = 0; i0 < count; i0 += 32 * N) {
                     if (i0) load(i0 + lane);
 #pragma unroll
@@ -908,7 +937,7 @@ __global__ void __launch_bounds__(256) adapter_prepare_kernel(const PrepareArgs 
                         const int i = i0 + lane + 32 * n;
                         if (i >= count) continue;
                         uint2 hi, lo;
-                        split_16<BF16>(make_float4(v[n].x * scale, v[n].y * scale, v[n].z * scale, v[n].w * scale), hi, lo);
+                        split_fp16(make_float4(v[n].x * scale, v[n].y * scale, v[n].z * scale, v[n].w * scale), hi, lo);
                         uint16_t *to = a.planes[which] + (long long)(s + i / pieces) * a.rank + 64 * j + i % pieces * 4;
                         *reinterpret_cast<uint2 *>(to) = hi;
                         *reinterpret_cast<uint2 *>(to + (long long)a.n_slots * a.rank) = lo;
@@ -924,15 +953,15 @@ __global__ void __launch_bounds__(256) adapter_prepare_kernel(const PrepareArgs 
 // summed index is the slot, so both operands lie across it (MN-major): a stage holds 64 slots of 128 features of P and of up
 // to NT columns of Q in blocks of 64.  Whole slices of rows in slot order come as a box per block; gathered rows and the last
 // slice of a group by row number, those behind the group's end named out of range: zeros, whatever lies there.
-// With `pair` a block of columns of Q is a hi and a lo plane, added up when the result is stored, and each group's values have been
-// multiplied by a power of two (adapter_prepare_kernel): the result is by its inverse.
+// In a launch of two products (a `pair`) a block of columns of Q is a hi and a lo plane of n_slots rows, added up when the result is stored; in fp16 each group's values have
+// been multiplied by a power of two (adapter_prepare_kernel), and the result is by its inverse.
 struct TcOuter {
     CUtensorMap p_rows, p_tile, q_rows, q_tile;  // boxes of one row / of 64
     const int *group_ptr, *slot_row;  // slot_row: rows of P (NULL: in slot order)
     int n_groups, n_slots, n_p_rows;
     int i, j;                         // features of P, columns of Q
-    bool bf16, pair;                  // pair: Q is two planes of n_slots rows
-    const int *exponents;             //   and the exponent field of the power of two by [group][column / 64] (NULL: one)
+    bool bf16;
+    const int *exponents;             // pair: the exponent field of the power of two by [group][column / 64] (NULL: one)
     void *out;
     long long out_group, out_f, out_c;
     int split;
@@ -966,7 +995,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     __shared__ TcPipe pipe;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t ring = (smem_addr(s_raw) + 1023) & ~1023u, staging = ring + kTcRing;
-    const int split = a.split, part = split > 1 ? (int)cluster_rank() : 0;
+    const int split = S::kReduce > 0 ? a.split : 1, part = split > 1 ? (int)cluster_rank() : 0;
     const int stages = split > 1 ? S::kSplitStages : S::kStages;
     const uint32_t partial = ring + (uint32_t)S::kSplitStages * S::kStage;
     constexpr bool PAIRED = S::kPaired;
@@ -986,15 +1015,16 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
     tc_fence_after();
     const uint32_t tmem = pipe.tmem;
     volatile int *gave_up = &pipe.gave_up;
-    const int cols = a.pair ? NT / 2 : NT;  // result columns per tile
+    constexpr bool pair = TWO;
+    constexpr int cols = pair ? NT / 2 : NT;  // result columns per tile
     const int i_tiles = (a.i + TILE_F - 1) / TILE_F, j_tiles = (a.j + cols - 1) / cols;
     const int per_group = i_tiles * j_tiles, n_tiles = a.n_groups * per_group;  // below 2^31 (host)
     const int worker = block / group_blocks, workers = blocks / group_blocks, shift = split == 1 ? 0 : split == 2 ? 1 : split == 4 ? 2 : 3;
-    const bool gather = a.slot_row != nullptr;
+    const bool gather = pair || a.slot_row != nullptr;
     const uint32_t full0 = PAIRED ? in_block(smem_addr(&pipe.full[0]), 0) : smem_addr(&pipe.full[0]);
     RingAt pos;
     int turn = -1;  // tiles with products before this one
-    const int q_end = (a.pair ? 2 : 1) * a.n_slots;  // out of range of Q
+    const int q_end = (pair ? 2 : 1) * a.n_slots;  // out of range of Q
     const bool on_16 = ((uintptr_t)a.out & 15) == 0;
     const bool wide = a.out_f == 1 && a.i % 8 == 0 && on_16, own_rows = a.out_c == 1 && a.j % 8 == 0 && on_16;  // rows of features / of columns
     int2 ends = make_int2(0, 0);  // of the next tile's group: read a tile ahead
@@ -1020,7 +1050,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
         const int total = (slots.y - slots.x + kTcDepth - 1) / kTcDepth;
         const int s0 = (int)((long long)total * part >> shift), s1 = (int)((long long)total * (part + 1) >> shift);
         const int buf = turn & 1;
-        const int p_blocks = PAIRED || a.i - f0 > 64 ? 2 : 1, q_blocks = a.pair || a.j - c0 > NT / 2 ? 2 : 1;
+        const int p_blocks = PAIRED || a.i - f0 > 64 ? 2 : 1, q_blocks = pair || a.j - c0 > NT / 2 ? 2 : 1;
         const int q0 = c0 + half * q_blocks * 64;  // the columns this block loads
         if (warp == 0) {
             if (elect_one()) {
@@ -1034,7 +1064,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     if (!gather)
                         for (int b = 0; b < p_blocks; ++b) tma_2d<PAIRED>(dst + b * kBlock64, &a.p_tile, f0 + b * 64, slot, bar);
                     for (int b = 0; b < q_blocks; ++b)
-                        tma_2d<PAIRED>(dst + (2 + b) * kBlock64, &a.q_tile, a.pair ? c0 : q0 + b * 64, a.pair ? b * a.n_slots + slot : slot, bar);
+                        tma_2d<PAIRED>(dst + (2 + b) * kBlock64, &a.q_tile, pair ? c0 : q0 + b * 64, pair ? b * a.n_slots + slot : slot, bar);
                 }
                 if (max(s0, whole) < s1) {  // part of a slice: by row number, zeros behind the group's end up to what the products read
                     const int st = pos.stage, slot = slots.x + (s1 - 1) * kTcDepth;
@@ -1046,7 +1076,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     for (int b = gather ? 2 : 0; b < 2 + q_blocks; ++b) {
                         if (b >= p_blocks && b < 2) continue;
                         const bool q = b >= 2;
-                        const int x = !q ? f0 + b * 64 : a.pair ? c0 : q0 + (b - 2) * 64, plane = q && a.pair ? (b - 2) * a.n_slots : 0;
+                        const int x = !q ? f0 + b * 64 : pair ? c0 : q0 + (b - 2) * 64, plane = q && pair ? (b - 2) * a.n_slots : 0;
 #pragma unroll 1
                         for (int i = 0; i < n_read; i += 4) {
                             auto line = [&](int j) { return slot + i + j < slots.y ? plane + slot + i + j : q ? q_end : a.n_p_rows; };
@@ -1119,9 +1149,12 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
             const int feature = quad * 32 + lane;
             const bool none = s0 == s1;
             float inverse = 1.0f;
-            if (a.exponents && slots.x < slots.y) inverse = __uint_as_float((uint32_t)(254 - __ldcg(a.exponents + (long long)g * ((a.j + 63) / 64) + (c0 >> 6))) << 23);
+            if (pair && a.exponents && slots.x < slots.y) inverse = __uint_as_float((uint32_t)(254 - __ldcg(a.exponents + (long long)g * ((a.j + 63) / 64) + (c0 >> 6))) << 23);
             // an infinite sum of hi values is the result, whatever an infinite factor made of the lo ones
-            auto join = [&](float hi, float lo) { return (fabsf(hi) < INFINITY ? hi + lo : hi) * inverse; };
+            auto join = [&](float hi, float lo) {
+                const float sum = hi + lo;
+                return (sum == sum ? sum : hi) * inverse;
+            };
             if (wide && split == 1) {
 #pragma unroll 1
                 for (int c = 0; c < cols && c0 + c < a.j; c += 64) {
@@ -1130,7 +1163,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                     for (int h = 0; h < 2; ++h) tmem_start(lanes + c + 32 * h, v[h]);
 #pragma unroll
                     for (int h = 0; h < 2; ++h) tmem_wait(v[h]);
-                    if (a.pair) {
+                    if (pair) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
                             float w[32];
@@ -1159,7 +1192,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) tc_outer_kernel(const __grid_co
                 float v[32] = {};
                 if (!none) {
                     tmem_load(lanes + c, v);
-                    if (a.pair) {
+                    if (pair) {
                         float w[32];
                         tmem_load(lanes + cols + c, w);
 #pragma unroll

@@ -278,6 +278,18 @@ __device__ __forceinline__ float tf32_second(float v) {
     return v == 0.0f ? 0.0f : copysignf(__uint_as_float(rest < 0x00800000u ? 0x00800000u : rest), v);
 }
 
+// The same of four values in bf16, two to a word: 2^-16 of a value lost.
+__device__ __forceinline__ uint32_t bf16_first(float v) { return v != v ? 0x7fffu : __float_as_uint(v) >> 16; }
+__device__ __forceinline__ uint32_t bf16_second(float v) {
+    const float rest = fabsf(v) < INFINITY ? v - __uint_as_float(bf16_first(v) << 16) : 0.0f;
+    const uint32_t bits = __bfloat16_as_ushort(__float2bfloat16_rn(fabsf(rest)));
+    return v == 0.0f ? 0u : (bits < 0x0080u ? 0x0080u : bits) | (__float_as_uint(v) >> 16 & 0x8000u);
+}
+__device__ __forceinline__ void split_bf16(float4 v, uint2 &first, uint2 &second) {
+    first = make_uint2(bf16_first(v.x) | bf16_first(v.y) << 16, bf16_first(v.z) | bf16_first(v.w) << 16);
+    second = make_uint2(bf16_second(v.x) | bf16_second(v.y) << 16, bf16_second(v.z) | bf16_second(v.w) << 16);
+}
+
 // the products of one slice: `steps` (1..4) times 32 bytes of summed elements, the first overwriting the accumulator unless `add`
 template <bool PAIRED, bool TF32 = false>
 __device__ __forceinline__ void tc_slice(uint32_t d, uint64_t a, uint64_t b, uint64_t a_step, uint64_t b_step, uint32_t idesc, int steps, bool add) {
