@@ -399,6 +399,7 @@ Cut best_cut(int slots, int groups, int features, int steps, bool gather, int sm
 
 // Blocks for two products side by side, in proportion to their work; each at least a cluster, none more than it has tiles for.
 void share_blocks(long long clusters, int cluster, const long long (&tiles)[2], const double (&work)[2], long long (&blocks)[2]) {
+    if (tiles[1] && clusters < 2) clusters = 2;  // one each, whatever the device has room for
     long long first = tiles[1] ? (long long)(clusters * work[0] / (work[0] + work[1]) + 0.5) : clusters;
     if (tiles[1]) first = first < 1 ? 1 : first > clusters - 1 ? clusters - 1 : first;
     const long long second = tiles[1] < clusters - first ? tiles[1] : clusters - first;  // what one has no use for goes to the other

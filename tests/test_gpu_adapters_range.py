@@ -185,3 +185,71 @@ def test_infinite_matrices(mps, cuda, dtype, rows):
     v = f64(t["dy"])[mine] @ f64(t["b"])[2, :, 3]
     assert (f64(dx)[mine, 9] == np.sign(v) * math.inf).all()
     assert torch.isfinite(dx).sum() == dx.numel() - len(mine)
+
+
+def both(mps, t, d_ids, groups):
+    return [mps.adapters(t["x"], t["w"], t["a"], t["b"], d_ids, groups, t["scale"]),
+            *mps.adapters_backward(t["dy"], t["x"], t["w"], t["a"], t["b"], d_ids, groups, t["scale"])]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [1, 60, 1500, 3000])
+def test_captured_and_on_two_streams(mps, cuda, dtype, rows):
+    """Two graphs replayed at once on two streams, on inputs that changed since; and eager calls side by side."""
+    cases = [case(dtype, rows, 5, 40, 512, 1024, 1.0, 1.0, size, seed=i) for i, size in enumerate((1.0, 1e-4))]
+    lists = [mps.group_rows(d_ids, 5) for _, d_ids, _ in cases]
+    want = [both(mps, t, d_ids, g) for (_, d_ids, t), g in zip(cases, lists)]
+    torch.cuda.synchronize()
+    held = [{k: v.clone() for k, v in cases[0][2].items()} for _ in range(2)]
+    ids = [cases[0][1].clone() for _ in range(2)]
+    groups = [mps.Groups(*(p.clone() for p in lists[0])) for _ in range(2)]
+    graphs, results = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i in range(2):
+        with torch.cuda.graph(graphs[i]):
+            results.append(both(mps, held[i], ids[i], groups[i]))
+    for k, v in cases[1][2].items():
+        held[1][k].copy_(v)
+    ids[1].copy_(cases[1][1])
+    for p, q in zip(groups[1], lists[1]):
+        p.copy_(q)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        eager = []
+        for s, g, (_, d_ids, t), l in zip(streams, graphs, cases, lists):
+            with torch.cuda.stream(s):
+                g.replay()
+                eager.append(both(mps, t, d_ids, l))
+                g.replay()
+        torch.cuda.synchronize()
+        for got in (results, eager):
+            assert all(torch.equal(a, b) for r, w in zip(got, want) for a, b in zip(r, w))
+    mps.routed_check()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("rows", [60, 1500])
+def test_wrong_lists_are_reported_and_harmless(mps, cuda, dtype, rows):
+    """Rows and offsets out of range in the caller's list: reported, nothing outside the arrays touched, and the adapters whose lists are
+    right keep their gradients."""
+    ids, d_ids, t = case(dtype, rows, 4, 16, 256, 384, 1.0, 1.0, 1.0)
+    groups = mps.group_rows(d_ids, 4)
+    want = both(mps, t, d_ids, groups)
+    ptr = groups.ptr.tolist()
+    row = groups.row.clone()
+    row[ptr[1]], row[ptr[1] + 1] = -7, rows + 5
+    got = both(mps, t, d_ids, mps.Groups(groups.ptr, row, None))
+    with pytest.raises(mps.MpsError) as e:
+        mps.routed_check()
+    assert e.value.code == mps.capi.ERR_ARG
+    for a, b in ((got[2], want[2]), (got[3], want[3])):
+        assert torch.equal(a[[0, 2, 3]], b[[0, 2, 3]]) and torch.isfinite(a).all()
+    for bad in ([0, ptr[1], 2**31 - 1, -5, ptr[4]], [5, 1, 3, 2, rows], [-2**31] * 5, [rows] * 5):
+        both(mps, t, d_ids, mps.Groups(torch.tensor(bad, dtype=torch.int32, device="cuda"), groups.row, None))
+        torch.cuda.synchronize()
+        try:
+            mps.routed_check()
+        except mps.MpsError as x:
+            assert x.code == mps.capi.ERR_ARG
+    assert all(torch.equal(a, b) for a, b in zip(both(mps, t, d_ids, groups), want))
+    mps.routed_check()
