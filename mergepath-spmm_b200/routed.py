@@ -2,8 +2,9 @@
 
 The routing is kept as the rows listed by group (`Groups`): `ptr` is the row_ptr over groups, `row` the col_idx (the input row
 in every slot), `slot` the slot of every (row, choice).  Thin wrappers of the mps_route* / mps_routed_* / mps_adapters* entry
-points of include/mps.h over torch CUDA tensors (float32, float16 or bfloat16); no reference counterpart.  Gradients are
-functions of their own.  `stream` is where a call runs and what it returns belongs to.  Nothing synchronises; `routed_check()`
+points of include/mps.h over torch CUDA tensors (float32, float16 or bfloat16); no reference counterpart.  Results are not part
+of an autograd graph, whatever the inputs ask for: gradients are functions of their own, which a user's autograd function calls.
+`stream` is where a call runs and what it returns belongs to.  Nothing synchronises; `routed_check()`
 waits and reports what the device met out of range.
 """
 from __future__ import annotations
@@ -118,7 +119,7 @@ def _spec(n_experts, top_k, score, n_groups, top_groups, group_top, renormalise,
 def route(logits, top_k: int, *, score: str = "softmax", bias=None, n_groups: int = 1, top_groups: int = 1, group_top: int = 1,
           renormalise: bool = True, scale: float = 1.0, group: bool = True, stream=None):
     """(ids, weights, groups): the top_k experts of every row of `logits` (rows, experts) by score + bias among the best
-    `top_groups` of `n_groups` expert groups, their weights (fp32), and the rows listed by expert (None with group=False)."""
+    `top_groups` of `n_groups` expert groups, their weights (fp32), and the rows listed by expert (None with group=False).  Gradient: route_backward."""
     rows, experts = _shape("logits", logits)
     dev = logits.device
     at = dev.index
@@ -171,7 +172,8 @@ def group_rows(ids, n_groups: int, *, stream=None) -> Groups:
 
 def routed_product(x, w, groups: Groups, *, gather: bool = True, transpose: bool = False, out=None, stream=None):
     """y[s] = x[groups.row[s]] @ w[g].T for the slots s of every group g (x[s] itself with gather=False); transpose=True
-    multiplies by w[g] instead.  w (groups, n, k).  Rows of `out` behind the last slot in use are left as they were."""
+    multiplies by w[g] instead.  w (groups, n, k).  Rows of `out` behind the last slot in use are left as they were.  Gradients: this
+    with transpose the other way (of the slots) and routed_wgrad."""
     n_groups, n, k = _shape("w", w, 3)
     inner, outer = (n, k) if transpose else (k, n)
     dev, rows, slots = x.device, _shape("x", x)[0], groups.row.numel()
@@ -205,7 +207,8 @@ def routed_wgrad(x, dy, groups: Groups, *, gather: bool = True, out=None, stream
 
 
 def routed_combine(rows, slot, weights=None, *, out=None, stream=None):
-    """y[t] = sum over j of weights[t, j] * rows[slot[t, j]]; no term for a negative slot, weights None: 1 each."""
+    """y[t] = sum over j of weights[t, j] * rows[slot[t, j]]; no term for a negative slot, weights None: 1 each.  Gradients:
+    routed_combine_backward."""
     dev, (n_slots, dim), (n, per_row) = rows.device, _shape("rows", rows), _shape("slot", slot)
     if out is None:
         out = _new(stream, rows, (n, dim))
@@ -257,7 +260,8 @@ def _workspace_bytes(*sizes) -> int:
 
 def adapters(x, w, a, b, ids, groups: Groups, scale=None, *, out=None, stream=None):
     """y[t] = x[t] @ w.T + scale[i] * (x[t] @ a[i].T) @ b[i].T with i = ids[t] (a negative id: the projection alone).
-    w (n, k), a (adapters, rank, k), b (adapters, n, rank), groups = group_rows(ids, adapters), scale fp32 or None (1)."""
+    w (n, k), a (adapters, rank, k), b (adapters, n, rank), groups = group_rows(ids, adapters), scale fp32 or None (1).
+    Gradients: adapters_backward."""
     sizes = rows, k, n, _, _ = _adapter_sizes(x, w, a, b, ids, groups, scale)
     if out is None:
         out = _new(stream, x, (rows, n))
