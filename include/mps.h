@@ -461,7 +461,7 @@ MPS_API int mps_routed_combine_backward(int32_t n_rows, int32_t per_row, int32_t
  * d_x n_rows x k, d_w n x k, d_a n_adapters x rank x k, d_b n_adapters x n x rank, d_scale n_adapters fp32 (NULL: 1), d_y
  * n_rows x n.  d_group_ptr and d_slot_row list the rows by adapter (mps_group_rows of d_ids, per_row 1).  n_adapters <= 1024,
  * rank <= 4096.  The intermediate scale * x A^T is kept in fp32; with 16-bit types the second product may read it as the sum of two
- * values (2^-16 of it at most lost in bf16, 2^-21 in fp16).  A group's rows may be listed in any order.  d_workspace: mps_adapters_workspace bytes (a negative return is an error), 256-byte aligned, for this call
+ * values (2^-16 of it at most lost in bf16, 2^-134 where that is more; 2^-21 in fp16).  A group's rows may be listed in any order.  d_workspace: mps_adapters_workspace bytes (a negative return is an error), 256-byte aligned, for this call
  * alone while it runs. */
 MPS_API int64_t mps_adapters_workspace(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, int backward);
 MPS_API int mps_adapters(int32_t n_rows, int32_t k, int32_t n, int32_t n_adapters, int32_t rank, int dtype, const int32_t *d_ids,

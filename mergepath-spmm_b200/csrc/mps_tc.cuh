@@ -270,12 +270,12 @@ __device__ __forceinline__ float4 load_shared_float4(uint32_t addr) {
 __device__ __forceinline__ void store_shared_f32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
 
 // An fp32 value as the sum of two tf32 values, off by 2^-21 of it at most: its first eleven bits, and what is left rounded to
-// eleven.  The second has the first's sign and is no zero unless the value is one, so that an infinite factor gives the infinity
-// that the value would; of an infinite value it is next to nothing.
+// eleven.  The second has the first's sign and (from 2^-100 up, where the least normal number is nothing) is no zero, so that an
+// infinite factor gives the infinity that the value would; of an infinite value it is next to nothing.
 __device__ __forceinline__ float tf32_first(float v) { return v != v ? v : __uint_as_float(__float_as_uint(v) & 0xffffe000u); }
 __device__ __forceinline__ float tf32_second(float v) {
     const uint32_t rest = fabsf(v) < INFINITY ? (__float_as_uint(fabsf(v - tf32_first(v))) + 0x1000u) & 0xffffe000u : 0u;
-    return v == 0.0f ? 0.0f : copysignf(__uint_as_float(rest < 0x00800000u ? 0x00800000u : rest), v);
+    return copysignf(__uint_as_float(rest < 0x00800000u && fabsf(v) >= 0x1p-100f ? 0x00800000u : rest), v);
 }
 
 // The same of four values in bf16, two to a word: 2^-16 of a value lost.
@@ -283,7 +283,7 @@ __device__ __forceinline__ uint32_t bf16_first(float v) { return v != v ? 0x7fff
 __device__ __forceinline__ uint32_t bf16_second(float v) {
     const float rest = fabsf(v) < INFINITY ? v - __uint_as_float(bf16_first(v) << 16) : 0.0f;
     const uint32_t bits = __bfloat16_as_ushort(__float2bfloat16_rn(fabsf(rest)));
-    return v == 0.0f ? 0u : (bits < 0x0080u ? 0x0080u : bits) | (__float_as_uint(v) >> 16 & 0x8000u);
+    return (bits < 0x0080u && fabsf(v) >= 0x1p-100f ? 0x0080u : bits) | (__float_as_uint(v) >> 16 & 0x8000u);
 }
 __device__ __forceinline__ void split_bf16(float4 v, uint2 &first, uint2 &second) {
     first = make_uint2(bf16_first(v.x) | bf16_first(v.y) << 16, bf16_first(v.z) | bf16_first(v.w) << 16);

@@ -253,3 +253,25 @@ def test_wrong_lists_are_reported_and_harmless(mps, cuda, dtype, rows):
             assert x.code == mps.capi.ERR_ARG
     assert all(torch.equal(a, b) for a, b in zip(both(mps, t, d_ids, groups), want))
     mps.routed_check()
+
+
+@pytest.mark.parametrize("rows,why", ROWS)
+@pytest.mark.parametrize("x_size,b_size", [(1e-17, 1e22), (1e-18, 1e23), (1e17, 1e-20)])
+def test_bf16_intermediates_at_the_ends_of_its_range(mps, cuda, rows, why, x_size, b_size):
+    """Sums of eight products, so that what the intermediate itself loses shows: about 1e-34, 1e-35 and 1e34 (by matrices of the same
+    size as x); the gradients likewise.  A value's second part is what bf16 rounds it to: half a step of 2^-16 of the value, or, below
+    2^-118, where that part is subnormal, half a step of 2^-133 of it, which meets |b| (or |a|).  At 1e-35 some values are."""
+    ids, d_ids, t = case(BF16, rows, 3, 8, 8, 64, x_size, 1.0, b_size, a_size=x_size)
+    wide = {name: f64(v) for name, v in t.items()}
+    want = o.adapters(wide["x"], wide["w"], wide["a"], wide["b"], ids, wide["scale"])
+    close(f64(mps.adapters(t["x"], t["w"], t["a"], t["b"], d_ids, mps.group_rows(d_ids, 3), t["scale"])), want[0], BF16, 8 + 8 + 2, want[1],
+          o.PAIR[BF16] * want[2] + 2.0 ** -134 * want[3])
+    gen = gen_of(rows)  # dx = dy W + (scale dy B) A with dy and B small (large), A large (small)
+    t = dict(x=rand(gen, BF16, rows, 64), w=rand(gen, BF16, 8, 64, scale=x_size), a=rand(gen, BF16, 3, 8, 64, scale=b_size), b=rand(gen, BF16, 3, 8, 8, scale=x_size),
+             dy=rand(gen, BF16, rows, 8, scale=x_size), scale=torch.ones(3, device="cuda"))
+    groups = mps.group_rows(d_ids, 3)
+    wide = {name: f64(v) for name, v in t.items()}
+    dx, _, _ = mps.adapters_backward(t["dy"], t["x"], t["w"], t["a"], t["b"], d_ids, groups, t["scale"])
+    want = o.adapters_grad(wide["dy"], wide["x"], wide["w"], wide["a"], wide["b"], ids, wide["scale"])[0]
+    close(f64(dx), want[0], BF16, 8 + 8 + 2, want[1], o.PAIR[BF16] * want[2] + 2.0 ** -134 * want[3])
+    mps.routed_check()
