@@ -183,8 +183,8 @@ __device__ __forceinline__ bool keep_groups(F (&key)[VPL], const F (&value)[VPL]
 
 // The top_k largest keys: lane j returns the j-th expert (or -1) in `mine`.  Every lane keeps the best two of its keys at hand, so
 // that most picks cost two warp reductions and no pass over the keys.  EXACT keys are compared as they are; others must be
-// `clearance` apart unless they belong to equal logits and equal biases.  Picking goes on behind the last place until a key is
-// that far away: behind one that equals the last pick there may be one that only seems to.  Returns false where keys are closer.
+// `clearance` apart unless they belong to equal logits and equal biases, and so must the last pick and every key that is left (not
+// the next one alone: behind one that equals the last pick there may be one that only seems to).  Returns false where they are not.
 template <bool EXACT, bool SIGMOID, typename F, int VPL, typename T>
 __device__ __forceinline__ bool choose(F (&key)[VPL], const RouteArgs &a, const T *logits, const float *bias, int lane, int &mine) {
     F one, two;
@@ -206,20 +206,23 @@ __device__ __forceinline__ bool choose(F (&key)[VPL], const RouteArgs &a, const 
     bool clear = true;
     float prev = INFINITY;
     int prev_at = -1;
-    for (int j = 0; !EXACT || j < a.top_k; ++j) {
+    auto equal = [&](int e, int o) { return to_f32(logits[e]) == to_f32(logits[o]) && bias[e] == bias[o]; };
+    for (int j = 0; j < a.top_k; ++j) {
         F best = one;
         int at = lane + 32 * one_at;
         warp_best(best, at);
-        if (!(best > neg_inf<F>())) break;
+        if (!(best > neg_inf<F>())) {
+            prev_at = -1;  // nothing is left
+            break;
+        }
         if (!EXACT) {
             const float v = (float)best;
-            const bool close = prev_at >= 0 && prev - v <= clearance<SIGMOID>(v);
-            clear = !close || (to_f32(logits[prev_at]) == to_f32(logits[at]) && bias[prev_at] == bias[at]);
-            if (!clear || (j >= a.top_k && !close)) break;
+            clear = !(prev_at >= 0 && prev - v <= clearance<SIGMOID>(v)) || equal(prev_at, at);
+            if (!clear) break;
             prev = v;
             prev_at = at;
         }
-        if (lane == j && j < a.top_k) mine = at;
+        if (lane == j) mine = at;
         if ((at & 31) == lane) {
 #pragma unroll
             for (int i = 0; i < VPL; ++i)
@@ -230,6 +233,13 @@ __device__ __forceinline__ bool choose(F (&key)[VPL], const RouteArgs &a, const 
                 two = neg_inf<F>();
             } else scan();
         }
+    }
+    if (!EXACT && clear && prev_at >= 0 && __any_sync(kAll, prev - (float)one <= clearance<SIGMOID>((float)one))) {
+        bool close = false;
+#pragma unroll
+        for (int i = 0; i < VPL; ++i)
+            if (key[i] > neg_inf<F>() && prev - (float)key[i] <= clearance<SIGMOID>((float)key[i])) close = close || !equal(prev_at, lane + 32 * i);
+        clear = !__any_sync(kAll, close);
     }
     return clear;
 }
@@ -360,12 +370,35 @@ __global__ void __launch_bounds__(32 * kRouteWarps, VPL <= 8 ? 8 : 1) route_kern
     }
 }
 
+// the fp32 key of an expert, all of its bits
+template <typename T, bool SIGMOID>
+__device__ __forceinline__ float whole_key(const T *line, const float *bias, float peak, float total, int e) {
+    const float x = to_f32(line[e]);
+    return bias ? (SIGMOID ? key_sigmoid(x) : key_div(key_exp(x - peak), total)) + bias[e] : x;
+}
+
+// Whether one of `count` experts from `first` that was not picked, and is not equal to the last pick by what its key is made of, may
+// belong before it.  Out of line: few rows ask.
+template <typename T, bool SIGMOID>
+__device__ __noinline__ bool may_be_lost(const T *line, const float *bias, float peak, float total, int first, int count, int last, const int *picks, int top_k) {
+    const float key = whole_key<T, SIGMOID>(line, bias, peak, total, last);
+    for (int e = first; e < first + count; ++e) {
+        const float k = whole_key<T, SIGMOID>(line, bias, peak, total, e);
+        if (!(to_f32(line[e]) > -INFINITY && k > -INFINITY && key - k <= (bias ? clearance<SIGMOID>(k) : 0.0f))) continue;
+        if (to_f32(line[e]) == to_f32(line[last]) && (!bias || bias[e] == bias[last])) continue;
+        bool picked = false;
+        for (int r = 0; r < top_k; ++r) picked = picked || picks[r] == e;
+        if (!picked) return true;
+    }
+    return false;
+}
+
 // Many rows: eight lanes per row, four rows per warp, so that a pick's reductions serve four rows.  A lane holds a contiguous
 // eighth of the experts (a part of one group: 1, 2, 4 or 8 groups) as integers that order like the keys, the low five bits
 // replaced by the place in the lane: the lane's best is one integer maximum, equal keys go to the lower place by themselves, and
 // taking an expert out is a comparison with the value that won.  Keys that differ in the five bits only count as close (of
-// 16-bit logits without a bias they are zeros); behind the last place every key is compared with the last pick until they are
-// too far down for the five bits to matter.  16384 rows of 256 experts, top 8 of 4 of 8 groups:
+// 16-bit logits without a bias they are zeros); where a key that is left may be as large as the last pick, every one is looked at
+// again.  16384 rows of 256 experts, top 8 of 4 of 8 groups:
 // 30 us, 42 with a warp per row (which keeps fewer rows, other group counts and more experts).
 constexpr int kOctetRows = 2048;  // from here on there are rows enough for a B200's 148 SMs
 
@@ -487,36 +520,26 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 6) route_octet_kernel(const 
 #pragma unroll
         for (int i = 0; i < VPL; ++i) best = max(best, key[i]);
         int prev_at = -1;
-        for (int j = 0;; ++j) {
+        for (int j = 0; j < a.top_k; ++j) {
             unsigned top = (best & ~31u) | (best ? 8 - sub : 0);  // the lower lane among equals
 #pragma unroll
             for (int d = 1; d < 8; d <<= 1) top = max(top, __shfl_xor_sync(kAll, top, d));
             const int owner = 8 - (int)(top & 31u);  // 8: none left in this row
             const unsigned won = __shfl_sync(kAll, best, (quad << 3) | (owner & 7));
             const int at = owner < 8 ? owner * chunk + 31 - (int)(won & 31u) : -1;
-            bool near = false;  // this key or one behind it may be close to the one picked before
             if (at >= 0 && prev_at >= 0 && !whole) {
                 const float p = key_of(prev), v = key_of(top);
                 bool close = (prev & ~31u) == (top & ~31u);
-                near = close;
                 if (has_bias && p - v <= clearance<SIGMOID>(v) + 8e-6f * fmaxf(fabsf(p), fabsf(v))) {  // within the five bits: by the whole keys
-                    auto whole_key = [&](int e) {
-                        const float x = to_f32(line[e]);
-                        return (SIGMOID ? key_sigmoid(x) : key_div(key_exp(x - peak), total)) + bias[e];
-                    };
-                    const float k = whole_key(at);
-                    near = true;
-                    close = close || whole_key(prev_at) - k <= clearance<SIGMOID>(k);
+                    const float k = whole_key<T, SIGMOID>(line, bias, peak, total, at);
+                    close = close || whole_key<T, SIGMOID>(line, bias, peak, total, prev_at) - k <= clearance<SIGMOID>(k);
                 }
                 if (close) clear = clear && to_f32(line[prev_at]) == to_f32(line[at]) && (!has_bias || bias[prev_at] == bias[at]);
             }
-            if (j < a.top_k) {
-                prev = top;
-                prev_at = at;
-                if (sub == 0) s_pick[warp][quad][j] = at;
-            }
-            const bool more = j + 1 < a.top_k || (!whole && (j + 1 == a.top_k || near));
-            if (!__any_sync(kAll, at >= 0 && clear && more)) {
+            prev = top;
+            prev_at = at;
+            if (sub == 0) s_pick[warp][quad][j] = at;
+            if (!__any_sync(kAll, at >= 0 && clear)) {
                 for (int r = j + 1; sub == 0 && r < a.top_k; ++r) s_pick[warp][quad][r] = -1;
                 break;
             }
@@ -528,6 +551,20 @@ __global__ void __launch_bounds__(32 * kRouteWarps, 6) route_octet_kernel(const 
                     best = max(best, key[i]);
                 }
             }
+        }
+        if (!whole) {
+            // the best key that is left to this lane, against the last pick: as far as the five bits tell
+            bool close = false;
+            if (prev_at >= 0 && clear && best) {
+                const float p = key_of(prev), v = key_of(best);
+                close = has_bias ? p - v <= clearance<SIGMOID>(v) + 8e-6f * fmaxf(fabsf(p), fabsf(v)) : (prev & ~31u) == (best & ~31u);
+            }
+            if (__any_sync(kAll, close)) {
+                __syncwarp();  // the picks are read below
+                if (close) close = may_be_lost<T, SIGMOID>(line, bias, peak, total, first, chunk, prev_at, s_pick[warp][quad], a.top_k);
+            }
+            const unsigned lanes_close = __ballot_sync(kAll, close);
+            clear = clear && !(lanes_close >> (quad * 8) & 0xff);
         }
         __syncwarp();
         // rows that fp32 keys do not decide, by the whole warp
